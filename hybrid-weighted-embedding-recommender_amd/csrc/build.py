@@ -19,6 +19,9 @@ OBJ_TAG = "" if os.path.basename(LIB) == "libhwer_hip.so" else "." + os.path.bas
 SOURCES = ["rowops.hip", "knn_screen.hip", "knn_small.hip", "knn_select.hip", "knn_select_f64.hip", "fit_pca.hip", "rows_f64.hip", "knn_wide.hip"]
 HEADERS = ["hwer_common.h", "knn_internal.h", "knn_select_kernels.h", os.path.join(ROOT, "include", "hwer_hip.h")]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math",
+         # no packed float32 instructions (v_pk_add / mul / fma_f32): -O3 forms them from ordinary float code, and some of their forms have given
+         # wrong results on this chip now and then (hipcc's host pass does not know the feature and warns: harmless)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-I" + os.path.join(ROOT, "include"), "-I" + HERE, "-Wno-unused-result"] + os.environ.get("HIPCC_EXTRA", "").split()
 # HIPCC_EXTRA=-DHWER_DIAG_STAMPS builds the screen kernel with its s_memtime phase stamps (diagnosis only: the stamps carry
 # scheduling barriers; the production build has none)
