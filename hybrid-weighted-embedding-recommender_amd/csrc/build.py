@@ -16,8 +16,9 @@ LIBDIR = os.path.join(os.path.dirname(HERE), "lib")
 # HWER_LIB_NAME=libhwer_hip_diag.so HIPCC_EXTRA=-DHWER_DIAG_STAMPS python build.py: a diagnostic library beside the production one (own objects)
 LIB = os.path.join(LIBDIR, os.environ.get("HWER_LIB_NAME", "libhwer_hip.so"))
 OBJ_TAG = "" if os.path.basename(LIB) == "libhwer_hip.so" else "." + os.path.basename(LIB).replace(".so", "")
-SOURCES = ["rowops.hip", "knn_screen.hip", "knn_small.hip", "knn_select.hip", "knn_select_f64.hip", "fit_pca.hip", "rows_f64.hip", "knn_wide.hip"]
-HEADERS = ["hwer_common.h", "knn_internal.h", "knn_select_kernels.h", os.path.join(ROOT, "include", "hwer_hip.h")]
+SOURCES = ["rowops.hip", "knn_screen.hip", "knn_small.hip", "knn_select.hip", "knn_select_f64.hip", "fit_pca.hip", "rows_f64.hip", "knn_wide.hip", "head_norm.hip", "matmul_q8.hip",
+           "catalogue_ce.hip"]
+HEADERS = ["hwer_common.h", "head_common.h", "knn_internal.h", "knn_select_kernels.h", os.path.join(ROOT, "include", "hwer_hip.h")]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math",
          # no packed float32 instructions (v_pk_add / mul / fma_f32): -O3 forms them from ordinary float code, and some of their forms have given
          # wrong results on this chip now and then (hipcc's host pass does not know the feature and warns: harmless)

@@ -1,0 +1,850 @@
+// Softmax cross entropy of query rows over a whole catalogue of item rows, and its gradients, without the logits ever being in memory.
+//
+//   z_rv = s <x_r, e_v> + b_v      lse_r = log sum_v exp z_rv      loss_r = lse_r - z_{r, t_r}      p_rv = exp(z_rv - lse_r)
+//   dx_r = s g_r (sum_v p_rv e_v - e_{t_r})      de_v = s sum_r g_r (p_rv - [v = t_r]) x_r      db_v = sum_r g_r (p_rv - [v = t_r])
+//
+// A row's target stands apart from its other classes throughout, so that a row that has learnt its target (p_t close to 1) keeps its digits:
+// with lse' and p' over the classes but the target,  x = lse' - z_t,  loss = log(1 + e^x),  1 - p_t = 1 / (1 + e^-x),
+//   dx_r = s g_r (1 - p_t) (sum_{v /= t} p'_v e_v - e_t)        and the target's weight in de is  -g_r (1 - p_t).
+//
+// Two passes of ONE kernel shape.  A wave keeps 32 "stationary" rows as matrix operands in registers and walks over tiles of "streaming" rows in LDS:
+//   S^T = streaming . stationary^T     (a lane holds one stationary row, its 16 registers 16 streaming rows)
+//   W   = f(S^T)                       in registers
+//   O^T += streaming^T . W             (W is already laid out as the second product's operand; the tile is read transposed from LDS)
+// Pass 1: stationary = queries, streaming = catalogue, f = exp with a running maximum: gives lse' and sum_v p'_v e_v, all that dx needs, at once.
+// Pass 2: stationary = catalogue, streaming = queries, f = the finished probabilities, the targets' put in: gives de (and db).
+// 8 N V d operations in all against 6 N V d with stored logits (4 bytes each way per logit): the recomputed product is cheaper than their traffic.
+//
+// float32 rows: each value is split into two float16 terms, x 2^e = hi + lo, with one power of two for a whole operand that puts its largest value in
+// [2^14, 2^15): 22 bits wherever a value is above 2^-18 of the largest, an absolute error of 2^-40 of it below.  A product then is
+// hi hi + hi lo + lo hi on the float16 matrix instructions with float32 sums (the missing lo lo term is below 2^-22): three times the work of a
+// 16-bit product, five times faster than the float32 matrix instructions.
+#include <algorithm>
+
+#include "head_common.h"
+#include "knn_internal.h"   // lds_dma16_v, lds_addr
+
+namespace hwer {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr double kLn2d = 0.6931471805599453;
+constexpr float kLowest = -INFINITY;
+// The weights are rounded to the rows' 16-bit type for the second product.  bfloat16 has float32's range.  float16 ends at 2^16 above, and below 2^-14
+// its steps stay at 2^-24, so float16 weights carry a power of two that uses the range up: pass 1, whose weights may exceed the maximum they are
+// taken against by 2^kStale before it is renewed, 2^11 (weights are kept to 2^-36 of a row's largest); pass 2, whose weights are at most 1, 2^15
+// (kept to 2^-40).
+constexpr float kStale = 4.f;
+template <typename E> struct CeType;
+template <> struct CeType<f16_t> {
+    static constexpr float offset[2] = {11.f, 15.f};
+    typedef f16x8 x8;
+    static __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct CeType<bf16_t> {
+    static constexpr float offset[2] = {0.f, 0.f};
+    typedef bf16x8 x8;
+    static __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+
+// device-side scalars of a call (in its workspace)
+struct CeScalars {
+    float unscale_s, unscale_q, unscale_e;      // 2^-(eq + ee), 2^-eq, 2^-ee: what undoes the operands' powers of two (1 for 16-bit rows)
+    float fac_e, fac_b;                          // factors of de and db
+    float g_top;                                 // largest |upstream gradient| of a row
+};
+
+struct CePass {
+    const short *stat, *stat_lo, *strm, *strm_lo;      // 16-bit terms; rows of DP values (lo: second term of float32 rows)
+    int64_t ld_stat, ld_strm, n_stat, n_strm;
+    const float* bias;           // per catalogue row
+    float scale;
+    const CeScalars* sc;
+    int tiles_per_split, n_splits, stat_blocks;
+    float *m, *l, *o;            // pass 1: (split, n_stat) maxima and sums, (split, n_stat, DP) weighted sums; pass 2: l, o likewise when split
+    const int64_t* target;       // pass 1: per query its target
+    float* zt;                   // pass 1: per query its target's logit, in the unit of m
+    const float4* rowp;          // pass 2: per query {what is taken off its logits, factor of its weights, its target's weight, target (int bits) or -1}
+    void* out;                   // pass 2, one split: de in the rows' type, and db
+    float* out_b;
+    int64_t ld_out;
+    int d, out_vec;
+};
+
+enum { kLse = 0, kMean = 1, kTable = 2 };
+
+// streaming rows per LDS tile: 16 - 32 KB a buffer
+template <int TERMS, int DP> constexpr int ce_sub() { return TERMS * DP <= 64 ? 4 : TERMS * DP <= 256 ? 2 : 1; }
+
+// LDS image: rows of DP / 8 chunks of 16 bytes, chunk c of row r at c ^ f(r).  Eight consecutive rows have eight different f, so the fragment reads
+// (8 rows, one chunk) and the transposed reads (4 rows, two neighbouring chunks) both touch every bank once.
+__device__ __forceinline__ int ce_swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+
+template <typename E, int TERMS, int DP, int MODE, bool BIAS, bool ROWG>
+__global__ __launch_bounds__(256, (TERMS * DP > 256 ? 1 : 2)) void ce_pass_kernel(CePass a) {
+    typedef CeType<E> X;
+    constexpr int KC = DP / 16, DB = DP / 32, SB = ce_sub<TERMS, DP>(), TS = 32 * SB, ROWB = DP * 2, PLANE = TS * ROWB;
+    // The factor carries a query's own upstream gradient, and the part of its lse that float32 cannot hold beside |lse| ~ 40 (2^-19 of a weight):
+    // of no account in 16-bit gradients, so plain 16-bit passes save the multiplication.
+    constexpr bool MUL = MODE == kTable && (ROWG || BIAS || TERMS == 2);
+    constexpr float OFF = X::offset[MODE == kTable];
+    __shared__ __align__(16) char s_tile[2][TERMS][PLANE];
+    __shared__ float s_x[2][TS];                          // pass 1: bias; pass 2: what is taken off the query's logits
+    __shared__ float s_mul[MUL ? 2 : 1][MUL ? TS : 1];    // pass 2: ... factor of its weights
+    __shared__ float s_hot[2][MODE == kTable ? TS : 1];   // ... its target's weight
+    __shared__ int s_tgt[2][MODE == kTable ? TS : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l31 = lane & 31;
+    // consecutive numbers stay on one XCD (workgroup id mod 8), and consecutive numbers share a split: the tiles they stream meet in that XCD's L2
+    const int total = a.stat_blocks * a.n_splits, per = (total + 7) / 8;
+    const int id = int(blockIdx.x & 7) * per + int(blockIdx.x >> 3);
+    if (int(blockIdx.x >> 3) >= per || id >= total) return;
+    const int split = id / a.stat_blocks, sblock = id % a.stat_blocks;
+    const int64_t row0 = int64_t(sblock) * 128 + wave * 32, my = row0 + l31;
+    const int64_t myc = my < a.n_stat ? my : a.n_stat - 1;
+
+    s16x8 xf[TERMS][KC];
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int k = 0; k < KC; ++k) xf[t][k] = *reinterpret_cast<const s16x8*>((t ? a.stat_lo : a.stat) + myc * a.ld_stat + 16 * k + 8 * half);
+    f32x16 o[MODE == kLse ? 1 : DB];
+#pragma unroll
+    for (int i = 0; i < (MODE == kLse ? 1 : DB); ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+    const float scl = a.scale * a.sc->unscale_s, c = fmaxf(scl * kLog2e, 1.2e-38f);      // (never 0: 0 * -inf)
+    const float thr = BIAS ? kStale * kLn2 : kStale / c;
+    float m = kLowest, renew = kLowest, l = 0.f;
+    int64_t target = MODE != kTable && my < a.n_stat ? a.target[my] : -1;
+    float zt = 0.f;
+    bool has_zt = false;
+    const float my_bias = (BIAS && MODE == kTable) ? a.bias[myc] : 0.f;
+
+    const int n_tiles = int((a.n_strm + TS - 1) / TS);
+    const int tile0 = split * a.tiles_per_split, tile1 = min(n_tiles, tile0 + a.tiles_per_split);
+    auto stage = [&](int tile, int buf) {
+        constexpr int RPI = 1024 / ROWB, PER_WAVE = PLANE / 4096;      // rows per DMA instruction (1 KB); instructions of a wave and term
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int i = 0; i < PER_WAVE; ++i) {
+                const int piece = wave * PER_WAVE + i, r = piece * RPI + lane / (ROWB / 16), ch = (lane % (ROWB / 16)) ^ ce_swz(r);
+                const int64_t g = min(int64_t(tile) * TS + r, a.n_strm - 1);      // rows past the end repeat the last one; their weights are zero
+                lds_dma16_v((t ? a.strm_lo : a.strm) + g * a.ld_strm + 8 * ch, __builtin_amdgcn_readfirstlane(lds_addr(&s_tile[buf][t][piece * 1024])));
+            }
+    };
+    float4 next_row = {0.f, 0.f, 0.f, 0.f};
+    auto fetch_params = [&](int tile) {
+        const int64_t g = int64_t(tile) * TS + threadIdx.x;
+        if (int(threadIdx.x) < TS) {
+            if (MODE == kTable) {
+                next_row = g < a.n_strm ? a.rowp[g] : float4{INFINITY, 0.f, 0.f, __int_as_float(-1)};
+            } else if (BIAS) {
+                next_row.x = g < a.n_strm ? a.bias[g] : kLowest;
+            }
+        }
+    };
+    auto put_params = [&](int buf) {
+        if (int(threadIdx.x) < TS) {
+            if (MODE == kTable || BIAS) s_x[buf][threadIdx.x] = next_row.x;
+            if (MUL) s_mul[buf][threadIdx.x] = next_row.y;
+            if (MODE == kTable) {
+                s_hot[buf][threadIdx.x] = next_row.z;
+                s_tgt[buf][threadIdx.x] = __float_as_int(next_row.w);
+            }
+        }
+    };
+    if (tile0 < tile1) {
+        stage(tile0, 0);
+        fetch_params(tile0);
+        put_params(0);
+    }
+    // lane-constant parts of the LDS addresses (bytes)
+    int fr_off[4], tr_off[2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) fr_off[k] = l31 * ROWB + 16 * ((2 * k + half) ^ ce_swz(l31));
+    {
+        const int r = 4 * half + ((lane & 15) >> 2), cl = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) tr_off[k] = r * ROWB + 16 * ((4 * k + cl) ^ ce_swz(r)) + 8 * (lane & 1);
+    }
+    for (int tile = tile0; tile < tile1; ++tile) {
+        const int buf = (tile - tile0) & 1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();      // this tile is staged, and everyone is done with the other buffer
+        if (tile + 1 < tile1) {
+            stage(tile + 1, buf ^ 1);
+            fetch_params(tile + 1);
+        }
+        const int64_t from_tile = target - int64_t(tile) * TS;
+        const int my_target = MODE != kTable && from_tile >= 0 && from_tile < TS ? int(from_tile) : -1;
+        bool hit = false;      // does any of the tile's queries have its target among this wave's rows?
+        if (MODE == kTable) {
+            bool h = false;
+#pragma unroll
+            for (int i = 0; i < (TS + 63) / 64; ++i) {
+                const int t = (TS >= 64 || lane < TS) ? s_tgt[buf][i * 64 + (lane & (TS - 1 < 63 ? TS - 1 : 63))] : -1;
+                h = h || (t >= row0 && t < row0 + 32);
+            }
+            hit = __any(h);
+        }
+#pragma unroll
+        for (int sb = 0; sb < SB; ++sb) {
+            f32x16 s;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[j] = 0.f;
+            const char* t_hi = s_tile[buf][0] + sb * 32 * ROWB;
+            const char* t_lo = s_tile[buf][TERMS - 1] + sb * 32 * ROWB;
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                const s16x8 fh = *reinterpret_cast<const s16x8*>(t_hi + fr_off[k & 3] + 128 * (k >> 2));
+                s = X::mfma(fh, xf[0][k], s);
+                if constexpr (TERMS == 2) {
+                    const s16x8 fl = *reinterpret_cast<const s16x8*>(t_lo + fr_off[k & 3] + 128 * (k >> 2));
+                    s = X::mfma(fl, xf[0][k], s);
+                    s = X::mfma(fh, xf[1][k], s);
+                }
+            }
+            // register j of this lane: streaming row 8 (j / 4) + 4 half + j % 4 of the 32
+            float w[16];
+            if constexpr (MODE == kTable) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = sb * 32 + 8 * q + 4 * half + j;
+                        float v;
+                        if (BIAS) v = __builtin_amdgcn_exp2f(fmaf((fmaf(s[4 * q + j], scl, my_bias) - s_x[buf][r]), kLog2e, OFF));
+                        else v = __builtin_amdgcn_exp2f(fmaf(s[4 * q + j], c, -s_x[buf][r]));
+                        if (MUL) v *= s_mul[buf][r];
+                        w[4 * q + j] = v;
+                    }
+                if (hit) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int r = sb * 32 + 8 * q + 4 * half + j;
+                            if (s_tgt[buf][r] == int(my)) w[4 * q + j] = s_hot[buf][r];
+                        }
+                }
+                if (BIAS) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) l += w[j];
+                }
+            } else {
+                if (!BIAS && tile == n_tiles - 1) {      // (with a bias, rows past the end have one of -inf)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (int64_t(tile) * TS + sb * 32 + 8 * (j >> 2) + 4 * half + (j & 3) >= a.n_strm) s[j] = kLowest;
+                }
+                if (BIAS) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) s[j] = fmaf(s[j], scl, s_x[buf][sb * 32 + 8 * (j >> 2) + 4 * half + (j & 3)]);
+                }
+                const int at = my_target - sb * 32;      // the target among these 32 rows: its logit is noted, and it is left out
+                if (__any(unsigned(at) < 32u)) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (at == 8 * (j >> 2) + 4 * half + (j & 3)) {
+                            zt = s[j];
+                            has_zt = true;
+                            s[j] = kLowest;
+                        }
+                }
+                float mx = s[0];
+#pragma unroll
+                for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
+                mx = fmaxf(mx, __uint_as_float(lane_xor32<32>(__float_as_uint(mx))));
+                if (__any(mx > renew)) {
+                    const float mn = fmaxf(m, mx);
+                    // (m = -inf: nothing so far, l and o are 0; differences first: a bias of float32's lowest value must not overflow)
+                    const float f = m == kLowest ? 1.f : __builtin_amdgcn_exp2f((m - mn) * (BIAS ? kLog2e : c));
+                    m = mn;
+                    renew = m == kLowest ? kLowest : m + thr;
+                    l *= f;
+                    if constexpr (MODE == kMean) {
+#pragma unroll
+                        for (int i = 0; i < DB; ++i)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[i][j] *= f;
+                    }
+                }
+                const float mu = m == kLowest ? 0.f : m, sub = OFF - mu * c;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    w[j] = BIAS ? __builtin_amdgcn_exp2f(fmaf(s[j] - mu, kLog2e, OFF)) : __builtin_amdgcn_exp2f(fmaf(s[j], c, sub));
+                    l += w[j];
+                }
+            }
+            if constexpr (MODE != kLse) {
+                s16x8 ph[2], pl[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    typename X::x8 hi, lo;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        hi[j] = E(w[8 * k + j]);
+                        if (TERMS == 2) lo[j] = E(w[8 * k + j] - float(hi[j]));
+                    }
+                    ph[k] = __builtin_bit_cast(s16x8, hi);
+                    if (TERMS == 2) pl[k] = __builtin_bit_cast(s16x8, lo);
+                }
+                typedef __attribute__((address_space(3))) s16x4* lds4;
+                auto transposed = [&](const char* t, int i, int k) {      // 16 streaming rows x 32 columns, as the product's row operand
+                    const char* p = t + tr_off[i & 1] + 128 * (i >> 1) + 16 * k * ROWB;
+                    const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p));
+                    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 8 * ROWB));
+                    return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+                };
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const s16x8 eh = transposed(t_hi, i, k);
+                        o[i] = X::mfma(eh, ph[k], o[i]);
+                        if constexpr (TERMS == 2) {
+                            const s16x8 el = transposed(t_lo, i, k);
+                            o[i] = X::mfma(el, ph[k], o[i]);
+                            o[i] = X::mfma(eh, pl[k], o[i]);
+                        }
+                    }
+            }
+        }
+        if (tile + 1 < tile1) put_params(buf ^ 1);
+    }
+
+    l += __uint_as_float(lane_xor32<32>(__float_as_uint(l)));
+    if (my >= a.n_stat) return;
+    if (MODE != kTable && has_zt) a.zt[my] = zt;
+    const bool direct = MODE == kTable && a.n_splits == 1;
+    if (!direct) {
+        const int64_t at = int64_t(split) * a.n_stat + my;
+        if (half == 0) {
+            if (MODE != kTable) a.m[at] = m;
+            if (MODE != kTable || BIAS) a.l[at] = l;
+        }
+        if constexpr (MODE != kLse) {
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<float4*>(a.o + at * DP + 32 * i + 8 * q + 4 * half) = float4{o[i][4 * q], o[i][4 * q + 1], o[i][4 * q + 2], o[i][4 * q + 3]};
+        }
+        return;
+    }
+    if constexpr (MODE == kTable) {
+        typedef typename std::conditional<TERMS == 2, float, E>::type OUT;
+        const float f = a.sc->fac_e;
+        OUT* out = static_cast<OUT*>(a.out) + my * a.ld_out;
+        if (BIAS && half == 0 && a.out_b) a.out_b[my] = l * a.sc->fac_b;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int col = 32 * i + 8 * q + 4 * half;
+                typedef OUT out4 __attribute__((ext_vector_type(4)));
+                const out4 v = {OUT(o[i][4 * q] * f), OUT(o[i][4 * q + 1] * f), OUT(o[i][4 * q + 2] * f), OUT(o[i][4 * q + 3] * f)};
+                if (a.out_vec) {
+                    if (col < a.d) *reinterpret_cast<out4*>(out + col) = v;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col + j < a.d) out[col + j] = v[j];
+                }
+            }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- operands
+// Rows that the passes cannot read in place (width not 64 / 128 / 256, rows not on 16 bytes, float32) are laid out once per call.
+struct CePack {
+    const void* src[2];
+    short *hi[2], *lo[2];
+    int64_t rows[2], ld[2];
+    int d, dp;
+    float* tops;             // (2, kTopBlocks) partial maxima of |value|
+    CeScalars* sc;
+};
+constexpr int kTopBlocks = 256;
+
+// 16-bit rows: copied with zeros behind them.  blockIdx.y: which operand.
+__global__ __launch_bounds__(256) void ce_pack16_kernel(CePack a) {
+    const int w = blockIdx.y, chunks = a.dp / 8;
+    if (!a.hi[w]) return;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < a.rows[w] * chunks; i += int64_t(gridDim.x) * 256) {
+        const int64_t r = i / chunks;
+        const int c = int(i % chunks) * 8;
+        const short* p = static_cast<const short*>(a.src[w]) + r * a.ld[w];
+        s16x8 v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < a.d ? p[c + j] : short(0);
+        *reinterpret_cast<s16x8*>(a.hi[w] + r * a.dp + c) = v;
+    }
+}
+
+__global__ __launch_bounds__(256) void ce_top_kernel(CePack a) {
+    __shared__ float s[4];
+    const int w = blockIdx.y;
+    float top = 0.f;
+    for (int64_t r = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); r < a.rows[w]; r += int64_t(gridDim.x) * 4) {
+        const float* p = static_cast<const float*>(a.src[w]) + r * a.ld[w];
+        for (int c = threadIdx.x & 63; c < a.d; c += 64) top = fmaxf(top, fabsf(p[c]));
+    }
+    top = wave_max_f32(top);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) a.tops[w * kTopBlocks + blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+}
+
+// exponent that puts `top` into [2^14, 2^15)
+__device__ __forceinline__ int ce_exponent(float top) {
+    if (!(top > 0.f) || !(top < INFINITY)) return 0;
+    return max(-100, min(100, 14 - ilogbf(top)));
+}
+
+__global__ __launch_bounds__(256) void ce_split_kernel(CePack a) {
+    __shared__ float s[2];
+    const int w = blockIdx.y, lane = threadIdx.x & 63;
+    if (threadIdx.x < 128) {      // a wave per operand
+        float top = 0.f;
+        for (int i = lane; i < kTopBlocks; i += 64) top = fmaxf(top, a.tops[(threadIdx.x >> 6) * kTopBlocks + i]);
+        top = wave_max_f32(top);
+        if (lane == 0) s[threadIdx.x >> 6] = top;
+    }
+    __syncthreads();
+    const int eq = ce_exponent(s[0]), ee = ce_exponent(s[1]);
+    if (blockIdx.x == 0 && w == 0 && threadIdx.x == 0) {
+        a.sc->unscale_s = ldexpf(1.f, -eq - ee);
+        a.sc->unscale_q = ldexpf(1.f, -eq);
+        a.sc->unscale_e = ldexpf(1.f, -ee);
+    }
+    const float f = ldexpf(1.f, w ? ee : eq);
+    const int chunks = a.dp / 8;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < a.rows[w] * chunks; i += int64_t(gridDim.x) * 256) {
+        const int64_t r = i / chunks;
+        const int c = int(i % chunks) * 8;
+        const float* p = static_cast<const float*>(a.src[w]) + r * a.ld[w];
+        f16x8 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = c + j < a.d ? p[c + j] * f : 0.f;
+            hi[j] = f16_t(v);
+            lo[j] = f16_t(v - float(hi[j]));
+        }
+        *reinterpret_cast<f16x8*>(a.hi[w] + r * a.dp + c) = hi;
+        *reinterpret_cast<f16x8*>(a.lo[w] + r * a.dp + c) = lo;
+    }
+}
+
+__global__ void ce_scalars_kernel(CeScalars* sc) {
+    sc->unscale_s = sc->unscale_q = sc->unscale_e = 1.f;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- rows
+struct CeRows {
+    const void *q, *e;
+    int64_t ldq, lde;
+    const float* bias;
+    const int64_t* target;
+    int64_t n, v;
+    int d, dp, n_splits;
+    float scale;
+    const float *m, *l, *o;       // partials of pass 1 (o nullable)
+    CeScalars* sc;
+    const float* zt;              // targets' logits (unit of m)
+    float* loss_rows;
+    float4* state;                // per row {lse, its low part, 1 - p_t, -}: with a bias in natural units, without in powers of two
+    float* mean;                  // (n, d) sum_{v /= t} p'_v e_v, nullable
+    // backward
+    const float *counted, *grad;  // number of counted rows; upstream gradient (1, or n values when per_row), nullable = 1
+    int reduction, per_row;       // 0 none, 1 mean, 2 sum
+    void* dq;
+    int64_t lddq;
+    float4* rowp;
+    float off;
+};
+
+// Joins the splits of pass 1: one wave per row.  loss_r, lse_r, 1 - p_t and sum_{v /= t} p'_v e_v.
+template <bool BIAS>
+__global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (r >= a.n) return;
+    const float unit = BIAS ? kLog2e : fmaxf(a.scale * a.sc->unscale_s * kLog2e, 1.2e-38f);      // from the maxima's unit to powers of two (as in the pass)
+    float top = kLowest;
+    for (int s = lane; s < a.n_splits; s += 64) top = fmaxf(top, a.m[int64_t(s) * a.n + r]);
+    top = wave_max_f32(top);
+    float sum = 0.f;
+    for (int s = lane; s < a.n_splits; s += 64) {
+        const float m = a.m[int64_t(s) * a.n + r], l = a.l[int64_t(s) * a.n + r];
+        sum += m == kLowest ? l : l * __builtin_amdgcn_exp2f((m - top) * unit);      // (a split without classes has l = 0, or NaN from NaN rows)
+    }
+    sum = lanes_sum<64>(sum);
+    if (a.mean) {
+        const float f = sum == 0.f ? 0.f : a.sc->unscale_e / sum;
+        for (int c = lane; c < a.d; c += 64) {
+            float v = 0.f;
+            for (int s = 0; s < a.n_splits; ++s) {
+                const float m = a.m[int64_t(s) * a.n + r];
+                const float x = a.o[(int64_t(s) * a.n + r) * a.dp + c];
+                v += m == kLowest ? x : x * __builtin_amdgcn_exp2f((m - top) * unit);
+            }
+            a.mean[r * a.d + c] = v * f;
+        }
+    }
+    if (lane) return;
+    // in powers of two, 64 bits: the other classes' lse (all of them where no target counts) and the target's logit
+    const int64_t t = a.target[r];
+    const double rest = sum == 0.f ? -double(INFINITY) : double(top) * double(unit) + log2(double(sum)) - double(a.off);
+    double lse = rest, miss = 0.0, loss = 0.0;
+    if (t >= 0 && t < a.v) {
+        const double z = double(a.zt[r]) * double(unit), x = rest - z;
+        const bool none = sum == 0.f && z == -double(INFINITY);      // every class masked
+        loss = none ? double(INFINITY) : x > 64.0 ? x * kLn2d : log1p(exp2(x));
+        miss = none ? 1.0 : 1.0 / (1.0 + exp2(-x));
+        if (!none && z != -double(INFINITY)) lse = z + loss / kLn2d;
+    } else if (t != -1) {
+        loss = NAN;      // no such class: nothing to learn from, and seen in the loss
+    }
+    if (BIAS) lse *= kLn2d;
+    const float hi = float(lse);
+    a.loss_rows[r] = float(loss);
+    a.state[r] = {hi, hi == kLowest ? 0.f : float(lse - double(hi)), float(miss), 0.f};
+}
+
+// Sum or mean of the rows' losses, and how many rows count; with no row counted the mean is 0.  One workgroup, 64-bit sums in a fixed order.
+__global__ __launch_bounds__(1024) void ce_stats_kernel(const float* loss_rows, const int64_t* target, int64_t n, int reduction, float* loss, float* counted) {
+    __shared__ double s_sum[16];
+    __shared__ int s_cnt[16];
+    double sum = 0.0;
+    int cnt = 0;      // n < 2^31
+    for (int64_t r = threadIdx.x; r < n; r += 1024) {
+        sum += double(loss_rows[r]);
+        cnt += target[r] != -1;
+    }
+    sum = wave_sum_f64(sum);
+    cnt = wave_sum_i32(cnt);
+    if ((threadIdx.x & 63) == 0) {
+        s_sum[threadIdx.x >> 6] = sum;
+        s_cnt[threadIdx.x >> 6] = cnt;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; ++i) sum += s_sum[i], cnt += s_cnt[i];
+        if (loss) *loss = float(reduction == 1 ? sum / double(max(cnt, 1)) : sum);
+        *counted = float(cnt);
+    }
+}
+
+__global__ __launch_bounds__(1024) void ce_grad_top_kernel(const float* grad, int64_t n, CeScalars* sc) {
+    __shared__ float s[16];
+    float top = 0.f;
+    for (int64_t r = threadIdx.x; r < n; r += 1024) top = fmaxf(top, fabsf(grad[r]));
+    top = wave_max_f32(top);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        sc->g_top = top;
+    }
+}
+
+// dx, and what pass 2 needs of every query (CePass::rowp).  One wave per row.
+template <typename E, bool BIAS>
+__global__ __launch_bounds__(256) void ce_dq_kernel(CeRows a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    // the gradient of a counted row, or with one per row what they are relative to
+    const float g = a.per_row ? a.sc->g_top : (a.grad ? a.grad[0] : 1.f) / (a.reduction == 1 ? fmaxf(a.counted[0], 1.f) : 1.f);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        const float unoff = __builtin_amdgcn_exp2f(-a.off);
+        a.sc->fac_e = a.scale * g * unoff * a.sc->unscale_q;
+        a.sc->fac_b = g * unoff;
+    }
+    if (r >= a.n) return;
+    const int64_t t = a.target[r];
+    const bool on = t >= 0 && t < a.v;
+    const float4 st = a.state[r];
+    const float gr = a.per_row ? a.grad[r] : g;
+    if (a.rowp && lane == 0) {
+        const float rel = !on ? 0.f : a.per_row ? (g > 0.f ? gr / g : gr) : 1.f;
+        const bool some = on && st.x != kLowest;
+        a.rowp[r] = {some ? (BIAS ? st.x : st.x - a.off) : INFINITY, rel * __builtin_amdgcn_exp2f(BIAS ? -st.y * kLog2e : -st.y),
+                     -rel * st.z * __builtin_amdgcn_exp2f(a.off), __int_as_float(on ? int(t) : -1)};
+    }
+    if (a.dq) {
+        E* dq = static_cast<E*>(a.dq) + r * a.lddq;
+        const E* e = static_cast<const E*>(a.e) + (on ? t : 0) * a.lde;
+        const float f = a.scale * gr * st.z;
+        for (int c = lane; c < a.d; c += 64) dq[c] = E(on ? f * (a.mean[r * a.d + c] - float(e[c])) : 0.f);
+    }
+}
+
+// Joins the splits of pass 2
+template <typename E>
+__global__ __launch_bounds__(256) void ce_de_kernel(const float* __restrict__ o, const float* __restrict__ l, int n_splits, int64_t v, int d, int dp,
+                                                   const CeScalars* sc, E* __restrict__ de, int64_t ldde, float* __restrict__ db) {
+    const int per = dp / 4;
+    const float fe = sc->fac_e, fb = sc->fac_b;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < v * per; i += int64_t(gridDim.x) * 256) {
+        const int64_t r = i / per;
+        const int c = int(i % per) * 4;
+        if (c < d) {
+            float4 s = *reinterpret_cast<const float4*>(o + r * dp + c);
+            for (int k = 1; k < n_splits; ++k) {
+                const float4 t = *reinterpret_cast<const float4*>(o + (int64_t(k) * v + r) * dp + c);
+                s.x += t.x, s.y += t.y, s.z += t.z, s.w += t.w;
+            }
+            E* out = de + r * ldde + c;
+            out[0] = E(s.x * fe);
+            if (c + 1 < d) out[1] = E(s.y * fe);
+            if (c + 2 < d) out[2] = E(s.z * fe);
+            if (c + 3 < d) out[3] = E(s.w * fe);
+        }
+        if (db && c == 0) {
+            float s = l[r];
+            for (int k = 1; k < n_splits; ++k) s += l[int64_t(k) * v + r];
+            db[r] = s * fb;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+static int ce_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+static bool ce_direct(const void* p, int64_t ld, int d, int dtype) {
+    return dtype != HWER_F32 && d == ce_padded(d) && aligned_to(p, ld * 2, 16);
+}
+
+// Splits of the streaming side: enough workgroups for every CU to hold its share (two, or one of the widest float32 rows), whole tiles each.
+struct CeSplit {
+    int blocks, splits, tiles_per_split;
+};
+static CeSplit ce_split(int64_t n_stat, int64_t n_strm, int d, int dtype) {
+    const int terms = dtype == HWER_F32 ? 2 : 1, dp = ce_padded(d), w = terms * dp;
+    const int ts = 32 * (w <= 64 ? 4 : w <= 256 ? 2 : 1), target = w > 256 ? 256 : 512;
+    const int64_t blocks = cdiv64(n_stat, 128), tiles = cdiv64(n_strm, ts);
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(tiles, target / std::max<int64_t>(blocks, 1)));
+    const int64_t per = std::max<int64_t>(1, cdiv64(tiles, want));
+    return {int(blocks), int(std::max<int64_t>(1, cdiv64(tiles, per))), int(per)};
+}
+
+static size_t up(size_t b) { return (b + 255) & ~size_t(255); }
+
+// Where a call's workspace keeps what.  The head (scalars, laid-out operands) stays for the backward call of the same operands; the rest is each call's own.
+struct CeLayout {
+    size_t tops, q_hi, q_lo, e_hi, e_lo, head, zt, m, l, o, fwd_end, rowp, l2, o2, bwd_end;
+};
+static CeLayout ce_layout(int64_t n, int64_t v, int d, int dtype, bool q_direct, bool e_direct, bool want_mean) {
+    const size_t dp = ce_padded(d);
+    CeLayout y{};
+    size_t at = 256;      // CeScalars
+    y.tops = at, at += dtype == HWER_F32 ? 2 * kTopBlocks * 4 : 0;
+    y.q_hi = at, at += q_direct ? 0 : up(size_t(n) * dp * 2);
+    y.q_lo = at, at += dtype == HWER_F32 ? up(size_t(n) * dp * 2) : 0;
+    y.e_hi = at, at += e_direct ? 0 : up(size_t(v) * dp * 2);
+    y.e_lo = at, at += dtype == HWER_F32 ? up(size_t(v) * dp * 2) : 0;
+    y.head = at;
+    const CeSplit f = ce_split(n, v, d, dtype), b = ce_split(v, n, d, dtype);
+    y.zt = at, at += up(size_t(n) * 4);
+    y.m = at, at += up(size_t(f.splits) * n * 4);
+    y.l = at, at += up(size_t(f.splits) * n * 4);
+    y.o = at, at += want_mean ? up(size_t(f.splits) * n * dp * 4) : 0;
+    y.fwd_end = at;
+    at = y.head;
+    y.rowp = at, at += up(size_t(n) * 16);
+    y.l2 = at, at += b.splits > 1 ? up(size_t(b.splits) * v * 4) : 0;
+    y.o2 = at, at += b.splits > 1 ? up(size_t(b.splits) * v * dp * 4) : 0;
+    y.bwd_end = at;
+    return y;
+}
+
+struct CeCall {
+    const void *q, *e;
+    int64_t ldq, lde, n, v;
+    int d, dtype;
+    const float* bias;
+    float scale;
+    unsigned char* ws;
+    CeLayout y;
+    bool q_direct, e_direct;
+    hipStream_t st;
+    CeScalars* sc() const { return reinterpret_cast<CeScalars*>(ws); }
+    const short* q_hi() const { return q_direct ? static_cast<const short*>(q) : reinterpret_cast<const short*>(ws + y.q_hi); }
+    const short* e_hi() const { return e_direct ? static_cast<const short*>(e) : reinterpret_cast<const short*>(ws + y.e_hi); }
+    const short* q_lo() const { return dtype == HWER_F32 ? reinterpret_cast<const short*>(ws + y.q_lo) : nullptr; }
+    const short* e_lo() const { return dtype == HWER_F32 ? reinterpret_cast<const short*>(ws + y.e_lo) : nullptr; }
+    int64_t q_ld() const { return q_direct ? ldq : ce_padded(d); }
+    int64_t e_ld() const { return e_direct ? lde : ce_padded(d); }
+};
+
+static int ce_prepare(const CeCall& c) {
+    const int dp = ce_padded(c.d);
+    CePack p{{c.q, c.e}, {nullptr, nullptr}, {nullptr, nullptr}, {c.n, c.v}, {c.ldq, c.lde}, c.d, dp, reinterpret_cast<float*>(c.ws + c.y.tops), c.sc()};
+    if (!c.q_direct) p.hi[0] = reinterpret_cast<short*>(c.ws + c.y.q_hi);
+    if (!c.e_direct) p.hi[1] = reinterpret_cast<short*>(c.ws + c.y.e_hi);
+    const unsigned blocks = unsigned(std::min<int64_t>(cdiv64(std::max(c.n, c.v) * (dp / 8), 256), kMaxStreamBlocks));
+    if (c.dtype == HWER_F32) {
+        p.lo[0] = reinterpret_cast<short*>(c.ws + c.y.q_lo);
+        p.lo[1] = reinterpret_cast<short*>(c.ws + c.y.e_lo);
+        ce_top_kernel<<<dim3(kTopBlocks, 2), dim3(256), 0, c.st>>>(p);
+        ce_split_kernel<<<dim3(blocks, 2), dim3(256), 0, c.st>>>(p);
+        return check_launch("catalogue_ce(split)");
+    }
+    ce_scalars_kernel<<<dim3(1), dim3(1), 0, c.st>>>(c.sc());
+    if (p.hi[0] || p.hi[1]) ce_pack16_kernel<<<dim3(blocks, 2), dim3(256), 0, c.st>>>(p);
+    return check_launch("catalogue_ce(pack)");
+}
+
+template <typename E, int TERMS, int DP, int MODE>
+static void ce_pass_launch(const CePass& a, bool rowg, hipStream_t st) {
+    const dim3 grid(unsigned((int64_t(a.stat_blocks) * a.n_splits + 7) / 8 * 8)), block(256);
+    if constexpr (MODE == kTable) {
+        if (a.bias) rowg ? ce_pass_kernel<E, TERMS, DP, MODE, true, true><<<grid, block, 0, st>>>(a) : ce_pass_kernel<E, TERMS, DP, MODE, true, false><<<grid, block, 0, st>>>(a);
+        else rowg ? ce_pass_kernel<E, TERMS, DP, MODE, false, true><<<grid, block, 0, st>>>(a) : ce_pass_kernel<E, TERMS, DP, MODE, false, false><<<grid, block, 0, st>>>(a);
+    } else {
+        if (a.bias) ce_pass_kernel<E, TERMS, DP, MODE, true, false><<<grid, block, 0, st>>>(a);
+        else ce_pass_kernel<E, TERMS, DP, MODE, false, false><<<grid, block, 0, st>>>(a);
+    }
+}
+template <typename E, int TERMS, int MODE>
+static void ce_pass_width(const CePass& a, int dp, bool rowg, hipStream_t st) {
+    if (dp == 64) ce_pass_launch<E, TERMS, 64, MODE>(a, rowg, st);
+    else if (dp == 128) ce_pass_launch<E, TERMS, 128, MODE>(a, rowg, st);
+    else ce_pass_launch<E, TERMS, 256, MODE>(a, rowg, st);
+}
+template <int MODE>
+static void ce_pass_any(const CePass& a, int dp, int dtype, bool rowg, hipStream_t st) {
+    if (dtype == HWER_F32) ce_pass_width<f16_t, 2, MODE>(a, dp, rowg, st);
+    else if (dtype == HWER_F16) ce_pass_width<f16_t, 1, MODE>(a, dp, rowg, st);
+    else ce_pass_width<bf16_t, 1, MODE>(a, dp, rowg, st);
+}
+static float ce_offset(int dtype, int pass) { return dtype == HWER_BF16 ? CeType<bf16_t>::offset[pass] : CeType<f16_t>::offset[pass]; }
+
+static void ce_rows_launch(const CeRows& r, hipStream_t st) {
+    const dim3 grid(unsigned(cdiv64(r.n, 4))), block(256);
+    r.bias ? ce_rows_kernel<true><<<grid, block, 0, st>>>(r) : ce_rows_kernel<false><<<grid, block, 0, st>>>(r);
+}
+template <typename E>
+static void ce_dq_launch(const CeRows& r, hipStream_t st) {
+    const dim3 grid(unsigned(std::max<int64_t>(1, cdiv64(r.n, 4)))), block(256);      // (without rows it leaves the factors of zeros)
+    r.bias ? ce_dq_kernel<E, true><<<grid, block, 0, st>>>(r) : ce_dq_kernel<E, false><<<grid, block, 0, st>>>(r);
+}
+
+static int ce_check(const char* what, const void* q, int64_t ldq, const void* e, int64_t lde, const int64_t* target, int64_t n, int64_t v, int d, int dtype, float scale) {
+    if (!known_dtype(dtype)) return fail(HWER_EINVAL, "%s: unknown element type %d", what, dtype);
+    if (d < 1 || d > hwer_catalogue_ce_max_dim()) return fail(HWER_EINVAL, "%s: d=%d unsupported (1..%d)", what, d, hwer_catalogue_ce_max_dim());
+    const int64_t most = (int64_t(1) << 31) - 256;
+    if (n < 0 || v < 1 || n > most || v > most) return fail(HWER_EINVAL, "%s: %lld rows, %lld classes", what, (long long)n, (long long)v);
+    if (!(scale > 0.f) || !(scale < INFINITY)) return fail(HWER_EINVAL, "%s: scale must be positive and finite", what);
+    if (n && (!q || !target)) return fail(HWER_EINVAL, "%s: null queries or targets", what);
+    if (!e || ldq < d || lde < d) return fail(HWER_EINVAL, "%s: null table or a row stride below d", what);
+    return HWER_OK;
+}
+
+}  // namespace hwer
+
+using namespace hwer;
+
+extern "C" {
+
+int hwer_catalogue_ce_max_dim(void) { return 256; }
+
+int hwer_catalogue_ce_reads_in_place(const void* rows, int64_t ld, int d, int dtype) { return ce_direct(rows, ld, d, dtype) ? 1 : 0; }
+
+size_t hwer_catalogue_ce_workspace_bytes(int64_t n, int64_t v, int d, int dtype, int q_in_place, int e_in_place, int want_gradients) {
+    if (!known_dtype(dtype) || d < 1 || d > hwer_catalogue_ce_max_dim() || n < 0 || v < 1) return 0;
+    const CeLayout y = ce_layout(n, v, d, dtype, q_in_place != 0, e_in_place != 0, want_gradients != 0);
+    return std::max<size_t>(256, want_gradients ? std::max(y.fwd_end, y.bwd_end) : y.fwd_end);
+}
+
+int hwer_catalogue_ce(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int d, int dtype,
+                      float scale, int reduction, float* loss_rows, float* state, float* loss, float* counted, float* mean, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = ce_check("catalogue_ce", q, ldq, e, lde, target, n, v, d, dtype, scale)) return rc;
+    if (reduction < 0 || reduction > 2) return fail(HWER_EINVAL, "catalogue_ce: unknown reduction %d", reduction);
+    if (!counted || (reduction && !loss) || (n && (!loss_rows || !state))) return fail(HWER_EINVAL, "catalogue_ce: null output");
+    const bool qd = ce_direct(q, ldq, d, dtype), ed = ce_direct(e, lde, d, dtype);
+    const size_t need = hwer_catalogue_ce_workspace_bytes(n, v, d, dtype, qd, ed, mean != nullptr);
+    if (!workspace || workspace_bytes < need) return fail(HWER_EWORKSPACE, "catalogue_ce: workspace of %zu bytes needed", need);
+    hipStream_t st = as_stream(stream);
+    CeCall c{q, e, ldq, lde, n, v, d, dtype, bias, scale, static_cast<unsigned char*>(workspace), ce_layout(n, v, d, dtype, qd, ed, mean != nullptr), qd, ed, st};
+    if (n) {
+        if (int rc = ce_prepare(c)) return rc;
+        const CeSplit s = ce_split(n, v, d, dtype);
+        const int dp = ce_padded(d);
+        CePass p{};
+        p.stat = c.q_hi(), p.stat_lo = c.q_lo(), p.strm = c.e_hi(), p.strm_lo = c.e_lo();
+        p.ld_stat = c.q_ld(), p.ld_strm = c.e_ld(), p.n_stat = n, p.n_strm = v;
+        p.bias = bias, p.scale = scale, p.sc = c.sc();
+        p.tiles_per_split = s.tiles_per_split, p.n_splits = s.splits, p.stat_blocks = s.blocks;
+        p.m = reinterpret_cast<float*>(c.ws + c.y.m), p.l = reinterpret_cast<float*>(c.ws + c.y.l), p.o = reinterpret_cast<float*>(c.ws + c.y.o);
+        p.target = target, p.zt = reinterpret_cast<float*>(c.ws + c.y.zt), p.d = d;
+        mean ? ce_pass_any<kMean>(p, dp, dtype, false, st) : ce_pass_any<kLse>(p, dp, dtype, false, st);
+        if (int rc = check_launch("catalogue_ce(pass)")) return rc;
+        CeRows r{};
+        r.q = q, r.e = e, r.ldq = ldq, r.lde = lde, r.bias = bias, r.target = target, r.n = n, r.v = v, r.d = d, r.dp = dp, r.n_splits = s.splits, r.scale = scale;
+        r.m = p.m, r.l = p.l, r.o = p.o, r.sc = c.sc(), r.zt = p.zt, r.loss_rows = loss_rows, r.state = reinterpret_cast<float4*>(state), r.mean = mean, r.off = ce_offset(dtype, 0);
+        ce_rows_launch(r, st);
+    }
+    ce_stats_kernel<<<dim3(1), dim3(1024), 0, st>>>(loss_rows, target, n, reduction, loss, counted);
+    return check_launch("catalogue_ce");
+}
+
+int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int d,
+                               int dtype, float scale, int reduction, const float* grad, const float* state, const float* counted, const float* mean, void* dq, int64_t lddq,
+                               void* de, int64_t ldde, float* dbias, int operands_ready, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = ce_check("catalogue_ce_backward", q, ldq, e, lde, target, n, v, d, dtype, scale)) return rc;
+    if (reduction < 0 || reduction > 2 || (reduction == 0 && !grad)) return fail(HWER_EINVAL, "catalogue_ce_backward: unknown reduction %d, or rows' losses without their gradients", reduction);
+    if (!counted || (n && (!state || (dq && !mean)))) return fail(HWER_EINVAL, "catalogue_ce_backward: what the forward call left is missing");
+    if ((dq && lddq < d) || (de && ldde < d)) return fail(HWER_EINVAL, "catalogue_ce_backward: a row stride is below d");
+    if (dbias && (!bias || !de)) return fail(HWER_EINVAL, "catalogue_ce_backward: dbias needs the bias, and comes with the table's gradient");
+    const bool qd = ce_direct(q, ldq, d, dtype), ed = ce_direct(e, lde, d, dtype);
+    const size_t need = hwer_catalogue_ce_workspace_bytes(n, v, d, dtype, qd, ed, 1);
+    if (!workspace || workspace_bytes < need) return fail(HWER_EWORKSPACE, "catalogue_ce_backward: workspace of %zu bytes needed", need);
+    hipStream_t st = as_stream(stream);
+    CeCall c{q, e, ldq, lde, n, v, d, dtype, bias, scale, static_cast<unsigned char*>(workspace), ce_layout(n, v, d, dtype, qd, ed, true), qd, ed, st};
+    if (!operands_ready || n == 0)
+        if (int rc = ce_prepare(c)) return rc;
+    const int dp = ce_padded(d);
+    CeRows r{};
+    r.q = q, r.e = e, r.ldq = ldq, r.lde = lde, r.bias = bias, r.target = target, r.n = n, r.v = v, r.d = d, r.dp = dp, r.scale = scale, r.sc = c.sc();
+    r.state = reinterpret_cast<float4*>(const_cast<float*>(state)), r.mean = const_cast<float*>(mean), r.counted = counted, r.grad = grad, r.reduction = reduction, r.per_row = reduction == 0;
+    r.dq = dq, r.lddq = lddq, r.off = ce_offset(dtype, 1);
+    r.rowp = de ? reinterpret_cast<float4*>(c.ws + c.y.rowp) : nullptr;
+    if (reduction == 0 && n) ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, st>>>(grad, n, c.sc());
+    if (dtype == HWER_F32) ce_dq_launch<float>(r, st);
+    else if (dtype == HWER_F16) ce_dq_launch<f16_t>(r, st);
+    else ce_dq_launch<bf16_t>(r, st);
+    if (int rc = check_launch("catalogue_ce_backward(rows)")) return rc;
+    if (!de) return HWER_OK;
+    const CeSplit s = ce_split(v, n, d, dtype);
+    CePass p{};
+    p.stat = c.e_hi(), p.stat_lo = c.e_lo(), p.strm = c.q_hi(), p.strm_lo = c.q_lo();
+    p.ld_stat = c.e_ld(), p.ld_strm = c.q_ld(), p.n_stat = v, p.n_strm = n;
+    p.bias = bias, p.scale = scale, p.sc = c.sc();
+    p.tiles_per_split = s.tiles_per_split, p.n_splits = s.splits, p.stat_blocks = s.blocks;
+    p.l = reinterpret_cast<float*>(c.ws + c.y.l2), p.o = reinterpret_cast<float*>(c.ws + c.y.o2);
+    p.rowp = r.rowp, p.out = de, p.out_b = dbias, p.ld_out = ldde, p.d = d;
+    p.out_vec = d % 4 == 0 && aligned_to(de, ldde * dtype_bytes(dtype), 4 * dtype_bytes(dtype));
+    ce_pass_any<kTable>(p, dp, dtype, reduction == 0, st);
+    if (int rc = check_launch("catalogue_ce_backward(pass)")) return rc;
+    if (s.splits > 1) {
+        const dim3 grid(unsigned(std::min<int64_t>(cdiv64(v * (dp / 4), 256), 4 * kMaxStreamBlocks)));
+        if (dtype == HWER_F32) ce_de_kernel<float><<<grid, dim3(256), 0, st>>>(p.o, p.l, s.splits, v, d, dp, c.sc(), static_cast<float*>(de), ldde, dbias);
+        else if (dtype == HWER_F16) ce_de_kernel<f16_t><<<grid, dim3(256), 0, st>>>(p.o, p.l, s.splits, v, d, dp, c.sc(), static_cast<f16_t*>(de), ldde, dbias);
+        else ce_de_kernel<bf16_t><<<grid, dim3(256), 0, st>>>(p.o, p.l, s.splits, v, d, dp, c.sc(), static_cast<bf16_t*>(de), ldde, dbias);
+    }
+    return check_launch("catalogue_ce_backward");
+}
+
+}  // extern "C"

@@ -1,0 +1,240 @@
+// Product of 8-bit rows:  out[m][n] = (sum_k A[m][k] B[n][k]) sa[m] sb[n] (+ bias[n]),  int8 codes with one float32 scale for each row of either side
+// (a token's on the left, a channel's or catalogue row's on the right).  Sums are exact 32-bit integers (K <= 131 071: K * 128 * 128 < 2^31), so
+// they depend on no order and no split; one rounding per product with a scale and one to the output's type follow.
+//
+//   matmul_q8_tile   both sides long: tiles of C on the 8-bit matrix instructions, operands staged in LDS by DMA
+//   matmul_q8_few    one side short (<= 64 rows): the long side streams from memory once, K split over the waves of a workgroup
+#include <algorithm>
+
+#include "head_common.h"
+#include "knn_internal.h"   // lds_dma16_v, lds_addr
+
+namespace hwer {
+
+typedef int i4_t __attribute__((ext_vector_type(4)));
+typedef int i16_t __attribute__((ext_vector_type(16)));
+
+struct QmmArgs {
+    const int8_t *a, *b;      // rows of the output / columns of the output
+    const float *sa, *sb, *bias;
+    void* out;
+    int64_t m, n, lda, ldb, ldo;
+    int k;
+};
+
+// what a DMA lane reads where a row or a K chunk does not exist
+__device__ const uint32_t kZero16[4] = {0u, 0u, 0u, 0u};
+
+// 16 bytes of a row at byte k, zeros past the row's end.  ALIGNED: K, the row strides and the pointers are multiples of 16.
+template <bool ALIGNED>
+__device__ __forceinline__ i4_t load16(const int8_t* row, int k, int K) {
+    i4_t v = {0, 0, 0, 0};
+    if constexpr (ALIGNED) {
+        if (k < K) v = *reinterpret_cast<const i4_t*>(row + k);
+    } else if (k + 16 <= K) {
+        __builtin_memcpy(&v, row + k, 16);      // any alignment: global loads need none
+    } else if (k < K) {
+        int8_t t[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t[i] = k + i < K ? row[k + i] : int8_t(0);
+        __builtin_memcpy(&v, t, 16);
+    }
+    return v;
+}
+
+template <typename O>
+__device__ __forceinline__ O finish(int acc, float sa, float sb, float bias) {
+    return O(float(acc) * sa * sb + bias);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- both sides long
+constexpr int kTM = 128, kTN = 128, kTK = 128;   // tile of C, bytes of K per step
+
+// LDS image of a 128-row operand tile: 128 bytes (8 chunks of 16) a row, chunk c of row r at c ^ (r & 7): the 8 lanes that a ds_read_b128 serves
+// together read 8 rows' same chunk from 8 different 16-byte slots of the banks
+template <bool ALIGNED>
+__device__ __forceinline__ void stage(const int8_t* base, int64_t ld, int64_t row0, int64_t rows, int k0, int K, int8_t* lds, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {               // a wave stages 32 of the 128 rows, 8 rows (1 KB) at a time
+        const int r = wave * 32 + i * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
+        const bool in = row0 + r < rows;
+        const int8_t* row = base + (in ? row0 + r : 0) * ld;
+        if constexpr (ALIGNED) {
+            const void* p = in && k0 + 16 * c < K ? static_cast<const void*>(row + k0 + 16 * c) : static_cast<const void*>(kZero16);
+            lds_dma16_v(p, __builtin_amdgcn_readfirstlane(lds_addr(lds + (wave * 32 + i * 8) * kTK)));
+        } else {
+            const i4_t v = in ? load16<false>(row, k0 + 16 * c, K) : i4_t{0, 0, 0, 0};
+            *reinterpret_cast<i4_t*>(lds + (wave * 32 + i * 8) * kTK + lane * 16) = v;
+        }
+    }
+}
+
+template <typename O, bool ALIGNED>
+__global__ __launch_bounds__(256, 2) void matmul_q8_tile_kernel(QmmArgs g, int tiles_m, int tiles_n) {
+    __shared__ __align__(16) int8_t s_a[2][kTM * kTK];
+    __shared__ __align__(16) int8_t s_b[2][kTN * kTK];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l31 = lane & 31;
+    // tiles of one XCD (workgroup id mod 8) are neighbours: 8 rows of tiles, walked along the columns
+    const int total = tiles_m * tiles_n, per = (total + 7) / 8;
+    const int id = int(blockIdx.x & 7) * per + int(blockIdx.x >> 3);
+    if (int(blockIdx.x >> 3) >= per || id >= total) return;
+    const int band = id / (8 * tiles_n), in_band = id % (8 * tiles_n), bh = min(8, tiles_m - 8 * band);
+    const int tm = band * 8 + in_band % bh, tn = in_band / bh;
+    const int64_t m0 = int64_t(tm) * kTM, n0 = int64_t(tn) * kTN;
+    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+    i16_t acc[2][2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[x][y][i] = 0;
+    const int steps = (g.k + kTK - 1) / kTK;
+    if (steps) {
+        stage<ALIGNED>(g.a, g.lda, m0, g.m, 0, g.k, s_a[0], wave, lane);
+        stage<ALIGNED>(g.b, g.ldb, n0, g.n, 0, g.k, s_b[0], wave, lane);
+    }
+    for (int s = 0; s < steps; ++s) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();      // step s is staged, and everyone is done with the other buffers
+        if (s + 1 < steps) {
+            stage<ALIGNED>(g.a, g.lda, m0, g.m, (s + 1) * kTK, g.k, s_a[(s + 1) & 1], wave, lane);
+            stage<ALIGNED>(g.b, g.ldb, n0, g.n, (s + 1) * kTK, g.k, s_b[(s + 1) & 1], wave, lane);
+        }
+        const int8_t *pa = s_a[s & 1], *pb = s_b[s & 1];
+#pragma unroll
+        for (int kc = 0; kc < kTK / 32; ++kc) {
+            i4_t fa[2], fb[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int ra = wm + 32 * x + l31, rb = wn + 32 * x + l31, c = 2 * kc + half;
+                fa[x] = *reinterpret_cast<const i4_t*>(pa + ra * kTK + 16 * (c ^ (ra & 7)));
+                fb[x] = *reinterpret_cast<const i4_t*>(pb + rb * kTK + 16 * (c ^ (rb & 7)));
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[y], fa[x], acc[x][y], 0, 0, 0);
+        }
+    }
+    // C fragment: column (lane & 31) = row m of the output, register rows = 4 consecutive n at a time
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int64_t m = m0 + wm + 32 * x + l31;
+        if (m >= g.m) continue;
+        const float sa = g.sa[m];
+        O* out = static_cast<O*>(g.out) + m * g.ldo;
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t n = n0 + wn + 32 * y + 8 * q + 4 * half;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (n + j < g.n) out[n + j] = finish<O>(acc[x][y][4 * q + j], sa, g.sb[n + j], g.bias ? g.bias[n + j] : 0.f);
+            }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- one side short
+// `few` (at most 16 FT rows) against `many`: a workgroup takes 16 rows of `many`, its 4 waves a quarter of K each.  16x16x64 matrix instruction: the
+// register rows are rows of `many`, the columns rows of `few`.  A lane reads 32 consecutive bytes of a row per step, 4 lanes a whole 128-byte line.
+struct QmmFewArgs {
+    const int8_t *few, *many;
+    const float *s_few, *s_many, *bias;
+    void* out;
+    int64_t n_many, ld_few, ld_many, o_few, o_many;     // output strides along either side
+    int n_few, k, bias_many;                              // bias_many: the bias belongs to `many`'s rows
+};
+
+template <typename O, int FT, bool ALIGNED>
+__global__ __launch_bounds__(256) void matmul_q8_few_kernel(QmmFewArgs g) {
+    __shared__ int s_part[3][FT * 4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, quad = lane >> 4;
+    const int64_t r0 = int64_t(blockIdx.x) * 16;
+    const int64_t mr = std::min<int64_t>(r0 + l15, g.n_many - 1);       // rows past the end are read as the last one and not written
+    const int8_t* many = g.many + mr * g.ld_many;
+    const int8_t* few[FT];
+#pragma unroll
+    for (int f = 0; f < FT; ++f) few[f] = g.few + int64_t(std::min(16 * f + l15, g.n_few - 1)) * g.ld_few;
+    i4_t acc[FT];
+#pragma unroll
+    for (int f = 0; f < FT; ++f) acc[f] = i4_t{0, 0, 0, 0};
+    const int steps = (g.k + 127) / 128, per = (steps + 3) / 4;
+    const int s1 = std::min(steps, (wave + 1) * per);
+#pragma unroll 4
+    for (int s = wave * per; s < s1; ++s) {
+        const int k = s * 128 + quad * 32;
+        const i4_t m0 = load16<ALIGNED>(many, k, g.k), m1 = load16<ALIGNED>(many, k + 16, g.k);
+#pragma unroll
+        for (int f = 0; f < FT; ++f) {
+            const i4_t f0 = load16<ALIGNED>(few[f], k, g.k), f1 = load16<ALIGNED>(few[f], k + 16, g.k);
+            acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(m0, f0, acc[f], 0, 0, 0);
+            acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(m1, f1, acc[f], 0, 0, 0);
+        }
+    }
+    if (wave > 0) {
+#pragma unroll
+        for (int f = 0; f < FT; ++f)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_part[wave - 1][4 * f + i][lane] = acc[f][i];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int f = 0; f < FT; ++f) {
+        const int row = 16 * f + l15;
+        if (row >= g.n_few) continue;
+        const float sf = g.s_few[row], bf = g.bias && !g.bias_many ? g.bias[row] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t r = r0 + 4 * quad + i;
+            if (r >= g.n_many) continue;
+            const int v = acc[f][i] + s_part[0][4 * f + i][lane] + s_part[1][4 * f + i][lane] + s_part[2][4 * f + i][lane];
+            const float bias = g.bias && g.bias_many ? g.bias[r] : bf, sm = g.s_many[r];
+            // the left side's scale first, whichever side is the short one
+            static_cast<O*>(g.out)[row * g.o_few + r * g.o_many] = g.bias_many ? finish<O>(v, sf, sm, bias) : finish<O>(v, sm, sf, bias);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+constexpr int kFewRows = 64;
+
+template <typename O, bool ALIGNED>
+static void matmul_q8_launch(const QmmArgs& g, hipStream_t st) {
+    if (std::min(g.m, g.n) <= kFewRows) {
+        const bool left = g.m <= g.n;      // which side is short
+        QmmFewArgs f{left ? g.a : g.b, left ? g.b : g.a, left ? g.sa : g.sb, left ? g.sb : g.sa, g.bias, g.out, left ? g.n : g.m, left ? g.lda : g.ldb,
+                     left ? g.ldb : g.lda, left ? g.ldo : 1, left ? 1 : g.ldo, int(left ? g.m : g.n), g.k, left ? 1 : 0};
+        const dim3 grid(unsigned(cdiv64(f.n_many, 16)));
+        if (f.n_few <= 16) matmul_q8_few_kernel<O, 1, ALIGNED><<<grid, dim3(256), 0, st>>>(f);
+        else if (f.n_few <= 32) matmul_q8_few_kernel<O, 2, ALIGNED><<<grid, dim3(256), 0, st>>>(f);
+        else matmul_q8_few_kernel<O, 4, ALIGNED><<<grid, dim3(256), 0, st>>>(f);
+        return;
+    }
+    const int tm = int(cdiv64(g.m, kTM)), tn = int(cdiv64(g.n, kTN));
+    matmul_q8_tile_kernel<O, ALIGNED><<<dim3(unsigned((int64_t(tm) * tn + 7) / 8 * 8)), dim3(256), 0, st>>>(g, tm, tn);
+}
+
+}  // namespace hwer
+
+using namespace hwer;
+
+extern "C" int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* b, int64_t ldb, const float* b_scale, const float* bias,
+                              int64_t m, int64_t n, int k, void* out, int64_t ldo, int out_dtype, void* stream) {
+    if (!known_dtype(out_dtype)) return fail(HWER_EINVAL, "matmul_q8: unknown output type %d", out_dtype);
+    if (m < 0 || n < 0 || k < 0 || k > 131071) return fail(HWER_EINVAL, "matmul_q8: m=%lld, n=%lld, k=%d (k <= 131071: sums stay in 32 bits)", (long long)m, (long long)n, k);
+    if (m == 0 || n == 0) return HWER_OK;
+    if (m > (int64_t(1) << 31) - 256 || n > (int64_t(1) << 31) - 256 || cdiv64(m, kTM) * cdiv64(n, kTN) > (int64_t(1) << 30))
+        return fail(HWER_EINVAL, "matmul_q8: m=%lld, n=%lld: too many tiles for one call", (long long)m, (long long)n);
+    if ((k && (!a || !b)) || !a_scale || !b_scale || !out) return fail(HWER_EINVAL, "matmul_q8: null operand");
+    if (lda < k || ldb < k || ldo < n) return fail(HWER_EINVAL, "matmul_q8: a row stride is below the row's length");
+    const QmmArgs g{a, b, a_scale, b_scale, bias, out, m, n, lda, ldb, ldo, k};
+    hipStream_t st = as_stream(stream);
+    const bool al = k % 16 == 0 && aligned_to(a, lda, 16) && aligned_to(b, ldb, 16);
+    if (out_dtype == HWER_F32) al ? matmul_q8_launch<float, true>(g, st) : matmul_q8_launch<float, false>(g, st);
+    else if (out_dtype == HWER_F16) al ? matmul_q8_launch<f16_t, true>(g, st) : matmul_q8_launch<f16_t, false>(g, st);
+    else al ? matmul_q8_launch<bf16_t, true>(g, st) : matmul_q8_launch<bf16_t, false>(g, st);
+    return check_launch("matmul_q8");
+}

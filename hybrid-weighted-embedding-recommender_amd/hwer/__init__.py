@@ -9,6 +9,16 @@ from .content_recommender import ContentRecommendation, ContentRecommender  # no
 from .embed import BaseEmbed, IdentityEmbedding  # noqa: F401
 from .utils import NodeNotFoundException  # noqa: F401
 
+_HEAD = ("rms_norm", "rms_norm_grads", "rms_norm_q8", "quantize_rows_q8", "matmul_q8", "catalogue_cross_entropy", "catalogue_cross_entropy_grads")
+
+
+def __getattr__(name):      # the learned head's operators (hwer/head.py) import torch: on first use, as everywhere in this package
+    if name in _HEAD:
+        from . import head
+        globals().update((n, getattr(head, n)) for n in _HEAD)
+        return globals()[name]
+    raise AttributeError("module %r has no attribute %r" % (__name__, name))
+
 
 class VectorIndex(RecommendationBase):
     """RecommendationBase over vectors that were trained elsewhere: fit(nodes, vectors)."""

@@ -1,0 +1,298 @@
+"""The learned head in front of the search: operators that train the rows `DeviceIndex` serves, and serve them in 8 bits.
+
+  rms_norm / rms_norm_grads          a tower's last norm, with the residual's addition, and its gradients
+  catalogue_cross_entropy(_grads)    softmax cross entropy of query rows over ALL item rows, with gradients, logits never stored
+  rms_norm_q8 / quantize_rows_q8     rows as int8 codes with one scale each (queries on their way out of the tower; the catalogue)
+  matmul_q8                          scores (or a layer) from two sets of 8-bit rows
+
+Everything takes and returns device tensors on their own device, runs on its current stream, never synchronises and may be captured into a
+hipGraph.  `rms_norm` and `catalogue_cross_entropy` take part in autograd where an input requires a gradient; the `_grads` functions return
+the gradients directly and keep nothing (what a resident training step calls).  The reference trains in DGL / PyTorch (hwer/gcn_ncf.py:126-327:
+out of scope here); what it hands to the search are rows (hwer/gcn_ncf.py:431,447-456).
+
+Errors: wrong shapes, types or devices raise before anything is launched (ValueError / TypeError; HwerNativeError from the library).  Values are
+never checked on the host (that would wait for the GPU): a target that names no class makes its loss NaN."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import native
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+P = native.ptr
+
+
+def _check_rows(name, t, dtypes=_DTYPES, dim=2):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s: a device tensor is needed, got %s" % (name, type(t).__name__))
+    if t.dtype not in dtypes:
+        raise TypeError("%s: unsupported type %s" % (name, t.dtype))
+    if dim is not None and t.dim() != dim:
+        raise ValueError("%s: %d dimensions needed, got shape %s" % (name, dim, tuple(t.shape)))
+
+
+def _check_device(t, *others):
+    if t.device.type != "cuda":
+        raise native.HwerNativeError("hwer (MI355X build) needs device tensors: got one on %s; there is no CPU fallback for this path" % t.device)
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise ValueError("operands on two devices: %s and %s" % (t.device, o.device))
+
+
+def _rows(t):
+    """(tensor, row stride) of 2-d rows whose elements are contiguous; anything else (a transposed view, a broadcast row) is copied."""
+    n, d = t.shape
+    if (t.stride(1) == 1 or d == 1) and (t.stride(0) >= d or n <= 1):
+        return t, max(t.stride(0), d)
+    t = t.contiguous()
+    return t, max(t.stride(0), d)
+
+
+def _flat(t):
+    """... of rows along the last dimension of any number of leading ones"""
+    return _rows(t.reshape(-1, t.shape[-1]))
+
+
+def _weight(weight, x):
+    if weight is None:
+        return None, 0
+    if weight.dtype not in (torch.float32, x.dtype):
+        raise TypeError("weight: float32 or the rows' type (%s), got %s" % (x.dtype, weight.dtype))
+    if tuple(weight.shape) != (x.shape[-1],):
+        raise ValueError("weight: shape (%d,) needed, got %s" % (x.shape[-1], tuple(weight.shape)))
+    return weight.contiguous(), _DTYPES[weight.dtype]
+
+
+def _norm_checks(x, weight, residual, eps):
+    _check_rows("x", x, dim=None)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x: rows of at least one element needed, got shape %s" % (tuple(x.shape),))
+    _check_device(x, weight, residual)
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
+        raise ValueError("residual: shape and type of x needed (%s %s), got %s %s" % (tuple(x.shape), x.dtype, tuple(residual.shape), residual.dtype))
+    if not 0.0 <= float(eps) < float("inf"):
+        raise ValueError("eps must be finite and not negative")
+
+
+# ---------------------------------------------------------------------------------------------------------------- root-mean-square norm
+def _norm_forward(x, weight, residual, eps):
+    w, wt = _weight(weight, x)
+    xr, ldx = _flat(x)
+    rr, ldr = _flat(residual) if residual is not None else (None, 0)
+    n, d = xr.shape
+    with native.device_guard(x.device):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+        native.check(native.lib().hwer_rms_norm(P(xr), ldx, P(rr), ldr, P(w), wt, n, d, _DTYPES[x.dtype], eps, P(y), d, P(h), d, native.stream_ptr()), "rms_norm")
+    return y, h
+
+
+def rms_norm_grads(dy, h, weight=None, eps: float = 1e-6, dh=None):
+    """Gradients of `rms_norm`: -> (dx, dweight).  dx is the gradient of x and of the residual alike; dweight is None without a weight.
+    h: what the norm was taken of (the second result of `rms_norm` with a residual, x without one).  dh: the gradient that reaches h by other ways."""
+    _norm_checks(h, weight, dh, eps)
+    if dy.shape != h.shape or dy.dtype != h.dtype:
+        raise ValueError("dy: shape and type of h needed")
+    _check_device(h, dy)
+    w, wt = _weight(weight, h)
+    (hr, ldh), (gr, ldg) = _flat(h), _flat(dy)
+    ar, lda = _flat(dh) if dh is not None else (None, 0)
+    n, d = hr.shape
+    lib = native.lib()
+    with native.device_guard(h.device):
+        dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        dw = torch.empty_like(w) if w is not None else None
+        nbytes = lib.hwer_rms_norm_backward_workspace_bytes(n, d) if w is not None else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device) if nbytes else None
+        native.check(lib.hwer_rms_norm_backward(P(gr), ldg, P(hr), ldh, P(w), wt, P(ar), lda, n, d, _DTYPES[h.dtype], eps, P(dx), d, P(dw), P(ws), nbytes,
+                                                native.stream_ptr()), "rms_norm_backward")
+    return dx, dw
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, h = _norm_forward(x, weight, residual, eps)
+        ctx.save_for_backward(x if h is None else h, weight)
+        ctx.eps, ctx.two = eps, h is not None
+        ctx.set_materialize_grads(False)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight = ctx.saved_tensors
+        if dy is None:       # only h was used further
+            return dh, None if weight is None or not ctx.needs_input_grad[1] else torch.zeros_like(weight), dh if ctx.two else None, None
+        w = weight if ctx.needs_input_grad[1] else (None if weight is None else weight.detach())
+        dx, dw = rms_norm_grads(dy, h, w, ctx.eps, dh)
+        return (dx if ctx.needs_input_grad[0] else None, dw if ctx.needs_input_grad[1] else None, dx if ctx.two and ctx.needs_input_grad[2] else None, None)
+
+
+def rms_norm(x, weight=None, residual=None, eps: float = 1e-6):
+    """y = h * weight / sqrt(mean(h^2, last dimension) + eps) with h = x, or h = x + residual rounded to their type: -> y, or (y, h) with a residual.
+    x: float32 / float16 / bfloat16, any number of leading dimensions; weight: (d,) float32 or x's type, None = ones."""
+    _norm_checks(x, weight, residual, eps)
+    eps = float(eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+        return _RmsNorm.apply(x, weight, residual, eps)
+    y, h = _norm_forward(x, weight, residual, eps)
+    return y if h is None else (y, h)
+
+
+def _codes(x, weight, residual, eps, norm):
+    w, wt = _weight(weight, x)
+    xr, ldx = _flat(x)
+    rr, ldr = _flat(residual) if residual is not None else (None, 0)
+    n, d = xr.shape
+    with native.device_guard(x.device):
+        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+        native.check(native.lib().hwer_rms_norm_q8(P(xr), ldx, P(rr), ldr, P(w), wt, n, d, _DTYPES[x.dtype], norm, eps, P(q), d, P(scale), P(h), d,
+                                                   native.stream_ptr()), "rms_norm_q8")
+    return (q, scale) if h is None else (q, scale, h)
+
+
+def rms_norm_q8(x, weight=None, residual=None, eps: float = 1e-6):
+    """`rms_norm` whose y comes as int8 codes and one float32 scale for each row: -> (codes, scales) or (codes, scales, h).  y = codes * scale to half a
+    step, max|y| / 254.  No gradient (codes are for serving)."""
+    _norm_checks(x, weight, residual, eps)
+    return _codes(x, weight, residual, float(eps), 1)
+
+
+def quantize_rows_q8(x):
+    """Rows as int8 codes and one float32 scale each, x = codes * scale to half a step: -> (codes, scales).  What a catalogue is stored as for `matmul_q8`."""
+    _norm_checks(x, None, None, 0.0)
+    return _codes(x, None, None, 0.0, 0)
+
+
+# ---------------------------------------------------------------------------------------------------------------- 8-bit product
+def matmul_q8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
+    """out = (a @ b.T) * a_scale[:, None] * b_scale (+ bias): a (m, k) and b (n, k) int8 codes, a_scale (m,), b_scale (n,), bias (n,) float32;
+    out (m, n) float32 / float16 / bfloat16.  The integer sums are exact (k <= 131 071)."""
+    _check_rows("a", a, (torch.int8,))
+    _check_rows("b", b, (torch.int8,))
+    _check_device(a, b, a_scale, b_scale, bias)
+    if a.shape[1] != b.shape[1]:
+        raise ValueError("rows of %d against rows of %d codes" % (a.shape[1], b.shape[1]))
+    if out_dtype not in _DTYPES:
+        raise TypeError("out_dtype: float32, float16 or bfloat16, got %s" % out_dtype)
+    for name, t, n in (("a_scale", a_scale, a.shape[0]), ("b_scale", b_scale, b.shape[0]), ("bias", bias, b.shape[0])):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (n,)):
+            raise ValueError("%s: float32 of shape (%d,) needed, got %s %s" % (name, n, t.dtype, tuple(t.shape)))
+    (ar, lda), (br, ldb) = _rows(a), _rows(b)
+    m, n, k = a.shape[0], b.shape[0], a.shape[1]
+    sa, sb, bi = a_scale.contiguous(), b_scale.contiguous(), None if bias is None else bias.contiguous()
+    with native.device_guard(a.device):
+        out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+        native.check(native.lib().hwer_matmul_q8(P(ar), lda, P(sa), P(br), ldb, P(sb), P(bi), m, n, k, P(out), n, _DTYPES[out_dtype], native.stream_ptr()), "matmul_q8")
+    return out
+
+
+# ---------------------------------------------------------------------------------------------------------------- cross entropy over the catalogue
+class _CeCall:
+    """Checked operands of one call, and its two launches."""
+
+    def __init__(self, queries, table, targets, scale, bias, reduction):
+        _check_rows("queries", queries)
+        _check_rows("table", table)
+        if table.dtype != queries.dtype or table.shape[1] != queries.shape[1]:
+            raise ValueError("table: rows of the queries' width and type needed (%d %s), got %s %s" % (queries.shape[1], queries.dtype, tuple(table.shape), table.dtype))
+        _check_device(queries, table, targets, bias)
+        if targets.dtype not in (torch.int64, torch.int32) or tuple(targets.shape) != (queries.shape[0],):
+            raise ValueError("targets: int64 or int32 of shape (%d,) needed, got %s %s" % (queries.shape[0], targets.dtype, tuple(targets.shape)))
+        if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (table.shape[0],)):
+            raise ValueError("bias: float32 of shape (%d,) needed, got %s %s" % (table.shape[0], bias.dtype, tuple(bias.shape)))
+        if reduction not in _REDUCTIONS:
+            raise ValueError("reduction: one of %s, got %r" % (sorted(_REDUCTIONS), reduction))
+        self.scale = float(scale)
+        if not 0.0 < self.scale < float("inf"):
+            raise ValueError("scale must be positive and finite")
+        self.lib = native.lib()
+        self.n, self.d = queries.shape
+        self.v = table.shape[0]
+        if self.v < 1 or not 1 <= self.d <= self.lib.hwer_catalogue_ce_max_dim():
+            raise ValueError("table: at least one row of 1..%d elements needed, got shape %s" % (self.lib.hwer_catalogue_ce_max_dim(), tuple(table.shape)))
+        self.q, self.ldq = _rows(queries)
+        self.e, self.lde = _rows(table)
+        self.t = targets.to(torch.int64).contiguous()
+        self.b = None if bias is None else bias.contiguous()
+        self.dtype, self.code, self.reduction, self.dev = queries.dtype, _DTYPES[queries.dtype], _REDUCTIONS[reduction], queries.device
+
+    def workspace(self, gradients):
+        lib = self.lib
+        nbytes = lib.hwer_catalogue_ce_workspace_bytes(self.n, self.v, self.d, self.code, lib.hwer_catalogue_ce_reads_in_place(P(self.q), self.ldq, self.d, self.code),
+                                                       lib.hwer_catalogue_ce_reads_in_place(P(self.e), self.lde, self.d, self.code), gradients)
+        return torch.empty(nbytes, dtype=torch.uint8, device=self.dev)
+
+    def forward(self, want_mean, ws):
+        f32 = dict(dtype=torch.float32, device=self.dev)
+        self.rows, self.state = torch.empty(self.n, **f32), torch.empty((self.n, 4), **f32)
+        loss, self.counted = torch.empty((), **f32), torch.empty((), **f32)
+        self.mean = torch.empty((self.n, self.d), **f32) if want_mean else None
+        native.check(self.lib.hwer_catalogue_ce(P(self.q), self.ldq, P(self.e), self.lde, P(self.b), P(self.t), self.n, self.v, self.d, self.code, self.scale,
+                                                self.reduction, P(self.rows), P(self.state), P(loss), P(self.counted), P(self.mean), P(ws), ws.numel(),
+                                                native.stream_ptr()), "catalogue_cross_entropy")
+        return self.rows if self.reduction == 0 else loss
+
+    def backward(self, grad, want_q, want_e, want_b, ws, ready):
+        dq = torch.empty((self.n, self.d), dtype=self.dtype, device=self.dev) if want_q else None
+        de = torch.empty((self.v, self.d), dtype=self.dtype, device=self.dev) if want_e or want_b else None
+        db = torch.empty(self.v, dtype=torch.float32, device=self.dev) if want_b else None
+        native.check(self.lib.hwer_catalogue_ce_backward(P(self.q), self.ldq, P(self.e), self.lde, P(self.b), P(self.t), self.n, self.v, self.d, self.code, self.scale,
+                                                         self.reduction, P(grad), P(self.state), P(self.counted), P(self.mean), P(dq), self.d, P(de), self.d, P(db), ready,
+                                                         P(ws), ws.numel(), native.stream_ptr()), "catalogue_cross_entropy(backward)")
+        return dq, de if want_e else None, db
+
+
+class _CatalogueCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, queries, table, bias, targets, scale, reduction):
+        call = _CeCall(queries, table, targets, scale, bias, reduction)
+        with native.device_guard(call.dev):
+            loss = call.forward(ctx.needs_input_grad[0], call.workspace(bool(ctx.needs_input_grad[0])))
+        ctx.save_for_backward(queries, table, bias, targets, call.state, call.counted, call.mean)
+        ctx.args = (scale, reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        queries, table, bias, targets, state, counted, mean = ctx.saved_tensors
+        call = _CeCall(queries, table, targets, ctx.args[0], bias, ctx.args[1])
+        call.state, call.counted, call.mean = state, counted, mean
+        want = ctx.needs_input_grad
+        with native.device_guard(call.dev):
+            dq, de, db = call.backward(grad.float().contiguous(), want[0], want[1], want[2], call.workspace(True), 0)
+        return dq, de, db, None, None, None
+
+
+def catalogue_cross_entropy(queries, table, targets, scale: float = 1.0, bias: Optional[torch.Tensor] = None, reduction: str = "mean"):
+    """Softmax cross entropy over the whole catalogue: logits scale * queries @ table.T + bias, target = row of `table`; -> the loss (float32; with
+    reduction "none" one for each row).  Logits are never in memory; gradients for queries, table and bias through autograd.
+
+    queries (n, d), table (v, d): float32 / float16 / bfloat16 of one type, 1 <= d <= 256.  targets (n,): -1 = the row does not count (an unknown
+    node, as everywhere in this package); any other value outside the table makes its loss NaN.  scale > 0: 1 / temperature.  bias (v,) float32,
+    e.g. a correction for popularity; -inf takes a row out of the catalogue.  "mean" divides by the counted rows and is 0 without any."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (queries, table, bias)):
+        return _CatalogueCrossEntropy.apply(queries, table, bias, targets, scale, reduction)
+    call = _CeCall(queries, table, targets, scale, bias, reduction)
+    with native.device_guard(call.dev):
+        return call.forward(False, call.workspace(False))
+
+
+def catalogue_cross_entropy_grads(queries, table, targets, scale: float = 1.0, bias: Optional[torch.Tensor] = None, reduction: str = "mean"):
+    """The loss of `catalogue_cross_entropy` ("mean" or "sum") and its gradients in one go, without autograd: -> (loss, dqueries, dtable), and with a
+    bias (loss, dqueries, dtable, dbias).  float32 operands are laid out for the matrix instructions once for both directions."""
+    if reduction == "none":
+        raise ValueError("reduction: \"mean\" or \"sum\" (gradients of which loss?)")
+    call = _CeCall(queries, table, targets, scale, bias, reduction)
+    with native.device_guard(call.dev):
+        ws = call.workspace(True)
+        loss = call.forward(True, ws)
+        dq, de, db = call.backward(None, True, True, bias is not None, ws, 1 if call.n else 0)
+    return (loss, dq, de) if bias is None else (loss, dq, de, db)
