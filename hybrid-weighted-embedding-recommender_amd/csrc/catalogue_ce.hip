@@ -58,7 +58,7 @@ template <> struct CeType<bf16_t> {
 
 // device-side scalars of a call (in its workspace)
 struct CeScalars {
-    float unscale_s, unscale_q, unscale_e;      // 2^-(eq + ee), 2^-eq, 2^-ee: what undoes the operands' powers of two (1 for 16-bit rows)
+    float unscale_s, unscale_q, unscale_e;      // float32 rows: 2^-(eq + ee), 2^-eq, 2^-ee, which undo the operands' powers of two
     float fac_e, fac_b;                          // factors of de and db
     float g_top;                                 // largest |upstream gradient| of a row
 };
@@ -71,7 +71,11 @@ struct CePass {
     const CeScalars* sc;
     int tiles_per_split, n_splits, stat_blocks;
     float *m, *l, *o;            // pass 1: (split, n_stat) maxima and sums, (split, n_stat, DP) weighted sums; pass 2: l, o likewise when split
-    const int64_t* target;       // pass 1: per query its target
+    const int64_t* target;       // per query its target
+    int* counts;                 // pass 1: counted rows of each 32 queries
+    const float* loss_rows;      // pass 2, nullable: the queries' losses, reduced by one more workgroup
+    float* loss;
+    int reduction;
     float* zt;                   // pass 1: per query its target's logit, in the unit of m
     const float4* rowp;          // pass 2: per query {what is taken off its logits, factor of its weights, its target's weight, target (int bits) or -1}
     void* out;                   // pass 2, one split: de in the rows' type, and db
@@ -89,7 +93,36 @@ template <int TERMS, int DP> constexpr int ce_sub() { return TERMS * DP <= 64 ? 
 // (8 rows, one chunk) and the transposed reads (4 rows, two neighbouring chunks) both touch every bank once.
 __device__ __forceinline__ int ce_swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
 
-template <typename E, int TERMS, int DP, int MODE, bool BIAS, bool ROWG>
+// WT: 16-bit terms of a weight.  Two for float32 rows; and where a sum has few terms (kFewTerms), whose roundings do not average out: with four queries
+// one rounding of each target's weight is the error of its class's whole gradient (1.6 times the plain form's, measured).
+constexpr int kFewTerms = 128;
+
+// Sum or mean of the rows' losses, and how many rows count; with no row counted the mean is 0.  One workgroup, 64-bit sums in a fixed order.
+template <int T>
+__device__ __forceinline__ void ce_reduce_loss(const float* loss_rows, const int64_t* target, int64_t n, int reduction, float* loss, float* counted) {
+    __shared__ double s_sum[T / 64];
+    __shared__ int s_cnt[T / 64];
+    double sum = 0.0;
+    int cnt = 0;      // n < 2^31
+    for (int64_t r = threadIdx.x; r < n; r += T) {
+        sum += double(loss_rows[r]);
+        cnt += target[r] != -1;
+    }
+    sum = wave_sum_f64(sum);
+    cnt = wave_sum_i32(cnt);
+    if ((threadIdx.x & 63) == 0) {
+        s_sum[threadIdx.x >> 6] = sum;
+        s_cnt[threadIdx.x >> 6] = cnt;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < T / 64; ++i) sum += s_sum[i], cnt += s_cnt[i];
+        if (loss) *loss = float(reduction == 1 ? sum / double(max(cnt, 1)) : sum);
+        if (counted) *counted = float(cnt);
+    }
+}
+
+template <typename E, int TERMS, int WT, int DP, int MODE, bool BIAS, bool ROWG>
 __global__ __launch_bounds__(256, (TERMS * DP > 256 ? 1 : 2)) void ce_pass_kernel(CePass a) {
     typedef CeType<E> X;
     constexpr int KC = DP / 16, DB = DP / 32, SB = ce_sub<TERMS, DP>(), TS = 32 * SB, ROWB = DP * 2, PLANE = TS * ROWB;
@@ -103,6 +136,9 @@ __global__ __launch_bounds__(256, (TERMS * DP > 256 ? 1 : 2)) void ce_pass_kerne
     __shared__ float s_hot[2][MODE == kTable ? TS : 1];   // ... its target's weight
     __shared__ int s_tgt[2][MODE == kTable ? TS : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l31 = lane & 31;
+    if constexpr (MODE == kTable) {
+        if (blockIdx.x + 1 == gridDim.x && a.loss) return ce_reduce_loss<256>(a.loss_rows, a.target, a.n_strm, a.reduction, a.loss, nullptr);
+    }
     // consecutive numbers stay on one XCD (workgroup id mod 8), and consecutive numbers share a split: the tiles they stream meet in that XCD's L2
     const int total = a.stat_blocks * a.n_splits, per = (total + 7) / 8;
     const int id = int(blockIdx.x & 7) * per + int(blockIdx.x >> 3);
@@ -121,10 +157,14 @@ __global__ __launch_bounds__(256, (TERMS * DP > 256 ? 1 : 2)) void ce_pass_kerne
     for (int i = 0; i < (MODE == kLse ? 1 : DB); ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-    const float scl = a.scale * a.sc->unscale_s, c = fmaxf(scl * kLog2e, 1.2e-38f);      // (never 0: 0 * -inf)
+    const float scl = TERMS == 2 ? a.scale * a.sc->unscale_s : a.scale, c = fmaxf(scl * kLog2e, 1.2e-38f);      // (never 0: 0 * -inf)
     const float thr = BIAS ? kStale * kLn2 : kStale / c;
     float m = kLowest, renew = kLowest, l = 0.f;
-    int64_t target = MODE != kTable && my < a.n_stat ? a.target[my] : -1;
+    const int64_t target = MODE != kTable && my < a.n_stat ? a.target[my] : -1;
+    if (MODE != kTable && split == 0) {      // (-1 once per row: both halves of a wave hold the same rows)
+        const int cnt = __builtin_popcountll(__ballot(half == 0 && target != -1));
+        if (lane == 0) a.counts[4 * sblock + wave] = cnt;
+    }
     float zt = 0.f;
     bool has_zt = false;
     const float my_bias = (BIAS && MODE == kTable) ? a.bias[myc] : 0.f;
@@ -294,10 +334,10 @@ __global__ __launch_bounds__(256, (TERMS * DP > 256 ? 1 : 2)) void ce_pass_kerne
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         hi[j] = E(w[8 * k + j]);
-                        if (TERMS == 2) lo[j] = E(w[8 * k + j] - float(hi[j]));
+                        if (WT == 2) lo[j] = E(w[8 * k + j] - float(hi[j]));
                     }
                     ph[k] = __builtin_bit_cast(s16x8, hi);
-                    if (TERMS == 2) pl[k] = __builtin_bit_cast(s16x8, lo);
+                    if (WT == 2) pl[k] = __builtin_bit_cast(s16x8, lo);
                 }
                 typedef __attribute__((address_space(3))) s16x4* lds4;
                 auto transposed = [&](const char* t, int i, int k) {      // 16 streaming rows x 32 columns, as the product's row operand
@@ -315,8 +355,8 @@ __global__ __launch_bounds__(256, (TERMS * DP > 256 ? 1 : 2)) void ce_pass_kerne
                         if constexpr (TERMS == 2) {
                             const s16x8 el = transposed(t_lo, i, k);
                             o[i] = X::mfma(el, ph[k], o[i]);
-                            o[i] = X::mfma(eh, pl[k], o[i]);
                         }
+                        if constexpr (WT == 2) o[i] = X::mfma(eh, pl[k], o[i]);
                     }
             }
         }
@@ -374,16 +414,18 @@ struct CePack {
     int d, dp;
     float* tops;             // (2, kTopBlocks) partial maxima of |value|
     CeScalars* sc;
+    int vec[2];
 };
-constexpr int kTopBlocks = 256;
+constexpr int kTopBlocks = 512;
 
 // 16-bit rows: copied with zeros behind them.  blockIdx.y: which operand.
 __global__ __launch_bounds__(256) void ce_pack16_kernel(CePack a) {
     const int w = blockIdx.y, chunks = a.dp / 8;
     if (!a.hi[w]) return;
+    const int shift = 31 - __clz(chunks);      // chunks of a row: 8, 16 or 32
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < a.rows[w] * chunks; i += int64_t(gridDim.x) * 256) {
-        const int64_t r = i / chunks;
-        const int c = int(i % chunks) * 8;
+        const int64_t r = i >> shift;
+        const int c = int(i & (chunks - 1)) * 8;
         const short* p = static_cast<const short*>(a.src[w]) + r * a.ld[w];
         s16x8 v;
 #pragma unroll
@@ -392,13 +434,30 @@ __global__ __launch_bounds__(256) void ce_pack16_kernel(CePack a) {
     }
 }
 
+// 8 float32 values of a row from column c, zeros past its end
+__device__ __forceinline__ void ce_load8(const CePack& a, int w, int64_t r, int c, float (&v)[8]) {
+    const float* p = static_cast<const float*>(a.src[w]) + r * a.ld[w] + c;
+    if (a.vec[w]) {      // rows on 16 bytes, of a multiple of 4 values
+        float4 u = {0.f, 0.f, 0.f, 0.f}, t = u;
+        if (c < a.d) u = *reinterpret_cast<const float4*>(p);
+        if (c + 4 < a.d) t = *reinterpret_cast<const float4*>(p + 4);
+        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w, v[4] = t.x, v[5] = t.y, v[6] = t.z, v[7] = t.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < a.d ? p[j] : 0.f;
+    }
+}
+
 __global__ __launch_bounds__(256) void ce_top_kernel(CePack a) {
     __shared__ float s[4];
-    const int w = blockIdx.y;
+    const int w = blockIdx.y, chunks = a.dp / 8, shift = 31 - __clz(chunks);
     float top = 0.f;
-    for (int64_t r = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); r < a.rows[w]; r += int64_t(gridDim.x) * 4) {
-        const float* p = static_cast<const float*>(a.src[w]) + r * a.ld[w];
-        for (int c = threadIdx.x & 63; c < a.d; c += 64) top = fmaxf(top, fabsf(p[c]));
+#pragma unroll 4
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < a.rows[w] * chunks; i += kTopBlocks * 256) {
+        float v[8];
+        ce_load8(a, w, i >> shift, int(i & (chunks - 1)) * 8, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
     }
     top = wave_max_f32(top);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
@@ -429,31 +488,27 @@ __global__ __launch_bounds__(256) void ce_split_kernel(CePack a) {
         a.sc->unscale_e = ldexpf(1.f, -ee);
     }
     const float f = ldexpf(1.f, w ? ee : eq);
-    const int chunks = a.dp / 8;
+    const int chunks = a.dp / 8, shift = 31 - __clz(chunks);
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < a.rows[w] * chunks; i += int64_t(gridDim.x) * 256) {
-        const int64_t r = i / chunks;
-        const int c = int(i % chunks) * 8;
-        const float* p = static_cast<const float*>(a.src[w]) + r * a.ld[w];
+        const int64_t r = i >> shift;
+        const int c = int(i & (chunks - 1)) * 8;
+        float v[8];
+        ce_load8(a, w, r, c, v);
         f16x8 hi, lo;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float v = c + j < a.d ? p[c + j] * f : 0.f;
-            hi[j] = f16_t(v);
-            lo[j] = f16_t(v - float(hi[j]));
+            hi[j] = f16_t(v[j] * f);
+            lo[j] = f16_t(v[j] * f - float(hi[j]));
         }
         *reinterpret_cast<f16x8*>(a.hi[w] + r * a.dp + c) = hi;
         *reinterpret_cast<f16x8*>(a.lo[w] + r * a.dp + c) = lo;
     }
 }
 
-__global__ void ce_scalars_kernel(CeScalars* sc) {
-    sc->unscale_s = sc->unscale_q = sc->unscale_e = 1.f;
-}
-
 // ---------------------------------------------------------------------------------------------------------------- rows
 struct CeRows {
-    const void *q, *e;
-    int64_t ldq, lde;
+    const void* e;
+    int64_t lde;
     const float* bias;
     const int64_t* target;
     int64_t n, v;
@@ -471,43 +526,60 @@ struct CeRows {
     void* dq;
     int64_t lddq;
     float4* rowp;
-    float off;
+    const int* counts;            // counted rows (partial)
+    int n_counts;
+    float off, off2;              // powers of two that the weights of pass 1 / 2 carry
 };
+constexpr int kMaxSplits = 1024;
 
-// Joins the splits of pass 1: one wave per row.  loss_r, lse_r, 1 - p_t and sum_{v /= t} p'_v e_v.
+// What a row's state {lse, its low part, 1 - p_t} means to pass 2 (CePass::rowp); rel: its gradient relative to the largest
 template <bool BIAS>
+__device__ __forceinline__ float4 ce_rowp(bool on, float lse, float low, float miss, float rel, float off, int64_t t) {
+    const bool some = on && lse != kLowest;
+    return {some ? (BIAS ? lse : lse - off) : INFINITY, rel * __builtin_amdgcn_exp2f(BIAS ? -low * kLog2e : -low), -rel * miss * __builtin_amdgcn_exp2f(off),
+            __int_as_float(on ? int(t) : -1)};
+}
+
+// Joins the splits of pass 1: loss_r, lse_r, 1 - p_t and sum_{v /= t} p'_v e_v.  TR threads a row (a wave, or 256 where there are many splits); DP / 4 of
+// them hold 4 columns each, the groups of them share the splits.  GRADS: dx and pass 2's parameters at once (the loss's own gradient is 1).
+template <typename E, bool F32, bool BIAS, int TR, bool GRADS>
 __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t r = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (r >= a.n) return;
-    const float unit = BIAS ? kLog2e : fmaxf(a.scale * a.sc->unscale_s * kLog2e, 1.2e-38f);      // from the maxima's unit to powers of two (as in the pass)
+    __shared__ float s_m[TR > 64 ? kMaxSplits : 1], s_red[8];
+    __shared__ float4 s_o[TR > 64 ? 256 : 1];
+    const int lane = threadIdx.x & 63, t_in = threadIdx.x % TR;
+    const int64_t r = int64_t(blockIdx.x) * (256 / TR) + threadIdx.x / TR;
+    if (r >= a.n) return;      // (whole rows: with TR = 256 the whole workgroup)
+    const float unit = BIAS ? kLog2e : fmaxf((F32 ? a.scale * a.sc->unscale_s : a.scale) * kLog2e, 1.2e-38f);      // from the maxima's unit to powers of two (as in the pass)
     float top = kLowest;
-    for (int s = lane; s < a.n_splits; s += 64) top = fmaxf(top, a.m[int64_t(s) * a.n + r]);
+    for (int s = t_in; s < a.n_splits; s += TR) top = fmaxf(top, a.m[int64_t(s) * a.n + r]);
     top = wave_max_f32(top);
+    if constexpr (TR > 64) {
+        if (lane == 0) s_red[threadIdx.x >> 6] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    }
+    auto factor = [&](int s) {      // (a split without classes has l = 0, or NaN from NaN rows)
+        const float m = a.m[int64_t(s) * a.n + r];
+        return m == kLowest ? 1.f : __builtin_amdgcn_exp2f((m - top) * unit);
+    };
     float sum = 0.f;
-    for (int s = lane; s < a.n_splits; s += 64) {
-        const float m = a.m[int64_t(s) * a.n + r], l = a.l[int64_t(s) * a.n + r];
-        sum += m == kLowest ? l : l * __builtin_amdgcn_exp2f((m - top) * unit);      // (a split without classes has l = 0, or NaN from NaN rows)
+    for (int s = t_in; s < a.n_splits; s += TR) {
+        const float f = factor(s);
+        if constexpr (TR > 64) s_m[s] = f;
+        sum += a.l[int64_t(s) * a.n + r] * f;
     }
     sum = lanes_sum<64>(sum);
-    if (a.mean) {
-        const float f = sum == 0.f ? 0.f : a.sc->unscale_e / sum;
-        for (int c = lane; c < a.d; c += 64) {
-            float v = 0.f;
-            for (int s = 0; s < a.n_splits; ++s) {
-                const float m = a.m[int64_t(s) * a.n + r];
-                const float x = a.o[(int64_t(s) * a.n + r) * a.dp + c];
-                v += m == kLowest ? x : x * __builtin_amdgcn_exp2f((m - top) * unit);
-            }
-            a.mean[r * a.d + c] = v * f;
-        }
+    if constexpr (TR > 64) {
+        if (lane == 0) s_red[4 + (threadIdx.x >> 6)] = sum;
+        __syncthreads();
+        sum = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
     }
-    if (lane) return;
     // in powers of two, 64 bits: the other classes' lse (all of them where no target counts) and the target's logit
     const int64_t t = a.target[r];
+    const bool on = t >= 0 && t < a.v;
     const double rest = sum == 0.f ? -double(INFINITY) : double(top) * double(unit) + log2(double(sum)) - double(a.off);
     double lse = rest, miss = 0.0, loss = 0.0;
-    if (t >= 0 && t < a.v) {
+    if (on) {
         const double z = double(a.zt[r]) * double(unit), x = rest - z;
         const bool none = sum == 0.f && z == -double(INFINITY);      // every class masked
         loss = none ? double(INFINITY) : x > 64.0 ? x * kLn2d : log1p(exp2(x));
@@ -517,33 +589,63 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
         loss = NAN;      // no such class: nothing to learn from, and seen in the loss
     }
     if (BIAS) lse *= kLn2d;
-    const float hi = float(lse);
-    a.loss_rows[r] = float(loss);
-    a.state[r] = {hi, hi == kLowest ? 0.f : float(lse - double(hi)), float(miss), 0.f};
+    const float hi = float(lse), low = hi == kLowest ? 0.f : float(lse - double(hi));
+    float g = 1.f;
+    if constexpr (GRADS) {
+        if (a.reduction == 1) {
+            int cnt = 0;
+            for (int i = lane; i < a.n_counts; i += 64) cnt += a.counts[i];
+            g = 1.f / float(max(wave_sum_i32(cnt), 1));
+        }
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            const float unoff = __builtin_amdgcn_exp2f(-a.off2);
+            a.sc->fac_e = a.scale * g * unoff * (F32 ? a.sc->unscale_q : 1.f);
+            a.sc->fac_b = g * unoff;
+        }
+    }
+    if (t_in == 0) {
+        a.loss_rows[r] = float(loss);
+        if constexpr (GRADS) a.rowp[r] = ce_rowp<BIAS>(on, hi, low, float(miss), on ? 1.f : 0.f, a.off2, t);
+        else a.state[r] = {hi, low, float(miss), 0.f};
+    }
+    if (!GRADS && !a.mean) return;
+    const int per = a.dp / 4, groups = TR / per, c4 = t_in & (per - 1), grp = t_in / per;
+    float4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = grp; s < a.n_splits; s += groups) {
+        const float f = TR > 64 ? s_m[s] : factor(s);
+        const float4 x = *reinterpret_cast<const float4*>(a.o + (int64_t(s) * a.n + r) * a.dp + 4 * c4);
+        v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
+    }
+    if constexpr (TR > 64) {
+        s_o[threadIdx.x] = v;
+        __syncthreads();
+        if (grp) return;
+        for (int k = 1; k < groups; ++k) {
+            const float4 x = s_o[k * per + c4];
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        }
+    } else {
+        for (int k = per; k < 64; k <<= 1) {      // groups lie side by side in the wave
+            v.x += __shfl_xor(v.x, k, kWave), v.y += __shfl_xor(v.y, k, kWave), v.z += __shfl_xor(v.z, k, kWave), v.w += __shfl_xor(v.w, k, kWave);
+        }
+        if (grp) return;
+    }
+    const float f = sum == 0.f ? 0.f : (F32 ? a.sc->unscale_e : 1.f) / sum;
+    const float mean[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+    const E* e = static_cast<const E*>(a.e) + (on ? t : 0) * a.lde;
+    const float fq = a.scale * g * float(miss);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int c = 4 * c4 + j;
+        if (c >= a.d) break;
+        if constexpr (GRADS) static_cast<E*>(a.dq)[r * a.lddq + c] = E(on ? fq * (mean[j] - float(e[c])) : 0.f);
+        else a.mean[r * a.d + c] = mean[j];
+    }
 }
 
-// Sum or mean of the rows' losses, and how many rows count; with no row counted the mean is 0.  One workgroup, 64-bit sums in a fixed order.
-__global__ __launch_bounds__(1024) void ce_stats_kernel(const float* loss_rows, const int64_t* target, int64_t n, int reduction, float* loss, float* counted) {
-    __shared__ double s_sum[16];
-    __shared__ int s_cnt[16];
-    double sum = 0.0;
-    int cnt = 0;      // n < 2^31
-    for (int64_t r = threadIdx.x; r < n; r += 1024) {
-        sum += double(loss_rows[r]);
-        cnt += target[r] != -1;
-    }
-    sum = wave_sum_f64(sum);
-    cnt = wave_sum_i32(cnt);
-    if ((threadIdx.x & 63) == 0) {
-        s_sum[threadIdx.x >> 6] = sum;
-        s_cnt[threadIdx.x >> 6] = cnt;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 16; ++i) sum += s_sum[i], cnt += s_cnt[i];
-        if (loss) *loss = float(reduction == 1 ? sum / double(max(cnt, 1)) : sum);
-        *counted = float(cnt);
-    }
+__global__ __launch_bounds__(1024) void ce_loss_kernel(const float* loss_rows, const int64_t* target, int64_t n, int reduction, float* loss, float* counted) {
+    ce_reduce_loss<1024>(loss_rows, target, n, reduction, loss, counted);
 }
 
 __global__ __launch_bounds__(1024) void ce_grad_top_kernel(const float* grad, int64_t n, CeScalars* sc) {
@@ -559,16 +661,16 @@ __global__ __launch_bounds__(1024) void ce_grad_top_kernel(const float* grad, in
     }
 }
 
-// dx, and what pass 2 needs of every query (CePass::rowp).  One wave per row.
-template <typename E, bool BIAS>
+// Backward by itself: dx, and what pass 2 needs of every query (CePass::rowp).  One wave per row.
+template <typename E, bool F32, bool BIAS>
 __global__ __launch_bounds__(256) void ce_dq_kernel(CeRows a) {
     const int lane = threadIdx.x & 63;
     const int64_t r = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
     // the gradient of a counted row, or with one per row what they are relative to
     const float g = a.per_row ? a.sc->g_top : (a.grad ? a.grad[0] : 1.f) / (a.reduction == 1 ? fmaxf(a.counted[0], 1.f) : 1.f);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
-        const float unoff = __builtin_amdgcn_exp2f(-a.off);
-        a.sc->fac_e = a.scale * g * unoff * a.sc->unscale_q;
+        const float unoff = __builtin_amdgcn_exp2f(-a.off2);
+        a.sc->fac_e = a.scale * g * unoff * (F32 ? a.sc->unscale_q : 1.f);
         a.sc->fac_b = g * unoff;
     }
     if (r >= a.n) return;
@@ -576,12 +678,7 @@ __global__ __launch_bounds__(256) void ce_dq_kernel(CeRows a) {
     const bool on = t >= 0 && t < a.v;
     const float4 st = a.state[r];
     const float gr = a.per_row ? a.grad[r] : g;
-    if (a.rowp && lane == 0) {
-        const float rel = !on ? 0.f : a.per_row ? (g > 0.f ? gr / g : gr) : 1.f;
-        const bool some = on && st.x != kLowest;
-        a.rowp[r] = {some ? (BIAS ? st.x : st.x - a.off) : INFINITY, rel * __builtin_amdgcn_exp2f(BIAS ? -st.y * kLog2e : -st.y),
-                     -rel * st.z * __builtin_amdgcn_exp2f(a.off), __int_as_float(on ? int(t) : -1)};
-    }
+    if (a.rowp && lane == 0) a.rowp[r] = ce_rowp<BIAS>(on, st.x, st.y, st.z, !on ? 0.f : a.per_row ? (g > 0.f ? gr / g : gr) : 1.f, a.off2, t);
     if (a.dq) {
         E* dq = static_cast<E*>(a.dq) + r * a.lddq;
         const E* e = static_cast<const E*>(a.e) + (on ? t : 0) * a.lde;
@@ -594,13 +691,14 @@ __global__ __launch_bounds__(256) void ce_dq_kernel(CeRows a) {
 template <typename E>
 __global__ __launch_bounds__(256) void ce_de_kernel(const float* __restrict__ o, const float* __restrict__ l, int n_splits, int64_t v, int d, int dp,
                                                    const CeScalars* sc, E* __restrict__ de, int64_t ldde, float* __restrict__ db) {
-    const int per = dp / 4;
+    const int per = dp / 4, shift = 31 - __clz(per);
     const float fe = sc->fac_e, fb = sc->fac_b;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < v * per; i += int64_t(gridDim.x) * 256) {
-        const int64_t r = i / per;
-        const int c = int(i % per) * 4;
+        const int64_t r = i >> shift;
+        const int c = int(i & (per - 1)) * 4;
         if (c < d) {
             float4 s = *reinterpret_cast<const float4*>(o + r * dp + c);
+#pragma unroll 4
             for (int k = 1; k < n_splits; ++k) {
                 const float4 t = *reinterpret_cast<const float4*>(o + (int64_t(k) * v + r) * dp + c);
                 s.x += t.x, s.y += t.y, s.z += t.z, s.w += t.w;
@@ -632,7 +730,7 @@ struct CeSplit {
 };
 static CeSplit ce_split(int64_t n_stat, int64_t n_strm, int d, int dtype) {
     const int terms = dtype == HWER_F32 ? 2 : 1, dp = ce_padded(d), w = terms * dp;
-    const int ts = 32 * (w <= 64 ? 4 : w <= 256 ? 2 : 1), target = w > 256 ? 256 : 512;
+    const int ts = 32 * (w <= 64 ? 4 : w <= 256 ? 2 : 1), target = w > 256 ? 256 : 512;      // target <= kMaxSplits
     const int64_t blocks = cdiv64(n_stat, 128), tiles = cdiv64(n_strm, ts);
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(tiles, target / std::max<int64_t>(blocks, 1)));
     const int64_t per = std::max<int64_t>(1, cdiv64(tiles, want));
@@ -641,116 +739,192 @@ static CeSplit ce_split(int64_t n_stat, int64_t n_strm, int d, int dtype) {
 
 static size_t up(size_t b) { return (b + 255) & ~size_t(255); }
 
-// Where a call's workspace keeps what.  The head (scalars, laid-out operands) stays for the backward call of the same operands; the rest is each call's own.
+// Where a call's workspace keeps what.  The head (scalars, laid-out operands) serves both passes of a call.
 struct CeLayout {
-    size_t tops, q_hi, q_lo, e_hi, e_lo, head, zt, m, l, o, fwd_end, rowp, l2, o2, bwd_end;
+    size_t tops, q_hi, q_lo, e_hi, e_lo, loss_rows, counts, rowp, head, zt, m, l, o, fwd_end, l2, o2, bwd_end;
 };
 static CeLayout ce_layout(int64_t n, int64_t v, int d, int dtype, bool q_direct, bool e_direct, bool want_mean) {
     const size_t dp = ce_padded(d);
     CeLayout y{};
+    const CeSplit f = ce_split(n, v, d, dtype), b = ce_split(v, n, d, dtype);
     size_t at = 256;      // CeScalars
     y.tops = at, at += dtype == HWER_F32 ? 2 * kTopBlocks * 4 : 0;
     y.q_hi = at, at += q_direct ? 0 : up(size_t(n) * dp * 2);
     y.q_lo = at, at += dtype == HWER_F32 ? up(size_t(n) * dp * 2) : 0;
     y.e_hi = at, at += e_direct ? 0 : up(size_t(v) * dp * 2);
     y.e_lo = at, at += dtype == HWER_F32 ? up(size_t(v) * dp * 2) : 0;
+    y.counts = at, at += up(size_t(f.blocks) * 16);
+    y.loss_rows = at, at += want_mean ? up(size_t(n) * 4) : 0;
+    y.rowp = at, at += want_mean ? up(size_t(n) * 16) : 0;
     y.head = at;
-    const CeSplit f = ce_split(n, v, d, dtype), b = ce_split(v, n, d, dtype);
     y.zt = at, at += up(size_t(n) * 4);
     y.m = at, at += up(size_t(f.splits) * n * 4);
     y.l = at, at += up(size_t(f.splits) * n * 4);
     y.o = at, at += want_mean ? up(size_t(f.splits) * n * dp * 4) : 0;
     y.fwd_end = at;
     at = y.head;
-    y.rowp = at, at += up(size_t(n) * 16);
     y.l2 = at, at += b.splits > 1 ? up(size_t(b.splits) * v * 4) : 0;
     y.o2 = at, at += b.splits > 1 ? up(size_t(b.splits) * v * dp * 4) : 0;
     y.bwd_end = at;
     return y;
 }
 
+// One call: checked operands, and the steps that the entries below are made of.
 struct CeCall {
     const void *q, *e;
-    int64_t ldq, lde, n, v;
-    int d, dtype;
+    int64_t ldq, lde;
     const float* bias;
+    const int64_t* target;
+    int64_t n, v;
+    int d, dtype;
     float scale;
+    int reduction;
     unsigned char* ws;
-    CeLayout y;
-    bool q_direct, e_direct;
     hipStream_t st;
-    CeScalars* sc() const { return reinterpret_cast<CeScalars*>(ws); }
-    const short* q_hi() const { return q_direct ? static_cast<const short*>(q) : reinterpret_cast<const short*>(ws + y.q_hi); }
-    const short* e_hi() const { return e_direct ? static_cast<const short*>(e) : reinterpret_cast<const short*>(ws + y.e_hi); }
-    const short* q_lo() const { return dtype == HWER_F32 ? reinterpret_cast<const short*>(ws + y.q_lo) : nullptr; }
-    const short* e_lo() const { return dtype == HWER_F32 ? reinterpret_cast<const short*>(ws + y.e_lo) : nullptr; }
-    int64_t q_ld() const { return q_direct ? ldq : ce_padded(d); }
-    int64_t e_ld() const { return e_direct ? lde : ce_padded(d); }
+    bool q_direct, e_direct;
+    int dp;
+    CeLayout y;
+
+    template <typename T> T* at(size_t off) const { return reinterpret_cast<T*>(ws + off); }
+    const short* q_hi() const { return q_direct ? static_cast<const short*>(q) : at<short>(y.q_hi); }
+    const short* e_hi() const { return e_direct ? static_cast<const short*>(e) : at<short>(y.e_hi); }
+    const short* q_lo() const { return dtype == HWER_F32 ? at<short>(y.q_lo) : nullptr; }
+    const short* e_lo() const { return dtype == HWER_F32 ? at<short>(y.e_lo) : nullptr; }
+    int64_t q_ld() const { return q_direct ? ldq : dp; }
+    int64_t e_ld() const { return e_direct ? lde : dp; }
+
+    int check(const char* what, void* workspace, size_t bytes, bool want_mean, void* stream) {
+        if (!known_dtype(dtype)) return fail(HWER_EINVAL, "%s: unknown element type %d", what, dtype);
+        if (d < 1 || d > hwer_catalogue_ce_max_dim()) return fail(HWER_EINVAL, "%s: d=%d unsupported (1..%d)", what, d, hwer_catalogue_ce_max_dim());
+        const int64_t most = (int64_t(1) << 31) - 256;
+        if (n < 0 || v < 1 || n > most || v > most) return fail(HWER_EINVAL, "%s: %lld rows, %lld classes", what, (long long)n, (long long)v);
+        if (!(scale > 0.f) || !(scale < INFINITY)) return fail(HWER_EINVAL, "%s: scale must be positive and finite", what);
+        if (n && (!q || !target)) return fail(HWER_EINVAL, "%s: null queries or targets", what);
+        if (!e || ldq < d || lde < d) return fail(HWER_EINVAL, "%s: null table or a row stride below d", what);
+        q_direct = ce_direct(q, ldq, d, dtype), e_direct = ce_direct(e, lde, d, dtype), dp = ce_padded(d);
+        y = ce_layout(n, v, d, dtype, q_direct, e_direct, want_mean);
+        const size_t need = hwer_catalogue_ce_workspace_bytes(n, v, d, dtype, q_direct, e_direct, want_mean);
+        if (!workspace || bytes < need) return fail(HWER_EWORKSPACE, "%s: workspace of %zu bytes needed", what, need);
+        ws = static_cast<unsigned char*>(workspace), st = as_stream(stream);
+        return HWER_OK;
+    }
+
+    // lays out what the passes cannot read in place
+    int prepare() const {
+        CePack p{{q, e}, {nullptr, nullptr}, {nullptr, nullptr}, {n, v}, {ldq, lde}, d, dp, at<float>(y.tops), at<CeScalars>(0), {0, 0}};
+        if (!q_direct) p.hi[0] = at<short>(y.q_hi);
+        if (!e_direct) p.hi[1] = at<short>(y.e_hi);
+        const dim3 grid(unsigned(std::max<int64_t>(1, std::min<int64_t>(cdiv64(std::max(n, v) * (dp / 8), 256), kMaxStreamBlocks))), 2);
+        if (dtype == HWER_F32) {
+            p.lo[0] = at<short>(y.q_lo), p.lo[1] = at<short>(y.e_lo);
+            p.vec[0] = d % 4 == 0 && aligned_to(q, ldq * 4, 16), p.vec[1] = d % 4 == 0 && aligned_to(e, lde * 4, 16);
+            ce_top_kernel<<<dim3(kTopBlocks, 2), dim3(256), 0, st>>>(p);
+            ce_split_kernel<<<grid, dim3(256), 0, st>>>(p);
+        } else if (p.hi[0] || p.hi[1]) {
+            ce_pack16_kernel<<<grid, dim3(256), 0, st>>>(p);
+        }
+        return check_launch("catalogue_ce(operands)");
+    }
+
+    int pass1(bool mean, CeRows& r) const {
+        const CeSplit s = ce_split(n, v, d, dtype);
+        CePass p{};
+        p.stat = q_hi(), p.stat_lo = q_lo(), p.strm = e_hi(), p.strm_lo = e_lo();
+        p.ld_stat = q_ld(), p.ld_strm = e_ld(), p.n_stat = n, p.n_strm = v;
+        p.bias = bias, p.scale = scale, p.sc = at<CeScalars>(0);
+        p.tiles_per_split = s.tiles_per_split, p.n_splits = s.splits, p.stat_blocks = s.blocks;
+        p.m = at<float>(y.m), p.l = at<float>(y.l), p.o = at<float>(y.o);
+        p.target = target, p.zt = at<float>(y.zt), p.counts = at<int>(y.counts), p.d = d;
+        mean ? ce_pass_any<kMean>(p, dp, dtype, false, st) : ce_pass_any<kLse>(p, dp, dtype, false, st);
+        r = rows();
+        r.n_splits = s.splits, r.m = p.m, r.l = p.l, r.o = p.o, r.zt = p.zt, r.counts = p.counts, r.n_counts = 4 * s.blocks;
+        return check_launch("catalogue_ce(pass)");
+    }
+
+    CeRows rows() const {
+        CeRows r{};
+        r.e = e, r.lde = lde, r.bias = bias, r.target = target, r.n = n, r.v = v, r.d = d, r.dp = dp, r.scale = scale, r.sc = at<CeScalars>(0);
+        r.reduction = reduction, r.off = ce_offset(dtype, 0), r.off2 = ce_offset(dtype, 1);
+        return r;
+    }
+
+    int pass2(void* de, int64_t ldde, float* dbias, bool rowg, const float* loss_rows, float* loss) const {
+        const CeSplit s = ce_split(v, n, d, dtype);
+        CePass p{};
+        p.stat = e_hi(), p.stat_lo = e_lo(), p.strm = q_hi(), p.strm_lo = q_lo();
+        p.ld_stat = e_ld(), p.ld_strm = q_ld(), p.n_stat = v, p.n_strm = n;
+        p.bias = bias, p.scale = scale, p.sc = at<CeScalars>(0);
+        p.tiles_per_split = s.tiles_per_split, p.n_splits = s.splits, p.stat_blocks = s.blocks;
+        p.l = at<float>(y.l2), p.o = at<float>(y.o2);
+        p.rowp = at<float4>(y.rowp), p.out = de, p.out_b = dbias, p.ld_out = ldde, p.d = d;
+        p.out_vec = d % 4 == 0 && aligned_to(de, ldde * dtype_bytes(dtype), 4 * dtype_bytes(dtype));
+        p.target = target, p.loss_rows = loss_rows, p.loss = loss, p.reduction = reduction;
+        ce_pass_any<kTable>(p, dp, dtype, rowg, st);
+        if (int rc = check_launch("catalogue_ce(table pass)")) return rc;
+        if (s.splits > 1) {
+            const dim3 grid(unsigned(std::min<int64_t>(cdiv64(v * (dp / 4), 256), 4 * kMaxStreamBlocks)));
+            if (dtype == HWER_F32) ce_de_kernel<float><<<grid, dim3(256), 0, st>>>(p.o, p.l, s.splits, v, d, dp, p.sc, static_cast<float*>(de), ldde, dbias);
+            else if (dtype == HWER_F16) ce_de_kernel<f16_t><<<grid, dim3(256), 0, st>>>(p.o, p.l, s.splits, v, d, dp, p.sc, static_cast<f16_t*>(de), ldde, dbias);
+            else ce_de_kernel<bf16_t><<<grid, dim3(256), 0, st>>>(p.o, p.l, s.splits, v, d, dp, p.sc, static_cast<bf16_t*>(de), ldde, dbias);
+        }
+        return check_launch("catalogue_ce(table)");
+    }
+
+    template <typename E, int TERMS, int WT, int DP, int MODE>
+    static void ce_pass_launch(const CePass& a, bool rowg, hipStream_t st) {
+        const bool more = MODE == kTable && a.loss;      // one more workgroup reduces the losses
+        const dim3 grid(unsigned((int64_t(a.stat_blocks) * a.n_splits + 7) / 8 * 8 + more)), block(256);
+        if constexpr (MODE == kTable) {
+            if (a.bias) rowg ? ce_pass_kernel<E, TERMS, WT, DP, MODE, true, true><<<grid, block, 0, st>>>(a) : ce_pass_kernel<E, TERMS, WT, DP, MODE, true, false><<<grid, block, 0, st>>>(a);
+            else rowg ? ce_pass_kernel<E, TERMS, WT, DP, MODE, false, true><<<grid, block, 0, st>>>(a) : ce_pass_kernel<E, TERMS, WT, DP, MODE, false, false><<<grid, block, 0, st>>>(a);
+        } else {
+            if (a.bias) ce_pass_kernel<E, TERMS, WT, DP, MODE, true, false><<<grid, block, 0, st>>>(a);
+            else ce_pass_kernel<E, TERMS, WT, DP, MODE, false, false><<<grid, block, 0, st>>>(a);
+        }
+    }
+    template <typename E, int TERMS, int WT, int MODE>
+    static void ce_pass_width(const CePass& a, int dp, bool rowg, hipStream_t st) {
+        if (dp == 64) ce_pass_launch<E, TERMS, WT, 64, MODE>(a, rowg, st);
+        else if (dp == 128) ce_pass_launch<E, TERMS, WT, 128, MODE>(a, rowg, st);
+        else ce_pass_launch<E, TERMS, WT, 256, MODE>(a, rowg, st);
+    }
+    template <int MODE>
+    static void ce_pass_any(const CePass& a, int dp, int dtype, bool rowg, hipStream_t st) {
+        const bool two = MODE != kLse && a.n_strm <= kFewTerms;
+        constexpr int W2 = MODE == kLse ? 1 : 2;
+        if (dtype == HWER_F32) ce_pass_width<f16_t, 2, W2, MODE>(a, dp, rowg, st);
+        else if (dtype == HWER_F16) two ? ce_pass_width<f16_t, 1, W2, MODE>(a, dp, rowg, st) : ce_pass_width<f16_t, 1, 1, MODE>(a, dp, rowg, st);
+        else two ? ce_pass_width<bf16_t, 1, W2, MODE>(a, dp, rowg, st) : ce_pass_width<bf16_t, 1, 1, MODE>(a, dp, rowg, st);
+    }
+    static float ce_offset(int dtype, int pass) { return dtype == HWER_BF16 ? CeType<bf16_t>::offset[pass] : CeType<f16_t>::offset[pass]; }
+
+    template <bool GRADS>
+    int join(const CeRows& r) const {
+        if (dtype == HWER_F32) join_typed<float, true, GRADS>(r);
+        else if (dtype == HWER_F16) join_typed<f16_t, false, GRADS>(r);
+        else join_typed<bf16_t, false, GRADS>(r);
+        return check_launch("catalogue_ce(rows)");
+    }
+    template <typename E, bool F32, bool GRADS>
+    void join_typed(const CeRows& r) const {
+        // a wave per row walks over a few splits in less than a microsecond; hundreds of them (few rows, long catalogue) took 230 us at 466
+        const bool wave = r.n_splits <= 16;
+        const dim3 grid(unsigned(wave ? cdiv64(n, 4) : n)), block(256);
+        if (bias) wave ? ce_rows_kernel<E, F32, true, 64, GRADS><<<grid, block, 0, st>>>(r) : ce_rows_kernel<E, F32, true, 256, GRADS><<<grid, block, 0, st>>>(r);
+        else wave ? ce_rows_kernel<E, F32, false, 64, GRADS><<<grid, block, 0, st>>>(r) : ce_rows_kernel<E, F32, false, 256, GRADS><<<grid, block, 0, st>>>(r);
+    }
+    template <typename E, bool F32>
+    void dq_typed(const CeRows& r) const {
+        const dim3 grid(unsigned(std::max<int64_t>(1, cdiv64(n, 4)))), block(256);      // (without rows it leaves the factors of zeros)
+        bias ? ce_dq_kernel<E, F32, true><<<grid, block, 0, st>>>(r) : ce_dq_kernel<E, F32, false><<<grid, block, 0, st>>>(r);
+    }
+    int backward_rows(const CeRows& r) const {
+        if (dtype == HWER_F32) dq_typed<float, true>(r);
+        else if (dtype == HWER_F16) dq_typed<f16_t, false>(r);
+        else dq_typed<bf16_t, false>(r);
+        return check_launch("catalogue_ce(row gradients)");
+    }
 };
-
-static int ce_prepare(const CeCall& c) {
-    const int dp = ce_padded(c.d);
-    CePack p{{c.q, c.e}, {nullptr, nullptr}, {nullptr, nullptr}, {c.n, c.v}, {c.ldq, c.lde}, c.d, dp, reinterpret_cast<float*>(c.ws + c.y.tops), c.sc()};
-    if (!c.q_direct) p.hi[0] = reinterpret_cast<short*>(c.ws + c.y.q_hi);
-    if (!c.e_direct) p.hi[1] = reinterpret_cast<short*>(c.ws + c.y.e_hi);
-    const unsigned blocks = unsigned(std::min<int64_t>(cdiv64(std::max(c.n, c.v) * (dp / 8), 256), kMaxStreamBlocks));
-    if (c.dtype == HWER_F32) {
-        p.lo[0] = reinterpret_cast<short*>(c.ws + c.y.q_lo);
-        p.lo[1] = reinterpret_cast<short*>(c.ws + c.y.e_lo);
-        ce_top_kernel<<<dim3(kTopBlocks, 2), dim3(256), 0, c.st>>>(p);
-        ce_split_kernel<<<dim3(blocks, 2), dim3(256), 0, c.st>>>(p);
-        return check_launch("catalogue_ce(split)");
-    }
-    ce_scalars_kernel<<<dim3(1), dim3(1), 0, c.st>>>(c.sc());
-    if (p.hi[0] || p.hi[1]) ce_pack16_kernel<<<dim3(blocks, 2), dim3(256), 0, c.st>>>(p);
-    return check_launch("catalogue_ce(pack)");
-}
-
-template <typename E, int TERMS, int DP, int MODE>
-static void ce_pass_launch(const CePass& a, bool rowg, hipStream_t st) {
-    const dim3 grid(unsigned((int64_t(a.stat_blocks) * a.n_splits + 7) / 8 * 8)), block(256);
-    if constexpr (MODE == kTable) {
-        if (a.bias) rowg ? ce_pass_kernel<E, TERMS, DP, MODE, true, true><<<grid, block, 0, st>>>(a) : ce_pass_kernel<E, TERMS, DP, MODE, true, false><<<grid, block, 0, st>>>(a);
-        else rowg ? ce_pass_kernel<E, TERMS, DP, MODE, false, true><<<grid, block, 0, st>>>(a) : ce_pass_kernel<E, TERMS, DP, MODE, false, false><<<grid, block, 0, st>>>(a);
-    } else {
-        if (a.bias) ce_pass_kernel<E, TERMS, DP, MODE, true, false><<<grid, block, 0, st>>>(a);
-        else ce_pass_kernel<E, TERMS, DP, MODE, false, false><<<grid, block, 0, st>>>(a);
-    }
-}
-template <typename E, int TERMS, int MODE>
-static void ce_pass_width(const CePass& a, int dp, bool rowg, hipStream_t st) {
-    if (dp == 64) ce_pass_launch<E, TERMS, 64, MODE>(a, rowg, st);
-    else if (dp == 128) ce_pass_launch<E, TERMS, 128, MODE>(a, rowg, st);
-    else ce_pass_launch<E, TERMS, 256, MODE>(a, rowg, st);
-}
-template <int MODE>
-static void ce_pass_any(const CePass& a, int dp, int dtype, bool rowg, hipStream_t st) {
-    if (dtype == HWER_F32) ce_pass_width<f16_t, 2, MODE>(a, dp, rowg, st);
-    else if (dtype == HWER_F16) ce_pass_width<f16_t, 1, MODE>(a, dp, rowg, st);
-    else ce_pass_width<bf16_t, 1, MODE>(a, dp, rowg, st);
-}
-static float ce_offset(int dtype, int pass) { return dtype == HWER_BF16 ? CeType<bf16_t>::offset[pass] : CeType<f16_t>::offset[pass]; }
-
-static void ce_rows_launch(const CeRows& r, hipStream_t st) {
-    const dim3 grid(unsigned(cdiv64(r.n, 4))), block(256);
-    r.bias ? ce_rows_kernel<true><<<grid, block, 0, st>>>(r) : ce_rows_kernel<false><<<grid, block, 0, st>>>(r);
-}
-template <typename E>
-static void ce_dq_launch(const CeRows& r, hipStream_t st) {
-    const dim3 grid(unsigned(std::max<int64_t>(1, cdiv64(r.n, 4)))), block(256);      // (without rows it leaves the factors of zeros)
-    r.bias ? ce_dq_kernel<E, true><<<grid, block, 0, st>>>(r) : ce_dq_kernel<E, false><<<grid, block, 0, st>>>(r);
-}
-
-static int ce_check(const char* what, const void* q, int64_t ldq, const void* e, int64_t lde, const int64_t* target, int64_t n, int64_t v, int d, int dtype, float scale) {
-    if (!known_dtype(dtype)) return fail(HWER_EINVAL, "%s: unknown element type %d", what, dtype);
-    if (d < 1 || d > hwer_catalogue_ce_max_dim()) return fail(HWER_EINVAL, "%s: d=%d unsupported (1..%d)", what, d, hwer_catalogue_ce_max_dim());
-    const int64_t most = (int64_t(1) << 31) - 256;
-    if (n < 0 || v < 1 || n > most || v > most) return fail(HWER_EINVAL, "%s: %lld rows, %lld classes", what, (long long)n, (long long)v);
-    if (!(scale > 0.f) || !(scale < INFINITY)) return fail(HWER_EINVAL, "%s: scale must be positive and finite", what);
-    if (n && (!q || !target)) return fail(HWER_EINVAL, "%s: null queries or targets", what);
-    if (!e || ldq < d || lde < d) return fail(HWER_EINVAL, "%s: null table or a row stride below d", what);
-    return HWER_OK;
-}
 
 }  // namespace hwer
 
@@ -769,82 +943,63 @@ size_t hwer_catalogue_ce_workspace_bytes(int64_t n, int64_t v, int d, int dtype,
 }
 
 int hwer_catalogue_ce(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int d, int dtype,
-                      float scale, int reduction, float* loss_rows, float* state, float* loss, float* counted, float* mean, void* workspace, size_t workspace_bytes, void* stream) {
-    if (int rc = ce_check("catalogue_ce", q, ldq, e, lde, target, n, v, d, dtype, scale)) return rc;
+                      float scale, int reduction, float* loss_rows, float* state, float* loss, float* counted, float* mean, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+    CeCall c{q, e, ldq, lde, bias, target, n, v, d, dtype, scale, reduction};
+    if (int rc = c.check("catalogue_ce", workspace, workspace_bytes, mean != nullptr, stream)) return rc;
     if (reduction < 0 || reduction > 2) return fail(HWER_EINVAL, "catalogue_ce: unknown reduction %d", reduction);
     if (!counted || (reduction && !loss) || (n && (!loss_rows || !state))) return fail(HWER_EINVAL, "catalogue_ce: null output");
-    const bool qd = ce_direct(q, ldq, d, dtype), ed = ce_direct(e, lde, d, dtype);
-    const size_t need = hwer_catalogue_ce_workspace_bytes(n, v, d, dtype, qd, ed, mean != nullptr);
-    if (!workspace || workspace_bytes < need) return fail(HWER_EWORKSPACE, "catalogue_ce: workspace of %zu bytes needed", need);
-    hipStream_t st = as_stream(stream);
-    CeCall c{q, e, ldq, lde, n, v, d, dtype, bias, scale, static_cast<unsigned char*>(workspace), ce_layout(n, v, d, dtype, qd, ed, mean != nullptr), qd, ed, st};
     if (n) {
-        if (int rc = ce_prepare(c)) return rc;
-        const CeSplit s = ce_split(n, v, d, dtype);
-        const int dp = ce_padded(d);
-        CePass p{};
-        p.stat = c.q_hi(), p.stat_lo = c.q_lo(), p.strm = c.e_hi(), p.strm_lo = c.e_lo();
-        p.ld_stat = c.q_ld(), p.ld_strm = c.e_ld(), p.n_stat = n, p.n_strm = v;
-        p.bias = bias, p.scale = scale, p.sc = c.sc();
-        p.tiles_per_split = s.tiles_per_split, p.n_splits = s.splits, p.stat_blocks = s.blocks;
-        p.m = reinterpret_cast<float*>(c.ws + c.y.m), p.l = reinterpret_cast<float*>(c.ws + c.y.l), p.o = reinterpret_cast<float*>(c.ws + c.y.o);
-        p.target = target, p.zt = reinterpret_cast<float*>(c.ws + c.y.zt), p.d = d;
-        mean ? ce_pass_any<kMean>(p, dp, dtype, false, st) : ce_pass_any<kLse>(p, dp, dtype, false, st);
-        if (int rc = check_launch("catalogue_ce(pass)")) return rc;
-        CeRows r{};
-        r.q = q, r.e = e, r.ldq = ldq, r.lde = lde, r.bias = bias, r.target = target, r.n = n, r.v = v, r.d = d, r.dp = dp, r.n_splits = s.splits, r.scale = scale;
-        r.m = p.m, r.l = p.l, r.o = p.o, r.sc = c.sc(), r.zt = p.zt, r.loss_rows = loss_rows, r.state = reinterpret_cast<float4*>(state), r.mean = mean, r.off = ce_offset(dtype, 0);
-        ce_rows_launch(r, st);
+        CeRows r;
+        if (int rc = c.prepare()) return rc;
+        if (int rc = c.pass1(mean != nullptr, r)) return rc;
+        r.loss_rows = loss_rows, r.state = reinterpret_cast<float4*>(state), r.mean = mean;
+        if (int rc = c.join<false>(r)) return rc;
     }
-    ce_stats_kernel<<<dim3(1), dim3(1024), 0, st>>>(loss_rows, target, n, reduction, loss, counted);
+    ce_loss_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(loss_rows, target, n, reduction, loss, counted);
     return check_launch("catalogue_ce");
 }
 
 int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int d,
-                               int dtype, float scale, int reduction, const float* grad, const float* state, const float* counted, const float* mean, void* dq, int64_t lddq,
-                               void* de, int64_t ldde, float* dbias, int operands_ready, void* workspace, size_t workspace_bytes, void* stream) {
-    if (int rc = ce_check("catalogue_ce_backward", q, ldq, e, lde, target, n, v, d, dtype, scale)) return rc;
+                               int dtype, float scale, int reduction, const float* grad, const float* state, const float* counted, const float* mean, void* dq,
+                               int64_t lddq, void* de, int64_t ldde, float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+    CeCall c{q, e, ldq, lde, bias, target, n, v, d, dtype, scale, reduction};
+    if (int rc = c.check("catalogue_ce_backward", workspace, workspace_bytes, true, stream)) return rc;
     if (reduction < 0 || reduction > 2 || (reduction == 0 && !grad)) return fail(HWER_EINVAL, "catalogue_ce_backward: unknown reduction %d, or rows' losses without their gradients", reduction);
     if (!counted || (n && (!state || (dq && !mean)))) return fail(HWER_EINVAL, "catalogue_ce_backward: what the forward call left is missing");
     if ((dq && lddq < d) || (de && ldde < d)) return fail(HWER_EINVAL, "catalogue_ce_backward: a row stride is below d");
     if (dbias && (!bias || !de)) return fail(HWER_EINVAL, "catalogue_ce_backward: dbias needs the bias, and comes with the table's gradient");
-    const bool qd = ce_direct(q, ldq, d, dtype), ed = ce_direct(e, lde, d, dtype);
-    const size_t need = hwer_catalogue_ce_workspace_bytes(n, v, d, dtype, qd, ed, 1);
-    if (!workspace || workspace_bytes < need) return fail(HWER_EWORKSPACE, "catalogue_ce_backward: workspace of %zu bytes needed", need);
-    hipStream_t st = as_stream(stream);
-    CeCall c{q, e, ldq, lde, n, v, d, dtype, bias, scale, static_cast<unsigned char*>(workspace), ce_layout(n, v, d, dtype, qd, ed, true), qd, ed, st};
-    if (!operands_ready || n == 0)
-        if (int rc = ce_prepare(c)) return rc;
-    const int dp = ce_padded(d);
-    CeRows r{};
-    r.q = q, r.e = e, r.ldq = ldq, r.lde = lde, r.bias = bias, r.target = target, r.n = n, r.v = v, r.d = d, r.dp = dp, r.scale = scale, r.sc = c.sc();
-    r.state = reinterpret_cast<float4*>(const_cast<float*>(state)), r.mean = const_cast<float*>(mean), r.counted = counted, r.grad = grad, r.reduction = reduction, r.per_row = reduction == 0;
-    r.dq = dq, r.lddq = lddq, r.off = ce_offset(dtype, 1);
-    r.rowp = de ? reinterpret_cast<float4*>(c.ws + c.y.rowp) : nullptr;
-    if (reduction == 0 && n) ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, st>>>(grad, n, c.sc());
-    if (dtype == HWER_F32) ce_dq_launch<float>(r, st);
-    else if (dtype == HWER_F16) ce_dq_launch<f16_t>(r, st);
-    else ce_dq_launch<bf16_t>(r, st);
-    if (int rc = check_launch("catalogue_ce_backward(rows)")) return rc;
-    if (!de) return HWER_OK;
-    const CeSplit s = ce_split(v, n, d, dtype);
-    CePass p{};
-    p.stat = c.e_hi(), p.stat_lo = c.e_lo(), p.strm = c.q_hi(), p.strm_lo = c.q_lo();
-    p.ld_stat = c.e_ld(), p.ld_strm = c.q_ld(), p.n_stat = v, p.n_strm = n;
-    p.bias = bias, p.scale = scale, p.sc = c.sc();
-    p.tiles_per_split = s.tiles_per_split, p.n_splits = s.splits, p.stat_blocks = s.blocks;
-    p.l = reinterpret_cast<float*>(c.ws + c.y.l2), p.o = reinterpret_cast<float*>(c.ws + c.y.o2);
-    p.rowp = r.rowp, p.out = de, p.out_b = dbias, p.ld_out = ldde, p.d = d;
-    p.out_vec = d % 4 == 0 && aligned_to(de, ldde * dtype_bytes(dtype), 4 * dtype_bytes(dtype));
-    ce_pass_any<kTable>(p, dp, dtype, reduction == 0, st);
-    if (int rc = check_launch("catalogue_ce_backward(pass)")) return rc;
-    if (s.splits > 1) {
-        const dim3 grid(unsigned(std::min<int64_t>(cdiv64(v * (dp / 4), 256), 4 * kMaxStreamBlocks)));
-        if (dtype == HWER_F32) ce_de_kernel<float><<<grid, dim3(256), 0, st>>>(p.o, p.l, s.splits, v, d, dp, c.sc(), static_cast<float*>(de), ldde, dbias);
-        else if (dtype == HWER_F16) ce_de_kernel<f16_t><<<grid, dim3(256), 0, st>>>(p.o, p.l, s.splits, v, d, dp, c.sc(), static_cast<f16_t*>(de), ldde, dbias);
-        else ce_de_kernel<bf16_t><<<grid, dim3(256), 0, st>>>(p.o, p.l, s.splits, v, d, dp, c.sc(), static_cast<bf16_t*>(de), ldde, dbias);
+    if (de || dtype == HWER_F32)
+        if (int rc = c.prepare()) return rc;
+    CeRows r = c.rows();
+    r.state = reinterpret_cast<float4*>(const_cast<float*>(state)), r.mean = const_cast<float*>(mean), r.counted = counted, r.grad = grad, r.per_row = reduction == 0;
+    r.dq = dq, r.lddq = lddq, r.rowp = de ? c.at<float4>(c.y.rowp) : nullptr;
+    if (reduction == 0) ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(grad, n, r.sc);
+    if (int rc = c.backward_rows(r)) return rc;
+    return de ? c.pass2(de, ldde, dbias, reduction == 0, nullptr, nullptr) : HWER_OK;
+}
+
+int hwer_catalogue_ce_grads(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int d, int dtype,
+                            float scale, int reduction, float* loss, void* dq, int64_t lddq, void* de, int64_t ldde, float* dbias, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+    CeCall c{q, e, ldq, lde, bias, target, n, v, d, dtype, scale, reduction};
+    if (int rc = c.check("catalogue_ce_grads", workspace, workspace_bytes, true, stream)) return rc;
+    if (reduction < 1 || reduction > 2) return fail(HWER_EINVAL, "catalogue_ce_grads: reduction %d: 1 (mean) or 2 (sum)", reduction);
+    if (!loss || !de || (n && !dq) || lddq < d || ldde < d) return fail(HWER_EINVAL, "catalogue_ce_grads: null output or a row stride below d");
+    if (dbias && !bias) return fail(HWER_EINVAL, "catalogue_ce_grads: a gradient of a bias that is not there");
+    if (int rc = c.prepare()) return rc;
+    float* loss_rows = c.at<float>(c.y.loss_rows);
+    CeRows r = c.rows();
+    if (n) {
+        if (int rc = c.pass1(true, r)) return rc;
+        r.loss_rows = loss_rows, r.dq = dq, r.lddq = lddq, r.rowp = c.at<float4>(c.y.rowp);
+        if (int rc = c.join<true>(r)) return rc;
+    } else {
+        r.per_row = 1, r.grad = loss_rows;      // no rows: the factors of a sum over nothing
+        ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(loss_rows, 0, r.sc);
+        if (int rc = c.backward_rows(r)) return rc;
     }
-    return check_launch("catalogue_ce_backward");
+    return c.pass2(de, ldde, dbias, false, loss_rows, loss);
 }
 
 }  // extern "C"

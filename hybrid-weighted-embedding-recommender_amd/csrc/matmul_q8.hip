@@ -48,31 +48,35 @@ __device__ __forceinline__ O finish(int acc, float sa, float sb, float bias) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- both sides long
-constexpr int kTM = 128, kTN = 128, kTK = 128;   // tile of C, bytes of K per step
+// A workgroup of WM x WN waves makes a tile of C; a wave XM x XN blocks of 32 x 32.  Operands go through LDS in steps of 128 bytes of K, by DMA, the
+// next step's while this one's is multiplied (STAGES = 2).
+constexpr int kTK = 128;
 
-// LDS image of a 128-row operand tile: 128 bytes (8 chunks of 16) a row, chunk c of row r at c ^ (r & 7): the 8 lanes that a ds_read_b128 serves
-// together read 8 rows' same chunk from 8 different 16-byte slots of the banks
-template <bool ALIGNED>
+// LDS image of an operand: 128 bytes (8 chunks of 16) a row, chunk c of row r at c ^ (r & 7): the 8 lanes that a ds_read_b128 serves together read 8
+// rows' same chunk from 8 different 16-byte slots of the banks
+template <bool ALIGNED, int ROWS, int WAVES>
 __device__ __forceinline__ void stage(const int8_t* base, int64_t ld, int64_t row0, int64_t rows, int k0, int K, int8_t* lds, int wave, int lane) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {               // a wave stages 32 of the 128 rows, 8 rows (1 KB) at a time
-        const int r = wave * 32 + i * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
+    for (int i = 0; i < ROWS / (8 * WAVES); ++i) {      // 8 rows (1 KB) at a time
+        const int r8 = (wave * (ROWS / (8 * WAVES)) + i) * 8, r = r8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
         const bool in = row0 + r < rows;
         const int8_t* row = base + (in ? row0 + r : 0) * ld;
         if constexpr (ALIGNED) {
             const void* p = in && k0 + 16 * c < K ? static_cast<const void*>(row + k0 + 16 * c) : static_cast<const void*>(kZero16);
-            lds_dma16_v(p, __builtin_amdgcn_readfirstlane(lds_addr(lds + (wave * 32 + i * 8) * kTK)));
+            lds_dma16_v(p, __builtin_amdgcn_readfirstlane(lds_addr(lds + r8 * kTK)));
         } else {
             const i4_t v = in ? load16<false>(row, k0 + 16 * c, K) : i4_t{0, 0, 0, 0};
-            *reinterpret_cast<i4_t*>(lds + (wave * 32 + i * 8) * kTK + lane * 16) = v;
+            *reinterpret_cast<i4_t*>(lds + r8 * kTK + lane * 16) = v;
         }
     }
 }
 
-template <typename O, bool ALIGNED>
-__global__ __launch_bounds__(256, 2) void matmul_q8_tile_kernel(QmmArgs g, int tiles_m, int tiles_n) {
-    __shared__ __align__(16) int8_t s_a[2][kTM * kTK];
-    __shared__ __align__(16) int8_t s_b[2][kTN * kTK];
+template <typename O, bool ALIGNED, int WM, int WN, int XM, int XN, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN, (WM * WN > 4 ? 2 : STAGES == 1 ? 4 : 2)) void matmul_q8_tile_kernel(QmmArgs g, int tiles_m, int tiles_n, int vec) {
+    constexpr int WAVES = WM * WN, TM = 32 * XM * WM, TN = 32 * XN * WN, STAGE = (TM + TN) * kTK;
+    constexpr int OC = 32 * XN, OROW = OC * int(sizeof(O)) + 16, OUT = WAVES * 32 * OROW;      // a wave's 32 output rows on their way out
+    __shared__ __align__(16) int8_t s_buf[STAGES * STAGE > OUT ? STAGES * STAGE : OUT];
+    __shared__ __align__(16) float s_scale[TN], s_bias[TN];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l31 = lane & 31;
     // tiles of one XCD (workgroup id mod 8) are neighbours: 8 rows of tiles, walked along the columns
     const int total = tiles_m * tiles_n, per = (total + 7) / 8;
@@ -80,59 +84,93 @@ __global__ __launch_bounds__(256, 2) void matmul_q8_tile_kernel(QmmArgs g, int t
     if (int(blockIdx.x >> 3) >= per || id >= total) return;
     const int band = id / (8 * tiles_n), in_band = id % (8 * tiles_n), bh = min(8, tiles_m - 8 * band);
     const int tm = band * 8 + in_band % bh, tn = in_band / bh;
-    const int64_t m0 = int64_t(tm) * kTM, n0 = int64_t(tn) * kTN;
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-    i16_t acc[2][2];
+    const int64_t m0 = int64_t(tm) * TM, n0 = int64_t(tn) * TN;
+    const int wm = (wave % WM) * 32 * XM, wn = (wave / WM) * 32 * XN;
+    i16_t acc[XM][XN];
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < XM; ++x)
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < XN; ++y)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[x][y][i] = 0;
     const int steps = (g.k + kTK - 1) / kTK;
-    if (steps) {
-        stage<ALIGNED>(g.a, g.lda, m0, g.m, 0, g.k, s_a[0], wave, lane);
-        stage<ALIGNED>(g.b, g.ldb, n0, g.n, 0, g.k, s_b[0], wave, lane);
+    auto put = [&](int s, int buf) {
+        stage<ALIGNED, TM, WAVES>(g.a, g.lda, m0, g.m, s * kTK, g.k, s_buf + buf * STAGE, wave, lane);
+        stage<ALIGNED, TN, WAVES>(g.b, g.ldb, n0, g.n, s * kTK, g.k, s_buf + buf * STAGE + TM * kTK, wave, lane);
+    };
+    if (steps) put(0, 0);
+    if (int(threadIdx.x) < TN) {      // (read after the barriers below)
+        const int64_t n = std::min<int64_t>(n0 + threadIdx.x, g.n - 1);
+        s_scale[threadIdx.x] = g.sb[n];
+        s_bias[threadIdx.x] = g.bias ? g.bias[n] : 0.f;
     }
     for (int s = 0; s < steps; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();      // step s is staged, and everyone is done with the other buffers
-        if (s + 1 < steps) {
-            stage<ALIGNED>(g.a, g.lda, m0, g.m, (s + 1) * kTK, g.k, s_a[(s + 1) & 1], wave, lane);
-            stage<ALIGNED>(g.b, g.ldb, n0, g.n, (s + 1) * kTK, g.k, s_b[(s + 1) & 1], wave, lane);
+        const int buf = STAGES == 1 ? 0 : s & 1;
+        if (STAGES == 1 && s) {
+            __syncthreads();      // everyone is done with the last step
+            put(s, 0);
         }
-        const int8_t *pa = s_a[s & 1], *pb = s_b[s & 1];
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();          // step s is staged, and everyone is done with the other buffer
+        if (STAGES == 2 && s + 1 < steps) put(s + 1, buf ^ 1);
+        const int8_t *pa = s_buf + buf * STAGE, *pb = pa + TM * kTK;
 #pragma unroll
         for (int kc = 0; kc < kTK / 32; ++kc) {
-            i4_t fa[2], fb[2];
+            i4_t fa[XM], fb[XN];
+            const int c = 2 * kc + half;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int ra = wm + 32 * x + l31, rb = wn + 32 * x + l31, c = 2 * kc + half;
-                fa[x] = *reinterpret_cast<const i4_t*>(pa + ra * kTK + 16 * (c ^ (ra & 7)));
-                fb[x] = *reinterpret_cast<const i4_t*>(pb + rb * kTK + 16 * (c ^ (rb & 7)));
+            for (int y = 0; y < XN; ++y) {
+                const int r = wn + 32 * y + l31;
+                fb[y] = *reinterpret_cast<const i4_t*>(pb + r * kTK + 16 * (c ^ (r & 7)));
             }
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < XM; ++x) {
+                const int r = wm + 32 * x + l31;
+                fa[x] = *reinterpret_cast<const i4_t*>(pa + r * kTK + 16 * (c ^ (r & 7)));
+            }
 #pragma unroll
-                for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[y], fa[x], acc[x][y], 0, 0, 0);
+            for (int x = 0; x < XM; ++x)
+#pragma unroll
+                for (int y = 0; y < XN; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[y], fa[x], acc[x][y], 0, 0, 0);
         }
     }
-    // C fragment: column (lane & 31) = row m of the output, register rows = 4 consecutive n at a time
+    // C fragment: column (lane & 31) = row m of the output, register rows = 4 consecutive n at a time.  Written through LDS, 32 rows at a time, so that
+    // lanes write neighbouring bytes of a row.
+    __syncthreads();
+    int8_t* mine = s_buf + wave * 32 * OROW;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const int64_t m = m0 + wm + 32 * x + l31;
-        if (m >= g.m) continue;
-        const float sa = g.sa[m];
-        O* out = static_cast<O*>(g.out) + m * g.ldo;
+    for (int x = 0; x < XM; ++x) {
+        const int64_t mb = m0 + wm + 32 * x;
+        const float sa = g.sa[std::min<int64_t>(mb + l31, g.m - 1)];
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < XN; ++y)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int64_t n = n0 + wn + 32 * y + 8 * q + 4 * half;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (n + j < g.n) out[n + j] = finish<O>(acc[x][y][4 * q + j], sa, g.sb[n + j], g.bias ? g.bias[n + j] : 0.f);
+                typedef O o4 __attribute__((ext_vector_type(4)));
+                const float4 sb = *reinterpret_cast<const float4*>(s_scale + wn + 32 * y + 8 * q + 4 * half);
+                const float4 bi = *reinterpret_cast<const float4*>(s_bias + wn + 32 * y + 8 * q + 4 * half);
+                const o4 v = {finish<O>(acc[x][y][4 * q], sa, sb.x, bi.x), finish<O>(acc[x][y][4 * q + 1], sa, sb.y, bi.y),
+                              finish<O>(acc[x][y][4 * q + 2], sa, sb.z, bi.z), finish<O>(acc[x][y][4 * q + 3], sa, sb.w, bi.w)};
+                *reinterpret_cast<o4*>(mine + l31 * OROW + (32 * y + 8 * q + 4 * half) * int(sizeof(O))) = v;
             }
+        wave_lds_sync();
+        const int64_t nb = n0 + wn;
+        O* out = static_cast<O*>(g.out) + mb * g.ldo + nb;
+        const int rows = int(std::min<int64_t>(32, g.m - mb)), cols = int(std::min<int64_t>(OC, g.n - nb));
+        if (vec) {      // whole 16-byte pieces (n and the row stride are multiples of a piece)
+            constexpr int PIECE = 16 / int(sizeof(O)), LPR = OC / PIECE, RPI = 64 / LPR;      // lanes of a row, rows of an instruction
+            const int c = (lane % LPR) * PIECE;
+#pragma unroll
+            for (int i = 0; i < 32 / RPI; ++i) {
+                const int r = i * RPI + lane / LPR;
+                const i4_t v = *reinterpret_cast<const i4_t*>(mine + r * OROW + c * int(sizeof(O)));
+                if (r < rows && c < cols) *reinterpret_cast<i4_t*>(out + int64_t(r) * g.ldo + c) = v;
+            }
+        } else {
+            for (int r = 0; r < rows; ++r)
+                for (int c = lane; c < cols; c += 64) out[int64_t(r) * g.ldo + c] = *reinterpret_cast<const O*>(mine + r * OROW + c * int(sizeof(O)));
+        }
+        wave_lds_sync();
     }
 }
 
@@ -213,8 +251,12 @@ static void matmul_q8_launch(const QmmArgs& g, hipStream_t st) {
         else matmul_q8_few_kernel<O, 4, ALIGNED><<<grid, dim3(256), 0, st>>>(f);
         return;
     }
-    const int tm = int(cdiv64(g.m, kTM)), tn = int(cdiv64(g.n, kTN));
-    matmul_q8_tile_kernel<O, ALIGNED><<<dim3(unsigned((int64_t(tm) * tn + 7) / 8 * 8)), dim3(256), 0, st>>>(g, tm, tn);
+    const int vec = (g.n * int64_t(sizeof(O))) % 16 == 0 && aligned_to(g.out, g.ldo * int64_t(sizeof(O)), 16);
+    auto tiles = [&](int tm, int tn) { return cdiv64(g.m, tm) * cdiv64(g.n, tn); };
+    auto grid = [&](int tm, int tn) { return dim3(unsigned((tiles(tm, tn) + 7) / 8 * 8)); };
+    if (g.k > kTK && tiles(256, 256) >= 192) matmul_q8_tile_kernel<O, ALIGNED, 2, 4, 4, 2, 2><<<grid(256, 256), dim3(512), 0, st>>>(g, int(cdiv64(g.m, 256)), int(cdiv64(g.n, 256)), vec);
+    else if (g.k > kTK) matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 2><<<grid(128, 128), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 128)), int(cdiv64(g.n, 128)), vec);
+    else matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 1><<<grid(128, 128), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 128)), int(cdiv64(g.n, 128)), vec);
 }
 
 }  // namespace hwer
@@ -226,7 +268,7 @@ extern "C" int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale
     if (!known_dtype(out_dtype)) return fail(HWER_EINVAL, "matmul_q8: unknown output type %d", out_dtype);
     if (m < 0 || n < 0 || k < 0 || k > 131071) return fail(HWER_EINVAL, "matmul_q8: m=%lld, n=%lld, k=%d (k <= 131071: sums stay in 32 bits)", (long long)m, (long long)n, k);
     if (m == 0 || n == 0) return HWER_OK;
-    if (m > (int64_t(1) << 31) - 256 || n > (int64_t(1) << 31) - 256 || cdiv64(m, kTM) * cdiv64(n, kTN) > (int64_t(1) << 30))
+    if (m > (int64_t(1) << 31) - 256 || n > (int64_t(1) << 31) - 256 || cdiv64(m, 128) * cdiv64(n, 128) > (int64_t(1) << 30))
         return fail(HWER_EINVAL, "matmul_q8: m=%lld, n=%lld: too many tiles for one call", (long long)m, (long long)n);
     if ((k && (!a || !b)) || !a_scale || !b_scale || !out) return fail(HWER_EINVAL, "matmul_q8: null operand");
     if (lda < k || ldb < k || ldo < n) return fail(HWER_EINVAL, "matmul_q8: a row stride is below the row's length");

@@ -14,6 +14,7 @@ Errors: wrong shapes, types or devices raise before anything is launched (ValueE
 never checked on the host (that would wait for the GPU): a target that names no class makes its loss NaN."""
 from __future__ import annotations
 
+import contextlib
 from typing import Optional
 
 import torch
@@ -22,7 +23,23 @@ from . import native
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
-P = native.ptr
+# A call on a single row is a few microseconds of GPU time: what the host does per call is kept short (addresses as plain integers, the device switched
+# only where it is another one, the raw stream handle).
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_STAY = contextlib.nullcontext()
+
+
+def P(t):
+    return None if t is None else t.data_ptr()
+
+
+def _on(t):
+    """Context in which `t`'s device is the current one."""
+    return _STAY if t.get_device() == torch.cuda.current_device() else native.device_guard(t.device)
+
+
+def _stream(t):
+    return _stream_of(t.get_device())
 
 
 def _check_rows(name, t, dtypes=_DTYPES, dim=2):
@@ -35,25 +52,28 @@ def _check_rows(name, t, dtypes=_DTYPES, dim=2):
 
 
 def _check_device(t, *others):
-    if t.device.type != "cuda":
+    index = t.get_device()
+    if index < 0:
         raise native.HwerNativeError("hwer (MI355X build) needs device tensors: got one on %s; there is no CPU fallback for this path" % t.device)
     for o in others:
-        if o is not None and o.device != t.device:
+        if o is not None and o.get_device() != index:
             raise ValueError("operands on two devices: %s and %s" % (t.device, o.device))
 
 
 def _rows(t):
     """(tensor, row stride) of 2-d rows whose elements are contiguous; anything else (a transposed view, a broadcast row) is copied."""
     n, d = t.shape
-    if (t.stride(1) == 1 or d == 1) and (t.stride(0) >= d or n <= 1):
-        return t, max(t.stride(0), d)
-    t = t.contiguous()
-    return t, max(t.stride(0), d)
+    if t.is_contiguous():
+        return t, d
+    row, one = t.stride()
+    if (one == 1 or d == 1) and (row >= d or n <= 1):
+        return t, max(row, d)
+    return t.contiguous(), d
 
 
 def _flat(t):
     """... of rows along the last dimension of any number of leading ones"""
-    return _rows(t.reshape(-1, t.shape[-1]))
+    return _rows(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
 
 
 def _weight(weight, x):
@@ -63,7 +83,7 @@ def _weight(weight, x):
         raise TypeError("weight: float32 or the rows' type (%s), got %s" % (x.dtype, weight.dtype))
     if tuple(weight.shape) != (x.shape[-1],):
         raise ValueError("weight: shape (%d,) needed, got %s" % (x.shape[-1], tuple(weight.shape)))
-    return weight.contiguous(), _DTYPES[weight.dtype]
+    return (weight if weight.is_contiguous() else weight.contiguous()), _DTYPES[weight.dtype]
 
 
 def _norm_checks(x, weight, residual, eps):
@@ -83,16 +103,20 @@ def _norm_forward(x, weight, residual, eps):
     xr, ldx = _flat(x)
     rr, ldr = _flat(residual) if residual is not None else (None, 0)
     n, d = xr.shape
-    with native.device_guard(x.device):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
-        native.check(native.lib().hwer_rms_norm(P(xr), ldx, P(rr), ldr, P(w), wt, n, d, _DTYPES[x.dtype], eps, P(y), d, P(h), d, native.stream_ptr()), "rms_norm")
+    with _on(x):
+        y = x.new_empty(x.shape)
+        h = x.new_empty(x.shape) if residual is not None else None
+        native.check(native.lib().hwer_rms_norm(P(xr), ldx, P(rr), ldr, P(w), wt, n, d, _DTYPES[x.dtype], eps, P(y), d, P(h), d, _stream(x)), "rms_norm")
     return y, h
 
 
 def rms_norm_grads(dy, h, weight=None, eps: float = 1e-6, dh=None):
     """Gradients of `rms_norm`: -> (dx, dweight).  dx is the gradient of x and of the residual alike; dweight is None without a weight.
     h: what the norm was taken of (the second result of `rms_norm` with a residual, x without one).  dh: the gradient that reaches h by other ways."""
+    return _norm_backward(dy, h, weight, eps, dh, weight is not None)
+
+
+def _norm_backward(dy, h, weight, eps, dh, want_dw):
     _norm_checks(h, weight, dh, eps)
     if dy.shape != h.shape or dy.dtype != h.dtype:
         raise ValueError("dy: shape and type of h needed")
@@ -102,13 +126,13 @@ def rms_norm_grads(dy, h, weight=None, eps: float = 1e-6, dh=None):
     ar, lda = _flat(dh) if dh is not None else (None, 0)
     n, d = hr.shape
     lib = native.lib()
-    with native.device_guard(h.device):
-        dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-        dw = torch.empty_like(w) if w is not None else None
-        nbytes = lib.hwer_rms_norm_backward_workspace_bytes(n, d) if w is not None else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device) if nbytes else None
+    with _on(h):
+        dx = h.new_empty(h.shape)
+        dw = torch.empty_like(w) if want_dw else None
+        nbytes = lib.hwer_rms_norm_backward_workspace_bytes(n, d) if want_dw else 0
+        ws = h.new_empty(nbytes, dtype=torch.uint8) if want_dw else None
         native.check(lib.hwer_rms_norm_backward(P(gr), ldg, P(hr), ldh, P(w), wt, P(ar), lda, n, d, _DTYPES[h.dtype], eps, P(dx), d, P(dw), P(ws), nbytes,
-                                                native.stream_ptr()), "rms_norm_backward")
+                                                _stream(h)), "rms_norm_backward")
     return dx, dw
 
 
@@ -127,9 +151,8 @@ class _RmsNorm(torch.autograd.Function):
         h, weight = ctx.saved_tensors
         if dy is None:       # only h was used further
             return dh, None if weight is None or not ctx.needs_input_grad[1] else torch.zeros_like(weight), dh if ctx.two else None, None
-        w = weight if ctx.needs_input_grad[1] else (None if weight is None else weight.detach())
-        dx, dw = rms_norm_grads(dy, h, w, ctx.eps, dh)
-        return (dx if ctx.needs_input_grad[0] else None, dw if ctx.needs_input_grad[1] else None, dx if ctx.two and ctx.needs_input_grad[2] else None, None)
+        dx, dw = _norm_backward(dy, h, weight, ctx.eps, dh, ctx.needs_input_grad[1])
+        return dx if ctx.needs_input_grad[0] else None, dw, dx if ctx.two and ctx.needs_input_grad[2] else None, None
 
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-6):
@@ -148,12 +171,12 @@ def _codes(x, weight, residual, eps, norm):
     xr, ldx = _flat(x)
     rr, ldr = _flat(residual) if residual is not None else (None, 0)
     n, d = xr.shape
-    with native.device_guard(x.device):
-        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    with _on(x):
+        q = x.new_empty(x.shape, dtype=torch.int8)
+        scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        h = x.new_empty(x.shape) if residual is not None else None
         native.check(native.lib().hwer_rms_norm_q8(P(xr), ldx, P(rr), ldr, P(w), wt, n, d, _DTYPES[x.dtype], norm, eps, P(q), d, P(scale), P(h), d,
-                                                   native.stream_ptr()), "rms_norm_q8")
+                                                   _stream(x)), "rms_norm_q8")
     return (q, scale) if h is None else (q, scale, h)
 
 
@@ -182,14 +205,14 @@ def matmul_q8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
     if out_dtype not in _DTYPES:
         raise TypeError("out_dtype: float32, float16 or bfloat16, got %s" % out_dtype)
     for name, t, n in (("a_scale", a_scale, a.shape[0]), ("b_scale", b_scale, b.shape[0]), ("bias", bias, b.shape[0])):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (n,)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (n,)):
             raise ValueError("%s: float32 of shape (%d,) needed, got %s %s" % (name, n, t.dtype, tuple(t.shape)))
     (ar, lda), (br, ldb) = _rows(a), _rows(b)
     m, n, k = a.shape[0], b.shape[0], a.shape[1]
     sa, sb, bi = a_scale.contiguous(), b_scale.contiguous(), None if bias is None else bias.contiguous()
-    with native.device_guard(a.device):
-        out = torch.empty((m, n), dtype=out_dtype, device=a.device)
-        native.check(native.lib().hwer_matmul_q8(P(ar), lda, P(sa), P(br), ldb, P(sb), P(bi), m, n, k, P(out), n, _DTYPES[out_dtype], native.stream_ptr()), "matmul_q8")
+    with _on(a):
+        out = a.new_empty((m, n), dtype=out_dtype)
+        native.check(native.lib().hwer_matmul_q8(P(ar), lda, P(sa), P(br), ldb, P(sb), P(bi), m, n, k, P(out), n, _DTYPES[out_dtype], _stream(a)), "matmul_q8")
     return out
 
 
@@ -219,42 +242,56 @@ class _CeCall:
             raise ValueError("table: at least one row of 1..%d elements needed, got shape %s" % (self.lib.hwer_catalogue_ce_max_dim(), tuple(table.shape)))
         self.q, self.ldq = _rows(queries)
         self.e, self.lde = _rows(table)
-        self.t = targets.to(torch.int64).contiguous()
-        self.b = None if bias is None else bias.contiguous()
-        self.dtype, self.code, self.reduction, self.dev = queries.dtype, _DTYPES[queries.dtype], _REDUCTIONS[reduction], queries.device
+        self.targets, self.b = targets, None if bias is None else bias.contiguous()
+        self.code, self.reduction = _DTYPES[queries.dtype], _REDUCTIONS[reduction]
+
+    def on(self):
+        """Context of the call's device; work that is enqueued belongs in it."""
+        return _on(self.q)
+
+    def operands(self):
+        self.t = self.targets.to(torch.int64).contiguous()
+        return P(self.q), self.ldq, P(self.e), self.lde, P(self.b), P(self.t), self.n, self.v, self.d, self.code, self.scale, self.reduction
 
     def workspace(self, gradients):
         lib = self.lib
         nbytes = lib.hwer_catalogue_ce_workspace_bytes(self.n, self.v, self.d, self.code, lib.hwer_catalogue_ce_reads_in_place(P(self.q), self.ldq, self.d, self.code),
                                                        lib.hwer_catalogue_ce_reads_in_place(P(self.e), self.lde, self.d, self.code), gradients)
-        return torch.empty(nbytes, dtype=torch.uint8, device=self.dev)
+        return self.q.new_empty(nbytes, dtype=torch.uint8), nbytes
 
-    def forward(self, want_mean, ws):
-        f32 = dict(dtype=torch.float32, device=self.dev)
-        self.rows, self.state = torch.empty(self.n, **f32), torch.empty((self.n, 4), **f32)
-        loss, self.counted = torch.empty((), **f32), torch.empty((), **f32)
-        self.mean = torch.empty((self.n, self.d), **f32) if want_mean else None
-        native.check(self.lib.hwer_catalogue_ce(P(self.q), self.ldq, P(self.e), self.lde, P(self.b), P(self.t), self.n, self.v, self.d, self.code, self.scale,
-                                                self.reduction, P(self.rows), P(self.state), P(loss), P(self.counted), P(self.mean), P(ws), ws.numel(),
-                                                native.stream_ptr()), "catalogue_cross_entropy")
+    def forward(self, want_mean):
+        new = lambda *shape: self.q.new_empty(shape, dtype=torch.float32)  # noqa: E731
+        ws, nbytes = self.workspace(want_mean)
+        self.rows, self.state, self.counted, loss = new(self.n), new(self.n, 4), new(), new()
+        self.mean = new(self.n, self.d) if want_mean else None
+        native.check(self.lib.hwer_catalogue_ce(*self.operands(), P(self.rows), P(self.state), P(loss), P(self.counted), P(self.mean), P(ws), nbytes, _stream(self.q)),
+                     "catalogue_cross_entropy")
         return self.rows if self.reduction == 0 else loss
 
-    def backward(self, grad, want_q, want_e, want_b, ws, ready):
-        dq = torch.empty((self.n, self.d), dtype=self.dtype, device=self.dev) if want_q else None
-        de = torch.empty((self.v, self.d), dtype=self.dtype, device=self.dev) if want_e or want_b else None
-        db = torch.empty(self.v, dtype=torch.float32, device=self.dev) if want_b else None
-        native.check(self.lib.hwer_catalogue_ce_backward(P(self.q), self.ldq, P(self.e), self.lde, P(self.b), P(self.t), self.n, self.v, self.d, self.code, self.scale,
-                                                         self.reduction, P(grad), P(self.state), P(self.counted), P(self.mean), P(dq), self.d, P(de), self.d, P(db), ready,
-                                                         P(ws), ws.numel(), native.stream_ptr()), "catalogue_cross_entropy(backward)")
+    def backward(self, grad, want_q, want_e, want_b):
+        ws, nbytes = self.workspace(True)
+        dq = self.q.new_empty((self.n, self.d)) if want_q else None
+        de = self.q.new_empty((self.v, self.d)) if want_e or want_b else None
+        db = self.q.new_empty(self.v, dtype=torch.float32) if want_b else None
+        native.check(self.lib.hwer_catalogue_ce_backward(*self.operands(), P(grad), P(self.state), P(self.counted), P(self.mean), P(dq), self.d, P(de), self.d, P(db),
+                                                         P(ws), nbytes, _stream(self.q)), "catalogue_cross_entropy(backward)")
         return dq, de if want_e else None, db
+
+    def gradients(self):
+        ws, nbytes = self.workspace(True)
+        loss, dq, de = self.q.new_empty((), dtype=torch.float32), self.q.new_empty((self.n, self.d)), self.q.new_empty((self.v, self.d))
+        db = None if self.b is None else self.q.new_empty(self.v, dtype=torch.float32)
+        native.check(self.lib.hwer_catalogue_ce_grads(*self.operands(), P(loss), P(dq), self.d, P(de), self.d, P(db), P(ws), nbytes, _stream(self.q)),
+                     "catalogue_cross_entropy_grads")
+        return (loss, dq, de) if db is None else (loss, dq, de, db)
 
 
 class _CatalogueCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, queries, table, bias, targets, scale, reduction):
         call = _CeCall(queries, table, targets, scale, bias, reduction)
-        with native.device_guard(call.dev):
-            loss = call.forward(ctx.needs_input_grad[0], call.workspace(bool(ctx.needs_input_grad[0])))
+        with call.on():
+            loss = call.forward(bool(ctx.needs_input_grad[0]))
         ctx.save_for_backward(queries, table, bias, targets, call.state, call.counted, call.mean)
         ctx.args = (scale, reduction)
         return loss
@@ -266,8 +303,8 @@ class _CatalogueCrossEntropy(torch.autograd.Function):
         call = _CeCall(queries, table, targets, ctx.args[0], bias, ctx.args[1])
         call.state, call.counted, call.mean = state, counted, mean
         want = ctx.needs_input_grad
-        with native.device_guard(call.dev):
-            dq, de, db = call.backward(grad.float().contiguous(), want[0], want[1], want[2], call.workspace(True), 0)
+        with call.on():
+            dq, de, db = call.backward(grad.float().contiguous(), want[0], want[1], want[2])
         return dq, de, db, None, None, None
 
 
@@ -281,8 +318,8 @@ def catalogue_cross_entropy(queries, table, targets, scale: float = 1.0, bias: O
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (queries, table, bias)):
         return _CatalogueCrossEntropy.apply(queries, table, bias, targets, scale, reduction)
     call = _CeCall(queries, table, targets, scale, bias, reduction)
-    with native.device_guard(call.dev):
-        return call.forward(False, call.workspace(False))
+    with call.on():
+        return call.forward(False)
 
 
 def catalogue_cross_entropy_grads(queries, table, targets, scale: float = 1.0, bias: Optional[torch.Tensor] = None, reduction: str = "mean"):
@@ -291,8 +328,5 @@ def catalogue_cross_entropy_grads(queries, table, targets, scale: float = 1.0, b
     if reduction == "none":
         raise ValueError("reduction: \"mean\" or \"sum\" (gradients of which loss?)")
     call = _CeCall(queries, table, targets, scale, bias, reduction)
-    with native.device_guard(call.dev):
-        ws = call.workspace(True)
-        loss = call.forward(True, ws)
-        dq, de, db = call.backward(None, True, True, bias is not None, ws, 1 if call.n else 0)
-    return (loss, dq, de) if bias is None else (loss, dq, de, db)
+    with call.on():
+        return call.gradients()

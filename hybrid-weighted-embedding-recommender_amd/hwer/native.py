@@ -117,9 +117,12 @@ PROTOTYPES = {
     "hwer_catalogue_ce_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int, c_int, c_int, c_int]),
     # q, ldq, e, lde, bias, target, n, v, d, dtype, scale, reduction, loss_rows, state, loss, counted, mean, workspace, workspace_bytes, stream
     "hwer_catalogue_ce": (c_int, [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int, c_int, c_float, c_int, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
-    # q, ldq, e, lde, bias, target, n, v, d, dtype, scale, reduction, grad, state, counted, mean, dq, lddq, de, ldde, dbias, operands_ready, workspace, bytes, stream
+    # q, ldq, e, lde, bias, target, n, v, d, dtype, scale, reduction, grad, state, counted, mean, dq, lddq, de, ldde, dbias, workspace, bytes, stream
     "hwer_catalogue_ce_backward": (c_int, [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int, c_int, c_float, c_int, _P, _P, _P, _P, _P, c_int64, _P, c_int64,
-                                           _P, c_int, _P, c_size_t, _P]),
+                                           _P, _P, c_size_t, _P]),
+    # q, ldq, e, lde, bias, target, n, v, d, dtype, scale, reduction, loss, dq, lddq, de, ldde, dbias, workspace, workspace_bytes, stream
+    "hwer_catalogue_ce_grads": (c_int, [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int, c_int, c_float, c_int, _P, _P, c_int64, _P, c_int64, _P, _P, c_size_t,
+                                        _P]),
     "hwer_merge_topk_lists": (c_int, [_P, _P, _P, c_int64, c_int, c_int64, c_int, c_int, c_int, _P, _P, _P, _P, _P]),
 }
 

@@ -562,7 +562,8 @@ int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int
  *   loss_rows (n), state (n, 4; 16-byte aligned: what the backward call needs of every row), loss (1, reduction 1 / 2), counted (1, the number of counted rows); mean (n, d) float32, nullable: the mean of a row's classes but its target under their probabilities, which the backward call needs for dq.
  * Backward: grad = upstream gradient of the reduced loss (one value, nullable = 1) or of each row (reduction 0).  dq, de, dbias nullable; dbias
  *   comes with de.  dq / de in the rows' type.  Every sum has a fixed order (no atomics).
- *   operands_ready: the workspace is the one of the forward call for the same operands (made with want_gradients = 1), untouched since.
+ * hwer_catalogue_ce_grads: loss (reduction 1 / 2) and gradients in one call, without what the two calls hand over; float32 rows are laid out for the
+ *   matrix instructions once.
  * Workspace: hwer_catalogue_ce_workspace_bytes(..., q_in_place, e_in_place = hwer_catalogue_ce_reads_in_place(rows, ld, d, dtype), ...). */
 int hwer_catalogue_ce_max_dim(void);
 int hwer_catalogue_ce_reads_in_place(const void* rows, int64_t ld, int d, int dtype);
@@ -573,7 +574,10 @@ int hwer_catalogue_ce(const void* q, int64_t ldq, const void* e, int64_t lde, co
 int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias /*nullable*/, const int64_t* target, int64_t n,
                                int64_t v, int d, int dtype, float scale, int reduction, const float* grad, const float* state, const float* counted,
                                const float* mean, void* dq /*nullable*/, int64_t lddq, void* de /*nullable*/, int64_t ldde, float* dbias /*nullable*/,
-                               int operands_ready, void* workspace, size_t workspace_bytes, void* stream);
+                               void* workspace, size_t workspace_bytes, void* stream);
+int hwer_catalogue_ce_grads(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias /*nullable*/, const int64_t* target, int64_t n, int64_t v,
+                            int d, int dtype, float scale, int reduction, float* loss, void* dq, int64_t lddq, void* de, int64_t ldde,
+                            float* dbias /*nullable*/, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

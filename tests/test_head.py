@@ -67,8 +67,10 @@ def test_c_entries_refuse_before_any_launch():
         assert ce(**bad) == E, bad
     assert ce(ws=None) == W and ce(nb=16) == W
     cb = lambda grad=p, red=1, mean=p, dq=p, de=p, ldde=8, bias=None, db=None, nb=big: lib.hwer_catalogue_ce_backward(  # noqa: E731
-        p, 8, p, 8, bias, p, 2, 3, 8, 0, 1.0, red, grad, p, p, mean, dq, 8, de, ldde, db, 0, p, nb, None)
+        p, 8, p, 8, bias, p, 2, 3, 8, 0, 1.0, red, grad, p, p, mean, dq, 8, de, ldde, db, p, nb, None)
     assert cb(red=0, grad=None) == E and cb(mean=None) == E and cb(ldde=7) == E and cb(db=p) == E and cb(bias=p, db=p, de=None) == E and cb(red=7) == E and cb(nb=64) == W
+    cg = lambda red=1, loss=p, dq=p, de=p, ldde=8, bias=None, db=None, ws=p: lib.hwer_catalogue_ce_grads(p, 8, p, 8, bias, p, 2, 3, 8, 0, 1.0, red, loss, dq, 8, de, ldde, db, ws, big, None)  # noqa: E731,E501
+    assert cg(red=0) == E and cg(loss=None) == E and cg(dq=None) == E and cg(de=None) == E and cg(ldde=7) == E and cg(db=p) == E and cg(ws=None) == W
     assert lib.hwer_catalogue_ce_workspace_bytes(1, 1, 300, 0, 0, 0, 1) == 0 and lib.hwer_catalogue_ce_workspace_bytes(0, 1, 8, 0, 0, 0, 1) > 0
 
 
@@ -595,7 +597,8 @@ def test_the_operators_together(hw):
     Y, _ = norm_reference(H, W, 1e-6)
     ref = torch.nn.functional.cross_entropy(0.2 * Y @ T.t(), t)
     ref.backward()
-    assert abs(float(loss) - float(ref)) <= 1e-5 * float(ref)
+    ref = float(ref.detach())
+    assert abs(float(loss) - ref) <= 1e-5 * ref
     for got, want in ((dx, X.grad), (dw, W.grad), (dtable, T.grad)):
         assert float((got.cpu().double() - want).norm()) <= 1e-5 * float(want.norm())
     # two factors in 8 bits: half a step of max / 127 each, in every one of the d products
