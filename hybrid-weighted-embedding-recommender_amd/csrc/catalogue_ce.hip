@@ -69,7 +69,7 @@ struct CePass {
     const float* bias;           // per catalogue row
     float scale;
     const CeScalars* sc;
-    int tiles_per_split, n_splits, stat_blocks;
+    int subs_per_split, n_splits, stat_blocks;      // a split takes so many times 32 streaming rows
     float *m, *l, *o;            // pass 1: (split, n_stat) maxima and sums, (split, n_stat, DP) weighted sums; pass 2: l, o likewise when split
     const int64_t* target;       // per query its target
     int* counts;                 // pass 1: counted rows of each 32 queries
@@ -77,7 +77,8 @@ struct CePass {
     float* loss;
     int reduction;
     float* zt;                   // pass 1: per query its target's logit, in the unit of m
-    const float4* rowp;          // pass 2: per query {what is taken off its logits, factor of its weights, its target's weight, target (int bits) or -1}
+    const float* rowp;           // pass 2: four arrays of ld_rowp, per query: what is taken off its logits, factor of its weights, its target's weight, its
+    int64_t ld_rowp;             // target (int bits) or -1; rows n_strm .. ld_rowp - 1 have weights of zero
     void* out;                   // pass 2, one split: de in the rows' type, and db
     float* out_b;
     int64_t ld_out;
@@ -86,12 +87,23 @@ struct CePass {
 
 enum { kLse = 0, kMean = 1, kTable = 2 };
 
-// streaming rows per LDS tile: 16 - 32 KB a buffer
-template <int TERMS, int DP> constexpr int ce_sub() { return TERMS * DP <= 64 ? 4 : TERMS * DP <= 256 ? 2 : 1; }
+// times 32 streaming rows in an LDS tile: 8 - 32 KB, so that two workgroups (rows of 256: one) fit a CU with four tiles each
+template <int TERMS, int DP> constexpr int ce_sub() { return TERMS * DP <= 128 || (TERMS == 1 && DP == 256) ? 2 : 1; }
 
-// LDS image: rows of DP / 8 chunks of 16 bytes, chunk c of row r at c ^ f(r).  Eight consecutive rows have eight different f, so the fragment reads
-// (8 rows, one chunk) and the transposed reads (4 rows, two neighbouring chunks) both touch every bank once.
-__device__ __forceinline__ int ce_swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+// Waves of a SIMD that registers are shared out for.  An MFMA occupies its own wave for all its passes, so a wave never overlaps its products with its
+// exponentials: only another wave's do.  Rows of 256 need all registers of a SIMD for one wave (128 accumulators, 64 or 128 of stationary rows).
+// Tried at 4 096 x 1.25 M x 128 bfloat16: two groups of 4 waves a CU held one phase apart by barriers 4.85 ms, against 5.00 ms of waves that run freely; the
+// larger workgroups cost 10 - 25 % at every smaller size, so waves run freely.
+template <int TERMS, int DP> constexpr int ce_waves() { return DP == 256 ? 1 : 2; }
+
+// LDS image: rows of DP / 8 chunks of 16 bytes, chunk c of row r at c ^ ce_swz(r).  The banks serve 256 bytes a cycle: 16 lanes of a fragment read (16 rows,
+// one chunk) or 32 of a transposed read (4 rows, four neighbouring chunks).  With this image either touches 16 different 16-byte slots; a swizzle of
+// 8 rows, enough for 128 bytes a cycle, spent half of the LDS cycles on conflicts.
+template <int DP>
+__device__ __forceinline__ int ce_swz(int r) {
+    if constexpr (DP == 64) return ((r & 2) << 1) | ((r >> 2) & 3);      // two rows to 256 bytes
+    else return ((r & 3) << 2) | ((r >> 2) & 3);
+}
 
 // WT: 16-bit terms of a weight.  Two for float32 rows; and where a sum has few terms (kFewTerms), whose roundings do not average out: with four queries
 // one rounding of each target's weight is the error of its class's whole gradient (1.6 times the plain form's, measured).
@@ -122,20 +134,30 @@ __device__ __forceinline__ void ce_reduce_loss(const float* loss_rows, const int
     }
 }
 
+// f(0 .. N - 1) with compile-time numbers
+template <int I, int N, class F>
+__device__ __forceinline__ void ce_static_for(F f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>());
+        ce_static_for<I + 1, N>(f);
+    }
+}
+
 template <typename E, int TERMS, int WT, int DP, int MODE, bool BIAS, bool ROWG>
-__global__ __launch_bounds__(256, (TERMS * DP > 256 ? 1 : 2)) void ce_pass_kernel(CePass a) {
+__global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(CePass a) {
     typedef CeType<E> X;
+    constexpr int WAVES = 4;
     constexpr int KC = DP / 16, DB = DP / 32, SB = ce_sub<TERMS, DP>(), TS = 32 * SB, ROWB = DP * 2, PLANE = TS * ROWB;
+    // Tiles in LDS: the last one, whose last 32 rows the second product still reads, the one at work, the next,
+    // and the one after that: a tile is fetched while two are worked on.
+    constexpr int RING = 4;
     // The factor carries a query's own upstream gradient, and the part of its lse that float32 cannot hold beside |lse| ~ 40 (2^-19 of a weight):
     // of no account in 16-bit gradients, so plain 16-bit passes save the multiplication.
     constexpr bool MUL = MODE == kTable && (ROWG || BIAS || TERMS == 2);
     constexpr float OFF = X::offset[MODE == kTable];
-    __shared__ __align__(16) char s_tile[2][TERMS][PLANE];
-    __shared__ float s_x[2][TS];                          // pass 1: bias; pass 2: what is taken off the query's logits
-    __shared__ float s_mul[MUL ? 2 : 1][MUL ? TS : 1];    // pass 2: ... factor of its weights
-    __shared__ float s_hot[2][MODE == kTable ? TS : 1];   // ... its target's weight
-    __shared__ int s_tgt[2][MODE == kTable ? TS : 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l31 = lane & 31;
+    __shared__ __align__(16) char s_tile[RING][TERMS][PLANE];
+    __shared__ __align__(16) float s_par[RING][MODE == kTable ? 4 : 1][TS];      // pass 1: bias; pass 2: CePass::rowp
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l31 = lane & 31;
     if constexpr (MODE == kTable) {
         if (blockIdx.x + 1 == gridDim.x && a.loss) return ce_reduce_loss<256>(a.loss_rows, a.target, a.n_strm, a.reduction, a.loss, nullptr);
     }
@@ -144,7 +166,7 @@ __global__ __launch_bounds__(256, (TERMS * DP > 256 ? 1 : 2)) void ce_pass_kerne
     const int id = int(blockIdx.x & 7) * per + int(blockIdx.x >> 3);
     if (int(blockIdx.x >> 3) >= per || id >= total) return;
     const int split = id / a.stat_blocks, sblock = id % a.stat_blocks;
-    const int64_t row0 = int64_t(sblock) * 128 + wave * 32, my = row0 + l31;
+    const int64_t row0 = int64_t(sblock) * (32 * WAVES) + wave * 32, my = row0 + l31;
     const int64_t myc = my < a.n_stat ? my : a.n_stat - 1;
 
     s16x8 xf[TERMS][KC];
@@ -157,210 +179,306 @@ __global__ __launch_bounds__(256, (TERMS * DP > 256 ? 1 : 2)) void ce_pass_kerne
     for (int i = 0; i < (MODE == kLse ? 1 : DB); ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-    const float scl = TERMS == 2 ? a.scale * a.sc->unscale_s : a.scale, c = fmaxf(scl * kLog2e, 1.2e-38f);      // (never 0: 0 * -inf)
+    const float scl = fmaxf(TERMS == 2 ? a.scale * a.sc->unscale_s : a.scale, 1.2e-38f), c = fmaxf(scl * kLog2e, 1.2e-38f);      // (never 0: 0 * -inf)
     const float thr = BIAS ? kStale * kLn2 : kStale / c;
     float m = kLowest, renew = kLowest, l = 0.f;
     const int64_t target = MODE != kTable && my < a.n_stat ? a.target[my] : -1;
     if (MODE != kTable && split == 0) {      // (-1 once per row: both halves of a wave hold the same rows)
         const int cnt = __builtin_popcountll(__ballot(half == 0 && target != -1));
-        if (lane == 0) a.counts[4 * sblock + wave] = cnt;
+        if (lane == 0) a.counts[WAVES * sblock + wave] = cnt;
     }
     float zt = 0.f;
     bool has_zt = false;
     const float my_bias = (BIAS && MODE == kTable) ? a.bias[myc] : 0.f;
 
-    const int n_tiles = int((a.n_strm + TS - 1) / TS);
-    const int tile0 = split * a.tiles_per_split, tile1 = min(n_tiles, tile0 + a.tiles_per_split);
-    auto stage = [&](int tile, int buf) {
-        constexpr int RPI = 1024 / ROWB, PER_WAVE = PLANE / 4096;      // rows per DMA instruction (1 KB); instructions of a wave and term
+    // this split's streaming rows: `subs` times 32 from strm0 on, in tiles of SB times 32
+    const int64_t strm0 = int64_t(split) * a.subs_per_split * 32;
+    const int subs = int(max(int64_t(0), min(int64_t(a.subs_per_split), (a.n_strm - strm0 + 31) / 32))), tiles = (subs + SB - 1) / SB;
+    constexpr int RPI = 1024 / ROWB, PER_WAVE = PLANE / (1024 * WAVES);      // rows of a DMA instruction (1 KB); instructions of a wave, tile and term
+    uint32_t piece_at[PER_WAVE];      // byte of this lane's 16 in a tile's memory
 #pragma unroll
-        for (int t = 0; t < TERMS; ++t)
+    for (int i = 0; i < PER_WAVE; ++i) {
+        const int r = (wave * PER_WAVE + i) * RPI + lane / (ROWB / 16);
+        piece_at[i] = uint32_t(r) * uint32_t(a.ld_strm * 2) + 16 * ((lane % (ROWB / 16)) ^ ce_swz<DP>(r));
+    }
+    auto fetch = [&](int tile, int slot) __attribute__((always_inline)) {
+        const int64_t first_row = strm0 + int64_t(tile) * TS;
+        const bool whole = first_row + TS <= a.n_strm;
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+            const short* base = (t ? a.strm_lo : a.strm) + first_row * a.ld_strm;
 #pragma unroll
             for (int i = 0; i < PER_WAVE; ++i) {
-                const int piece = wave * PER_WAVE + i, r = piece * RPI + lane / (ROWB / 16), ch = (lane % (ROWB / 16)) ^ ce_swz(r);
-                const int64_t g = min(int64_t(tile) * TS + r, a.n_strm - 1);      // rows past the end repeat the last one; their weights are zero
-                lds_dma16_v((t ? a.strm_lo : a.strm) + g * a.ld_strm + 8 * ch, __builtin_amdgcn_readfirstlane(lds_addr(&s_tile[buf][t][piece * 1024])));
-            }
-    };
-    float4 next_row = {0.f, 0.f, 0.f, 0.f};
-    auto fetch_params = [&](int tile) {
-        const int64_t g = int64_t(tile) * TS + threadIdx.x;
-        if (int(threadIdx.x) < TS) {
-            if (MODE == kTable) {
-                next_row = g < a.n_strm ? a.rowp[g] : float4{INFINITY, 0.f, 0.f, __int_as_float(-1)};
-            } else if (BIAS) {
-                next_row.x = g < a.n_strm ? a.bias[g] : kLowest;
+                const int piece = wave * PER_WAVE + i;
+                const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(&s_tile[slot][t][piece * 1024]));
+                if (whole) {
+                    lds_dma16(base, piece_at[i], to);
+                } else {      // rows past the end repeat the last one; their weights are zero
+                    const int r = piece * RPI + lane / (ROWB / 16), in = int(min(int64_t(r), a.n_strm - 1 - first_row));
+                    lds_dma16_v(base + int64_t(in) * a.ld_strm + 8 * ((lane % (ROWB / 16)) ^ ce_swz<DP>(r)), to);
+                }
             }
         }
     };
-    auto put_params = [&](int buf) {
-        if (int(threadIdx.x) < TS) {
-            if (MODE == kTable || BIAS) s_x[buf][threadIdx.x] = next_row.x;
-            if (MUL) s_mul[buf][threadIdx.x] = next_row.y;
-            if (MODE == kTable) {
-                s_hot[buf][threadIdx.x] = next_row.z;
-                s_tgt[buf][threadIdx.x] = __float_as_int(next_row.w);
-            }
-        }
-    };
-    if (tile0 < tile1) {
-        stage(tile0, 0);
-        fetch_params(tile0);
-        put_params(0);
-    }
-    // lane-constant parts of the LDS addresses (bytes)
-    int fr_off[4], tr_off[2];
+    // ... and the rows' parameters: wave i of the first four brings array i
+    auto fetch_params = [&](int tile, int slot) __attribute__((always_inline)) {
+        if (MODE == kTable ? wave < 4 : (BIAS && wave == 0)) {
+            const int64_t first_row = strm0 + int64_t(tile) * TS;
+            if (TS >= 64 || lane < TS) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) fr_off[k] = l31 * ROWB + 16 * ((2 * k + half) ^ ce_swz(l31));
+                for (int i = 0; i < (TS + 63) / 64; ++i) {
+                    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(&s_par[slot][MODE == kTable ? wave : 0][i * 64]));
+                    // (a bias is the caller's: rows past the end repeat the last one)
+                    if (MODE == kTable) lds_dma4(a.rowp + wave * a.ld_rowp + first_row, uint32_t(i * 64 + lane) * 4, to);
+                    else lds_dma4(a.bias + first_row, uint32_t(min(int64_t(i * 64 + lane), a.n_strm - 1 - first_row)) * 4, to);
+                }
+            }
+        }
+    };
+    // This wave's share of tile `tile`, and of its parameters, has arrived (before a barrier: everyone's has).  What was fetched after it, the next tile's rows,
+    // may be under way.
+    auto arrived = [&](int tile) __attribute__((always_inline)) {
+        if (tile + 1 < tiles) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TERMS * PER_WAVE) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
+    if (tiles) {
+        __builtin_amdgcn_s_waitcnt(0);      // (nothing of the above is counted below)
+        fetch_params(0, 0);
+        fetch(0, 0);
+        if (tiles > 1) fetch(1, 1);
+        arrived(0);
+    }
+    __syncthreads();
+
+    // LDS addresses of this lane's pieces of the next fragments (bytes; they move on with the tiles), the rest of an address is a constant
+    constexpr int SWZ = DP == 64 ? 8 : 16;      // chunks that are exchanged among each other
+    constexpr int SLOT = TERMS * PLANE;
+    // Chunk 2 k + half, or 4 k + cl, of a lane's row is at the address of k = 0 with 32 k, or 64 k, exclusive-or'd in; held for each k where registers allow.
+    constexpr bool HELD = DP < 256;
+    uint32_t fr_at[HELD ? SWZ / 2 : 1], tr_at[HELD ? SWZ / 4 : 1];
+    fr_at[0] = lds_addr(s_tile) + l31 * ROWB + 16 * (half ^ ce_swz<DP>(l31));
     {
         const int r = 4 * half + ((lane & 15) >> 2), cl = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) tr_off[k] = r * ROWB + 16 * ((4 * k + cl) ^ ce_swz(r)) + 8 * (lane & 1);
+        tr_at[0] = lds_addr(s_tile) + r * ROWB + 8 * (lane & 1) + 16 * (cl ^ ce_swz<DP>(r));
     }
-    for (int tile = tile0; tile < tile1; ++tile) {
-        const int buf = (tile - tile0) & 1;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();      // this tile is staged, and everyone is done with the other buffer
-        if (tile + 1 < tile1) {
-            stage(tile + 1, buf ^ 1);
-            fetch_params(tile + 1);
-        }
-        const int64_t from_tile = target - int64_t(tile) * TS;
-        const int my_target = MODE != kTable && from_tile >= 0 && from_tile < TS ? int(from_tile) : -1;
-        bool hit = false;      // does any of the tile's queries have its target among this wave's rows?
-        if (MODE == kTable) {
-            bool h = false;
 #pragma unroll
-            for (int i = 0; i < (TS + 63) / 64; ++i) {
-                const int t = (TS >= 64 || lane < TS) ? s_tgt[buf][i * 64 + (lane & (TS - 1 < 63 ? TS - 1 : 63))] : -1;
-                h = h || (t >= row0 && t < row0 + 32);
-            }
-            hit = __any(h);
-        }
+    for (int k = 1; k < (HELD ? SWZ / 2 : 1); ++k) fr_at[k] = fr_at[0] ^ (32 * k);
 #pragma unroll
-        for (int sb = 0; sb < SB; ++sb) {
-            f32x16 s;
+    for (int k = 1; k < (HELD ? SWZ / 4 : 1); ++k) tr_at[k] = tr_at[0] ^ (64 * k);
+
+    f32x16 s;
+    s16x8 ph[2], pl[2];      // weights of the last 32 streaming rows, as the second product's operand
+    // A product phase is N2 + N1 steps, each with a fragment (two with two terms) from LDS: the second product of 32 rows (O^T += rows^T . weights), then the
+    // first of the next 32 (S^T = rows . stationary^T).  Fragments are read DEPTH steps ahead, the first of them before the phase begins.
+    constexpr int N2 = MODE == kLse ? 0 : 2 * DB, N1 = KC, DEPTH = TERMS * DP >= 256 ? 4 : 8, PRE = N2 < 2 ? N2 : 2;
+    s16x8 ring[DEPTH][TERMS];
+    typedef const __attribute__((address_space(3))) s16x8* lds8_t;
+    typedef __attribute__((address_space(3))) s16x4* lds4_t;
+    auto read = [&](auto u_, auto sb2_, auto sb1_) __attribute__((always_inline)) {
+        constexpr int u = decltype(u_)::value, sb2 = decltype(sb2_)::value, sb1 = decltype(sb1_)::value;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) s[j] = 0.f;
-            const char* t_hi = s_tile[buf][0] + sb * 32 * ROWB;
-            const char* t_lo = s_tile[buf][TERMS - 1] + sb * 32 * ROWB;
-#pragma unroll
-            for (int k = 0; k < KC; ++k) {
-                const s16x8 fh = *reinterpret_cast<const s16x8*>(t_hi + fr_off[k & 3] + 128 * (k >> 2));
-                s = X::mfma(fh, xf[0][k], s);
-                if constexpr (TERMS == 2) {
-                    const s16x8 fl = *reinterpret_cast<const s16x8*>(t_lo + fr_off[k & 3] + 128 * (k >> 2));
-                    s = X::mfma(fl, xf[0][k], s);
-                    s = X::mfma(fh, xf[1][k], s);
-                }
-            }
-            // register j of this lane: streaming row 8 (j / 4) + 4 half + j % 4 of the 32
-            float w[16];
-            if constexpr (MODE == kTable) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = sb * 32 + 8 * q + 4 * half + j;
-                        float v;
-                        if (BIAS) v = __builtin_amdgcn_exp2f(fmaf((fmaf(s[4 * q + j], scl, my_bias) - s_x[buf][r]), kLog2e, OFF));
-                        else v = __builtin_amdgcn_exp2f(fmaf(s[4 * q + j], c, -s_x[buf][r]));
-                        if (MUL) v *= s_mul[buf][r];
-                        w[4 * q + j] = v;
-                    }
-                if (hit) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int r = sb * 32 + 8 * q + 4 * half + j;
-                            if (s_tgt[buf][r] == int(my)) w[4 * q + j] = s_hot[buf][r];
-                        }
-                }
-                if (BIAS) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) l += w[j];
-                }
+        for (int t = 0; t < TERMS; ++t) {
+            if constexpr (u < N2) {      // 16 streaming rows x 32 columns, transposed
+                constexpr int k = u / DB, i = u % DB;
+                const uint32_t p = HELD ? tr_at[i % (SWZ / 4) * HELD] : tr_at[0] ^ (64 * (i % (SWZ / 4)));
+                const int off = t * PLANE + (sb2 * 32 + 16 * k) * ROWB + 16 * SWZ * (i / (SWZ / 4));
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds4_t>(p + off));
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds4_t>((p ^ 32) + (off + 8 * ROWB)));      // (8 rows on, the swizzle differs by 2)
+                ring[u % DEPTH][t] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
             } else {
-                if (!BIAS && tile == n_tiles - 1) {      // (with a bias, rows past the end have one of -inf)
+                constexpr int k = u - N2;
+                ring[u % DEPTH][t] = *reinterpret_cast<lds8_t>((HELD ? fr_at[k % (SWZ / 2) * HELD] : fr_at[0] ^ (32 * (k % (SWZ / 2)))) + (t * PLANE + sb1 * 32 * ROWB + 16 * SWZ * (k / (SWZ / 2))));
+            }
+        }
+    };
+    auto multiply = [&](auto u_) __attribute__((always_inline)) {
+        constexpr int u = decltype(u_)::value;
+        const s16x8 hi = ring[u % DEPTH][0], lo = ring[u % DEPTH][TERMS - 1];
+        if constexpr (u < N2) {
+            constexpr int k = u / DB, i = u % DB;
+            o[i] = X::mfma(hi, ph[k], o[i]);
+            if constexpr (TERMS == 2) o[i] = X::mfma(lo, ph[k], o[i]);
+            if constexpr (WT == 2) o[i] = X::mfma(hi, pl[k], o[i]);
+        } else {
+            constexpr int k = u - N2;
+            if constexpr (k == 0) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (int64_t(tile) * TS + sb * 32 + 8 * (j >> 2) + 4 * half + (j & 3) >= a.n_strm) s[j] = kLowest;
+                for (int j = 0; j < 16; ++j) s[j] = 0.f;
+            }
+            s = X::mfma(hi, xf[0][k], s);
+            if constexpr (TERMS == 2) {
+                s = X::mfma(lo, xf[0][k], s);
+                s = X::mfma(hi, xf[1][k], s);
+            }
+        }
+    };
+    auto steps = [&](auto from_, auto to_, auto sb2, auto sb1) __attribute__((always_inline)) {      // steps from .. to - 1, their first reads done up to `from + PRE`
+        constexpr int from = decltype(from_)::value, to = decltype(to_)::value;
+        ce_static_for<from, to>([&](auto u) __attribute__((always_inline)) {
+            multiply(u);
+            constexpr int v = decltype(u)::value + DEPTH;
+            if constexpr (v < to) read(std::integral_constant<int, v>(), sb2, sb1);
+            __builtin_amdgcn_sched_barrier(0);      // the compiler would put every read right before its use
+        });
+    };
+    // What the weights of 32 streaming rows take besides S (registers 4 q + j: row 8 q + 4 half + j of the 32), read before their phase where registers allow
+    constexpr bool HAS_X = MODE == kTable || BIAS, EARLY = HAS_X && TERMS * DP <= 256;
+    float px[HAS_X ? 16 : 1], pm[MUL ? 16 : 1];
+    auto read_params = [&](int slot, int sb) __attribute__((always_inline)) {
+        if constexpr (HAS_X) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 v = *reinterpret_cast<const float4*>(&s_par[slot][0][sb * 32 + 4 * half + 8 * q]);
+                px[4 * q] = v.x, px[4 * q + 1] = v.y, px[4 * q + 2] = v.z, px[4 * q + 3] = v.w;
+                if constexpr (MUL) {
+                    const float4 u = *reinterpret_cast<const float4*>(&s_par[slot][1][sb * 32 + 4 * half + 8 * q]);
+                    pm[4 * q] = u.x, pm[4 * q + 1] = u.y, pm[4 * q + 2] = u.z, pm[4 * q + 3] = u.w;
                 }
-                if (BIAS) {
+            }
+        }
+    };
+    // S -> weights.  row: the first of the 32; reads: the first fragment reads of the product phase, issued before the exponentials
+    float sub = BIAS ? 0.f : OFF;      // what exponents are taken against (without a maximum yet: 0)
+    auto weights = [&](int slot, int sb, int64_t row, int my_target, bool hit, auto reads) __attribute__((always_inline)) {
+        if constexpr (HAS_X && !EARLY) read_params(slot, sb);
+        float w[16];
+        if constexpr (MODE == kTable) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) s[j] = fmaf(s[j], scl, s_x[buf][sb * 32 + 8 * (j >> 2) + 4 * half + (j & 3)]);
-                }
-                const int at = my_target - sb * 32;      // the target among these 32 rows: its logit is noted, and it is left out
-                if (__any(unsigned(at) < 32u)) {
+            for (int j = 0; j < 16; ++j) w[j] = BIAS ? fmaf(fmaf(s[j], scl, my_bias) - px[j], kLog2e, OFF) : fmaf(s[j], c, -px[j]);
+            reads();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (at == 8 * (j >> 2) + 4 * half + (j & 3)) {
-                            zt = s[j];
-                            has_zt = true;
-                            s[j] = kLowest;
-                        }
-                }
-                float mx = s[0];
-#pragma unroll
-                for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
-                mx = fmaxf(mx, __uint_as_float(lane_xor32<32>(__float_as_uint(mx))));
-                if (__any(mx > renew)) {
-                    const float mn = fmaxf(m, mx);
-                    // (m = -inf: nothing so far, l and o are 0; differences first: a bias of float32's lowest value must not overflow)
-                    const float f = m == kLowest ? 1.f : __builtin_amdgcn_exp2f((m - mn) * (BIAS ? kLog2e : c));
-                    m = mn;
-                    renew = m == kLowest ? kLowest : m + thr;
-                    l *= f;
-                    if constexpr (MODE == kMean) {
-#pragma unroll
-                        for (int i = 0; i < DB; ++i)
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) o[i][j] *= f;
-                    }
-                }
-                const float mu = m == kLowest ? 0.f : m, sub = OFF - mu * c;
+            for (int j = 0; j < 16; ++j) {
+                w[j] = __builtin_amdgcn_exp2f(w[j]);
+                if constexpr (MUL) w[j] *= pm[j];
+            }
+            if (hit) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    w[j] = BIAS ? __builtin_amdgcn_exp2f(fmaf(s[j] - mu, kLog2e, OFF)) : __builtin_amdgcn_exp2f(fmaf(s[j], c, sub));
-                    l += w[j];
+                    const int r = sb * 32 + 8 * (j >> 2) + 4 * half + (j & 3);
+                    if (__float_as_int(s_par[slot][3][r]) == int(my)) w[j] = s_par[slot][2][r];
                 }
             }
-            if constexpr (MODE != kLse) {
-                s16x8 ph[2], pl[2];
+            if (BIAS) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    typename X::x8 hi, lo;
+                for (int j = 0; j < 16; ++j) l += w[j];
+            }
+        } else {
+            if (row + 32 > a.n_strm) {      // rows past the end
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        hi[j] = E(w[8 * k + j]);
-                        if (WT == 2) lo[j] = E(w[8 * k + j] - float(hi[j]));
+                for (int j = 0; j < 16; ++j)
+                    if (row + 4 * half + 8 * (j >> 2) + (j & 3) >= a.n_strm) s[j] = kLowest;
+            }
+            if (BIAS) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[j] = fmaf(s[j], scl, px[j]);
+            }
+            if (hit) {      // a target in this tile, and perhaps among these 32 rows: its logit is noted, and it is left out
+                const int at = my_target - sb * 32;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (at == 8 * (j >> 2) + 4 * half + (j & 3)) {
+                        zt = s[j];
+                        has_zt = true;
+                        s[j] = kLowest;
                     }
-                    ph[k] = __builtin_bit_cast(s16x8, hi);
-                    if (WT == 2) pl[k] = __builtin_bit_cast(s16x8, lo);
+            }
+            float mx = fmaxf(fmaxf(s[0], s[1]), s[2]);      // (pairs of them are one instruction)
+#pragma unroll
+            for (int j = 3; j < 15; j += 2) mx = fmaxf(fmaxf(mx, s[j]), s[j + 1]);
+            mx = fmaxf(mx, s[15]);
+            mx = fmaxf(mx, __uint_as_float(lane_xor32<32>(__float_as_uint(mx))));
+            if (__any(mx > renew)) {
+                const float mn = fmaxf(m, mx);
+                // (m = -inf: nothing so far, l and o are 0; differences first: a bias of float32's lowest value must not overflow)
+                const float f = m == kLowest ? 1.f : __builtin_amdgcn_exp2f((m - mn) * (BIAS ? kLog2e : c));
+                m = mn;
+                renew = m == kLowest ? kLowest : m + thr;
+                sub = m == kLowest ? (BIAS ? 0.f : OFF) : (BIAS ? m : OFF - m * c);
+                l *= f;
+                if constexpr (MODE == kMean) {
+#pragma unroll
+                    for (int i = 0; i < DB; ++i)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[i][j] *= f;
                 }
-                typedef __attribute__((address_space(3))) s16x4* lds4;
-                auto transposed = [&](const char* t, int i, int k) {      // 16 streaming rows x 32 columns, as the product's row operand
-                    const char* p = t + tr_off[i & 1] + 128 * (i >> 1) + 16 * k * ROWB;
-                    const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p));
-                    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 8 * ROWB));
-                    return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
-                };
+            }
 #pragma unroll
-                for (int i = 0; i < DB; ++i)
+            for (int j = 0; j < 16; ++j) w[j] = BIAS ? fmaf(s[j] - sub, kLog2e, OFF) : fmaf(s[j], c, sub);
+            reads();
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const s16x8 eh = transposed(t_hi, i, k);
-                        o[i] = X::mfma(eh, ph[k], o[i]);
-                        if constexpr (TERMS == 2) {
-                            const s16x8 el = transposed(t_lo, i, k);
-                            o[i] = X::mfma(el, ph[k], o[i]);
-                        }
-                        if constexpr (WT == 2) o[i] = X::mfma(eh, pl[k], o[i]);
-                    }
+            for (int j = 0; j < 16; ++j) {
+                w[j] = __builtin_amdgcn_exp2f(w[j]);
+                l += w[j];
             }
         }
-        if (tile + 1 < tile1) put_params(buf ^ 1);
+        if constexpr (MODE != kLse) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                typename X::x8 hi, lo;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    hi[j] = E(w[8 * k + j]);
+                    if (WT == 2) lo[j] = E(w[8 * k + j] - float(hi[j]));
+                }
+                ph[k] = __builtin_bit_cast(s16x8, hi);
+                if (WT == 2) pl[k] = __builtin_bit_cast(s16x8, lo);
+            }
+        }
+    };
+
+    // first(0), weights(0), second(0) first(1), weights(1), ...; one barrier a tile, before its last 32 rows' products: the next tile is there then
+    typedef std::integral_constant<int, 0> zero_t;
+    if (tiles) {
+        ce_static_for<N2, N2 + (DEPTH < N1 ? DEPTH : N1)>([&](auto u) __attribute__((always_inline)) { read(u, zero_t(), zero_t()); });
+        steps(std::integral_constant<int, N2>(), std::integral_constant<int, N2 + N1>(), zero_t(), zero_t());
+        if (EARLY) read_params(0, 0);
+    }
+    int slot = 0, at = 0;      // at: number of the 32 rows at work
+    for (int tile = 0; tile < tiles; ++tile) {
+        const int next = (slot + 1) % RING;
+        const int64_t row = strm0 + int64_t(tile) * TS, from_tile = target - row;
+        const int my_target = MODE != kTable && from_tile >= 0 && from_tile < TS ? int(from_tile) : -1;
+        bool hit = __any(my_target >= 0);
+        if (MODE == kTable) {      // does any of the tile's queries have its target among this wave's rows?
+            const int t = (TS >= 64 || lane < TS) ? __float_as_int(s_par[slot][MODE == kTable ? 3 : 0][lane & (TS - 1)]) : -1;
+            static_assert(TS <= 64, "a lane a row");
+            hit = __any(t >= row0 && t < row0 + 32);
+        }
+        ce_static_for<0, SB>([&](auto sb_) __attribute__((always_inline)) {
+            constexpr int sb = decltype(sb_)::value, sb1 = sb == SB - 1 ? 0 : sb + 1;
+            if (at >= subs) return;      // (uniform: the last tile may be shorter)
+            if (sb == 0 && tile + 1 < tiles) {      // (the slot that is filled held the tile before the last: all waves have passed the last one's barrier)
+                fetch_params(tile + 1, next);
+                if (tile + 2 < tiles) fetch(tile + 2, (slot + 2) % RING);
+            }
+            weights(slot, sb, row + sb * 32, my_target, hit, [&]() __attribute__((always_inline)) {
+                __builtin_amdgcn_sched_barrier(0);
+                ce_static_for<0, PRE>([&](auto u) __attribute__((always_inline)) { read(u, sb_, std::integral_constant<int, sb1>()); });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            if (sb == SB - 1) {
+                if (tile + 1 < tiles) arrived(tile + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_s_barrier();      // (waits for the waves only, not for memory)
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+                const int move = (next - slot) * SLOT;
+#pragma unroll
+                for (int k = 0; k < (HELD ? SWZ / 2 : 1); ++k) fr_at[k] += move;
+            }
+            // (Behind the last 32 rows the first product reads what is there, and its result is not used.)
+            ce_static_for<PRE, DEPTH>([&](auto u) __attribute__((always_inline)) { read(u, sb_, std::integral_constant<int, sb1>()); });
+            __builtin_amdgcn_s_setprio(1);
+            steps(zero_t(), std::integral_constant<int, N2 + N1>(), sb_, std::integral_constant<int, sb1>());
+            __builtin_amdgcn_s_setprio(0);
+            if constexpr (EARLY) read_params(sb == SB - 1 ? next : slot, sb1);
+            ++at;
+        });
+        const int move = (next - slot) * SLOT;
+#pragma unroll
+        for (int k = 0; k < (HELD ? SWZ / 4 : 1); ++k) tr_at[k] += move;
+        slot = next;
     }
 
     l += __uint_as_float(lane_xor32<32>(__float_as_uint(l)));
@@ -525,19 +643,22 @@ struct CeRows {
     int reduction, per_row;       // 0 none, 1 mean, 2 sum
     void* dq;
     int64_t lddq;
-    float4* rowp;
+    float* rowp;                  // CePass::rowp
+    int64_t ld_rowp;
     const int* counts;            // counted rows (partial)
     int n_counts;
     float off, off2;              // powers of two that the weights of pass 1 / 2 carry
 };
-constexpr int kMaxSplits = 1024;
+constexpr int kCUs = 256, kMaxSplits = 512;      // splits of a streaming side
 
-// What a row's state {lse, its low part, 1 - p_t} means to pass 2 (CePass::rowp); rel: its gradient relative to the largest
+// What a row's state {lse, its low part, 1 - p_t} means to pass 2 (CePass::rowp); rel: its gradient relative to the largest.  Rows from n on: weights of zero.
 template <bool BIAS>
-__device__ __forceinline__ float4 ce_rowp(bool on, float lse, float low, float miss, float rel, float off, int64_t t) {
+__device__ __forceinline__ void ce_put_rowp(const CeRows& a, int64_t r, bool on, float lse, float low, float miss, float rel, int64_t t) {
     const bool some = on && lse != kLowest;
-    return {some ? (BIAS ? lse : lse - off) : INFINITY, rel * __builtin_amdgcn_exp2f(BIAS ? -low * kLog2e : -low), -rel * miss * __builtin_amdgcn_exp2f(off),
-            __int_as_float(on ? int(t) : -1)};
+    a.rowp[r] = some ? (BIAS ? lse : lse - a.off2) : INFINITY;
+    a.rowp[a.ld_rowp + r] = on ? rel * __builtin_amdgcn_exp2f(BIAS ? -low * kLog2e : -low) : 0.f;
+    a.rowp[2 * a.ld_rowp + r] = -rel * miss * __builtin_amdgcn_exp2f(a.off2);
+    a.rowp[3 * a.ld_rowp + r] = __int_as_float(on ? int(t) : -1);
 }
 
 // Joins the splits of pass 1: loss_r, lse_r, 1 - p_t and sum_{v /= t} p'_v e_v.  TR threads a row (a wave, or 256 where there are many splits); DP / 4 of
@@ -548,7 +669,10 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
     __shared__ float4 s_o[TR > 64 ? 256 : 1];
     const int lane = threadIdx.x & 63, t_in = threadIdx.x % TR;
     const int64_t r = int64_t(blockIdx.x) * (256 / TR) + threadIdx.x / TR;
-    if (r >= a.n) return;      // (whole rows: with TR = 256 the whole workgroup)
+    if (r >= a.n) {      // (whole rows: with TR = 256 the whole workgroup)
+        if (GRADS && r < a.ld_rowp && t_in == 0) ce_put_rowp<BIAS>(a, r, false, 0.f, 0.f, 0.f, 0.f, -1);
+        return;
+    }
     const float unit = BIAS ? kLog2e : fmaxf((F32 ? a.scale * a.sc->unscale_s : a.scale) * kLog2e, 1.2e-38f);      // from the maxima's unit to powers of two (as in the pass)
     float top = kLowest;
     for (int s = t_in; s < a.n_splits; s += TR) top = fmaxf(top, a.m[int64_t(s) * a.n + r]);
@@ -605,7 +729,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
     }
     if (t_in == 0) {
         a.loss_rows[r] = float(loss);
-        if constexpr (GRADS) a.rowp[r] = ce_rowp<BIAS>(on, hi, low, float(miss), on ? 1.f : 0.f, a.off2, t);
+        if constexpr (GRADS) ce_put_rowp<BIAS>(a, r, on, hi, low, float(miss), on ? 1.f : 0.f, t);
         else a.state[r] = {hi, low, float(miss), 0.f};
     }
     if (!GRADS && !a.mean) return;
@@ -673,12 +797,15 @@ __global__ __launch_bounds__(256) void ce_dq_kernel(CeRows a) {
         a.sc->fac_e = a.scale * g * unoff * (F32 ? a.sc->unscale_q : 1.f);
         a.sc->fac_b = g * unoff;
     }
-    if (r >= a.n) return;
+    if (r >= a.n) {
+        if (a.rowp && r < a.ld_rowp && lane == 0) ce_put_rowp<BIAS>(a, r, false, 0.f, 0.f, 0.f, 0.f, -1);
+        return;
+    }
     const int64_t t = a.target[r];
     const bool on = t >= 0 && t < a.v;
     const float4 st = a.state[r];
     const float gr = a.per_row ? a.grad[r] : g;
-    if (a.rowp && lane == 0) a.rowp[r] = ce_rowp<BIAS>(on, st.x, st.y, st.z, !on ? 0.f : a.per_row ? (g > 0.f ? gr / g : gr) : 1.f, a.off2, t);
+    if (a.rowp && lane == 0) ce_put_rowp<BIAS>(a, r, on, st.x, st.y, st.z, !on ? 0.f : a.per_row ? (g > 0.f ? gr / g : gr) : 1.f, t);
     if (a.dq) {
         E* dq = static_cast<E*>(a.dq) + r * a.lddq;
         const E* e = static_cast<const E*>(a.e) + (on ? t : 0) * a.lde;
@@ -721,21 +848,31 @@ __global__ __launch_bounds__(256) void ce_de_kernel(const float* __restrict__ o,
 static int ce_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 static bool ce_direct(const void* p, int64_t ld, int d, int dtype) {
-    return dtype != HWER_F32 && d == ce_padded(d) && aligned_to(p, ld * 2, 16);
+    return dtype != HWER_F32 && d == ce_padded(d) && aligned_to(p, ld * 2, 16) && ld < (1 << 23);      // (a tile's bytes are addressed in 32 bits)
 }
 
-// Splits of the streaming side: enough workgroups for every CU to hold its share (two, or one of the widest float32 rows), whole tiles each.
+// Splits of the streaming side, in 32s of its rows.  A call takes as long as its fullest CU (which holds two workgroups, or one of the widest rows): rounds of
+// workgroups times (a split's 32s + about 4 for its start and end); and each split leaves sums behind that are written and read again, about 2 MB in the
+// time of 32 rows.
 struct CeSplit {
-    int blocks, splits, tiles_per_split;
+    int blocks, splits, subs;
 };
-static CeSplit ce_split(int64_t n_stat, int64_t n_strm, int d, int dtype) {
-    const int terms = dtype == HWER_F32 ? 2 : 1, dp = ce_padded(d), w = terms * dp;
-    const int ts = 32 * (w <= 64 ? 4 : w <= 256 ? 2 : 1), target = w > 256 ? 256 : 512;      // target <= kMaxSplits
-    const int64_t blocks = cdiv64(n_stat, 128), tiles = cdiv64(n_strm, ts);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(tiles, target / std::max<int64_t>(blocks, 1)));
-    const int64_t per = std::max<int64_t>(1, cdiv64(tiles, want));
-    return {int(blocks), int(std::max<int64_t>(1, cdiv64(tiles, per))), int(per)};
+constexpr int kRows = 128;      // stationary rows of a workgroup
+static CeSplit ce_split(int64_t n_stat, int64_t n_strm, int d) {
+    const int dp = ce_padded(d);
+    const int64_t blocks = cdiv64(n_stat, kRows), subs = std::max<int64_t>(1, cdiv64(n_strm, 32)), slots = (dp == 256 ? 1 : 2) * kCUs;
+    double best = INFINITY;
+    int64_t per = subs;
+    for (int64_t s = 1; s <= std::min<int64_t>(subs, kMaxSplits) && (s == 1 || blocks * s <= 8 * slots); ++s) {
+        const int64_t p = cdiv64(subs, s), n = cdiv64(subs, p);
+        const double cost = double(cdiv64(blocks * n, slots) * (p + 4)) + (n > 1 ? double(blocks * kRows * dp * 8) * double(n) / 2e6 : 0.0);
+        if (cost < best) best = cost, per = p;
+    }
+    return {int(blocks), int(cdiv64(subs, per)), int(per)};
 }
+
+// queries with parameters for pass 2, whole tiles of at most 128 from any 32nd query on
+static int64_t ce_rowp_ld(int64_t n) { return cdiv64(n, 32) * 32 + 128; }
 
 static size_t up(size_t b) { return (b + 255) & ~size_t(255); }
 
@@ -746,7 +883,7 @@ struct CeLayout {
 static CeLayout ce_layout(int64_t n, int64_t v, int d, int dtype, bool q_direct, bool e_direct, bool want_mean) {
     const size_t dp = ce_padded(d);
     CeLayout y{};
-    const CeSplit f = ce_split(n, v, d, dtype), b = ce_split(v, n, d, dtype);
+    const CeSplit f = ce_split(n, v, d), b = ce_split(v, n, d);
     size_t at = 256;      // CeScalars
     y.tops = at, at += dtype == HWER_F32 ? 2 * kTopBlocks * 4 : 0;
     y.q_hi = at, at += q_direct ? 0 : up(size_t(n) * dp * 2);
@@ -755,7 +892,7 @@ static CeLayout ce_layout(int64_t n, int64_t v, int d, int dtype, bool q_direct,
     y.e_lo = at, at += dtype == HWER_F32 ? up(size_t(v) * dp * 2) : 0;
     y.counts = at, at += up(size_t(f.blocks) * 16);
     y.loss_rows = at, at += want_mean ? up(size_t(n) * 4) : 0;
-    y.rowp = at, at += want_mean ? up(size_t(n) * 16) : 0;
+    y.rowp = at, at += want_mean ? up(size_t(ce_rowp_ld(n)) * 16) : 0;
     y.head = at;
     y.zt = at, at += up(size_t(n) * 4);
     y.m = at, at += up(size_t(f.splits) * n * 4);
@@ -827,12 +964,12 @@ struct CeCall {
     }
 
     int pass1(bool mean, CeRows& r) const {
-        const CeSplit s = ce_split(n, v, d, dtype);
+        const CeSplit s = ce_split(n, v, d);
         CePass p{};
         p.stat = q_hi(), p.stat_lo = q_lo(), p.strm = e_hi(), p.strm_lo = e_lo();
         p.ld_stat = q_ld(), p.ld_strm = e_ld(), p.n_stat = n, p.n_strm = v;
         p.bias = bias, p.scale = scale, p.sc = at<CeScalars>(0);
-        p.tiles_per_split = s.tiles_per_split, p.n_splits = s.splits, p.stat_blocks = s.blocks;
+        p.subs_per_split = s.subs, p.n_splits = s.splits, p.stat_blocks = s.blocks;
         p.m = at<float>(y.m), p.l = at<float>(y.l), p.o = at<float>(y.o);
         p.target = target, p.zt = at<float>(y.zt), p.counts = at<int>(y.counts), p.d = d;
         mean ? ce_pass_any<kMean>(p, dp, dtype, false, st) : ce_pass_any<kLse>(p, dp, dtype, false, st);
@@ -844,19 +981,19 @@ struct CeCall {
     CeRows rows() const {
         CeRows r{};
         r.e = e, r.lde = lde, r.bias = bias, r.target = target, r.n = n, r.v = v, r.d = d, r.dp = dp, r.scale = scale, r.sc = at<CeScalars>(0);
-        r.reduction = reduction, r.off = ce_offset(dtype, 0), r.off2 = ce_offset(dtype, 1);
+        r.reduction = reduction, r.ld_rowp = ce_rowp_ld(n), r.off = ce_offset(dtype, 0), r.off2 = ce_offset(dtype, 1);
         return r;
     }
 
     int pass2(void* de, int64_t ldde, float* dbias, bool rowg, const float* loss_rows, float* loss) const {
-        const CeSplit s = ce_split(v, n, d, dtype);
+        const CeSplit s = ce_split(v, n, d);
         CePass p{};
         p.stat = e_hi(), p.stat_lo = e_lo(), p.strm = q_hi(), p.strm_lo = q_lo();
         p.ld_stat = e_ld(), p.ld_strm = q_ld(), p.n_stat = v, p.n_strm = n;
         p.bias = bias, p.scale = scale, p.sc = at<CeScalars>(0);
-        p.tiles_per_split = s.tiles_per_split, p.n_splits = s.splits, p.stat_blocks = s.blocks;
+        p.subs_per_split = s.subs, p.n_splits = s.splits, p.stat_blocks = s.blocks;
         p.l = at<float>(y.l2), p.o = at<float>(y.o2);
-        p.rowp = at<float4>(y.rowp), p.out = de, p.out_b = dbias, p.ld_out = ldde, p.d = d;
+        p.rowp = at<float>(y.rowp), p.ld_rowp = ce_rowp_ld(n), p.out = de, p.out_b = dbias, p.ld_out = ldde, p.d = d;
         p.out_vec = d % 4 == 0 && aligned_to(de, ldde * dtype_bytes(dtype), 4 * dtype_bytes(dtype));
         p.target = target, p.loss_rows = loss_rows, p.loss = loss, p.reduction = reduction;
         ce_pass_any<kTable>(p, dp, dtype, rowg, st);
@@ -909,13 +1046,14 @@ struct CeCall {
     void join_typed(const CeRows& r) const {
         // a wave per row walks over a few splits in less than a microsecond; hundreds of them (few rows, long catalogue) took 230 us at 466
         const bool wave = r.n_splits <= 16;
-        const dim3 grid(unsigned(wave ? cdiv64(n, 4) : n)), block(256);
+        const int64_t rows = GRADS ? ce_rowp_ld(n) : n;
+        const dim3 grid(unsigned(wave ? cdiv64(rows, 4) : rows)), block(256);
         if (bias) wave ? ce_rows_kernel<E, F32, true, 64, GRADS><<<grid, block, 0, st>>>(r) : ce_rows_kernel<E, F32, true, 256, GRADS><<<grid, block, 0, st>>>(r);
         else wave ? ce_rows_kernel<E, F32, false, 64, GRADS><<<grid, block, 0, st>>>(r) : ce_rows_kernel<E, F32, false, 256, GRADS><<<grid, block, 0, st>>>(r);
     }
     template <typename E, bool F32>
     void dq_typed(const CeRows& r) const {
-        const dim3 grid(unsigned(std::max<int64_t>(1, cdiv64(n, 4)))), block(256);      // (without rows it leaves the factors of zeros)
+        const dim3 grid(unsigned(cdiv64(ce_rowp_ld(n), 4))), block(256);      // (without rows it leaves the factors of zeros)
         bias ? ce_dq_kernel<E, F32, true><<<grid, block, 0, st>>>(r) : ce_dq_kernel<E, F32, false><<<grid, block, 0, st>>>(r);
     }
     int backward_rows(const CeRows& r) const {
@@ -973,7 +1111,7 @@ int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_
         if (int rc = c.prepare()) return rc;
     CeRows r = c.rows();
     r.state = reinterpret_cast<float4*>(const_cast<float*>(state)), r.mean = const_cast<float*>(mean), r.counted = counted, r.grad = grad, r.per_row = reduction == 0;
-    r.dq = dq, r.lddq = lddq, r.rowp = de ? c.at<float4>(c.y.rowp) : nullptr;
+    r.dq = dq, r.lddq = lddq, r.rowp = de ? c.at<float>(c.y.rowp) : nullptr;
     if (reduction == 0) ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(grad, n, r.sc);
     if (int rc = c.backward_rows(r)) return rc;
     return de ? c.pass2(de, ldde, dbias, reduction == 0, nullptr, nullptr) : HWER_OK;
@@ -992,7 +1130,7 @@ int hwer_catalogue_ce_grads(const void* q, int64_t ldq, const void* e, int64_t l
     CeRows r = c.rows();
     if (n) {
         if (int rc = c.pass1(true, r)) return rc;
-        r.loss_rows = loss_rows, r.dq = dq, r.lddq = lddq, r.rowp = c.at<float4>(c.y.rowp);
+        r.loss_rows = loss_rows, r.dq = dq, r.lddq = lddq, r.rowp = c.at<float>(c.y.rowp);
         if (int rc = c.join<true>(r)) return rc;
     } else {
         r.per_row = 1, r.grad = loss_rows;      // no rows: the factors of a sum over nothing
