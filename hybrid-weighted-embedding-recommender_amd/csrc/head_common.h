@@ -28,6 +28,30 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 template <int T>
+__device__ __forceinline__ uint32_t lanes_max_u32(uint32_t v) {
+    v = max(v, lane_xor32<1>(v));
+    v = max(v, lane_xor32<2>(v));
+    v = max(v, lane_xor32<4>(v));
+    v = max(v, lane_xor32<8>(v));
+    if constexpr (T > 16) {
+        v = max(v, lane_xor32<16>(v));
+        v = max(v, lane_xor32<32>(v));
+    }
+    return v;
+}
+template <int T>
+__device__ __forceinline__ float lanes_max_f32(float v) {
+    v = fmaxf(v, __uint_as_float(lane_xor32<1>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(lane_xor32<2>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(lane_xor32<4>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(lane_xor32<8>(__float_as_uint(v))));
+    if constexpr (T > 16) {
+        v = fmaxf(v, __uint_as_float(lane_xor32<16>(__float_as_uint(v))));
+        v = fmaxf(v, __uint_as_float(lane_xor32<32>(__float_as_uint(v))));
+    }
+    return v;
+}
+template <int T>
 __device__ __forceinline__ double lanes_max(double v) {
     auto step = [](double a, uint64_t b) { return fmax(a, __longlong_as_double((long long)b)); };
     v = step(v, lane_xor64<1>((uint64_t)__double_as_longlong(v)));
