@@ -52,13 +52,13 @@ __device__ __forceinline__ O finish(int acc, float sa, float sb, float bias) {
 // next step's while this one's is multiplied (STAGES = 2).
 constexpr int kTK = 128;
 
-// LDS image of an operand: 128 bytes (8 chunks of 16) a row, chunk c of row r at c ^ (r & 7): the 8 lanes that a ds_read_b128 serves together read 8
-// rows' same chunk from 8 different 16-byte slots of the banks
+// LDS image of an operand: 128 bytes (8 chunks of 16) a row, chunk c of row r at c ^ ((r / 2) & 7).  The banks serve 256 bytes a cycle, two rows: the 16 lanes
+// of a ds_read_b128 that are served together read 16 rows' same chunk from 16 different 16-byte slots.  (r & 7 instead: two of them from each slot.)
 template <bool ALIGNED, int ROWS, int WAVES>
 __device__ __forceinline__ void stage(const int8_t* base, int64_t ld, int64_t row0, int64_t rows, int k0, int K, int8_t* lds, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < ROWS / (8 * WAVES); ++i) {      // 8 rows (1 KB) at a time
-        const int r8 = (wave * (ROWS / (8 * WAVES)) + i) * 8, r = r8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
+        const int r8 = (wave * (ROWS / (8 * WAVES)) + i) * 8, r = r8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
         const bool in = row0 + r < rows;
         const int8_t* row = base + (in ? row0 + r : 0) * ld;
         if constexpr (ALIGNED) {
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN > 4 ? 2 : STAGES == 1 ? 4 : 
     constexpr int OC = 32 * XN, OROW = OC * int(sizeof(O)) + 16, OUT = WAVES * 32 * OROW;      // a wave's 32 output rows on their way out
     __shared__ __align__(16) int8_t s_buf[STAGES * STAGE > OUT ? STAGES * STAGE : OUT];
     __shared__ __align__(16) float s_scale[TN], s_bias[TN];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l31 = lane & 31;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l31 = lane & 31;
     // tiles of one XCD (workgroup id mod 8) are neighbours: 8 rows of tiles, walked along the columns
     const int total = tiles_m * tiles_n, per = (total + 7) / 8;
     const int id = int(blockIdx.x & 7) * per + int(blockIdx.x >> 3);
@@ -94,7 +94,34 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN > 4 ? 2 : STAGES == 1 ? 4 : 
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[x][y][i] = 0;
     const int steps = (g.k + kTK - 1) / kTK;
-    auto put = [&](int s, int buf) {
+    // Whole steps of aligned operands: this lane's bytes of a panel as 32-bit offsets from a scalar address, rows past the end read as the last one (their
+    // results are not written).  The general form's addresses cost a third of the vector instructions of a long product.
+    constexpr int NA = TM / (8 * WAVES), NB = TN / (8 * WAVES);
+    uint32_t at_a[ALIGNED ? NA : 1], at_b[ALIGNED ? NB : 1];
+    if constexpr (ALIGNED) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int r = (wave * NA + i) * 8 + (lane >> 3);
+            at_a[i] = uint32_t(std::min<int64_t>(r, g.m - 1 - m0)) * uint32_t(g.lda) + 16 * ((lane & 7) ^ ((r >> 1) & 7));
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int r = (wave * NB + i) * 8 + (lane >> 3);
+            at_b[i] = uint32_t(std::min<int64_t>(r, g.n - 1 - n0)) * uint32_t(g.ldb) + 16 * ((lane & 7) ^ ((r >> 1) & 7));
+        }
+    }
+    auto put = [&](int s, int buf) __attribute__((always_inline)) {
+        if constexpr (ALIGNED) {
+            if ((s + 1) * kTK <= g.k) {
+                const int8_t *pa = g.a + m0 * g.lda + s * kTK, *pb = g.b + n0 * g.ldb + s * kTK;
+                const uint32_t to = lds_addr(s_buf) + buf * STAGE;
+#pragma unroll
+                for (int i = 0; i < NA; ++i) lds_dma16(pa, at_a[i], __builtin_amdgcn_readfirstlane(to + (wave * NA + i) * 8 * kTK));
+#pragma unroll
+                for (int i = 0; i < NB; ++i) lds_dma16(pb, at_b[i], __builtin_amdgcn_readfirstlane(to + (TM + (wave * NB + i) * 8) * kTK));
+                return;
+            }
+        }
         stage<ALIGNED, TM, WAVES>(g.a, g.lda, m0, g.m, s * kTK, g.k, s_buf + buf * STAGE, wave, lane);
         stage<ALIGNED, TN, WAVES>(g.b, g.ldb, n0, g.n, s * kTK, g.k, s_buf + buf * STAGE + TM * kTK, wave, lane);
     };
@@ -104,39 +131,72 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN > 4 ? 2 : STAGES == 1 ? 4 : 
         s_scale[threadIdx.x] = g.sb[n];
         s_bias[threadIdx.x] = g.bias ? g.bias[n] : 0.f;
     }
-    for (int s = 0; s < steps; ++s) {
-        const int buf = STAGES == 1 ? 0 : s & 1;
-        if (STAGES == 1 && s) {
-            __syncthreads();      // everyone is done with the last step
-            put(s, 0);
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();          // step s is staged, and everyone is done with the other buffer
-        if (STAGES == 2 && s + 1 < steps) put(s + 1, buf ^ 1);
+    constexpr int KC = kTK / 32;
+    i4_t fa[2][XM], fb[2][XN];
+    auto read = [&](int buf, int kc) __attribute__((always_inline)) {
         const int8_t *pa = s_buf + buf * STAGE, *pb = pa + TM * kTK;
+        const int c = 2 * kc + half;
 #pragma unroll
-        for (int kc = 0; kc < kTK / 32; ++kc) {
-            i4_t fa[XM], fb[XN];
-            const int c = 2 * kc + half;
+        for (int y = 0; y < XN; ++y) {
+            const int r = wn + 32 * y + l31;
+            fb[kc & 1][y] = *reinterpret_cast<const i4_t*>(pb + r * kTK + 16 * (c ^ ((r >> 1) & 7)));
+        }
 #pragma unroll
-            for (int y = 0; y < XN; ++y) {
-                const int r = wn + 32 * y + l31;
-                fb[y] = *reinterpret_cast<const i4_t*>(pb + r * kTK + 16 * (c ^ (r & 7)));
+        for (int x = 0; x < XM; ++x) {
+            const int r = wm + 32 * x + l31;
+            fa[kc & 1][x] = *reinterpret_cast<const i4_t*>(pa + r * kTK + 16 * (c ^ ((r >> 1) & 7)));
+        }
+    };
+    auto multiply = [&](int kc) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < XM; ++x)
+#pragma unroll
+            for (int y = 0; y < XN; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[kc & 1][y], fa[kc & 1][x], acc[x][y], 0, 0, 0);
+    };
+    // everything this wave has asked for is there, and everyone is here
+    auto meet = [&]() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    if constexpr (STAGES == 1) {
+        for (int s = 0; s < steps; ++s) {
+            if (s) {
+                __syncthreads();      // everyone is done with the last step
+                put(s, 0);
             }
+            meet();
 #pragma unroll
-            for (int x = 0; x < XM; ++x) {
-                const int r = wm + 32 * x + l31;
-                fa[x] = *reinterpret_cast<const i4_t*>(pa + r * kTK + 16 * (c ^ (r & 7)));
+            for (int kc = 0; kc < KC; ++kc) {
+                read(0, kc);
+                multiply(kc);
             }
+        }
+    } else if (steps) {
+        // Fragments are read one quarter of a step ahead.  The last quarter's are in registers when the waves meet: the buffer is free for the step after the
+        // next, whose loads have a whole step to arrive, and the next step's first fragments are read beside the last products.
+        meet();
+        if (steps > 1) put(1, 1);
+        read(0, 0);
+        for (int s = 0; s < steps; ++s) {
+            const int buf = s & 1;
 #pragma unroll
-            for (int x = 0; x < XM; ++x)
-#pragma unroll
-                for (int y = 0; y < XN; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[y], fa[x], acc[x][y], 0, 0, 0);
+            for (int kc = 0; kc < KC; ++kc) {
+                if (kc + 1 < KC) {
+                    read(buf, kc + 1);
+                } else if (s + 1 < steps) {
+                    meet();
+                    if (s + 2 < steps) put(s + 2, buf);
+                    read(buf ^ 1, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(kc);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
     // C fragment: column (lane & 31) = row m of the output, register rows = 4 consecutive n at a time.  Written through LDS, 32 rows at a time, so that
     // lanes write neighbouring bytes of a row.
-    __syncthreads();
+    meet();
     int8_t* mine = s_buf + wave * 32 * OROW;
 #pragma unroll
     for (int x = 0; x < XM; ++x) {
@@ -254,8 +314,8 @@ static void matmul_q8_launch(const QmmArgs& g, hipStream_t st) {
     const int vec = (g.n * int64_t(sizeof(O))) % 16 == 0 && aligned_to(g.out, g.ldo * int64_t(sizeof(O)), 16);
     auto tiles = [&](int tm, int tn) { return cdiv64(g.m, tm) * cdiv64(g.n, tn); };
     auto grid = [&](int tm, int tn) { return dim3(unsigned((tiles(tm, tn) + 7) / 8 * 8)); };
-    if (g.k > kTK && tiles(256, 256) >= 192) matmul_q8_tile_kernel<O, ALIGNED, 2, 4, 4, 2, 2><<<grid(256, 256), dim3(512), 0, st>>>(g, int(cdiv64(g.m, 256)), int(cdiv64(g.n, 256)), vec);
-    else if (g.k > kTK) matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 2><<<grid(128, 128), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 128)), int(cdiv64(g.n, 128)), vec);
+    if (g.k > 2 * kTK && tiles(256, 256) >= 192) matmul_q8_tile_kernel<O, ALIGNED, 2, 4, 4, 2, 2><<<grid(256, 256), dim3(512), 0, st>>>(g, int(cdiv64(g.m, 256)), int(cdiv64(g.n, 256)), vec);
+    else if (g.k > 2 * kTK) matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 2><<<grid(128, 128), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 128)), int(cdiv64(g.n, 128)), vec);
     else matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 1><<<grid(128, 128), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 128)), int(cdiv64(g.n, 128)), vec);
 }
 
@@ -274,7 +334,7 @@ extern "C" int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale
     if (lda < k || ldb < k || ldo < n) return fail(HWER_EINVAL, "matmul_q8: a row stride is below the row's length");
     const QmmArgs g{a, b, a_scale, b_scale, bias, out, m, n, lda, ldb, ldo, k};
     hipStream_t st = as_stream(stream);
-    const bool al = k % 16 == 0 && aligned_to(a, lda, 16) && aligned_to(b, ldb, 16);
+    const bool al = k % 16 == 0 && aligned_to(a, lda, 16) && aligned_to(b, ldb, 16) && std::max(lda, ldb) < (1 << 23);      // (a panel's bytes in 32 bits)
     if (out_dtype == HWER_F32) al ? matmul_q8_launch<float, true>(g, st) : matmul_q8_launch<float, false>(g, st);
     else if (out_dtype == HWER_F16) al ? matmul_q8_launch<f16_t, true>(g, st) : matmul_q8_launch<f16_t, false>(g, st);
     else al ? matmul_q8_launch<bf16_t, true>(g, st) : matmul_q8_launch<bf16_t, false>(g, st);
