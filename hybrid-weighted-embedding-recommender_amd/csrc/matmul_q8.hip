@@ -3,7 +3,8 @@
 // they depend on no order and no split; one rounding per product with a scale and one to the output's type follow.
 //
 //   matmul_q8_tile   both sides long: tiles of C on the 8-bit matrix instructions, operands staged in LDS by DMA
-//   matmul_q8_few    one side short (<= 64 rows): the long side streams from memory once, K split over the waves of a workgroup
+//   matmul_q8_few    one side short (<= 32 rows): the long side streams from memory once (1 x 8 192 x 8 192: 12.7 us, 5.3 TB/s; 1 x 400 k x 512: 31 us,
+//                    6.5 TB/s, part of it from the last-level cache)
 #include <algorithm>
 
 #include "head_common.h"
@@ -25,21 +26,53 @@ struct QmmArgs {
 // what a DMA lane reads where a row or a K chunk does not exist
 __device__ const uint32_t kZero16[4] = {0u, 0u, 0u, 0u};
 
+// 16 bytes at any address: the whole 4-byte words that hold them, shifted once they are there.  16-byte loads that are not on 4 bytes run at half the
+// rate of others (1 x 8 192 rows of 8 190: 31 us against 23.5; but tiles, whose loads are covered by products: 2 000 x 8 192 x 8 190 155 us with such
+// loads, 186 with these).
+__device__ __forceinline__ i4_t bytes16(const int8_t* p) {
+    i4_t v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+struct Words5 {
+    uint32_t d[5];
+    int off;
+    __device__ __forceinline__ void load(const int8_t* p) {
+        off = int(reinterpret_cast<uintptr_t>(p) & 3);
+        const int8_t* w = p - off;
+        __builtin_memcpy(d, __builtin_assume_aligned(w, 4), 16);
+        d[4] = *reinterpret_cast<const uint32_t*>(w + ((off + 15) & ~3));      // (the last word with a byte of the 16)
+    }
+    __device__ __forceinline__ void load(const int8_t* p, int n) {      // the first n (any number) of them, no word read that holds none
+        off = int(reinterpret_cast<uintptr_t>(p) & 3);
+        const int last = n > 0 ? (off + std::min(n, 16) - 1) & ~3 : 0;
+#pragma unroll
+        for (int i = 0; i < 5; ++i) d[i] = n > 0 ? *reinterpret_cast<const uint32_t*>(p - off + std::min(4 * i, last)) : 0u;
+    }
+    __device__ __forceinline__ i4_t get() const {
+        i4_t v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = int(__builtin_amdgcn_alignbyte(d[i + 1], d[i], off));
+        return v;
+    }
+    __device__ __forceinline__ i4_t get(int n) const {      // zeros after n bytes
+        i4_t v = get();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = n >= 4 * i + 4 ? v[i] : n <= 4 * i ? 0 : v[i] & int((1u << (8 * (n - 4 * i))) - 1u);
+        return v;
+    }
+};
+
 // 16 bytes of a row at byte k, zeros past the row's end.  ALIGNED: K, the row strides and the pointers are multiples of 16.
 template <bool ALIGNED>
 __device__ __forceinline__ i4_t load16(const int8_t* row, int k, int K) {
-    i4_t v = {0, 0, 0, 0};
     if constexpr (ALIGNED) {
-        if (k < K) v = *reinterpret_cast<const i4_t*>(row + k);
-    } else if (k + 16 <= K) {
-        __builtin_memcpy(&v, row + k, 16);      // any alignment: global loads need none
-    } else if (k < K) {
-        int8_t t[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) t[i] = k + i < K ? row[k + i] : int8_t(0);
-        __builtin_memcpy(&v, t, 16);
+        return k < K ? *reinterpret_cast<const i4_t*>(row + k) : i4_t{0, 0, 0, 0};
+    } else {
+        Words5 w;
+        w.load(row + k, K - k);
+        return w.get(K - k);
     }
-    return v;
 }
 
 template <typename O>
@@ -65,7 +98,7 @@ __device__ __forceinline__ void stage(const int8_t* base, int64_t ld, int64_t ro
             const void* p = in && k0 + 16 * c < K ? static_cast<const void*>(row + k0 + 16 * c) : static_cast<const void*>(kZero16);
             lds_dma16_v(p, __builtin_amdgcn_readfirstlane(lds_addr(lds + r8 * kTK)));
         } else {
-            const i4_t v = in ? load16<false>(row, k0 + 16 * c, K) : i4_t{0, 0, 0, 0};
+            const i4_t v = !in ? i4_t{0, 0, 0, 0} : k0 + kTK <= K ? bytes16(row + k0 + 16 * c) : load16<false>(row, k0 + 16 * c, K);
             *reinterpret_cast<i4_t*>(lds + r8 * kTK + lane * 16) = v;
         }
     }
@@ -125,12 +158,12 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN > 4 ? 2 : STAGES == 1 ? 4 : 
         stage<ALIGNED, TM, WAVES>(g.a, g.lda, m0, g.m, s * kTK, g.k, s_buf + buf * STAGE, wave, lane);
         stage<ALIGNED, TN, WAVES>(g.b, g.ldb, n0, g.n, s * kTK, g.k, s_buf + buf * STAGE + TM * kTK, wave, lane);
     };
-    if (steps) put(0, 0);
-    if (int(threadIdx.x) < TN) {      // (read after the barriers below)
+    if (int(threadIdx.x) < TN) {      // (TN <= threads; read after the barriers below)
         const int64_t n = std::min<int64_t>(n0 + threadIdx.x, g.n - 1);
         s_scale[threadIdx.x] = g.sb[n];
         s_bias[threadIdx.x] = g.bias ? g.bias[n] : 0.f;
     }
+    __builtin_amdgcn_s_waitcnt(0);      // (not counted below)
     constexpr int KC = kTK / 32;
     i4_t fa[2][XM], fb[2][XN];
     auto read = [&](int buf, int kc) __attribute__((always_inline)) {
@@ -153,18 +186,71 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN > 4 ? 2 : STAGES == 1 ? 4 : 
 #pragma unroll
             for (int y = 0; y < XN; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[kc & 1][y], fa[kc & 1][x], acc[x][y], 0, 0, 0);
     };
-    // everything this wave has asked for is there, and everyone is here
-    auto meet = [&]() __attribute__((always_inline)) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __syncthreads();
+    // What this wave has asked for is there - all of it, or all but the newest `LEFT` steps' loads - and everyone is here.
+    auto meet = [&](auto left) __attribute__((always_inline)) {
+        constexpr int LEFT = ALIGNED ? decltype(left)::value * (NA + NB) : 0;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
-    if constexpr (STAGES == 1) {
+    typedef std::integral_constant<int, 0> all_t;
+    if constexpr (!ALIGNED && STAGES > 1) {
+        // Any alignment: through registers, a step's loads under way while the last one is multiplied
+        i4_t va[NA], vb[NB];
+        const int8_t *pa[NA], *pb[NB];
+#pragma unroll
+        for (int i = 0; i < NA; ++i) pa[i] = g.a + std::min<int64_t>(m0 + (wave * NA + i) * 8 + (lane >> 3), g.m - 1) * g.lda + 16 * (lane & 7);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) pb[i] = g.b + std::min<int64_t>(n0 + (wave * NB + i) * 8 + (lane >> 3), g.n - 1) * g.ldb + 16 * (lane & 7);
+        auto load = [&](int s) __attribute__((always_inline)) {
+            if ((s + 1) * kTK <= g.k) {
+#pragma unroll
+                for (int i = 0; i < NA; ++i) va[i] = bytes16(pa[i] + s * kTK);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) vb[i] = bytes16(pb[i] + s * kTK);
+            } else {
+                const int n = g.k - 16 * (lane & 7);
+#pragma unroll
+                for (int i = 0; i < NA; ++i) va[i] = load16<false>(pa[i], s * kTK, n);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) vb[i] = load16<false>(pb[i], s * kTK, n);
+            }
+        };
+        auto store = [&](int buf) __attribute__((always_inline)) {
+            int8_t* to = s_buf + buf * STAGE;
+#pragma unroll
+            for (int i = 0; i < NA; ++i) {
+                const int r = (wave * NA + i) * 8 + (lane >> 3);
+                *reinterpret_cast<i4_t*>(to + r * kTK + 16 * ((lane & 7) ^ ((r >> 1) & 7))) = va[i];
+            }
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const int r = (wave * NB + i) * 8 + (lane >> 3);
+                *reinterpret_cast<i4_t*>(to + (TM + r) * kTK + 16 * ((lane & 7) ^ ((r >> 1) & 7))) = vb[i];
+            }
+        };
+        if (steps) {
+            load(0);
+            store(0);
+        }
+        for (int s = 0; s < steps; ++s) {
+            meet(all_t());      // step s is there, and everyone is done with the other buffer
+            if (s + 1 < steps) load(s + 1);
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) {
+                read(s & 1, kc);
+                multiply(kc);
+            }
+            if (s + 1 < steps) store((s + 1) & 1);
+        }
+    } else if constexpr (STAGES == 1) {
+        if (steps) put(0, 0);
         for (int s = 0; s < steps; ++s) {
             if (s) {
-                __syncthreads();      // everyone is done with the last step
+                meet(all_t());      // everyone is done with the last step
                 put(s, 0);
             }
-            meet();
+            meet(all_t());
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) {
                 read(0, kc);
@@ -172,31 +258,38 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN > 4 ? 2 : STAGES == 1 ? 4 : 
             }
         }
     } else if (steps) {
-        // Fragments are read one quarter of a step ahead.  The last quarter's are in registers when the waves meet: the buffer is free for the step after the
-        // next, whose loads have a whole step to arrive, and the next step's first fragments are read beside the last products.
-        meet();
-        if (steps > 1) put(1, 1);
+        // Fragments are read one quarter of a step ahead.  The last quarter's are in registers when the waves meet: the buffer is free for the step STAGES on,
+        // whose loads have STAGES - 1 steps to arrive, and the next step's first fragments are read beside the last products.
+        typedef std::integral_constant<int, STAGES - 2> later_t;
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s)
+            if (s < steps) put(s, s);
+        if (STAGES <= steps) meet(std::integral_constant<int, STAGES - 1>());
+        else meet(all_t());
         read(0, 0);
+        int buf = 0;
         for (int s = 0; s < steps; ++s) {
-            const int buf = s & 1;
+            const int next = buf == STAGES - 1 ? 0 : buf + 1;
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) {
                 if (kc + 1 < KC) {
                     read(buf, kc + 1);
                 } else if (s + 1 < steps) {
-                    meet();
-                    if (s + 2 < steps) put(s + 2, buf);
-                    read(buf ^ 1, 0);
+                    if (s + STAGES - 1 < steps) meet(later_t());
+                    else meet(all_t());
+                    if (s + STAGES < steps) put(s + STAGES, buf);
+                    read(next, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(kc);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            buf = next;
         }
     }
     // C fragment: column (lane & 31) = row m of the output, register rows = 4 consecutive n at a time.  Written through LDS, 32 rows at a time, so that
     // lanes write neighbouring bytes of a row.
-    meet();
+    meet(all_t());
     int8_t* mine = s_buf + wave * 32 * OROW;
 #pragma unroll
     for (int x = 0; x < XM; ++x) {
@@ -235,21 +328,23 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN > 4 ? 2 : STAGES == 1 ? 4 : 
 }
 
 // ---------------------------------------------------------------------------------------------------------------- one side short
-// `few` (at most 16 FT rows) against `many`: a workgroup takes 16 rows of `many`, its 4 waves a quarter of K each.  16x16x64 matrix instruction: the
-// register rows are rows of `many`, the columns rows of `few`.  A lane reads 32 consecutive bytes of a row per step, 4 lanes a whole 128-byte line.
+// `few` (at most 16 FT rows) against `many`: 16 rows of `many` belong to KS waves, each with its part of K; a workgroup of 4 waves takes 64 / KS rows.
+// 16x16x64 matrix instruction: the register rows are rows of `many`, the columns rows of `few`.  A lane reads 32 consecutive bytes of a row per step,
+// 4 lanes a whole 128-byte line.
 struct QmmFewArgs {
     const int8_t *few, *many;
     const float *s_few, *s_many, *bias;
     void* out;
     int64_t n_many, ld_few, ld_many, o_few, o_many;     // output strides along either side
-    int n_few, k, bias_many;                              // bias_many: the bias belongs to `many`'s rows
+    int n_few, k, bias_many, vec;                              // bias_many: the bias belongs to `many`'s rows
 };
 
-template <typename O, int FT, bool ALIGNED>
+template <typename O, int FT, bool ALIGNED, int KS>
 __global__ __launch_bounds__(256) void matmul_q8_few_kernel(QmmFewArgs g) {
-    __shared__ int s_part[3][FT * 4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, quad = lane >> 4;
-    const int64_t r0 = int64_t(blockIdx.x) * 16;
+    static_assert(KS == 1 || KS == 4, "a workgroup's waves have a block of rows each, or all the same");
+    __shared__ int s_part[KS - 1 ? KS - 1 : 1][FT * 4][64];
+    const int lane = threadIdx.x & 63, wave = KS == 1 ? 0 : threadIdx.x >> 6, l15 = lane & 15, quad = lane >> 4;
+    const int64_t r0 = (KS == 1 ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6) : int64_t(blockIdx.x)) * 16;
     const int64_t mr = std::min<int64_t>(r0 + l15, g.n_many - 1);       // rows past the end are read as the last one and not written
     const int8_t* many = g.many + mr * g.ld_many;
     const int8_t* few[FT];
@@ -258,65 +353,129 @@ __global__ __launch_bounds__(256) void matmul_q8_few_kernel(QmmFewArgs g) {
     i4_t acc[FT];
 #pragma unroll
     for (int f = 0; f < FT; ++f) acc[f] = i4_t{0, 0, 0, 0};
-    const int steps = (g.k + 127) / 128, per = (steps + 3) / 4;
+    const int steps = (g.k + 127) / 128, per = (steps + KS - 1) / KS;
     const int s1 = std::min(steps, (wave + 1) * per);
-#pragma unroll 4
-    for (int s = wave * per; s < s1; ++s) {
+    auto load = [&](i4_t (&v)[2 * FT + 2], int s, auto get) __attribute__((always_inline)) {
         const int k = s * 128 + quad * 32;
-        const i4_t m0 = load16<ALIGNED>(many, k, g.k), m1 = load16<ALIGNED>(many, k + 16, g.k);
 #pragma unroll
-        for (int f = 0; f < FT; ++f) {
-            const i4_t f0 = load16<ALIGNED>(few[f], k, g.k), f1 = load16<ALIGNED>(few[f], k + 16, g.k);
-            acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(m0, f0, acc[f], 0, 0, 0);
-            acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(m1, f1, acc[f], 0, 0, 0);
+        for (int h = 0; h < 2; ++h) {
+            v[h] = get(many, k + 16 * h);
+#pragma unroll
+            for (int f = 0; f < FT; ++f) v[2 * f + 2 + h] = get(few[f], k + 16 * h);
         }
+    };
+    auto multiply = [&](const i4_t (&v)[2 * FT + 2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int f = 0; f < FT; ++f) acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[h], v[2 * f + 2 + h], acc[f], 0, 0, 0);
+    };
+    auto plain = [](const int8_t* row, int k) __attribute__((always_inline)) {
+        if constexpr (ALIGNED) return *reinterpret_cast<const i4_t*>(row + k);
+        Words5 w;
+        w.load(row + k);
+        return w.get();
+    };
+    const int whole = std::min(s1, g.k / 128);
+    int s = wave * per;
+    // Whole steps, with no end to look for: the loads of AHEAD steps under way at once
+    constexpr int AHEAD = KS == 1 ? 2 : 4;
+    i4_t v[AHEAD][2 * FT + 2];
+    for (; s + AHEAD <= whole; s += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) load(v[u], s + u, plain);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) multiply(v[u]);
     }
-    if (wave > 0) {
+    for (; s < whole; ++s) {
+        load(v[0], s, plain);
+        multiply(v[0]);
+    }
+    if (s < s1) {      // the last, partial one
+        load(v[0], s, [&](const int8_t* row, int k) __attribute__((always_inline)) { return load16<ALIGNED>(row, k, g.k); });
+        multiply(v[0]);
+    }
+    if constexpr (KS > 1) {
+        if (wave > 0) {
+#pragma unroll
+            for (int f = 0; f < FT; ++f)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s_part[wave - 1][4 * f + i][lane] = acc[f][i];
+        }
+        __syncthreads();
+        if (wave > 0) return;
 #pragma unroll
         for (int f = 0; f < FT; ++f)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s_part[wave - 1][4 * f + i][lane] = acc[f][i];
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int w = 0; w < KS - 1; ++w) acc[f][i] += s_part[w][4 * f + i][lane];
     }
-    __syncthreads();
-    if (wave > 0) return;
+    const int64_t r = r0 + 4 * quad;
+    if (r >= g.n_many) return;
+    const int rows = int(std::min<int64_t>(4, g.n_many - r));
+    float sm[4], bm[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        sm[i] = g.s_many[r + std::min(i, rows - 1)];
+        bm[i] = g.bias && g.bias_many ? g.bias[r + std::min(i, rows - 1)] : 0.f;
+    }
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
         const int row = 16 * f + l15;
         if (row >= g.n_few) continue;
         const float sf = g.s_few[row], bf = g.bias && !g.bias_many ? g.bias[row] : 0.f;
+        typedef O o4 __attribute__((ext_vector_type(4)));
+        o4 v;
+        // the left side's scale first, whichever side is the short one
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t r = r0 + 4 * quad + i;
-            if (r >= g.n_many) continue;
-            const int v = acc[f][i] + s_part[0][4 * f + i][lane] + s_part[1][4 * f + i][lane] + s_part[2][4 * f + i][lane];
-            const float bias = g.bias && g.bias_many ? g.bias[r] : bf, sm = g.s_many[r];
-            // the left side's scale first, whichever side is the short one
-            static_cast<O*>(g.out)[row * g.o_few + r * g.o_many] = g.bias_many ? finish<O>(v, sf, sm, bias) : finish<O>(v, sm, sf, bias);
+        for (int i = 0; i < 4; ++i) v[i] = g.bias_many ? finish<O>(acc[f][i], sf, sm[i], bm[i]) : finish<O>(acc[f][i], sm[i], sf, bf);
+        O* out = static_cast<O*>(g.out) + row * g.o_few + r * g.o_many;
+        if (g.vec && rows == 4) {
+            *reinterpret_cast<o4*>(out) = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < rows) out[i * g.o_many] = v[i];
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
-constexpr int kFewRows = 64;
+// 64 x 8 192 x 8 192: 42 us streamed, 21 us as tiles of 64 x 64; 32 x 8 192 x 8 192: 24 us and 21, but with short sides on both ends (24 x 356 x 2 490)
+// 9 and 25
+constexpr int kFewRows = 32;
+// 1 x 1.6 M x 64: 27 us with a wave's own rows, 76 with K split over a workgroup's waves; 1 x 400 k x 512: 31 and 33; x 50 k x 1 024: 11.1 and 10.2;
+// 24 x 356 x 2 490: 20 and 9
+constexpr int kFewWholeK = 512;
 
 template <typename O, bool ALIGNED>
 static void matmul_q8_launch(const QmmArgs& g, hipStream_t st) {
     if (std::min(g.m, g.n) <= kFewRows) {
         const bool left = g.m <= g.n;      // which side is short
         QmmFewArgs f{left ? g.a : g.b, left ? g.b : g.a, left ? g.sa : g.sb, left ? g.sb : g.sa, g.bias, g.out, left ? g.n : g.m, left ? g.lda : g.ldb,
-                     left ? g.ldb : g.lda, left ? g.ldo : 1, left ? 1 : g.ldo, int(left ? g.m : g.n), g.k, left ? 1 : 0};
-        const dim3 grid(unsigned(cdiv64(f.n_many, 16)));
-        if (f.n_few <= 16) matmul_q8_few_kernel<O, 1, ALIGNED><<<grid, dim3(256), 0, st>>>(f);
-        else if (f.n_few <= 32) matmul_q8_few_kernel<O, 2, ALIGNED><<<grid, dim3(256), 0, st>>>(f);
-        else matmul_q8_few_kernel<O, 4, ALIGNED><<<grid, dim3(256), 0, st>>>(f);
+                     left ? g.ldb : g.lda, left ? g.ldo : 1, left ? 1 : g.ldo, int(left ? g.m : g.n), g.k, left ? 1 : 0, 0};
+        f.vec = left && aligned_to(g.out, g.ldo * int64_t(sizeof(O)), 4 * sizeof(O));
+        auto launch = [&](auto ft, auto ks) {
+            matmul_q8_few_kernel<O, decltype(ft)::value, ALIGNED, decltype(ks)::value><<<dim3(unsigned(cdiv64(f.n_many, 64 / decltype(ks)::value))), dim3(256), 0, st>>>(f);
+        };
+        typedef std::integral_constant<int, 1> one_t;
+        typedef std::integral_constant<int, 2> two_t;
+        typedef std::integral_constant<int, 4> four_t;
+        if (g.k <= kFewWholeK) f.n_few <= 16 ? launch(one_t(), one_t()) : launch(two_t(), one_t());
+        else f.n_few <= 16 ? launch(one_t(), four_t()) : launch(two_t(), four_t());
         return;
     }
     const int vec = (g.n * int64_t(sizeof(O))) % 16 == 0 && aligned_to(g.out, g.ldo * int64_t(sizeof(O)), 16);
     auto tiles = [&](int tm, int tn) { return cdiv64(g.m, tm) * cdiv64(g.n, tn); };
     auto grid = [&](int tm, int tn) { return dim3(unsigned((tiles(tm, tn) + 7) / 8 * 8)); };
-    if (g.k > 2 * kTK && tiles(256, 256) >= 192) matmul_q8_tile_kernel<O, ALIGNED, 2, 4, 4, 2, 2><<<grid(256, 256), dim3(512), 0, st>>>(g, int(cdiv64(g.m, 256)), int(cdiv64(g.n, 256)), vec);
-    else if (g.k > 2 * kTK) matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 2><<<grid(128, 128), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 128)), int(cdiv64(g.n, 128)), vec);
-    else matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 1><<<grid(128, 128), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 128)), int(cdiv64(g.n, 128)), vec);
+    // Few K steps: the output's traffic counts, many workgroups a CU (4 096 x 26 744 x 256: 62 us, 80 with two buffers).  Many: the largest tile of which there
+    // are enough for the CUs; the smallest has four buffers, as little work covers its loads.
+    if (g.k <= 2 * kTK) matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 1><<<grid(128, 128), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 128)), int(cdiv64(g.n, 128)), vec);
+    else if (tiles(256, 256) >= 192) matmul_q8_tile_kernel<O, ALIGNED, 2, 4, 4, 2, 2><<<grid(256, 256), dim3(512), 0, st>>>(g, int(cdiv64(g.m, 256)), int(cdiv64(g.n, 256)), vec);
+    else if (tiles(128, 128) >= 192) matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 2><<<grid(128, 128), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 128)), int(cdiv64(g.n, 128)), vec);
+    else matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 1, 1, 4><<<grid(64, 64), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 64)), int(cdiv64(g.n, 64)), vec);
 }
 
 }  // namespace hwer
@@ -328,7 +487,7 @@ extern "C" int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale
     if (!known_dtype(out_dtype)) return fail(HWER_EINVAL, "matmul_q8: unknown output type %d", out_dtype);
     if (m < 0 || n < 0 || k < 0 || k > 131071) return fail(HWER_EINVAL, "matmul_q8: m=%lld, n=%lld, k=%d (k <= 131071: sums stay in 32 bits)", (long long)m, (long long)n, k);
     if (m == 0 || n == 0) return HWER_OK;
-    if (m > (int64_t(1) << 31) - 256 || n > (int64_t(1) << 31) - 256 || cdiv64(m, 128) * cdiv64(n, 128) > (int64_t(1) << 30))
+    if (m > (int64_t(1) << 31) - 256 || n > (int64_t(1) << 31) - 256 || cdiv64(m, 64) * cdiv64(n, 64) > (int64_t(1) << 30))
         return fail(HWER_EINVAL, "matmul_q8: m=%lld, n=%lld: too many tiles for one call", (long long)m, (long long)n);
     if ((k && (!a || !b)) || !a_scale || !b_scale || !out) return fail(HWER_EINVAL, "matmul_q8: null operand");
     if (lda < k || ldb < k || ldo < n) return fail(HWER_EINVAL, "matmul_q8: a row stride is below the row's length");

@@ -304,6 +304,28 @@ def test_matmul_q8(hw, m, n, k):
 
 
 @gpu
+@pytest.mark.parametrize("k", [257, 272, 384, 512, 640, 1000, 1280])
+@pytest.mark.parametrize("m,n,views", [(33, 70, "whole"), (32, 70, "whole"), (70, 31, "whole"), (100, 450, "whole"), (1600, 2000, "whole"), (2900, 4200, "whole"),
+                                       (100, 450, "odd"), (1600, 2001, "odd"), (2900, 4200, "odd"), (24, 450, "odd")])
+def test_matmul_q8_tiles(hw, m, n, k, views):
+    """every size of tile, with fewer steps of K than it has buffers and more, partial last steps, partial tiles; rows on 16 bytes and not"""
+    from hwer import native
+    a, b = q8(m + k, m, k).cuda(), q8(n + k + 1, n, k).cuda()
+    if views == "odd":
+        a, b = (torch.cat([t.new_full((t.shape[0], 1), 77), t, t.new_full((t.shape[0], 2), -99)], 1)[:, 1:-2] for t in (a, b))
+    sa, sb = torch.ones(m, device="cuda"), torch.ones(n, device="cuda")
+    buf = torch.full((m + 1, n + 5), 7.0, device="cuda")
+    out = buf[:m, 2:2 + n]
+    lib = native.lib()
+    assert lib.hwer_matmul_q8(a.data_ptr(), a.stride(0), sa.data_ptr(), b.data_ptr(), b.stride(0), sb.data_ptr(), None, m, n, k, out.data_ptr(), n + 5, 0, torch.cuda.current_stream().cuda_stream) == 0
+    want = a.double() @ b.double().t()      # below 2^24 in magnitude at these K with scales of one: exact in float32
+    assert want.abs().max() < 2 ** 24 and torch.equal(out.double(), want)
+    assert (buf[m] == 7).all() and (buf[:, :2] == 7).all() and (buf[:, 2 + n:] == 7).all()
+    got = hw.matmul_q8(a, sa, b, sb, out_dtype=torch.bfloat16)
+    assert torch.equal(got, want.float().bfloat16())
+
+
+@gpu
 def test_matmul_q8_strides_and_order(hw):
     """rows of a wider table, rows that are not on 16 bytes, a transposed operand; the same product with the sides exchanged is the same, bit for bit"""
     a, b = q8(1, 100, 300).cuda(), q8(2, 200, 300).cuda()
