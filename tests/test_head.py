@@ -160,6 +160,14 @@ def test_norm_forward_and_gradients(hw, n, d, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,d", [(20011, 40), (7001, 1030), (2900, 4104), (1100, 20000), (40000, 3)])
+def test_norm_of_many_rows(hw, n, d, dtype):
+    """the weights' gradient joined from many workgroups' parts"""
+    test_norm_forward_and_gradients(hw, n, d, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_norm_gradients_against_differences(hw, dtype):
     """The gradient of sum(y * c) + sum(h * k) along a direction against the difference of the 64-bit formula on both sides."""
     x, res, c, k, v = (rnd(70 + i, 6, 40) for i in range(5))
@@ -428,6 +436,35 @@ def test_cross_entropy_and_gradients(hw, n, v, d, dtype):
     ce_check(hw, x, e, t, 6.0, None)
     t[::3] = -1
     ce_check(hw, x, e, t, 0.7, rnd(9, v).float(), reduction="sum")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,d", [(1000, 30000, 64), (16, 150000, 96), (200, 40000, 250), (9000, 300, 128), (5000, 129, 256), (2500, 4000, 100), (70, 20000, 3)])
+def test_cross_entropy_split_over_either_side(hw, n, v, d, dtype):
+    """a few and hundreds of splits in both passes, and their joins; rows with gradients of their own, of which some are zero"""
+    x, e, t, b = ce_inputs(n + v + d, n, v, d, dtype, bias=True)
+    t[::5] = -1
+    b[::11] = float("-inf")
+    t = torch.where(t % 11 == 0, t + 1, t).clamp_max(v - 1 if (v - 1) % 11 else v - 2)
+    up = rnd(7, n)
+    up[::4] = 0
+    up[1::8] *= 1e-4
+    ref = {k: a.cpu() for k, a in ce_reference(x.cuda(), e.cuda(), t.cuda(), 4.0, b.cuda(), up.cuda()).items()}
+    tol = ce_tolerances(ref, dtype, n, v, d)
+    xs, es, bs = x.cuda().requires_grad_(), e.cuda().requires_grad_(), b.cuda().requires_grad_()
+    rows = hw.catalogue_cross_entropy(xs, es, t.cuda(), scale=4.0, bias=bs, reduction="none")
+    close(rows, ref["rows"], tol["loss"] + ref["rows"].abs() * U32, "rows")
+    rows.backward(up.float().cuda())
+    # a row's gradient enters in float32, relative to the largest: two more roundings; in float16 a weight of the table's sum keeps 2^-40 of the largest
+    # gradient's (not of its own row's)
+    floor = 0.0 if dtype == torch.bfloat16 else 2.0 ** -40 * 4.0 * up.abs().max() * x.double().abs().sum(0)
+    close(xs.grad, ref["dx"], tol["dx"] + ref["dx_size"] * 4 * U32, "dqueries")
+    close(es.grad, ref["de"], tol["de"] + ref["de_size"] * 4 * U32 + floor, "dtable")
+    close(bs.grad, ref["db"], tol["db"] + ref["db_size"] * 4 * U32, "dbias")
+    again = [a.detach().clone().requires_grad_() for a in (xs, es, bs)]
+    hw.catalogue_cross_entropy(again[0], again[1], t.cuda(), scale=4.0, bias=again[2], reduction="none").backward(up.float().cuda())
+    assert all(torch.equal(p.grad, q.grad) for p, q in zip(again, (xs, es, bs)))
 
 
 @gpu
