@@ -105,18 +105,18 @@ __device__ __forceinline__ void stage(const int8_t* base, int64_t ld, int64_t ro
 }
 
 template <typename O, bool ALIGNED, int WM, int WN, int XM, int XN, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN, (WM * WN > 4 ? 2 : STAGES == 1 ? 4 : 2)) void matmul_q8_tile_kernel(QmmArgs g, int tiles_m, int tiles_n, int vec) {
+__global__ __launch_bounds__(64 * WM * WN, (STAGES == 1 ? 4 : 2)) void matmul_q8_tile_kernel(QmmArgs g, int tiles_m, int tiles_n, int rows, int vec) {
     constexpr int WAVES = WM * WN, TM = 32 * XM * WM, TN = 32 * XN * WN, STAGE = (TM + TN) * kTK;
-    constexpr int OC = 32 * XN, OROW = OC * int(sizeof(O)) + 16, OUT = WAVES * 32 * OROW;      // a wave's 32 output rows on their way out
+    constexpr int OROW = TN * int(sizeof(O)) + 16, OUT = 32 * WM * OROW;      // output rows on their way out: 32 of each wave's at a time
     __shared__ __align__(16) int8_t s_buf[STAGES * STAGE > OUT ? STAGES * STAGE : OUT];
     __shared__ __align__(16) float s_scale[TN], s_bias[TN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l31 = lane & 31;
-    // tiles of one XCD (workgroup id mod 8) are neighbours: 8 rows of tiles, walked along the columns
+    // tiles of one XCD (workgroup id mod 8) are neighbours: bands of `rows` rows of tiles, walked along the columns
     const int total = tiles_m * tiles_n, per = (total + 7) / 8;
     const int id = int(blockIdx.x & 7) * per + int(blockIdx.x >> 3);
     if (int(blockIdx.x >> 3) >= per || id >= total) return;
-    const int band = id / (8 * tiles_n), in_band = id % (8 * tiles_n), bh = min(8, tiles_m - 8 * band);
-    const int tm = band * 8 + in_band % bh, tn = in_band / bh;
+    const int band = id / (rows * tiles_n), in_band = id % (rows * tiles_n), bh = min(rows, tiles_m - rows * band);
+    const int tm = band * rows + in_band % bh, tn = in_band / bh;
     const int64_t m0 = int64_t(tm) * TM, n0 = int64_t(tn) * TN;
     const int wm = (wave % WM) * 32 * XM, wn = (wave / WM) * 32 * XN;
     i16_t acc[XM][XN];
@@ -158,12 +158,12 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN > 4 ? 2 : STAGES == 1 ? 4 : 
         stage<ALIGNED, TM, WAVES>(g.a, g.lda, m0, g.m, s * kTK, g.k, s_buf + buf * STAGE, wave, lane);
         stage<ALIGNED, TN, WAVES>(g.b, g.ldb, n0, g.n, s * kTK, g.k, s_buf + buf * STAGE + TM * kTK, wave, lane);
     };
-    if (int(threadIdx.x) < TN) {      // (TN <= threads; read after the barriers below)
-        const int64_t n = std::min<int64_t>(n0 + threadIdx.x, g.n - 1);
-        s_scale[threadIdx.x] = g.sb[n];
-        s_bias[threadIdx.x] = g.bias ? g.bias[n] : 0.f;
-    }
-    __builtin_amdgcn_s_waitcnt(0);      // (not counted below)
+    // (older than the loads that are counted below, written to LDS after them: TN <= threads)
+    const int64_t my_n = std::min<int64_t>(n0 + threadIdx.x % TN, g.n - 1);
+    const float my_scale = g.sb[my_n], my_bias = g.bias ? g.bias[my_n] : 0.f;
+    float row_scale[XM];
+#pragma unroll
+    for (int x = 0; x < XM; ++x) row_scale[x] = g.sa[std::min<int64_t>(m0 + wm + 32 * x + l31, g.m - 1)];
     constexpr int KC = kTK / 32;
     i4_t fa[2][XM], fb[2][XN];
     auto read = [&](int buf, int kc) __attribute__((always_inline)) {
@@ -287,43 +287,41 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN > 4 ? 2 : STAGES == 1 ? 4 : 
             buf = next;
         }
     }
-    // C fragment: column (lane & 31) = row m of the output, register rows = 4 consecutive n at a time.  Written through LDS, 32 rows at a time, so that
-    // lanes write neighbouring bytes of a row.
-    meet(all_t());
-    int8_t* mine = s_buf + wave * 32 * OROW;
+    if (int(threadIdx.x) < TN) s_scale[threadIdx.x] = my_scale, s_bias[threadIdx.x] = my_bias;
+    // C fragment: column (lane & 31) = row m of the output, register rows = 4 consecutive n at a time.  Written through LDS, 32 rows of each wave at a time, so
+    // that lanes write neighbouring bytes of a whole row of the tile: parts of memory lines cost as much as whole ones.
+    constexpr int PIECE = 16 / int(sizeof(O)), LPR = TN / PIECE, RPI = 64 / LPR;      // elements of 16 bytes, lanes of a row, rows of an instruction
+    const int cols = int(std::min<int64_t>(TN, g.n - n0));
 #pragma unroll
     for (int x = 0; x < XM; ++x) {
-        const int64_t mb = m0 + wm + 32 * x;
-        const float sa = g.sa[std::min<int64_t>(mb + l31, g.m - 1)];
+        meet(all_t());
 #pragma unroll
         for (int y = 0; y < XN; ++y)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 typedef O o4 __attribute__((ext_vector_type(4)));
-                const float4 sb = *reinterpret_cast<const float4*>(s_scale + wn + 32 * y + 8 * q + 4 * half);
-                const float4 bi = *reinterpret_cast<const float4*>(s_bias + wn + 32 * y + 8 * q + 4 * half);
+                const int c = wn + 32 * y + 8 * q + 4 * half;
+                const float4 sb = *reinterpret_cast<const float4*>(s_scale + c);
+                const float4 bi = *reinterpret_cast<const float4*>(s_bias + c);
+                const float sa = row_scale[x];
                 const o4 v = {finish<O>(acc[x][y][4 * q], sa, sb.x, bi.x), finish<O>(acc[x][y][4 * q + 1], sa, sb.y, bi.y),
                               finish<O>(acc[x][y][4 * q + 2], sa, sb.z, bi.z), finish<O>(acc[x][y][4 * q + 3], sa, sb.w, bi.w)};
-                *reinterpret_cast<o4*>(mine + l31 * OROW + (32 * y + 8 * q + 4 * half) * int(sizeof(O))) = v;
+                *reinterpret_cast<o4*>(s_buf + ((wave % WM) * 32 + l31) * OROW + c * int(sizeof(O))) = v;
             }
-        wave_lds_sync();
-        const int64_t nb = n0 + wn;
-        O* out = static_cast<O*>(g.out) + mb * g.ldo + nb;
-        const int rows = int(std::min<int64_t>(32, g.m - mb)), cols = int(std::min<int64_t>(OC, g.n - nb));
-        if (vec) {      // whole 16-byte pieces (n and the row stride are multiples of a piece)
-            constexpr int PIECE = 16 / int(sizeof(O)), LPR = OC / PIECE, RPI = 64 / LPR;      // lanes of a row, rows of an instruction
-            const int c = (lane % LPR) * PIECE;
+        meet(all_t());
+        constexpr int RPW = 32 * WM / WAVES;      // rows of a wave
 #pragma unroll
-            for (int i = 0; i < 32 / RPI; ++i) {
-                const int r = i * RPI + lane / LPR;
-                const i4_t v = *reinterpret_cast<const i4_t*>(mine + r * OROW + c * int(sizeof(O)));
-                if (r < rows && c < cols) *reinterpret_cast<i4_t*>(out + int64_t(r) * g.ldo + c) = v;
-            }
-        } else {
-            for (int r = 0; r < rows; ++r)
-                for (int c = lane; c < cols; c += 64) out[int64_t(r) * g.ldo + c] = *reinterpret_cast<const O*>(mine + r * OROW + c * int(sizeof(O)));
+        for (int i = 0; i < RPW / RPI; ++i) {
+            const int r = wave * RPW + i * RPI + lane / LPR, c = (lane % LPR) * PIECE;
+            const int64_t m = m0 + (r / 32) * 32 * XM + 32 * x + r % 32;
+            if (m >= g.m || c >= cols) continue;
+            const i4_t v = *reinterpret_cast<const i4_t*>(s_buf + r * OROW + c * int(sizeof(O)));
+            O* out = static_cast<O*>(g.out) + m * g.ldo + n0 + c;
+            if (vec) *reinterpret_cast<i4_t*>(out) = v;      // whole 16-byte pieces (n and the row stride are multiples of a piece)
+            else if (c + PIECE <= cols) __builtin_memcpy(out, &v, 16);
+            else
+                for (int k = 0; k < cols - c; ++k) out[k] = *reinterpret_cast<const O*>(s_buf + r * OROW + (c + k) * int(sizeof(O)));
         }
-        wave_lds_sync();
     }
 }
 
@@ -470,12 +468,20 @@ static void matmul_q8_launch(const QmmArgs& g, hipStream_t st) {
     const int vec = (g.n * int64_t(sizeof(O))) % 16 == 0 && aligned_to(g.out, g.ldo * int64_t(sizeof(O)), 16);
     auto tiles = [&](int tm, int tn) { return cdiv64(g.m, tm) * cdiv64(g.n, tn); };
     auto grid = [&](int tm, int tn) { return dim3(unsigned((tiles(tm, tn) + 7) / 8 * 8)); };
-    // Few K steps: the output's traffic counts, many workgroups a CU (4 096 x 26 744 x 256: 62 us, 80 with two buffers).  Many: the largest tile of which there
-    // are enough for the CUs; the smallest has four buffers, as little work covers its loads.
-    if (g.k <= 2 * kTK) matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 1><<<grid(128, 128), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 128)), int(cdiv64(g.n, 128)), vec);
-    else if (tiles(256, 256) >= 192) matmul_q8_tile_kernel<O, ALIGNED, 2, 4, 4, 2, 2><<<grid(256, 256), dim3(512), 0, st>>>(g, int(cdiv64(g.m, 256)), int(cdiv64(g.n, 256)), vec);
-    else if (tiles(128, 128) >= 192) matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 2><<<grid(128, 128), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 128)), int(cdiv64(g.n, 128)), vec);
-    else matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 1, 1, 4><<<grid(64, 64), dim3(256), 0, st>>>(g, int(cdiv64(g.m, 64)), int(cdiv64(g.n, 64)), vec);
+    auto go = [&](auto kernel, int tm, int tn, int threads, int band) {
+        kernel<<<grid(tm, tn), dim3(threads), 0, st>>>(g, int(cdiv64(g.m, tm)), int(cdiv64(g.n, tn)), band, vec);
+    };
+    // Few K steps: the output's traffic counts, one buffer and many workgroups a CU.  With few tiles smaller ones (943 x 1 682 x 64 bfloat16: 5.4 us, 6.8 as
+    // 128 x 128).  Rows of the output seldom begin on a memory line, so parts of one line come from two tiles: float32 tiles are wider and their bands are
+    // narrower, so that these meet sooner (4 096 x 26 744 x 256: 104 us, 120 as 128 x 128 in bands of 8 rows; bfloat16: 72 both ways, x 128: 61 and 60,
+    // with rows on 128 bytes 54 and 49).
+    constexpr bool wide = sizeof(O) == 4;
+    if (g.k <= 2 * kTK && tiles(128, 128) < 1024) go(matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 1, 2, 1>, 64, 128, 256, 4);
+    else if (g.k <= 2 * kTK) go(matmul_q8_tile_kernel<O, ALIGNED, 2, wide ? 4 : 2, 2, 2, 1>, 128, wide ? 256 : 128, wide ? 512 : 256, wide ? 2 : 8);
+    // Many: the largest tile of which there are enough for the CUs; the smallest has four buffers, as little work covers its loads.
+    else if (tiles(256, 256) >= 192) go(matmul_q8_tile_kernel<O, ALIGNED, 2, 4, 4, 2, 2>, 256, 256, 512, 8);
+    else if (tiles(128, 128) >= 192) go(matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 2, 2, 2>, 128, 128, 256, 8);
+    else go(matmul_q8_tile_kernel<O, ALIGNED, 2, 2, 1, 1, 4>, 64, 64, 256, 8);
 }
 
 }  // namespace hwer

@@ -312,9 +312,9 @@ def test_matmul_q8(hw, m, n, k):
 
 
 @gpu
-@pytest.mark.parametrize("k", [257, 272, 384, 512, 640, 1000, 1280])
+@pytest.mark.parametrize("k", [64, 250, 257, 272, 384, 512, 640, 1000, 1280])
 @pytest.mark.parametrize("m,n,views", [(33, 70, "whole"), (32, 70, "whole"), (70, 31, "whole"), (100, 450, "whole"), (1600, 2000, "whole"), (2900, 4200, "whole"),
-                                       (100, 450, "odd"), (1600, 2001, "odd"), (2900, 4200, "odd"), (24, 450, "odd")])
+                                       (100, 450, "odd"), (1600, 2001, "odd"), (2900, 4200, "odd"), (24, 450, "odd"), (3003, 6001, "whole"), (3003, 6001, "odd")])
 def test_matmul_q8_tiles(hw, m, n, k, views):
     """every size of tile, with fewer steps of K than it has buffers and more, partial last steps, partial tiles; rows on 16 bytes and not"""
     from hwer import native
