@@ -351,11 +351,15 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
                 w[j] = __builtin_amdgcn_exp2f(w[j]);
                 if constexpr (MUL) w[j] *= pm[j];
             }
-            if (hit) {
+            if (hit) {      // (popular classes are hit in every tile: four rows' targets and weights at a time, not one after the other)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int r = sb * 32 + 8 * (j >> 2) + 4 * half + (j & 3);
-                    if (__float_as_int(s_par[slot][3][r]) == int(my)) w[j] = s_par[slot][2][r];
+                for (int q = 0; q < 4; ++q) {
+                    const int r = sb * 32 + 8 * q + 4 * half;
+                    const float4 t = *reinterpret_cast<const float4*>(&s_par[slot][3][r]), v = *reinterpret_cast<const float4*>(&s_par[slot][2][r]);
+                    w[4 * q] = __float_as_int(t.x) == int(my) ? v.x : w[4 * q];
+                    w[4 * q + 1] = __float_as_int(t.y) == int(my) ? v.y : w[4 * q + 1];
+                    w[4 * q + 2] = __float_as_int(t.z) == int(my) ? v.z : w[4 * q + 2];
+                    w[4 * q + 3] = __float_as_int(t.w) == int(my) ? v.w : w[4 * q + 3];
                 }
             }
             if (BIAS) {
