@@ -858,6 +858,9 @@ static bool ce_direct(const void* p, int64_t ld, int d, int dtype) {
 // Splits of the streaming side, in 32s of its rows.  A call takes as long as its fullest CU (which holds two workgroups, or one of the widest rows): rounds of
 // workgroups times (a split's 32s + about 4 for its start and end); and each split leaves sums behind that are written and read again, about 2 MB in the
 // time of 32 rows.
+// Tried for pass 2: one workgroup for each place on the CUs with an equal share of all blocks' work.  No last round that is not full (1 037 x 50 021 x 250
+// float16 256 -> 241 us), but no workgroup takes over from a slower one either, and the loop over blocks costs registers: 4 096 x 1.25 M x 128 bfloat16
+// 4.90 -> 5.00 ms, x 400 k x 64 0.97 -> 1.04, x 400 k x 256 4.0 -> 4.7.
 struct CeSplit {
     int blocks, splits, subs;
 };

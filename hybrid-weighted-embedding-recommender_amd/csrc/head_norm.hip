@@ -15,7 +15,8 @@
 
 namespace hwer {
 
-constexpr int kNormBlock = 256;     // threads of a workgroup unless one row takes more
+// threads of a workgroup: 256 with rows of their own for each wave or part of one, or those of one row
+constexpr int norm_block(int t) { return t <= 64 ? 256 : t; }
 
 // N elements of a row from column c, and back: one access of 16 bytes (codes: N bytes) at any alignment; at the row's end element by element, zeros past it
 template <typename E, int N>
@@ -86,8 +87,8 @@ __device__ __forceinline__ float row_sum(float v, float* slots, int flip) {
 }
 
 template <typename E, typename W, int T, int VPT, int VW, bool Q8>
-__global__ __launch_bounds__(T > kNormBlock ? T : kNormBlock) void norm_fwd_kernel(NormFwdArgs a) {
-    constexpr int B = T > kNormBlock ? T : kNormBlock, R = B / T;     // R rows at a time
+__global__ __launch_bounds__(norm_block(T)) void norm_fwd_kernel(NormFwdArgs a) {
+    constexpr int B = norm_block(T), R = B / T;     // R rows at a time
     __shared__ float s_sum[2 * (T > 64 ? T / 64 : 1)];
     __shared__ uint32_t s_top[2 * (T > 64 ? T / 64 : 1)];
     __shared__ double s_exact[T > 64 ? T / 64 : 1];
@@ -252,8 +253,8 @@ struct NormBwdArgs {
 };
 
 template <typename E, typename W, int T, int VPT, int VW>
-__global__ __launch_bounds__(T > kNormBlock ? T : kNormBlock) void norm_bwd_kernel(NormBwdArgs a) {
-    constexpr int B = T > kNormBlock ? T : kNormBlock, R = B / T;
+__global__ __launch_bounds__(norm_block(T)) void norm_bwd_kernel(NormBwdArgs a) {
+    constexpr int B = norm_block(T), R = B / T;
     __shared__ float s_sum[4 * (T > 64 ? T / 64 : 1)];
     __shared__ float s_dw[R > 1 ? B * VPT * VW : 1];
     typedef Pack<E, VW> PE;
@@ -494,12 +495,12 @@ static NormPlan norm_plan(int d, int vw) {
 
 // workgroups of a launch: enough to fill the chip several times over, few enough that the weights are read once per many rows
 static int norm_grid(int64_t rows, int t) {
-    const int r = t >= kNormBlock ? 1 : kNormBlock / t;
+    const int r = norm_block(t) / t;
     return int(std::min<int64_t>(cdiv64(rows, r), kMaxStreamBlocks));
 }
 // ... of a backward launch: each leaves a partial sum of the weights' gradient behind
 static int norm_bwd_grid(int64_t rows, int t) {
-    const int r = t >= kNormBlock ? 1 : kNormBlock / t;
+    const int r = norm_block(t) / t;
     return int(std::min<int64_t>(cdiv64(rows, r), 1024));
 }
 constexpr int kWideDwParts = 32;
@@ -507,11 +508,17 @@ constexpr int kWideDwParts = 32;
 template <typename E, typename W, bool Q8>
 static void norm_fwd_launch(const NormFwdArgs& a, hipStream_t st) {
     constexpr int VW = 16 / int(sizeof(E));
-    const NormPlan p = norm_plan(a.d, VW);
+    NormPlan p = norm_plan(a.d, VW);
+    // Two waves that a row nearly fills, instead of one with twice the elements: 16 384 x 1 024 bfloat16 25 us, 30 as one wave; but 65 536 x 300 float32 87, 54
+    // as one wave, and the codes' second reduction 139, 116 (65 536 x 1 024).
+    if (!Q8 && a.d > 112 * VW && a.d <= 128 * VW) p = {128, 1};
     const int grid = norm_grid(a.rows, p.t ? p.t : kWideThreads);
 #define HWER_NORM_FWD(T, V) \
-    if (p.t == T && p.vpt == V) return norm_fwd_kernel<E, W, T, V, VW, Q8><<<dim3(grid), dim3(T > kNormBlock ? T : kNormBlock), 0, st>>>(a);
+    if (p.t == T && p.vpt == V) return norm_fwd_kernel<E, W, T, V, VW, Q8><<<dim3(grid), dim3(norm_block(T)), 0, st>>>(a);
     HWER_NORM_PLANS(HWER_NORM_FWD)
+    if constexpr (!Q8) {
+        HWER_NORM_FWD(128, 1)
+    }
 #undef HWER_NORM_FWD
     norm_fwd_wide_kernel<E, W, Q8><<<dim3(grid), dim3(kWideThreads), 0, st>>>(a);
 }
@@ -595,7 +602,7 @@ int hwer_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t 
         }
         parts = norm_bwd_grid(rows, p.t);
 #define HWER_NORM_BWD(T, V) \
-        if (p.t == T && p.vpt == V) return norm_bwd_kernel<E, W, T, V, VW><<<dim3(parts), dim3(T > kNormBlock ? T : kNormBlock), 0, st>>>(a);
+        if (p.t == T && p.vpt == V) return norm_bwd_kernel<E, W, T, V, VW><<<dim3(parts), dim3(norm_block(T)), 0, st>>>(a);
         HWER_NORM_PLANS(HWER_NORM_BWD)
 #undef HWER_NORM_BWD
     };
