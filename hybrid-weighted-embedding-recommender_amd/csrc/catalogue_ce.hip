@@ -392,7 +392,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
             mx = fmaxf(mx, s[15]);
             mx = fmaxf(mx, __uint_as_float(lane_xor32<32>(__float_as_uint(mx))));
             if (__any(mx > renew)) {
-                const float mn = fmaxf(m, mx);
+                const float mn = mx > renew ? fmaxf(m, mx) : m;      // (row by row: a row's result does not depend on the rows beside it)
                 // (m = -inf: nothing so far, l and o are 0; differences first: a bias of float32's lowest value must not overflow)
                 const float f = m == kLowest ? 1.f : __builtin_amdgcn_exp2f((m - mn) * (BIAS ? kLog2e : c));
                 m = mn;
@@ -528,7 +528,9 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
 }
 
 // ---------------------------------------------------------------------------------------------------------------- operands
-// Rows that the passes cannot read in place (width not 64 / 128 / 256, rows not on 16 bytes, float32) are laid out once per call.
+// Rows that the passes cannot read in place (width not 64 / 128 / 256, rows not on 16 bytes, float32, a table some of whose rows may be taken out) are laid
+// out once per call.  Queries that do not count and classes that are taken out become rows of zeros there: their weights are zero, and zero times what an
+// unused row holds (infinity, NaN) would be NaN in every other row's gradient.
 struct CePack {
     const void* src[2];
     short *hi[2], *lo[2];
@@ -537,6 +539,12 @@ struct CePack {
     float* tops;             // (2, kTopBlocks) partial maxima of |value|
     CeScalars* sc;
     int vec[2];
+    const int64_t* target;
+    const float* bias;
+    __device__ __forceinline__ bool used(int w, int64_t r) const {
+        if (w == 0) return target[r] >= 0 && target[r] < rows[1];
+        return !bias || bias[r] != -INFINITY;
+    }
 };
 constexpr int kTopBlocks = 512;
 
@@ -549,9 +557,10 @@ __global__ __launch_bounds__(256) void ce_pack16_kernel(CePack a) {
         const int64_t r = i >> shift;
         const int c = int(i & (chunks - 1)) * 8;
         const short* p = static_cast<const short*>(a.src[w]) + r * a.ld[w];
+        const int d = a.used(w, r) ? a.d : 0;
         s16x8 v;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < a.d ? p[c + j] : short(0);
+        for (int j = 0; j < 8; ++j) v[j] = c + j < d ? p[c + j] : short(0);
         *reinterpret_cast<s16x8*>(a.hi[w] + r * a.dp + c) = v;
     }
 }
@@ -559,14 +568,15 @@ __global__ __launch_bounds__(256) void ce_pack16_kernel(CePack a) {
 // 8 float32 values of a row from column c, zeros past its end
 __device__ __forceinline__ void ce_load8(const CePack& a, int w, int64_t r, int c, float (&v)[8]) {
     const float* p = static_cast<const float*>(a.src[w]) + r * a.ld[w] + c;
+    const int d = a.used(w, r) ? a.d : 0;
     if (a.vec[w]) {      // rows on 16 bytes, of a multiple of 4 values
         float4 u = {0.f, 0.f, 0.f, 0.f}, t = u;
-        if (c < a.d) u = *reinterpret_cast<const float4*>(p);
-        if (c + 4 < a.d) t = *reinterpret_cast<const float4*>(p + 4);
+        if (c < d) u = *reinterpret_cast<const float4*>(p);
+        if (c + 4 < d) t = *reinterpret_cast<const float4*>(p + 4);
         v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w, v[4] = t.x, v[5] = t.y, v[6] = t.z, v[7] = t.w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < a.d ? p[j] : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = c + j < d ? p[j] : 0.f;
     }
 }
 
@@ -579,7 +589,7 @@ __global__ __launch_bounds__(256) void ce_top_kernel(CePack a) {
         float v[8];
         ce_load8(a, w, i >> shift, int(i & (chunks - 1)) * 8, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+        for (int j = 0; j < 8; ++j) top = fabsf(v[j]) < INFINITY ? fmaxf(top, fabsf(v[j])) : top;      // (of the finite ones: a row with others spoils no other row)
     }
     top = wave_max_f32(top);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
@@ -652,6 +662,9 @@ struct CeRows {
     const int* counts;            // counted rows (partial)
     int n_counts;
     float off, off2;              // powers of two that the weights of pass 1 / 2 carry
+    const short* q;               // queries that pass 1 reads in place, nullable: copied for pass 2, rows that do not count as zeros (as CePack lays them out)
+    int64_t ldq;
+    short* q_copy;
 };
 constexpr int kCUs = 256, kMaxSplits = 512;      // splits of a streaming side
 
@@ -663,6 +676,11 @@ __device__ __forceinline__ void ce_put_rowp(const CeRows& a, int64_t r, bool on,
     a.rowp[a.ld_rowp + r] = on ? rel * __builtin_amdgcn_exp2f(BIAS ? -low * kLog2e : -low) : 0.f;
     a.rowp[2 * a.ld_rowp + r] = -rel * miss * __builtin_amdgcn_exp2f(a.off2);
     a.rowp[3 * a.ld_rowp + r] = __int_as_float(on ? int(t) : -1);
+}
+
+__device__ __forceinline__ void ce_copy_query(const CeRows& a, int64_t r, bool on, int t) {      // thread t of at least dp / 8
+    if (a.q && 8 * t < a.dp)
+        *reinterpret_cast<s16x8*>(a.q_copy + r * a.dp + 8 * t) = on ? *reinterpret_cast<const s16x8*>(a.q + r * a.ldq + 8 * t) : s16x8{0, 0, 0, 0, 0, 0, 0, 0};
 }
 
 // Joins the splits of pass 1: loss_r, lse_r, 1 - p_t and sum_{v /= t} p'_v e_v.  TR threads a row (a wave, or 256 where there are many splits); DP / 4 of
@@ -737,6 +755,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
         else a.state[r] = {hi, low, float(miss), 0.f};
     }
     if (!GRADS && !a.mean) return;
+    if constexpr (GRADS && !F32) ce_copy_query(a, r, on, t_in);
     const int per = a.dp / 4, groups = TR / per, c4 = t_in & (per - 1), grp = t_in / per;
     float4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
@@ -776,10 +795,11 @@ __global__ __launch_bounds__(1024) void ce_loss_kernel(const float* loss_rows, c
     ce_reduce_loss<1024>(loss_rows, target, n, reduction, loss, counted);
 }
 
-__global__ __launch_bounds__(1024) void ce_grad_top_kernel(const float* grad, int64_t n, CeScalars* sc) {
+// (of the rows that count: another row's gradient may be anything)
+__global__ __launch_bounds__(1024) void ce_grad_top_kernel(const float* grad, const int64_t* target, int64_t n, int64_t v, CeScalars* sc) {
     __shared__ float s[16];
     float top = 0.f;
-    for (int64_t r = threadIdx.x; r < n; r += 1024) top = fmaxf(top, fabsf(grad[r]));
+    for (int64_t r = threadIdx.x; r < n; r += 1024) top = fmaxf(top, target[r] >= 0 && target[r] < v ? fabsf(grad[r]) : 0.f);
     top = wave_max_f32(top);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
     __syncthreads();
@@ -810,6 +830,7 @@ __global__ __launch_bounds__(256) void ce_dq_kernel(CeRows a) {
     const float4 st = a.state[r];
     const float gr = a.per_row ? a.grad[r] : g;
     if (a.rowp && lane == 0) ce_put_rowp<BIAS>(a, r, on, st.x, st.y, st.z, !on ? 0.f : a.per_row ? (g > 0.f ? gr / g : gr) : 1.f, t);
+    if (!F32 && a.rowp) ce_copy_query(a, r, on, lane);
     if (a.dq) {
         E* dq = static_cast<E*>(a.dq) + r * a.lddq;
         const E* e = static_cast<const E*>(a.e) + (on ? t : 0) * a.lde;
@@ -893,7 +914,7 @@ static CeLayout ce_layout(int64_t n, int64_t v, int d, int dtype, bool q_direct,
     const CeSplit f = ce_split(n, v, d), b = ce_split(v, n, d);
     size_t at = 256;      // CeScalars
     y.tops = at, at += dtype == HWER_F32 ? 2 * kTopBlocks * 4 : 0;
-    y.q_hi = at, at += q_direct ? 0 : up(size_t(n) * dp * 2);
+    y.q_hi = at, at += q_direct && !want_mean ? 0 : up(size_t(n) * dp * 2);
     y.q_lo = at, at += dtype == HWER_F32 ? up(size_t(n) * dp * 2) : 0;
     y.e_hi = at, at += e_direct ? 0 : up(size_t(v) * dp * 2);
     y.e_lo = at, at += dtype == HWER_F32 ? up(size_t(v) * dp * 2) : 0;
@@ -945,7 +966,7 @@ struct CeCall {
         if (!(scale > 0.f) || !(scale < INFINITY)) return fail(HWER_EINVAL, "%s: scale must be positive and finite", what);
         if (n && (!q || !target)) return fail(HWER_EINVAL, "%s: null queries or targets", what);
         if (!e || ldq < d || lde < d) return fail(HWER_EINVAL, "%s: null table or a row stride below d", what);
-        q_direct = ce_direct(q, ldq, d, dtype), e_direct = ce_direct(e, lde, d, dtype), dp = ce_padded(d);
+        q_direct = ce_direct(q, ldq, d, dtype), e_direct = !bias && ce_direct(e, lde, d, dtype), dp = ce_padded(d);
         y = ce_layout(n, v, d, dtype, q_direct, e_direct, want_mean);
         const size_t need = hwer_catalogue_ce_workspace_bytes(n, v, d, dtype, q_direct, e_direct, want_mean);
         if (!workspace || bytes < need) return fail(HWER_EWORKSPACE, "%s: workspace of %zu bytes needed", what, need);
@@ -955,7 +976,7 @@ struct CeCall {
 
     // lays out what the passes cannot read in place
     int prepare() const {
-        CePack p{{q, e}, {nullptr, nullptr}, {nullptr, nullptr}, {n, v}, {ldq, lde}, d, dp, at<float>(y.tops), at<CeScalars>(0), {0, 0}};
+        CePack p{{q, e}, {nullptr, nullptr}, {nullptr, nullptr}, {n, v}, {ldq, lde}, d, dp, at<float>(y.tops), at<CeScalars>(0), {0, 0}, target, bias};
         if (!q_direct) p.hi[0] = at<short>(y.q_hi);
         if (!e_direct) p.hi[1] = at<short>(y.e_hi);
         const dim3 grid(unsigned(std::max<int64_t>(1, std::min<int64_t>(cdiv64(std::max(n, v) * (dp / 8), 256), kMaxStreamBlocks))), 2);
@@ -988,6 +1009,7 @@ struct CeCall {
     CeRows rows() const {
         CeRows r{};
         r.e = e, r.lde = lde, r.bias = bias, r.target = target, r.n = n, r.v = v, r.d = d, r.dp = dp, r.scale = scale, r.sc = at<CeScalars>(0);
+        if (q_direct) r.q = static_cast<const short*>(q), r.ldq = ldq, r.q_copy = at<short>(y.q_hi);
         r.reduction = reduction, r.ld_rowp = ce_rowp_ld(n), r.off = ce_offset(dtype, 0), r.off2 = ce_offset(dtype, 1);
         return r;
     }
@@ -995,8 +1017,8 @@ struct CeCall {
     int pass2(void* de, int64_t ldde, float* dbias, bool rowg, const float* loss_rows, float* loss) const {
         const CeSplit s = ce_split(v, n, d);
         CePass p{};
-        p.stat = e_hi(), p.stat_lo = e_lo(), p.strm = q_hi(), p.strm_lo = q_lo();
-        p.ld_stat = e_ld(), p.ld_strm = q_ld(), p.n_stat = v, p.n_strm = n;
+        p.stat = e_hi(), p.stat_lo = e_lo(), p.strm = at<short>(y.q_hi), p.strm_lo = q_lo();      // (queries: laid out, or copied by the rows' kernel)
+        p.ld_stat = e_ld(), p.ld_strm = dp, p.n_stat = v, p.n_strm = n;
         p.bias = bias, p.scale = scale, p.sc = at<CeScalars>(0);
         p.subs_per_split = s.subs, p.n_splits = s.splits, p.stat_blocks = s.blocks;
         p.l = at<float>(y.l2), p.o = at<float>(y.o2);
@@ -1119,7 +1141,7 @@ int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_
     CeRows r = c.rows();
     r.state = reinterpret_cast<float4*>(const_cast<float*>(state)), r.mean = const_cast<float*>(mean), r.counted = counted, r.grad = grad, r.per_row = reduction == 0;
     r.dq = dq, r.lddq = lddq, r.rowp = de ? c.at<float>(c.y.rowp) : nullptr;
-    if (reduction == 0) ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(grad, n, r.sc);
+    if (reduction == 0) ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(grad, target, n, v, r.sc);
     if (int rc = c.backward_rows(r)) return rc;
     return de ? c.pass2(de, ldde, dbias, reduction == 0, nullptr, nullptr) : HWER_OK;
 }
@@ -1141,7 +1163,7 @@ int hwer_catalogue_ce_grads(const void* q, int64_t ldq, const void* e, int64_t l
         if (int rc = c.join<true>(r)) return rc;
     } else {
         r.per_row = 1, r.grad = loss_rows;      // no rows: the factors of a sum over nothing
-        ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(loss_rows, 0, r.sc);
+        ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(loss_rows, target, 0, v, r.sc);
         if (int rc = c.backward_rows(r)) return rc;
     }
     return c.pass2(de, ldde, dbias, false, loss_rows, loss);

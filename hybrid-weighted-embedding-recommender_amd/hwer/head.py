@@ -255,8 +255,10 @@ class _CeCall:
 
     def workspace(self, gradients):
         lib = self.lib
+        # (with a bias the table is laid out anew: rows that it takes out may hold anything)
+        in_place = self.b is None and lib.hwer_catalogue_ce_reads_in_place(P(self.e), self.lde, self.d, self.code)
         nbytes = lib.hwer_catalogue_ce_workspace_bytes(self.n, self.v, self.d, self.code, lib.hwer_catalogue_ce_reads_in_place(P(self.q), self.ldq, self.d, self.code),
-                                                       lib.hwer_catalogue_ce_reads_in_place(P(self.e), self.lde, self.d, self.code), gradients)
+                                                       in_place, gradients)
         return self.q.new_empty(nbytes, dtype=torch.uint8), nbytes
 
     def forward(self, want_mean):
@@ -313,8 +315,9 @@ def catalogue_cross_entropy(queries, table, targets, scale: float = 1.0, bias: O
     reduction "none" one for each row).  Logits are never in memory; gradients for queries, table and bias through autograd.
 
     queries (n, d), table (v, d): float32 / float16 / bfloat16 of one type, 1 <= d <= 256.  targets (n,): -1 = the row does not count (an unknown
-    node, as everywhere in this package); any other value outside the table makes its loss NaN.  scale > 0: 1 / temperature.  bias (v,) float32,
-    e.g. a correction for popularity; -inf takes a row out of the catalogue.  "mean" divides by the counted rows and is 0 without any."""
+    node, as everywhere in this package; padding); any other value outside the table makes its loss NaN.  scale > 0: 1 / temperature.  bias (v,) float32,
+    e.g. a correction for popularity; -inf takes a row out of the catalogue.  Rows that do not count or are taken out may hold anything, NaN and
+    infinities included; their gradients are zero.  float32 products keep 2^-22 of an element and 2^-40 of its operand's largest one.  "mean" divides by the counted rows and is 0 without any."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (queries, table, bias)):
         return _CatalogueCrossEntropy.apply(queries, table, bias, targets, scale, reduction)
     call = _CeCall(queries, table, targets, scale, bias, reduction)

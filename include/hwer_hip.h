@@ -564,7 +564,10 @@ int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int
  *   comes with de.  dq / de in the rows' type.  Every sum has a fixed order (no atomics).
  * hwer_catalogue_ce_grads: loss (reduction 1 / 2) and gradients in one call, without what the two calls hand over; float32 rows are laid out for the
  *   matrix instructions once.
- * Workspace: hwer_catalogue_ce_workspace_bytes(..., q_in_place, e_in_place = hwer_catalogue_ce_reads_in_place(rows, ld, d, dtype), ...). */
+ *   float32 rows are multiplied as two float16 terms relative to the operand's largest finite element: elements keep 2^-22 of themselves and 2^-40 of it.
+ *   Rows of q that do not count, and rows of e whose bias is -inf, may hold anything (NaN, infinities): they reach no other row.
+ * Workspace: hwer_catalogue_ce_workspace_bytes(..., q_in_place, e_in_place = hwer_catalogue_ce_reads_in_place(rows, ld, d, dtype), ...); with a bias the table
+ *   is never read in place (e_in_place = 0). */
 int hwer_catalogue_ce_max_dim(void);
 int hwer_catalogue_ce_reads_in_place(const void* rows, int64_t ld, int d, int dtype);
 size_t hwer_catalogue_ce_workspace_bytes(int64_t n, int64_t v, int d, int dtype, int q_in_place, int e_in_place, int want_gradients);

@@ -546,6 +546,58 @@ def test_cross_entropy_masks(hw, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,d", [(70, 333, 64), (300, 150, 128), (129, 1000, 100), (40, 500, 256)])
+def test_cross_entropy_unused_rows_hold_anything(hw, n, v, d, dtype):
+    """NaN, infinities and huge values in queries that do not count (padding) and in classes that are taken out: the same as zeros there, bit for bit"""
+    x, e, t, b = ce_inputs(n + d, n, v, d, dtype, bias=True)
+    b[3::7] = float("-inf")
+    t = torch.where(torch.isinf(b[t]), t - 1, t)
+    t[::3] = -1
+    t[-1] = -1
+    top = torch.finfo(dtype).max
+    bad_x, bad_e, clean_x, clean_e = x.clone(), e.clone(), x.clone(), e.clone()
+    clean_x[t == -1], clean_e[torch.isinf(b)] = 0, 0
+    for i, value in enumerate((float("nan"), float("inf"), -float("inf"), top, -top)):
+        bad_x[torch.nonzero(t == -1)[i::5, 0], i::3] = value
+        bad_e[torch.nonzero(torch.isinf(b))[i::5, 0], i::4] = value
+    t = t.cuda()
+    for queries, table, bias in (((bad_x, clean_x), (e, e), None), ((bad_x, clean_x), (bad_e, clean_e), b.cuda())):
+        got, want = ([], [])
+        for out, q, tab in ((got, queries[0].cuda(), table[0].cuda()), (want, queries[1].cuda(), table[1].cuda())):
+            out.extend(hw.catalogue_cross_entropy_grads(q, tab, t, scale=4.0, bias=bias))
+            out.append(hw.catalogue_cross_entropy(q, tab, t, scale=4.0, bias=bias, reduction="none"))
+            for reduction in ("mean", "none"):
+                leaves = [None if a is None else a.clone().requires_grad_() for a in (q, tab, bias)]
+                loss = hw.catalogue_cross_entropy(leaves[0], leaves[1], t, scale=4.0, bias=leaves[2], reduction=reduction)
+                up = torch.linspace(-1, 1, n, device="cuda")
+                if out is got:      # and so may the gradients that reach them
+                    up[t == -1] = torch.tensor([float("inf"), float("nan"), 1e30], device="cuda").repeat(n)[:int((t == -1).sum())]
+                loss.backward(up if reduction == "none" else None)
+                out.extend([loss.detach()] + [a.grad for a in leaves if a is not None])
+        assert all(torch.isfinite(a).all() and torch.equal(a, c) for a, c in zip(got, want))
+        close(want[0], ce_reference(queries[1], table[1], t.cpu(), 4.0, None if bias is None else b, torch.ones(n, dtype=torch.float64))["rows"].sum() / int((t >= 0).sum()), 2e-3 if dtype != torch.float32 else 1e-4)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_cross_entropy_a_bad_row_stays_alone(hw, dtype):
+    """a counted query with an infinity or NaN: its own loss and gradient are lost (and the sums it enters), the other rows' are not"""
+    n, v, d = 50, 200, 64
+    x, e, t, _ = ce_inputs(11, n, v, d, dtype)
+    want = hw.catalogue_cross_entropy(x.cuda(), e.cuda(), t.cuda(), scale=4.0, reduction="none")
+    y = x.clone()
+    y[7, 3], y[20, 5] = float("inf"), float("nan")
+    q = y.cuda().requires_grad_()
+    got = hw.catalogue_cross_entropy(q, e.cuda(), t.cuda(), scale=4.0, reduction="none")
+    keep = torch.ones(n, dtype=torch.bool)
+    keep[[7, 20]] = False
+    assert torch.equal(got.detach()[keep], want[keep]) and not torch.isfinite(got.detach()[~keep]).any()
+    got[keep.cuda()].sum().backward()
+    assert torch.isfinite(q.grad[keep]).all()
+
+
+@gpu
 def test_cross_entropy_targets(hw):
     """rows that do not count, no row that counts, no row at all, and targets that name nothing"""
     x, e, t, _ = ce_inputs(5, 50, 90, 64, torch.float32)
