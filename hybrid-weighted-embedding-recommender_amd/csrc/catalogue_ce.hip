@@ -538,7 +538,6 @@ struct CePack {
     int d, dp;
     float* tops;             // (2, kTopBlocks) partial maxima of |value|
     CeScalars* sc;
-    int vec[2];
     const int64_t* target;
     const float* bias;
     __device__ __forceinline__ bool used(int w, int64_t r) const {
@@ -559,8 +558,10 @@ __global__ __launch_bounds__(256) void ce_pack16_kernel(CePack a) {
         const short* p = static_cast<const short*>(a.src[w]) + r * a.ld[w];
         const int d = a.used(w, r) ? a.d : 0;
         s16x8 v;
+        if (c + 8 <= d) __builtin_memcpy(&v, p + c, 16);      // (at any alignment: 50 021 x 250 float16 with 1 037 queries 11.5 us, 17 element by element)
+        else
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < d ? p[c + j] : short(0);
+            for (int j = 0; j < 8; ++j) v[j] = c + j < d ? p[c + j] : short(0);
         *reinterpret_cast<s16x8*>(a.hi[w] + r * a.dp + c) = v;
     }
 }
@@ -569,11 +570,8 @@ __global__ __launch_bounds__(256) void ce_pack16_kernel(CePack a) {
 __device__ __forceinline__ void ce_load8(const CePack& a, int w, int64_t r, int c, float (&v)[8]) {
     const float* p = static_cast<const float*>(a.src[w]) + r * a.ld[w] + c;
     const int d = a.used(w, r) ? a.d : 0;
-    if (a.vec[w]) {      // rows on 16 bytes, of a multiple of 4 values
-        float4 u = {0.f, 0.f, 0.f, 0.f}, t = u;
-        if (c < d) u = *reinterpret_cast<const float4*>(p);
-        if (c + 4 < d) t = *reinterpret_cast<const float4*>(p + 4);
-        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w, v[4] = t.x, v[5] = t.y, v[6] = t.z, v[7] = t.w;
+    if (c + 8 <= d) {
+        __builtin_memcpy(v, p, 32);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = c + j < d ? p[j] : 0.f;
@@ -976,13 +974,12 @@ struct CeCall {
 
     // lays out what the passes cannot read in place
     int prepare() const {
-        CePack p{{q, e}, {nullptr, nullptr}, {nullptr, nullptr}, {n, v}, {ldq, lde}, d, dp, at<float>(y.tops), at<CeScalars>(0), {0, 0}, target, bias};
+        CePack p{{q, e}, {nullptr, nullptr}, {nullptr, nullptr}, {n, v}, {ldq, lde}, d, dp, at<float>(y.tops), at<CeScalars>(0), target, bias};
         if (!q_direct) p.hi[0] = at<short>(y.q_hi);
         if (!e_direct) p.hi[1] = at<short>(y.e_hi);
         const dim3 grid(unsigned(std::max<int64_t>(1, std::min<int64_t>(cdiv64(std::max(n, v) * (dp / 8), 256), kMaxStreamBlocks))), 2);
         if (dtype == HWER_F32) {
             p.lo[0] = at<short>(y.q_lo), p.lo[1] = at<short>(y.e_lo);
-            p.vec[0] = d % 4 == 0 && aligned_to(q, ldq * 4, 16), p.vec[1] = d % 4 == 0 && aligned_to(e, lde * 4, 16);
             ce_top_kernel<<<dim3(kTopBlocks, 2), dim3(256), 0, st>>>(p);
             ce_split_kernel<<<grid, dim3(256), 0, st>>>(p);
         } else if (p.hi[0] || p.hi[1]) {

@@ -290,11 +290,17 @@ __global__ __launch_bounds__(64 * WM * WN, (STAGES == 1 ? 4 : 2)) void matmul_q8
     if (int(threadIdx.x) < TN) s_scale[threadIdx.x] = my_scale, s_bias[threadIdx.x] = my_bias;
     // C fragment: column (lane & 31) = row m of the output, register rows = 4 consecutive n at a time.  Written through LDS, 32 rows of each wave at a time, so
     // that lanes write neighbouring bytes of a whole row of the tile: parts of memory lines cost as much as whole ones.
+    // (Waves meet here with their LDS work done, not their stores: those of the last rows may be under way while the next ones are made.)
+    auto meet_lds = [&]() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
     constexpr int PIECE = 16 / int(sizeof(O)), LPR = TN / PIECE, RPI = 64 / LPR;      // elements of 16 bytes, lanes of a row, rows of an instruction
     const int cols = int(std::min<int64_t>(TN, g.n - n0));
 #pragma unroll
     for (int x = 0; x < XM; ++x) {
-        meet(all_t());
+        meet_lds();
 #pragma unroll
         for (int y = 0; y < XN; ++y)
 #pragma unroll
@@ -308,7 +314,7 @@ __global__ __launch_bounds__(64 * WM * WN, (STAGES == 1 ? 4 : 2)) void matmul_q8
                               finish<O>(acc[x][y][4 * q + 2], sa, sb.z, bi.z), finish<O>(acc[x][y][4 * q + 3], sa, sb.w, bi.w)};
                 *reinterpret_cast<o4*>(s_buf + ((wave % WM) * 32 + l31) * OROW + c * int(sizeof(O))) = v;
             }
-        meet(all_t());
+        meet_lds();
         constexpr int RPW = 32 * WM / WAVES;      // rows of a wave
 #pragma unroll
         for (int i = 0; i < RPW / RPI; ++i) {
