@@ -905,11 +905,13 @@ static size_t up(size_t b) { return (b + 255) & ~size_t(255); }
 // Where a call's workspace keeps what.  The head (scalars, laid-out operands) serves both passes of a call.
 struct CeLayout {
     size_t tops, q_hi, q_lo, e_hi, e_lo, loss_rows, counts, rowp, head, zt, m, l, o, fwd_end, l2, o2, bwd_end;
+    CeSplit f, b;      // of pass 1 and 2
+    size_t bytes(bool want_mean) const { return std::max<size_t>(256, want_mean ? std::max(fwd_end, bwd_end) : fwd_end); }
 };
 static CeLayout ce_layout(int64_t n, int64_t v, int d, int dtype, bool q_direct, bool e_direct, bool want_mean) {
     const size_t dp = ce_padded(d);
     CeLayout y{};
-    const CeSplit f = ce_split(n, v, d), b = ce_split(v, n, d);
+    const CeSplit f = y.f = ce_split(n, v, d), b = y.b = ce_split(v, n, d);
     size_t at = 256;      // CeScalars
     y.tops = at, at += dtype == HWER_F32 ? 2 * kTopBlocks * 4 : 0;
     y.q_hi = at, at += q_direct && !want_mean ? 0 : up(size_t(n) * dp * 2);
@@ -966,7 +968,7 @@ struct CeCall {
         if (!e || ldq < d || lde < d) return fail(HWER_EINVAL, "%s: null table or a row stride below d", what);
         q_direct = ce_direct(q, ldq, d, dtype), e_direct = !bias && ce_direct(e, lde, d, dtype), dp = ce_padded(d);
         y = ce_layout(n, v, d, dtype, q_direct, e_direct, want_mean);
-        const size_t need = hwer_catalogue_ce_workspace_bytes(n, v, d, dtype, q_direct, e_direct, want_mean);
+        const size_t need = y.bytes(want_mean);
         if (!workspace || bytes < need) return fail(HWER_EWORKSPACE, "%s: workspace of %zu bytes needed", what, need);
         ws = static_cast<unsigned char*>(workspace), st = as_stream(stream);
         return HWER_OK;
@@ -989,7 +991,7 @@ struct CeCall {
     }
 
     int pass1(bool mean, CeRows& r) const {
-        const CeSplit s = ce_split(n, v, d);
+        const CeSplit& s = y.f;
         CePass p{};
         p.stat = q_hi(), p.stat_lo = q_lo(), p.strm = e_hi(), p.strm_lo = e_lo();
         p.ld_stat = q_ld(), p.ld_strm = e_ld(), p.n_stat = n, p.n_strm = v;
@@ -1012,7 +1014,7 @@ struct CeCall {
     }
 
     int pass2(void* de, int64_t ldde, float* dbias, bool rowg, const float* loss_rows, float* loss) const {
-        const CeSplit s = ce_split(v, n, d);
+        const CeSplit& s = y.b;
         CePass p{};
         p.stat = e_hi(), p.stat_lo = e_lo(), p.strm = at<short>(y.q_hi), p.strm_lo = q_lo();      // (queries: laid out, or copied by the rows' kernel)
         p.ld_stat = e_ld(), p.ld_strm = dp, p.n_stat = v, p.n_strm = n;
@@ -1102,8 +1104,7 @@ int hwer_catalogue_ce_reads_in_place(const void* rows, int64_t ld, int d, int dt
 
 size_t hwer_catalogue_ce_workspace_bytes(int64_t n, int64_t v, int d, int dtype, int q_in_place, int e_in_place, int want_gradients) {
     if (!known_dtype(dtype) || d < 1 || d > hwer_catalogue_ce_max_dim() || n < 0 || v < 1) return 0;
-    const CeLayout y = ce_layout(n, v, d, dtype, q_in_place != 0, e_in_place != 0, want_gradients != 0);
-    return std::max<size_t>(256, want_gradients ? std::max(y.fwd_end, y.bwd_end) : y.fwd_end);
+    return ce_layout(n, v, d, dtype, q_in_place != 0, e_in_place != 0, want_gradients != 0).bytes(want_gradients != 0);
 }
 
 int hwer_catalogue_ce(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int d, int dtype,

@@ -684,6 +684,69 @@ def test_cross_entropy_is_the_same_every_time(hw):
         assert all(torch.equal(p, q) for p, q in zip(first, hw.catalogue_cross_entropy_grads(x, e, t, scale=5.0, bias=b)))
 
 
+# ---------------------------------------------------------------------------------------------------------------- offsets beyond 32 bits
+@gpu
+def test_rows_beyond_32_bits(hw):
+    """the last rows of operands and outputs of more than 2^32 bytes (and elements): the same as those rows by themselves"""
+    free = torch.cuda.mem_get_info()[0]
+    if free < 60 << 30:
+        pytest.skip("60 GB of device memory needed, %d GB free" % (free >> 30))
+    n, d = (1 << 21) + 5, 1024
+    g = torch.Generator("cuda").manual_seed(1)
+    x = torch.randn(n, d, device="cuda", dtype=torch.bfloat16, generator=g)
+    w = torch.randn(d, device="cuda", generator=g)
+    last = slice(n - 7, n)
+    y, h = hw.rms_norm(x, w, x)
+    want = hw.rms_norm(x[last].contiguous(), w, x[last].contiguous())
+    assert torch.equal(y[last], want[0]) and torch.equal(h[last], want[1])
+    dx, _ = hw.rms_norm_grads(y, h, w)
+    assert torch.equal(dx[last], hw.rms_norm_grads(y[last].contiguous(), h[last].contiguous(), w)[0])
+    del y, h, dx
+    q, s = hw.quantize_rows_q8(x)
+    qw, sw = hw.quantize_rows_q8(x[last].contiguous())
+    assert torch.equal(q[last], qw) and torch.equal(s[last], sw)
+    del x, q, s
+    # products: an output, and an operand
+    m, k = 66001, 64
+    a, b = (torch.randint(-127, 128, (m, k), device="cuda", dtype=torch.int8, generator=g) for _ in range(2))
+    one = torch.ones(m, device="cuda")
+    out = hw.matmul_q8(a, one, b, one, out_dtype=torch.bfloat16)
+    assert out.numel() > 1 << 32 and torch.equal(out[-200:, -200:], (a[-200:].double() @ b[-200:].double().t()).bfloat16())
+    del out
+    rows = 68_000_003
+    tall = torch.randint(-127, 128, (rows, k), device="cuda", dtype=torch.int8, generator=g)
+    one = torch.ones(rows, device="cuda")
+    for few in (3, 40):
+        out = hw.matmul_q8(tall, one, b[:few].contiguous(), one[:few], out_dtype=torch.bfloat16)
+        assert torch.equal(out[-100:], (tall[-100:].double() @ b[:few].double().t()).bfloat16())
+    out = hw.matmul_q8(b[:2].contiguous(), one[:2], tall, one)
+    assert torch.equal(out[:, -100:].double(), b[:2].double() @ tall[-100:].double().t())
+    del tall, out, one
+    # a catalogue of equal blocks: p is a block's, divided by their number
+    block, copies, n, d = 1 << 20, 17, 40, 128
+    e = torch.randn(block, d, device="cuda", dtype=torch.bfloat16, generator=g) / 8
+    table = e.repeat(copies, 1)
+    x = torch.randn(n, d, device="cuda", dtype=torch.bfloat16, generator=g) / 8
+    t = torch.randint(0, block, (n,), device="cuda", generator=g)
+    assert table.numel() * 2 > 1 << 32
+    far = t + (copies - 1) * block
+    got = hw.catalogue_cross_entropy(x, table, far, scale=4.0, reduction="none")
+    z = 4.0 * (x.double() @ e.double().t())
+    want = torch.logsumexp(z, 1) + math.log(copies) - z.gather(1, t[:, None])[:, 0]
+    close(got, want.cpu(), (2 * 30 * 8 * math.sqrt(3 * d) + 8 * math.sqrt(block * copies)) * U32, "rows")
+    loss, dx, de = hw.catalogue_cross_entropy_grads(x, table, far, scale=4.0)
+    # (a float32 sum of 17.8 M terms: 8 sqrt(v) 2^-24 = 2e-3 of the magnitudes, half of which is allowed beside the weights' roundings)
+    p = torch.softmax(z, 1)
+    dw = 4.0 / n * (p @ e.double() - e[t].double())
+    close(dx, dw.cpu(), dw.abs().cpu() * U[torch.bfloat16] + 4.0 / n * ((p @ e.double().abs()) * (U[torch.bfloat16] + 1e-3) + e[t].double().abs() * 1e-3).cpu(), "dx")
+    other = torch.ones(block, dtype=torch.bool, device="cuda")
+    other[t] = False
+    assert torch.equal(de[:block][other], de[-block:][other])
+    want = 4.0 / n * (p[:, t].t() @ x.double() / copies - torch.eye(n, device="cuda", dtype=torch.double) @ x.double())
+    if len(t.unique()) == n:
+        close(de[far], want.cpu(), want.abs().cpu() * U[torch.bfloat16] * 2 + 4.0 / n * x.double().abs().cpu() * 1e-3, "de")
+
+
 # ---------------------------------------------------------------------------------------------------------------- together, streams, graphs
 def _train_and_serve(hw, x, res, w, table, t):
     y, h = hw.rms_norm(x, w, res)
