@@ -377,12 +377,25 @@ __global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__
 }
 
 // ---------------------------------------------------------------------------------------------------------------- rows too wide for registers
+// Read twice, 16 bytes a lane, the second time from the caches while few rows are under way.
 constexpr int kWideThreads = 1024;
+
+template <typename W, int N>
+__device__ __forceinline__ Pack<W, N> load_weights(const W* w, int c, int d) {      // (none: ones)
+    if (w) return load_pack<W, N>(w, c, d);
+    Pack<W, N> v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v.e[j] = W(1.f);
+    return v;
+}
 
 template <typename E, typename W, bool Q8>
 __global__ __launch_bounds__(kWideThreads) void norm_fwd_wide_kernel(NormFwdArgs a) {
     __shared__ float s_sum[2 * (kWideThreads / 64)];
     __shared__ double s_top[kWideThreads / 64];
+    constexpr int VW = 16 / int(sizeof(E));
+    typedef Pack<E, VW> PE;
+    typedef Pack<W, VW> PW;
     const int t = threadIdx.x;
     const W* wp = static_cast<const W*>(a.w);
     int flip = 0;
@@ -390,17 +403,29 @@ __global__ __launch_bounds__(kWideThreads) void norm_fwd_wide_kernel(NormFwdArgs
         const E* x = static_cast<const E*>(a.x) + r * a.ldx;
         const E* q = a.res ? static_cast<const E*>(a.res) + r * a.ldr : nullptr;
         // the sum is formed again from the inputs in each pass: `h` may share memory with nothing, but is written once only
-        auto value = [&](int c) { return q ? float(E(float(x[c]) + float(q[c]))) : float(x[c]); };
+        auto load = [&](int c) {
+            PE h = load_pack<E, VW>(x, c, a.d);
+            if (q) {
+                const PE p = load_pack<E, VW>(q, c, a.d);
+#pragma unroll
+                for (int j = 0; j < VW; ++j) h.e[j] = E(float(h.e[j]) + float(p.e[j]));
+            }
+            return h;
+        };
         float ss = 0.f;
         double top = 0.0;
         float bad = 0.f;
-        for (int c = t; c < a.d; c += kWideThreads) {
-            const float hv = value(c);
-            ss = fmaf(hv, hv, ss);
-            if (Q8) {
-                    const float wv = wp ? float(wp[c]) : 1.f;
-                top = fmax(top, fabs(double(hv) * double(wv)));
-                bad = fmaf(hv * wv, 0.f, bad);      // becomes NaN with any NaN or infinity
+        for (int c = t * VW; c < a.d; c += kWideThreads * VW) {      // (past the row's end h is 0)
+            const PE h = load(c);
+            const PW w = Q8 ? load_weights<W, VW>(wp, c, a.d) : PW();
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                const float hv = float(h.e[j]);
+                ss = fmaf(hv, hv, ss);
+                if (Q8) {
+                    top = fmax(top, fabs(double(hv) * double(float(w.e[j]))));
+                    bad = fmaf(hv * float(w.e[j]), 0.f, bad);      // becomes NaN with any NaN or infinity
+                }
             }
         }
         float rstd = 1.f;
@@ -419,15 +444,25 @@ __global__ __launch_bounds__(kWideThreads) void norm_fwd_wide_kernel(NormFwdArgs
             inv = fine ? 127.f / float(top) : 0.f;
             if (t == 0) a.scale[r] = top < double(INFINITY) ? float(top) * rstd / 127.f : NAN;
         }
-        for (int c = t; c < a.d; c += kWideThreads) {
-            const float hv = value(c), wv = wp ? float(wp[c]) : 1.f;
-            if (a.res) static_cast<E*>(a.h)[r * a.ldh + c] = E(hv);
-            if (Q8) {
-                const float quo = hv * wv * inv, code = rintf(quo);
-                const bool open = top < 1e-30 || q8_open(quo, code);
-                static_cast<int8_t*>(a.y)[r * a.ldy + c] = !fine ? int8_t(0) : int8_t(open ? q8_exact(hv, wv, top) : int(code));
+        for (int c = t * VW; c < a.d; c += kWideThreads * VW) {
+            const PE h = load(c);
+            const PW w = load_weights<W, VW>(wp, c, a.d);
+            if (a.res) store_pack<E, VW>(static_cast<E*>(a.h) + r * a.ldh, c, a.d, h);
+            PE y;
+            Pack<int8_t, VW> code;
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                const float hv = float(h.e[j]), wv = float(w.e[j]);
+                if (Q8) {
+                    const float quo = hv * wv * inv, near = rintf(quo);
+                    const bool open = top < 1e-30 || q8_open(quo, near);
+                    code.e[j] = !fine ? int8_t(0) : int8_t(open ? q8_exact(hv, wv, top) : int(near));
+                } else {
+                    y.e[j] = E(hv * rstd * wv);
+                }
             }
-            else static_cast<E*>(a.y)[r * a.ldy + c] = E(hv * rstd * wv);
+            if constexpr (Q8) store_pack<int8_t, VW>(static_cast<int8_t*>(a.y) + r * a.ldy, c, a.d, code);
+            else store_pack<E, VW>(static_cast<E*>(a.y) + r * a.ldy, c, a.d, y);
         }
     }
 }
@@ -436,6 +471,9 @@ __global__ __launch_bounds__(kWideThreads) void norm_fwd_wide_kernel(NormFwdArgs
 template <typename E, typename W>
 __global__ __launch_bounds__(kWideThreads) void norm_bwd_wide_kernel(NormBwdArgs a, float* __restrict__ rstd_out) {
     __shared__ float s_sum[4 * (kWideThreads / 64)];
+    constexpr int VW = 16 / int(sizeof(E));
+    typedef Pack<E, VW> PE;
+    typedef Pack<W, VW> PW;
     const int t = threadIdx.x;
     const W* wp = static_cast<const W*>(a.w);
     int flip = 0;
@@ -443,19 +481,33 @@ __global__ __launch_bounds__(kWideThreads) void norm_bwd_wide_kernel(NormBwdArgs
         const E* h = static_cast<const E*>(a.h) + r * a.ldh;
         const E* g = static_cast<const E*>(a.dy) + r * a.lddy;
         float ss = 0.f, sc = 0.f;
-        for (int c = t; c < a.d; c += kWideThreads) {
-            const float hv = float(h[c]);
-            ss = fmaf(hv, hv, ss);
-            sc = fmaf(hv * (wp ? float(wp[c]) : 1.f), float(g[c]), sc);
+        for (int c = t * VW; c < a.d; c += kWideThreads * VW) {
+            const PE hp = load_pack<E, VW>(h, c, a.d), gp = load_pack<E, VW>(g, c, a.d);
+            const PW w = load_weights<W, VW>(wp, c, a.d);
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                const float hv = float(hp.e[j]);
+                ss = fmaf(hv, hv, ss);
+                sc = fmaf(hv * float(w.e[j]), float(gp.e[j]), sc);
+            }
         }
         ss = row_sum<kWideThreads>(ss, s_sum, flip);
         sc = row_sum<kWideThreads>(sc, s_sum + 2 * (kWideThreads / 64), flip);
         const float rstd = 1.f / sqrtf(ss / float(a.d) + a.eps);
         const float back = (sc / float(a.d)) * rstd * rstd;
-        for (int c = t; c < a.d; c += kWideThreads) {
-            float v = rstd * ((wp ? float(wp[c]) : 1.f) * float(g[c]) - float(h[c]) * back);
-            if (a.dh) v += float(static_cast<const E*>(a.dh)[r * a.lddh + c]);
-            static_cast<E*>(a.dx)[r * a.lddx + c] = E(v);
+        for (int c = t * VW; c < a.d; c += kWideThreads * VW) {
+            const PE hp = load_pack<E, VW>(h, c, a.d), gp = load_pack<E, VW>(g, c, a.d);
+            const PW w = load_weights<W, VW>(wp, c, a.d);
+            PE add;
+            if (a.dh) add = load_pack<E, VW>(static_cast<const E*>(a.dh) + r * a.lddh, c, a.d);
+            PE dx;
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                float v = rstd * (float(w.e[j]) * float(gp.e[j]) - float(hp.e[j]) * back);
+                if (a.dh) v += float(add.e[j]);
+                dx.e[j] = E(v);
+            }
+            store_pack<E, VW>(static_cast<E*>(a.dx) + r * a.lddx, c, a.d, dx);
         }
         if (rstd_out && t == 0) rstd_out[r] = rstd;
     }
@@ -595,7 +647,7 @@ int hwer_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t 
             const int grid = norm_grid(rows, kWideThreads);
             norm_bwd_wide_kernel<E, W><<<dim3(grid), dim3(kWideThreads), 0, st>>>(a, rstd);
             if (a.dw_part) {
-                parts = int(std::min<int64_t>(kWideDwParts, rows));
+                parts = int(std::min<int64_t>(kWideDwParts, cdiv64(rows, 64)));      // (16 waves share a part's rows)
                 norm_dw_wide_kernel<E><<<dim3((d + 63) / 64, parts), dim3(1024), 0, st>>>(a, rstd, int(cdiv64(rows, parts)));
             }
             return;
