@@ -647,7 +647,7 @@ int hwer_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t 
             const int grid = norm_grid(rows, kWideThreads);
             norm_bwd_wide_kernel<E, W><<<dim3(grid), dim3(kWideThreads), 0, st>>>(a, rstd);
             if (a.dw_part) {
-                parts = int(std::min<int64_t>(kWideDwParts, cdiv64(rows, 64)));      // (16 waves share a part's rows)
+                parts = int(std::min<int64_t>(kWideDwParts, cdiv64(rows, 64)));      // (16 waves share a part's rows: 152 x 20 000 bfloat16 5.3 us, 18.6 as 32 parts)
                 norm_dw_wide_kernel<E><<<dim3((d + 63) / 64, parts), dim3(1024), 0, st>>>(a, rstd, int(cdiv64(rows, parts)));
             }
             return;

@@ -42,6 +42,19 @@ def _stream(t):
     return _stream_of(t.get_device())
 
 
+def _like(t, dtype=None):
+    """An empty contiguous tensor of t's shape (two thirds of `new_empty`'s time)."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
+def _wants_grad(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def _check_rows(name, t, dtypes=_DTYPES, dim=2):
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s: a device tensor is needed, got %s" % (name, type(t).__name__))
@@ -104,8 +117,8 @@ def _norm_forward(x, weight, residual, eps):
     rr, ldr = _flat(residual) if residual is not None else (None, 0)
     n, d = xr.shape
     with _on(x):
-        y = x.new_empty(x.shape)
-        h = x.new_empty(x.shape) if residual is not None else None
+        y = _like(x)
+        h = _like(x) if residual is not None else None
         native.check(native.lib().hwer_rms_norm(P(xr), ldx, P(rr), ldr, P(w), wt, n, d, _DTYPES[x.dtype], eps, P(y), d, P(h), d, _stream(x)), "rms_norm")
     return y, h
 
@@ -127,7 +140,7 @@ def _norm_backward(dy, h, weight, eps, dh, want_dw):
     n, d = hr.shape
     lib = native.lib()
     with _on(h):
-        dx = h.new_empty(h.shape)
+        dx = _like(h)
         dw = torch.empty_like(w) if want_dw else None
         nbytes = lib.hwer_rms_norm_backward_workspace_bytes(n, d) if want_dw else 0
         ws = h.new_empty(nbytes, dtype=torch.uint8) if want_dw else None
@@ -160,7 +173,7 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-6):
     x: float32 / float16 / bfloat16, any number of leading dimensions; weight: (d,) float32 or x's type, None = ones."""
     _norm_checks(x, weight, residual, eps)
     eps = float(eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if _wants_grad(x, weight, residual):
         return _RmsNorm.apply(x, weight, residual, eps)
     y, h = _norm_forward(x, weight, residual, eps)
     return y if h is None else (y, h)
@@ -172,11 +185,13 @@ def _codes(x, weight, residual, eps, norm):
     rr, ldr = _flat(residual) if residual is not None else (None, 0)
     n, d = xr.shape
     with _on(x):
-        q = x.new_empty(x.shape, dtype=torch.int8)
-        scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
-        h = x.new_empty(x.shape) if residual is not None else None
+        q = _like(x, torch.int8)
+        scale = x.new_empty(n, dtype=torch.float32)
+        h = _like(x) if residual is not None else None
         native.check(native.lib().hwer_rms_norm_q8(P(xr), ldx, P(rr), ldr, P(w), wt, n, d, _DTYPES[x.dtype], norm, eps, P(q), d, P(scale), P(h), d,
                                                    _stream(x)), "rms_norm_q8")
+    if x.dim() != 2:
+        scale = scale.view(x.shape[:-1])
     return (q, scale) if h is None else (q, scale, h)
 
 
@@ -211,7 +226,7 @@ def matmul_q8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
     m, n, k = a.shape[0], b.shape[0], a.shape[1]
     sa, sb, bi = a_scale.contiguous(), b_scale.contiguous(), None if bias is None else bias.contiguous()
     with _on(a):
-        out = a.new_empty((m, n), dtype=out_dtype)
+        out = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=a.device)
         native.check(native.lib().hwer_matmul_q8(P(ar), lda, P(sa), P(br), ldb, P(sb), P(bi), m, n, k, P(out), n, _DTYPES[out_dtype], _stream(a)), "matmul_q8")
     return out
 
@@ -272,17 +287,17 @@ class _CeCall:
 
     def backward(self, grad, want_q, want_e, want_b):
         ws, nbytes = self.workspace(True)
-        dq = self.q.new_empty((self.n, self.d)) if want_q else None
-        de = self.q.new_empty((self.v, self.d)) if want_e or want_b else None
-        db = self.q.new_empty(self.v, dtype=torch.float32) if want_b else None
+        dq = _like(self.q) if want_q else None
+        de = _like(self.e) if want_e or want_b else None
+        db = _like(self.b) if want_b else None
         native.check(self.lib.hwer_catalogue_ce_backward(*self.operands(), P(grad), P(self.state), P(self.counted), P(self.mean), P(dq), self.d, P(de), self.d, P(db),
                                                          P(ws), nbytes, _stream(self.q)), "catalogue_cross_entropy(backward)")
         return dq, de if want_e else None, db
 
     def gradients(self):
         ws, nbytes = self.workspace(True)
-        loss, dq, de = self.q.new_empty((), dtype=torch.float32), self.q.new_empty((self.n, self.d)), self.q.new_empty((self.v, self.d))
-        db = None if self.b is None else self.q.new_empty(self.v, dtype=torch.float32)
+        loss, dq, de = self.q.new_empty((), dtype=torch.float32), _like(self.q), _like(self.e)
+        db = None if self.b is None else _like(self.b)
         native.check(self.lib.hwer_catalogue_ce_grads(*self.operands(), P(loss), P(dq), self.d, P(de), self.d, P(db), P(ws), nbytes, _stream(self.q)),
                      "catalogue_cross_entropy_grads")
         return (loss, dq, de) if db is None else (loss, dq, de, db)
@@ -318,7 +333,7 @@ def catalogue_cross_entropy(queries, table, targets, scale: float = 1.0, bias: O
     node, as everywhere in this package; padding); any other value outside the table makes its loss NaN.  scale > 0: 1 / temperature.  bias (v,) float32,
     e.g. a correction for popularity; -inf takes a row out of the catalogue.  Rows that do not count or are taken out may hold anything, NaN and
     infinities included; their gradients are zero.  float32 products keep 2^-22 of an element and 2^-40 of its operand's largest one.  "mean" divides by the counted rows and is 0 without any."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (queries, table, bias)):
+    if _wants_grad(queries, table, bias):
         return _CatalogueCrossEntropy.apply(queries, table, bias, targets, scale, reduction)
     call = _CeCall(queries, table, targets, scale, bias, reduction)
     with call.on():
