@@ -75,10 +75,9 @@ def _check_device(t, *others):
 
 def _rows(t):
     """(tensor, row stride) of 2-d rows whose elements are contiguous; anything else (a transposed view, a broadcast row) is copied."""
-    n, d = t.shape
     if t.is_contiguous():
-        return t, d
-    row, one = t.stride()
+        return t, t.shape[1]
+    (n, d), (row, one) = t.shape, t.stride()
     if (one == 1 or d == 1) and (row >= d or n <= 1):
         return t, max(row, d)
     return t.contiguous(), d
@@ -86,15 +85,21 @@ def _rows(t):
 
 def _flat(t):
     """... of rows along the last dimension of any number of leading ones"""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     return _rows(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
+
+
+def _is_vector(t, n):
+    return t.dim() == 1 and t.shape[0] == n
 
 
 def _weight(weight, x):
     if weight is None:
         return None, 0
-    if weight.dtype not in (torch.float32, x.dtype):
+    if weight.dtype is not torch.float32 and weight.dtype is not x.dtype:
         raise TypeError("weight: float32 or the rows' type (%s), got %s" % (x.dtype, weight.dtype))
-    if tuple(weight.shape) != (x.shape[-1],):
+    if not _is_vector(weight, x.shape[-1]):
         raise ValueError("weight: shape (%d,) needed, got %s" % (x.shape[-1], tuple(weight.shape)))
     return (weight if weight.is_contiguous() else weight.contiguous()), _DTYPES[weight.dtype]
 
@@ -115,7 +120,8 @@ def _norm_forward(x, weight, residual, eps):
     w, wt = _weight(weight, x)
     xr, ldx = _flat(x)
     rr, ldr = _flat(residual) if residual is not None else (None, 0)
-    n, d = xr.shape
+    d = x.shape[-1]
+    n = x.numel() // d
     with _on(x):
         y = _like(x)
         h = _like(x) if residual is not None else None
@@ -137,7 +143,8 @@ def _norm_backward(dy, h, weight, eps, dh, want_dw):
     w, wt = _weight(weight, h)
     (hr, ldh), (gr, ldg) = _flat(h), _flat(dy)
     ar, lda = _flat(dh) if dh is not None else (None, 0)
-    n, d = hr.shape
+    d = h.shape[-1]
+    n = h.numel() // d
     lib = native.lib()
     with _on(h):
         dx = _like(h)
@@ -183,7 +190,8 @@ def _codes(x, weight, residual, eps, norm):
     w, wt = _weight(weight, x)
     xr, ldx = _flat(x)
     rr, ldr = _flat(residual) if residual is not None else (None, 0)
-    n, d = xr.shape
+    d = x.shape[-1]
+    n = x.numel() // d
     with _on(x):
         q = _like(x, torch.int8)
         scale = x.new_empty(n, dtype=torch.float32)
@@ -209,6 +217,11 @@ def quantize_rows_q8(x):
 
 
 # ---------------------------------------------------------------------------------------------------------------- 8-bit product
+def _check_vector(name, t, n):
+    if t.dtype is not torch.float32 or not _is_vector(t, n):
+        raise ValueError("%s: float32 of shape (%d,) needed, got %s %s" % (name, n, t.dtype, tuple(t.shape)))
+
+
 def matmul_q8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
     """out = (a @ b.T) * a_scale[:, None] * b_scale (+ bias): a (m, k) and b (n, k) int8 codes, a_scale (m,), b_scale (n,), bias (n,) float32;
     out (m, n) float32 / float16 / bfloat16.  The integer sums are exact (k <= 131 071)."""
@@ -219,11 +232,12 @@ def matmul_q8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
         raise ValueError("rows of %d against rows of %d codes" % (a.shape[1], b.shape[1]))
     if out_dtype not in _DTYPES:
         raise TypeError("out_dtype: float32, float16 or bfloat16, got %s" % out_dtype)
-    for name, t, n in (("a_scale", a_scale, a.shape[0]), ("b_scale", b_scale, b.shape[0]), ("bias", bias, b.shape[0])):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (n,)):
-            raise ValueError("%s: float32 of shape (%d,) needed, got %s %s" % (name, n, t.dtype, tuple(t.shape)))
+    (m, k), n = a.shape, b.shape[0]
+    _check_vector("a_scale", a_scale, m)
+    _check_vector("b_scale", b_scale, n)
+    if bias is not None:
+        _check_vector("bias", bias, n)
     (ar, lda), (br, ldb) = _rows(a), _rows(b)
-    m, n, k = a.shape[0], b.shape[0], a.shape[1]
     sa, sb, bi = a_scale.contiguous(), b_scale.contiguous(), None if bias is None else bias.contiguous()
     with _on(a):
         out = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=a.device)
@@ -241,10 +255,10 @@ class _CeCall:
         if table.dtype != queries.dtype or table.shape[1] != queries.shape[1]:
             raise ValueError("table: rows of the queries' width and type needed (%d %s), got %s %s" % (queries.shape[1], queries.dtype, tuple(table.shape), table.dtype))
         _check_device(queries, table, targets, bias)
-        if targets.dtype not in (torch.int64, torch.int32) or tuple(targets.shape) != (queries.shape[0],):
+        if targets.dtype not in (torch.int64, torch.int32) or not _is_vector(targets, queries.shape[0]):
             raise ValueError("targets: int64 or int32 of shape (%d,) needed, got %s %s" % (queries.shape[0], targets.dtype, tuple(targets.shape)))
-        if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (table.shape[0],)):
-            raise ValueError("bias: float32 of shape (%d,) needed, got %s %s" % (table.shape[0], bias.dtype, tuple(bias.shape)))
+        if bias is not None:
+            _check_vector("bias", bias, table.shape[0])
         if reduction not in _REDUCTIONS:
             raise ValueError("reduction: one of %s, got %r" % (sorted(_REDUCTIONS), reduction))
         self.scale = float(scale)
@@ -265,7 +279,8 @@ class _CeCall:
         return _on(self.q)
 
     def operands(self):
-        self.t = self.targets.to(torch.int64).contiguous()
+        t = self.targets
+        self.t = t if t.dtype is torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
         return P(self.q), self.ldq, P(self.e), self.lde, P(self.b), P(self.t), self.n, self.v, self.d, self.code, self.scale, self.reduction
 
     def workspace(self, gradients):
