@@ -7,7 +7,8 @@
 
 Everything takes and returns device tensors on their own device, runs on its current stream, never synchronises and may be captured into a
 hipGraph.  `rms_norm` and `catalogue_cross_entropy` take part in autograd where an input requires a gradient; the `_grads` functions return
-the gradients directly and keep nothing (what a resident training step calls).  The reference trains in DGL / PyTorch (hwer/gcn_ncf.py:126-327:
+the gradients directly and keep nothing (what a resident training step calls, and the simple form to capture: torch's own accumulators of leaf
+gradients belong to the stream that made them, so a captured `backward()` needs leaves of which no graph from outside the capture is alive).  The reference trains in DGL / PyTorch (hwer/gcn_ncf.py:126-327:
 out of scope here); what it hands to the search are rows (hwer/gcn_ncf.py:431,447-456).
 
 Errors: wrong shapes, types or devices raise before anything is launched (ValueError / TypeError; HwerNativeError from the library).  Values are
