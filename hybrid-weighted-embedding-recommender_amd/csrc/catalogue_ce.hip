@@ -93,7 +93,8 @@ template <int TERMS, int DP> constexpr int ce_sub() { return TERMS * DP <= 128 |
 // Waves of a SIMD that registers are shared out for.  An MFMA occupies its own wave for all its passes, so a wave never overlaps its products with its
 // exponentials: only another wave's do.  Rows of 256 need all registers of a SIMD for one wave (128 accumulators, 64 or 128 of stationary rows).
 // Tried at 4 096 x 1.25 M x 128 bfloat16: two groups of 4 waves a CU held one phase apart by barriers 4.85 ms, against 5.00 ms of waves that run freely; the
-// larger workgroups cost 10 - 25 % at every smaller size, so waves run freely.
+// larger workgroups cost 10 - 25 % at every smaller size, so waves run freely.  (Priority for either phase of a wave: no difference.)  Under this load the card
+// runs at 1.8 - 1.9 GHz.
 template <int TERMS, int DP> constexpr int ce_waves() { return DP == 256 ? 1 : 2; }
 
 // LDS image: rows of DP / 8 chunks of 16 bytes, chunk c of row r at c ^ ce_swz(r).  The banks serve 256 bytes a cycle: 16 lanes of a fragment read (16 rows,
@@ -473,9 +474,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
             }
             // (Behind the last 32 rows the first product reads what is there, and its result is not used.)
             ce_static_for<PRE, DEPTH>([&](auto u) __attribute__((always_inline)) { read(u, sb_, std::integral_constant<int, sb1>()); });
-            __builtin_amdgcn_s_setprio(1);
             steps(zero_t(), std::integral_constant<int, N2 + N1>(), sb_, std::integral_constant<int, sb1>());
-            __builtin_amdgcn_s_setprio(0);
             if constexpr (EARLY) read_params(sb == SB - 1 ? next : slot, sb1);
             ++at;
         });
