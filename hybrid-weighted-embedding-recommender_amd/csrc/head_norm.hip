@@ -165,6 +165,7 @@ __global__ __launch_bounds__(norm_block(T)) void norm_fwd_kernel(NormFwdArgs a) 
             int8_t* q = static_cast<int8_t*>(a.y) + rc * a.ldy;
             constexpr bool PAIR = std::is_same<W, float>::value;      // weights of 24 bits: products have a low part (16-bit rows and weights: exact)
             float te = 0.f;      // low part of the largest product, needed where a code is open
+            bool settle = true;      // is any code of the row open: looked at for each again then (without low parts that is all there is to it)
             if constexpr (PAIR) {
                 if (wp) {
                     bool some = false;
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(norm_block(T)) void norm_fwd_kernel(NormFwdArgs a) 
                             const float v = float(h[p].e[j]) * w[p * VW + j] * inv;
                             some = some || q8_open(v, rintf(v));
                         }
-                    bool settle;      // the same for all that hold the row (a wave may hold several)
+                    // the same for all that hold the row (a wave may hold several)
                     if constexpr (T > 64) settle = __syncthreads_or(some);
                     else settle = __any(some);
                     if (settle) {
@@ -198,6 +199,15 @@ __global__ __launch_bounds__(norm_block(T)) void norm_fwd_kernel(NormFwdArgs a) 
                     }
                 }
             }
+            if (!settle) {
+#pragma unroll
+                for (int p = 0; p < VPT; ++p) {
+                    Pack<int8_t, VW> out;
+#pragma unroll
+                    for (int j = 0; j < VW; ++j) out.e[j] = fine ? int8_t(int(rintf(float(h[p].e[j]) * w[p * VW + j] * inv))) : int8_t(0);
+                    store_pack<int8_t, VW>(q, (p * T + t) * VW, own, out);
+                }
+            } else {
 #pragma unroll
             for (int p = 0; p < VPT; ++p) {
                 Pack<int8_t, VW> out;
@@ -209,6 +219,7 @@ __global__ __launch_bounds__(norm_block(T)) void norm_fwd_kernel(NormFwdArgs a) 
                     out.e[j] = fine ? int8_t(int(c)) : int8_t(0);
                 }
                 store_pack<int8_t, VW>(q, (p * T + t) * VW, own, out);
+            }
             }
             // Rows of nothing but tiny products: once more from memory, in 64 bits
             bool again;
@@ -581,7 +592,7 @@ static void norm_fwd_typed(const NormFwdArgs& a, bool q8, hipStream_t st) {
 
 static int norm_fwd_any(const NormFwdArgs& a, int dtype, int w_dtype, bool q8, const char* what, void* stream) {
     hipStream_t st = as_stream(stream);
-    const bool w32 = !a.w || w_dtype == HWER_F32;
+    const bool w32 = a.w && w_dtype == HWER_F32;      // (without weights products are the rows' own values: no low parts)
     if (dtype == HWER_F32) norm_fwd_typed<float, float>(a, q8, st);
     else if (dtype == HWER_F16) w32 ? norm_fwd_typed<f16_t, float>(a, q8, st) : norm_fwd_typed<f16_t, f16_t>(a, q8, st);
     else w32 ? norm_fwd_typed<bf16_t, float>(a, q8, st) : norm_fwd_typed<bf16_t, bf16_t>(a, q8, st);
