@@ -542,19 +542,30 @@ __global__ __launch_bounds__(1024) void norm_dw_wide_kernel(NormBwdArgs a, const
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
-// How a row of d elements is held: T lanes with VPT vectors of VW elements, T * VPT * VW >= d.  Few elements a lane keep many waves at work: at 32 768 rows
-// of 2 048 bfloat16 the 8-bit norm takes 152 us with 64 lanes of 32 elements and 131 with 256 of 8.
+// How a row of d elements is held: T lanes with VPT vectors of VW elements, T * VPT * VW >= d.
 struct NormPlan {
     int t, vpt;      // t = 0: the wide kernels
 };
 #define HWER_NORM_PLANS(X) X(16, 1) X(64, 1) X(64, 2) X(256, 1) X(512, 1) X(1024, 1) X(1024, 2)
-static NormPlan norm_plan(int d, int vw) {
+// Codes take two reductions and more work an element: 16 elements a lane, so that fewer waves meet.  32 768 x 2 048 bfloat16 with float32 weights 119 us, 136
+// with 8 elements, 176 with 32; 8 192 x 8 192 126, 155 and 175; 16 384 x 2 048 float32 (4, 8, 16 elements) 87, 89 and 82.
+#define HWER_NORM_CODE_PLANS_16(X) X(16, 1) X(64, 1) X(64, 2) X(128, 2) X(256, 2) X(512, 2) X(1024, 2)
+#define HWER_NORM_CODE_PLANS_32(X) X(16, 1) X(64, 1) X(64, 2) X(64, 4) X(128, 4) X(256, 4) X(512, 4)
 #define HWER_NORM_TRY(T, V) \
     if (int64_t(T) * V * vw >= d) return {T, V};
+static NormPlan norm_plan(int d, int vw) {
     HWER_NORM_PLANS(HWER_NORM_TRY)
-#undef HWER_NORM_TRY
     return {0, 0};
 }
+static NormPlan norm_code_plan(int d, int vw) {
+    if (vw == 8) {
+        HWER_NORM_CODE_PLANS_16(HWER_NORM_TRY)
+    } else {
+        HWER_NORM_CODE_PLANS_32(HWER_NORM_TRY)
+    }
+    return {0, 0};
+}
+#undef HWER_NORM_TRY
 
 // workgroups of a launch: enough to fill the chip several times over, few enough that the weights are read once per many rows
 static int norm_grid(int64_t rows, int t) {
@@ -571,16 +582,20 @@ constexpr int kWideDwParts = 32;
 template <typename E, typename W, bool Q8>
 static void norm_fwd_launch(const NormFwdArgs& a, hipStream_t st) {
     constexpr int VW = 16 / int(sizeof(E));
-    NormPlan p = norm_plan(a.d, VW);
+    NormPlan p = Q8 ? norm_code_plan(a.d, VW) : norm_plan(a.d, VW);
     // Two waves that a row nearly fills, instead of one with twice the elements: 16 384 x 1 024 bfloat16 25 us, 30 as one wave; but 65 536 x 300 float32 87, 54
-    // as one wave, and the codes' second reduction 139, 116 (65 536 x 1 024).
+    // as one wave.
     if (!Q8 && a.d > 112 * VW && a.d <= 128 * VW) p = {128, 1};
     const int grid = norm_grid(a.rows, p.t ? p.t : kWideThreads);
 #define HWER_NORM_FWD(T, V) \
     if (p.t == T && p.vpt == V) return norm_fwd_kernel<E, W, T, V, VW, Q8><<<dim3(grid), dim3(norm_block(T)), 0, st>>>(a);
-    HWER_NORM_PLANS(HWER_NORM_FWD)
     if constexpr (!Q8) {
+        HWER_NORM_PLANS(HWER_NORM_FWD)
         HWER_NORM_FWD(128, 1)
+    } else if constexpr (VW == 8) {
+        HWER_NORM_CODE_PLANS_16(HWER_NORM_FWD)
+    } else {
+        HWER_NORM_CODE_PLANS_32(HWER_NORM_FWD)
     }
 #undef HWER_NORM_FWD
     norm_fwd_wide_kernel<E, W, Q8><<<dim3(grid), dim3(kWideThreads), 0, st>>>(a);
