@@ -551,6 +551,8 @@ struct NormPlan {
 // with 8 elements, 176 with 32; 8 192 x 8 192 126, 155 and 175; 16 384 x 2 048 float32 (4, 8, 16 elements) 87, 89 and 82.
 #define HWER_NORM_CODE_PLANS_16(X) X(16, 1) X(64, 1) X(64, 2) X(128, 2) X(256, 2) X(512, 2) X(1024, 2)
 #define HWER_NORM_CODE_PLANS_32(X) X(16, 1) X(64, 1) X(64, 2) X(64, 4) X(128, 4) X(256, 4) X(512, 4)
+// Gradients of wide 16-bit rows: 16 384 x 4 096 bfloat16 105 us, 116 with 8 elements a lane (32 768 x 2 048 150 and 107: too few waves with two a row)
+#define HWER_NORM_BWD_PLANS_16(X) X(16, 1) X(64, 1) X(64, 2) X(256, 1) X(256, 2) X(512, 2) X(1024, 2)
 #define HWER_NORM_TRY(T, V) \
     if (int64_t(T) * V * vw >= d) return {T, V};
 static NormPlan norm_plan(int d, int vw) {
@@ -564,6 +566,13 @@ static NormPlan norm_code_plan(int d, int vw) {
         HWER_NORM_CODE_PLANS_32(HWER_NORM_TRY)
     }
     return {0, 0};
+}
+static NormPlan norm_bwd_plan(int d, int vw) {
+    if (vw == 8) {
+        HWER_NORM_BWD_PLANS_16(HWER_NORM_TRY)
+        return {0, 0};
+    }
+    return norm_plan(d, vw);
 }
 #undef HWER_NORM_TRY
 
@@ -667,7 +676,7 @@ int hwer_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t 
         typedef decltype(e) E;
         typedef decltype(wt) W;
         constexpr int VW = 16 / int(sizeof(E));
-        const NormPlan p = norm_plan(d, VW);
+        const NormPlan p = norm_bwd_plan(d, VW);
         if (p.t == 0) {
             float* rstd = a.dw_part ? a.dw_part + int64_t(kWideDwParts) * d : nullptr;
             const int grid = norm_grid(rows, kWideThreads);
@@ -681,7 +690,11 @@ int hwer_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t 
         parts = norm_bwd_grid(rows, p.t);
 #define HWER_NORM_BWD(T, V) \
         if (p.t == T && p.vpt == V) return norm_bwd_kernel<E, W, T, V, VW><<<dim3(parts), dim3(norm_block(T)), 0, st>>>(a);
-        HWER_NORM_PLANS(HWER_NORM_BWD)
+        if constexpr (VW == 8) {
+            HWER_NORM_BWD_PLANS_16(HWER_NORM_BWD)
+        } else {
+            HWER_NORM_PLANS(HWER_NORM_BWD)
+        }
 #undef HWER_NORM_BWD
     };
     const bool w32 = !weight || weight_dtype == HWER_F32;
