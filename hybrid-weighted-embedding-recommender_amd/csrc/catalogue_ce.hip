@@ -535,7 +535,8 @@ struct CePack {
     short *hi[2], *lo[2];
     int64_t rows[2], ld[2];
     int d, dp;
-    float* tops;             // (2, kTopBlocks) partial maxima of |value|
+    float* tops;             // (2, kTopBlocks) partial maxima of |value|, n_tops of them
+    int n_tops;
     CeScalars* sc;
     const int64_t* target;
     const float* bias;
@@ -582,7 +583,7 @@ __global__ __launch_bounds__(256) void ce_top_kernel(CePack a) {
     const int w = blockIdx.y, chunks = a.dp / 8, shift = 31 - __clz(chunks);
     float top = 0.f;
 #pragma unroll 4
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < a.rows[w] * chunks; i += kTopBlocks * 256) {
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < a.rows[w] * chunks; i += int64_t(gridDim.x) * 256) {
         float v[8];
         ce_load8(a, w, i >> shift, int(i & (chunks - 1)) * 8, v);
 #pragma unroll
@@ -605,7 +606,7 @@ __global__ __launch_bounds__(256) void ce_split_kernel(CePack a) {
     const int w = blockIdx.y, lane = threadIdx.x & 63;
     if (threadIdx.x < 128) {      // a wave per operand
         float top = 0.f;
-        for (int i = lane; i < kTopBlocks; i += 64) top = fmaxf(top, a.tops[(threadIdx.x >> 6) * kTopBlocks + i]);
+        for (int i = lane; i < a.n_tops; i += 64) top = fmaxf(top, a.tops[(threadIdx.x >> 6) * kTopBlocks + i]);
         top = wave_max_f32(top);
         if (lane == 0) s[threadIdx.x >> 6] = top;
     }
@@ -975,13 +976,14 @@ struct CeCall {
 
     // lays out what the passes cannot read in place
     int prepare() const {
-        CePack p{{q, e}, {nullptr, nullptr}, {nullptr, nullptr}, {n, v}, {ldq, lde}, d, dp, at<float>(y.tops), at<CeScalars>(0), target, bias};
+        CePack p{{q, e}, {nullptr, nullptr}, {nullptr, nullptr}, {n, v}, {ldq, lde}, d, dp, at<float>(y.tops), 0, at<CeScalars>(0), target, bias};
         if (!q_direct) p.hi[0] = at<short>(y.q_hi);
         if (!e_direct) p.hi[1] = at<short>(y.e_hi);
         const dim3 grid(unsigned(std::max<int64_t>(1, std::min<int64_t>(cdiv64(std::max(n, v) * (dp / 8), 256), kMaxStreamBlocks))), 2);
         if (dtype == HWER_F32) {
             p.lo[0] = at<short>(y.q_lo), p.lo[1] = at<short>(y.e_lo);
-            ce_top_kernel<<<dim3(kTopBlocks, 2), dim3(256), 0, st>>>(p);
+            p.n_tops = int(std::max<int64_t>(1, std::min<int64_t>(kTopBlocks, cdiv64(std::max(n, v) * (dp / 8), 256))));
+            ce_top_kernel<<<dim3(p.n_tops, 2), dim3(256), 0, st>>>(p);
             ce_split_kernel<<<grid, dim3(256), 0, st>>>(p);
         } else if (p.hi[0] || p.hi[1]) {
             ce_pack16_kernel<<<grid, dim3(256), 0, st>>>(p);
