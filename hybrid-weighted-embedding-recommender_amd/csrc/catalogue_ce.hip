@@ -875,8 +875,8 @@ static bool ce_direct(const void* p, int64_t ld, int d, int dtype) {
 }
 
 // Splits of the streaming side, in 32s of its rows.  A call takes as long as its fullest CU (which holds two workgroups, or one of the widest rows): rounds of
-// workgroups times (a split's 32s + about 4 for its start and end); and each split leaves sums behind that are written and read again, about 2 MB in the
-// time of 32 rows.
+// workgroups times (a split's 32s + about 4 for its start and end); and each split leaves sums behind that are written and read again, about 3 MB in the
+// time of 32 rows (with 2: 8 192 x 4 000 x 128 bfloat16 95 us, 83 so, 86 with 6; 2 000 x 3 000 x 100 float32 80, 76 and 73; 100 000 x 129 x 128 334, 337 and 339).
 // Tried for pass 2: one workgroup for each place on the CUs with an equal share of all blocks' work.  No last round that is not full (1 037 x 50 021 x 250
 // float16 256 -> 241 us), but no workgroup takes over from a slower one either, and the loop over blocks costs registers: 4 096 x 1.25 M x 128 bfloat16
 // 4.90 -> 5.00 ms, x 400 k x 64 0.97 -> 1.04, x 400 k x 256 4.0 -> 4.7.
@@ -891,7 +891,7 @@ static CeSplit ce_split(int64_t n_stat, int64_t n_strm, int d) {
     int64_t per = subs;
     for (int64_t s = 1; s <= std::min<int64_t>(subs, kMaxSplits) && (s == 1 || blocks * s <= 8 * slots); ++s) {
         const int64_t p = cdiv64(subs, s), n = cdiv64(subs, p);
-        const double cost = double(cdiv64(blocks * n, slots) * (p + 4)) + (n > 1 ? double(blocks * kRows * dp * 8) * double(n) / 2e6 : 0.0);
+        const double cost = double(cdiv64(blocks * n, slots) * (p + 4)) + (n > 1 ? double(blocks * kRows * dp * 8) * double(n) / 3e6 : 0.0);
         if (cost < best) best = cost, per = p;
     }
     return {int(blocks), int(cdiv64(subs, per)), int(per)};
