@@ -868,6 +868,8 @@ __global__ __launch_bounds__(256) void ce_de_kernel(const float* __restrict__ o,
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
+constexpr int kCeMaxDim = 256;
+static int ce_width(int64_t d) { return d >= 1 && d <= kCeMaxDim ? int(d) : 0; }      // 0: refused by CeCall::check
 static int ce_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 static bool ce_direct(const void* p, int64_t ld, int d, int dtype) {
@@ -960,7 +962,7 @@ struct CeCall {
 
     int check(const char* what, void* workspace, size_t bytes, bool want_mean, void* stream) {
         if (!known_dtype(dtype)) return fail(HWER_EINVAL, "%s: unknown element type %d", what, dtype);
-        if (d < 1 || d > hwer_catalogue_ce_max_dim()) return fail(HWER_EINVAL, "%s: d=%d unsupported (1..%d)", what, d, hwer_catalogue_ce_max_dim());
+        if (d < 1) return fail(HWER_EINVAL, "%s: rows of 1..%d elements are supported", what, kCeMaxDim);
         const int64_t most = (int64_t(1) << 31) - 256;
         if (n < 0 || v < 1 || n > most || v > most) return fail(HWER_EINVAL, "%s: %lld rows, %lld classes", what, (long long)n, (long long)v);
         if (!(scale > 0.f) || !(scale < INFINITY)) return fail(HWER_EINVAL, "%s: scale must be positive and finite", what);
@@ -1099,19 +1101,19 @@ using namespace hwer;
 
 extern "C" {
 
-int hwer_catalogue_ce_max_dim(void) { return 256; }
+int hwer_catalogue_ce_max_dim(void) { return kCeMaxDim; }
 
-int hwer_catalogue_ce_reads_in_place(const void* rows, int64_t ld, int d, int dtype) { return ce_direct(rows, ld, d, dtype) ? 1 : 0; }
+int hwer_catalogue_ce_reads_in_place(const void* rows, int64_t ld, int64_t d, int dtype) { return ce_width(d) && ce_direct(rows, ld, int(d), dtype) ? 1 : 0; }
 
-size_t hwer_catalogue_ce_workspace_bytes(int64_t n, int64_t v, int d, int dtype, int q_in_place, int e_in_place, int want_gradients) {
-    if (!known_dtype(dtype) || d < 1 || d > hwer_catalogue_ce_max_dim() || n < 0 || v < 1) return 0;
-    return ce_layout(n, v, d, dtype, q_in_place != 0, e_in_place != 0, want_gradients != 0).bytes(want_gradients != 0);
+size_t hwer_catalogue_ce_workspace_bytes(int64_t n, int64_t v, int64_t d, int dtype, int q_in_place, int e_in_place, int want_gradients) {
+    if (!known_dtype(dtype) || !ce_width(d) || n < 0 || v < 1) return 0;
+    return ce_layout(n, v, int(d), dtype, q_in_place != 0, e_in_place != 0, want_gradients != 0).bytes(want_gradients != 0);
 }
 
-int hwer_catalogue_ce(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int d, int dtype,
+int hwer_catalogue_ce(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int64_t d, int dtype,
                       float scale, int reduction, float* loss_rows, float* state, float* loss, float* counted, float* mean, void* workspace, size_t workspace_bytes,
                       void* stream) {
-    CeCall c{q, e, ldq, lde, bias, target, n, v, d, dtype, scale, reduction};
+    CeCall c{q, e, ldq, lde, bias, target, n, v, ce_width(d), dtype, scale, reduction};
     if (int rc = c.check("catalogue_ce", workspace, workspace_bytes, mean != nullptr, stream)) return rc;
     if (reduction < 0 || reduction > 2) return fail(HWER_EINVAL, "catalogue_ce: unknown reduction %d", reduction);
     if (!counted || (reduction && !loss) || (n && (!loss_rows || !state))) return fail(HWER_EINVAL, "catalogue_ce: null output");
@@ -1126,10 +1128,10 @@ int hwer_catalogue_ce(const void* q, int64_t ldq, const void* e, int64_t lde, co
     return check_launch("catalogue_ce");
 }
 
-int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int d,
+int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int64_t d,
                                int dtype, float scale, int reduction, const float* grad, const float* state, const float* counted, const float* mean, void* dq,
                                int64_t lddq, void* de, int64_t ldde, float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
-    CeCall c{q, e, ldq, lde, bias, target, n, v, d, dtype, scale, reduction};
+    CeCall c{q, e, ldq, lde, bias, target, n, v, ce_width(d), dtype, scale, reduction};
     if (int rc = c.check("catalogue_ce_backward", workspace, workspace_bytes, true, stream)) return rc;
     if (reduction < 0 || reduction > 2 || (reduction == 0 && !grad)) return fail(HWER_EINVAL, "catalogue_ce_backward: unknown reduction %d, or rows' losses without their gradients", reduction);
     if (!counted || (n && (!state || (dq && !mean)))) return fail(HWER_EINVAL, "catalogue_ce_backward: what the forward call left is missing");
@@ -1145,10 +1147,10 @@ int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_
     return de ? c.pass2(de, ldde, dbias, reduction == 0, nullptr, nullptr) : HWER_OK;
 }
 
-int hwer_catalogue_ce_grads(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int d, int dtype,
+int hwer_catalogue_ce_grads(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias, const int64_t* target, int64_t n, int64_t v, int64_t d, int dtype,
                             float scale, int reduction, float* loss, void* dq, int64_t lddq, void* de, int64_t ldde, float* dbias, void* workspace,
                             size_t workspace_bytes, void* stream) {
-    CeCall c{q, e, ldq, lde, bias, target, n, v, d, dtype, scale, reduction};
+    CeCall c{q, e, ldq, lde, bias, target, n, v, ce_width(d), dtype, scale, reduction};
     if (int rc = c.check("catalogue_ce_grads", workspace, workspace_bytes, true, stream)) return rc;
     if (reduction < 1 || reduction > 2) return fail(HWER_EINVAL, "catalogue_ce_grads: reduction %d: 1 (mean) or 2 (sum)", reduction);
     if (!loss || !de || (n && !dq) || lddq < d || ldde < d) return fail(HWER_EINVAL, "catalogue_ce_grads: null output or a row stride below d");

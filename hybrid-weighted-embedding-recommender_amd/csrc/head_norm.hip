@@ -587,6 +587,8 @@ static int norm_bwd_grid(int64_t rows, int t) {
     return int(std::min<int64_t>(cdiv64(rows, r), 1024));
 }
 constexpr int kWideDwParts = 32;
+// Columns are 32-bit numbers, which the wide kernels run past a row's end by up to kWideThreads * 8
+constexpr int64_t kNormMaxDim = (int64_t(1) << 31) - (int64_t(1) << 14);
 
 template <typename E, typename W, bool Q8>
 static void norm_fwd_launch(const NormFwdArgs& a, hipStream_t st) {
@@ -623,10 +625,10 @@ static int norm_fwd_any(const NormFwdArgs& a, int dtype, int w_dtype, bool q8, c
     return check_launch(what);
 }
 
-static int norm_check(const char* what, const void* x, int64_t ldx, const void* w, int w_dtype, int64_t rows, int d, int dtype, float eps) {
+static int norm_check(const char* what, const void* x, int64_t ldx, const void* w, int w_dtype, int64_t rows, int64_t d, int dtype, float eps) {
     if (!known_dtype(dtype)) return fail(HWER_EINVAL, "%s: unknown element type %d", what, dtype);
     if (w && w_dtype != HWER_F32 && w_dtype != dtype) return fail(HWER_EINVAL, "%s: the weights are float32 or of the rows' type", what);
-    if (rows < 0 || d < 1) return fail(HWER_EINVAL, "%s: rows=%lld, d=%d", what, (long long)rows, d);
+    if (rows < 0 || d < 1 || d > kNormMaxDim) return fail(HWER_EINVAL, "%s: rows=%lld, d=%lld (d <= %lld)", what, (long long)rows, (long long)d, (long long)kNormMaxDim);
     if (rows && (!x || ldx < d)) return fail(HWER_EINVAL, "%s: null rows or a row stride below d", what);
     if (!(eps >= 0.f) || !(eps < INFINITY)) return fail(HWER_EINVAL, "%s: eps must be finite and not negative", what);
     return HWER_OK;
@@ -638,52 +640,52 @@ using namespace hwer;
 
 extern "C" {
 
-int hwer_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int weight_dtype, int64_t rows, int d, int dtype,
+int hwer_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int weight_dtype, int64_t rows, int64_t d, int dtype,
                   float eps, void* y, int64_t ldy, void* h, int64_t ldh, void* stream) {
     if (int rc = norm_check("rms_norm", x, ldx, weight, weight_dtype, rows, d, dtype, eps)) return rc;
     if (rows == 0) return HWER_OK;
     if (!y || ldy < d || (residual && (!h || ldr < d || ldh < d))) return fail(HWER_EINVAL, "rms_norm: null output or a row stride below d");
-    const NormFwdArgs a{x, residual, weight, y, h, nullptr, rows, ldx, ldr, ldy, ldh, d, eps, 1};
+    const NormFwdArgs a{x, residual, weight, y, h, nullptr, rows, ldx, ldr, ldy, ldh, int(d), eps, 1};
     return norm_fwd_any(a, dtype, weight_dtype, false, "rms_norm", stream);
 }
 
-int hwer_rms_norm_q8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int weight_dtype, int64_t rows, int d, int dtype,
+int hwer_rms_norm_q8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int weight_dtype, int64_t rows, int64_t d, int dtype,
                      int norm, float eps, int8_t* q, int64_t ldq, float* scale, void* h, int64_t ldh, void* stream) {
     if (int rc = norm_check("rms_norm_q8", x, ldx, weight, weight_dtype, rows, d, dtype, eps)) return rc;
     if (rows == 0) return HWER_OK;
     if (!q || !scale || ldq < d || (residual && (!h || ldr < d || ldh < d))) return fail(HWER_EINVAL, "rms_norm_q8: null output or a row stride below d");
-    const NormFwdArgs a{x, residual, weight, q, h, scale, rows, ldx, ldr, ldq, ldh, d, eps, norm ? 1 : 0};
+    const NormFwdArgs a{x, residual, weight, q, h, scale, rows, ldx, ldr, ldq, ldh, int(d), eps, norm ? 1 : 0};
     return norm_fwd_any(a, dtype, weight_dtype, true, "rms_norm_q8", stream);
 }
 
-size_t hwer_rms_norm_backward_workspace_bytes(int64_t rows, int d) {
-    if (rows <= 0 || d < 1) return 16;
+size_t hwer_rms_norm_backward_workspace_bytes(int64_t rows, int64_t d) {
+    if (rows <= 0 || d < 1 || d > kNormMaxDim) return 16;
     // partial sums of dweight (at most 1 024 workgroups; rows too wide for registers: kWideDwParts and one r per row)
     return size_t(std::max<int64_t>(std::min<int64_t>(rows, 1024), kWideDwParts)) * d * 4 + size_t(rows) * 4;
 }
 
 int hwer_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* weight, int weight_dtype, const void* dh, int64_t lddh,
-                           int64_t rows, int d, int dtype, float eps, void* dx, int64_t lddx, void* dweight, void* workspace, size_t workspace_bytes, void* stream) {
+                           int64_t rows, int64_t d, int dtype, float eps, void* dx, int64_t lddx, void* dweight, void* workspace, size_t workspace_bytes, void* stream) {
     if (int rc = norm_check("rms_norm_backward", h, ldh, weight, weight_dtype, rows, d, dtype, eps)) return rc;
     if (dweight && !weight) return fail(HWER_EINVAL, "rms_norm_backward: a gradient of weights that are not there");
     if (rows && (!dy || !dx || lddy < d || lddx < d || (dh && lddh < d))) return fail(HWER_EINVAL, "rms_norm_backward: null rows or a row stride below d");
     if (dweight && (!workspace || workspace_bytes < hwer_rms_norm_backward_workspace_bytes(rows, d)))
         return fail(HWER_EWORKSPACE, "rms_norm_backward: workspace of %zu bytes needed", hwer_rms_norm_backward_workspace_bytes(rows, d));
     hipStream_t st = as_stream(stream);
-    NormBwdArgs a{dy, h, weight, dh, dx, dweight ? static_cast<float*>(workspace) : nullptr, rows, lddy, ldh, lddh, lddx, d, eps};
+    NormBwdArgs a{dy, h, weight, dh, dx, dweight ? static_cast<float*>(workspace) : nullptr, rows, lddy, ldh, lddh, lddx, int(d), eps};
     int parts = 0;
     auto run = [&](auto e, auto wt) {
         typedef decltype(e) E;
         typedef decltype(wt) W;
         constexpr int VW = 16 / int(sizeof(E));
-        const NormPlan p = norm_bwd_plan(d, VW);
+        const NormPlan p = norm_bwd_plan(a.d, VW);
         if (p.t == 0) {
             float* rstd = a.dw_part ? a.dw_part + int64_t(kWideDwParts) * d : nullptr;
             const int grid = norm_grid(rows, kWideThreads);
             norm_bwd_wide_kernel<E, W><<<dim3(grid), dim3(kWideThreads), 0, st>>>(a, rstd);
             if (a.dw_part) {
                 parts = int(std::min<int64_t>(kWideDwParts, cdiv64(rows, 64)));      // (16 waves share a part's rows: 152 x 20 000 bfloat16 5.3 us, 18.6 as 32 parts)
-                norm_dw_wide_kernel<E><<<dim3((d + 63) / 64, parts), dim3(1024), 0, st>>>(a, rstd, int(cdiv64(rows, parts)));
+                norm_dw_wide_kernel<E><<<dim3((a.d + 63) / 64, parts), dim3(1024), 0, st>>>(a, rstd, int(cdiv64(rows, parts)));
             }
             return;
         }
@@ -705,10 +707,10 @@ int hwer_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t 
         if (int rc = check_launch("rms_norm_backward")) return rc;
     }
     if (dweight) {      // no rows: a sum over nothing, zeros
-        const dim3 grid((d + 15) / 16);
-        if (w32) norm_dw_kernel<float><<<grid, dim3(1024), 0, st>>>(a.dw_part, parts, d, static_cast<float*>(dweight));
-        else if (dtype == HWER_F16) norm_dw_kernel<f16_t><<<grid, dim3(1024), 0, st>>>(a.dw_part, parts, d, static_cast<f16_t*>(dweight));
-        else norm_dw_kernel<bf16_t><<<grid, dim3(1024), 0, st>>>(a.dw_part, parts, d, static_cast<bf16_t*>(dweight));
+        const dim3 grid((a.d + 15) / 16);
+        if (w32) norm_dw_kernel<float><<<grid, dim3(1024), 0, st>>>(a.dw_part, parts, a.d, static_cast<float*>(dweight));
+        else if (dtype == HWER_F16) norm_dw_kernel<f16_t><<<grid, dim3(1024), 0, st>>>(a.dw_part, parts, a.d, static_cast<f16_t*>(dweight));
+        else norm_dw_kernel<bf16_t><<<grid, dim3(1024), 0, st>>>(a.dw_part, parts, a.d, static_cast<bf16_t*>(dweight));
     }
     return check_launch("rms_norm_backward(dweight)");
 }

@@ -495,15 +495,15 @@ static void matmul_q8_launch(const QmmArgs& g, hipStream_t st) {
 using namespace hwer;
 
 extern "C" int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* b, int64_t ldb, const float* b_scale, const float* bias,
-                              int64_t m, int64_t n, int k, void* out, int64_t ldo, int out_dtype, void* stream) {
+                              int64_t m, int64_t n, int64_t k, void* out, int64_t ldo, int out_dtype, void* stream) {
     if (!known_dtype(out_dtype)) return fail(HWER_EINVAL, "matmul_q8: unknown output type %d", out_dtype);
-    if (m < 0 || n < 0 || k < 0 || k > 131071) return fail(HWER_EINVAL, "matmul_q8: m=%lld, n=%lld, k=%d (k <= 131071: sums stay in 32 bits)", (long long)m, (long long)n, k);
+    if (m < 0 || n < 0 || k < 0 || k > 131071) return fail(HWER_EINVAL, "matmul_q8: m=%lld, n=%lld, k=%lld (k <= 131071: sums stay in 32 bits)", (long long)m, (long long)n, (long long)k);
     if (m == 0 || n == 0) return HWER_OK;
     if (m > (int64_t(1) << 31) - 256 || n > (int64_t(1) << 31) - 256 || cdiv64(m, 64) * cdiv64(n, 64) > (int64_t(1) << 30))
         return fail(HWER_EINVAL, "matmul_q8: m=%lld, n=%lld: too many tiles for one call", (long long)m, (long long)n);
     if ((k && (!a || !b)) || !a_scale || !b_scale || !out) return fail(HWER_EINVAL, "matmul_q8: null operand");
     if (lda < k || ldb < k || ldo < n) return fail(HWER_EINVAL, "matmul_q8: a row stride is below the row's length");
-    const QmmArgs g{a, b, a_scale, b_scale, bias, out, m, n, lda, ldb, ldo, k};
+    const QmmArgs g{a, b, a_scale, b_scale, bias, out, m, n, lda, ldb, ldo, int(k)};
     hipStream_t st = as_stream(stream);
     const bool al = k % 16 == 0 && aligned_to(a, lda, 16) && aligned_to(b, ldb, 16) && std::max(lda, ldb) < (1 << 23);      // (a panel's bytes in 32 bits)
     if (out_dtype == HWER_F32) al ? matmul_q8_launch<float, true>(g, st) : matmul_q8_launch<float, false>(g, st);

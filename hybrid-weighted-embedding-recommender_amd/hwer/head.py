@@ -23,6 +23,8 @@ import torch
 from . import native
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_MAX_WIDTH = (1 << 31) - (1 << 14)      # of a norm's rows
+_MAX_CODES = 131071                     # of a row of the 8-bit product: 128 * 128 times as many stay below 2^31
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 # A call on a single row is a few microseconds of GPU time: what the host does per call is kept short (addresses as plain integers, the device switched
 # only where it is another one, the raw stream handle).
@@ -109,6 +111,8 @@ def _norm_checks(x, weight, residual, eps):
     _check_rows("x", x, dim=None)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x: rows of at least one element needed, got shape %s" % (tuple(x.shape),))
+    if x.shape[-1] > _MAX_WIDTH:
+        raise ValueError("x: rows of at most %d elements, got %d" % (_MAX_WIDTH, x.shape[-1]))
     _check_device(x, weight, residual)
     if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
         raise ValueError("residual: shape and type of x needed (%s %s), got %s %s" % (tuple(x.shape), x.dtype, tuple(residual.shape), residual.dtype))
@@ -231,6 +235,8 @@ def matmul_q8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
     _check_device(a, b, a_scale, b_scale, bias)
     if a.shape[1] != b.shape[1]:
         raise ValueError("rows of %d against rows of %d codes" % (a.shape[1], b.shape[1]))
+    if a.shape[1] > _MAX_CODES:
+        raise ValueError("rows of at most %d codes, got %d" % (_MAX_CODES, a.shape[1]))
     if out_dtype not in _DTYPES:
         raise TypeError("out_dtype: float32, float16 or bfloat16, got %s" % out_dtype)
     (m, k), n = a.shape, b.shape[0]

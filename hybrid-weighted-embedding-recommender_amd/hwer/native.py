@@ -104,24 +104,24 @@ PROTOTYPES = {
                                         _P, _P, c_int, _P, c_size_t, _P]),
     "hwer_merge_topk_strided": (c_int, [_P, _P, _P, c_int64, c_int, c_int64, c_int, c_int, _P, _P, _P, _P]),
     # x, ldx, residual, ldr, weight, weight_dtype, rows, d, dtype, eps, y, ldy, h, ldh, stream
-    "hwer_rms_norm": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, c_int64, c_int, c_int, c_float, _P, c_int64, _P, c_int64, _P]),
+    "hwer_rms_norm": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, c_int64, c_int64, c_int, c_float, _P, c_int64, _P, c_int64, _P]),
     # x, ldx, residual, ldr, weight, weight_dtype, rows, d, dtype, norm, eps, q, ldq, scale, h, ldh, stream
-    "hwer_rms_norm_q8": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, c_int64, c_int, c_int, c_int, c_float, _P, c_int64, _P, _P, c_int64, _P]),
-    "hwer_rms_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int]),
+    "hwer_rms_norm_q8": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, c_int64, c_int64, c_int, c_int, c_float, _P, c_int64, _P, _P, c_int64, _P]),
+    "hwer_rms_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     # dy, lddy, h, ldh, weight, weight_dtype, dh, lddh, rows, d, dtype, eps, dx, lddx, dweight, workspace, workspace_bytes, stream
-    "hwer_rms_norm_backward": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, _P, c_int64, c_int64, c_int, c_int, c_float, _P, c_int64, _P, _P, c_size_t, _P]),
+    "hwer_rms_norm_backward": (c_int, [_P, c_int64, _P, c_int64, _P, c_int, _P, c_int64, c_int64, c_int64, c_int, c_float, _P, c_int64, _P, _P, c_size_t, _P]),
     # a, lda, a_scale, b, ldb, b_scale, bias, m, n, k, out, ldo, out_dtype, stream
-    "hwer_matmul_q8": (c_int, [_P, c_int64, _P, _P, c_int64, _P, _P, c_int64, c_int64, c_int, _P, c_int64, c_int, _P]),
+    "hwer_matmul_q8": (c_int, [_P, c_int64, _P, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, _P, c_int64, c_int, _P]),
     "hwer_catalogue_ce_max_dim": (c_int, []),
-    "hwer_catalogue_ce_reads_in_place": (c_int, [_P, c_int64, c_int, c_int]),
-    "hwer_catalogue_ce_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int, c_int, c_int, c_int]),
+    "hwer_catalogue_ce_reads_in_place": (c_int, [_P, c_int64, c_int64, c_int]),
+    "hwer_catalogue_ce_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int]),
     # q, ldq, e, lde, bias, target, n, v, d, dtype, scale, reduction, loss_rows, state, loss, counted, mean, workspace, workspace_bytes, stream
-    "hwer_catalogue_ce": (c_int, [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int, c_int, c_float, c_int, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
+    "hwer_catalogue_ce": (c_int, [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int, c_float, c_int, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
     # q, ldq, e, lde, bias, target, n, v, d, dtype, scale, reduction, grad, state, counted, mean, dq, lddq, de, ldde, dbias, workspace, bytes, stream
-    "hwer_catalogue_ce_backward": (c_int, [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int, c_int, c_float, c_int, _P, _P, _P, _P, _P, c_int64, _P, c_int64,
+    "hwer_catalogue_ce_backward": (c_int, [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int, c_float, c_int, _P, _P, _P, _P, _P, c_int64, _P, c_int64,
                                            _P, _P, c_size_t, _P]),
     # q, ldq, e, lde, bias, target, n, v, d, dtype, scale, reduction, loss, dq, lddq, de, ldde, dbias, workspace, workspace_bytes, stream
-    "hwer_catalogue_ce_grads": (c_int, [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int, c_int, c_float, c_int, _P, _P, c_int64, _P, c_int64, _P, _P, c_size_t,
+    "hwer_catalogue_ce_grads": (c_int, [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int, c_float, c_int, _P, _P, c_int64, _P, c_int64, _P, _P, c_size_t,
                                         _P]),
     "hwer_merge_topk_lists": (c_int, [_P, _P, _P, c_int64, c_int, c_int64, c_int, c_int, c_int, _P, _P, _P, _P, _P]),
 }

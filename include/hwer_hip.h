@@ -526,6 +526,7 @@ int hwer_pack_exchange(const int64_t* idx, const double* score, const double* di
  * reference, whose training runs in DGL / PyTorch, hwer/gcn_ncf.py:126-327; its outputs are the tables above).
  * Element types: HWER_F32 / HWER_F16 / HWER_BF16.  Rows are contiguous along their elements, strides `ld*` in ELEMENTS, any
  * alignment (rows on 16 bytes whose width is a multiple of 16 bytes run on wide loads).  Sums and statistics are float32 or wider.
+ * Widths are 64-bit arguments, so that one beyond a limit is refused and not cut off.
  * ------------------------------------------------------------------------------------------------- */
 #define HWER_F32 0
 #define HWER_F16 1
@@ -533,26 +534,26 @@ int hwer_pack_exchange(const int64_t* idx, const double* score, const double* di
 
 /* Root-mean-square norm:  h = x + residual rounded to the rows' type (written when there is a residual; outputs share memory with no input),
  *   y = h * weight / sqrt(mean(h^2) + eps).  weight (nullable = ones): float32 or the rows' type.  One pass over memory.
- * The sum of squares is float32: |h| below 1.8e19 / sqrt(d).  A NaN or an infinity stays in its row. */
+ * 1 <= d <= 2^31 - 2^14.  The sum of squares is float32: |h| below 1.8e19 / sqrt(d).  A NaN or an infinity stays in its row. */
 int hwer_rms_norm(const void* x, int64_t ldx, const void* residual /*nullable*/, int64_t ldr, const void* weight /*nullable*/, int weight_dtype,
-                  int64_t rows, int d, int dtype, float eps, void* y, int64_t ldy, void* h, int64_t ldh, void* stream);
+                  int64_t rows, int64_t d, int dtype, float eps, void* y, int64_t ldy, void* h, int64_t ldh, void* stream);
 /* The same rows as int8 codes with one scale a row: q = round_half_even(127 v / max|v|), v = h * weight, scale = max|v| / (127 sqrt(mean(h^2) + eps));
  * norm = 0: scale = max|v| / 127 (plain quantisation).  The codes are exact for their definition.  A row of zeros: codes 0, scale 0; a row
  * with a NaN or an infinity: codes 0, scale NaN. */
 int hwer_rms_norm_q8(const void* x, int64_t ldx, const void* residual /*nullable*/, int64_t ldr, const void* weight /*nullable*/, int weight_dtype,
-                     int64_t rows, int d, int dtype, int norm, float eps, int8_t* q, int64_t ldq, float* scale, void* h, int64_t ldh, void* stream);
+                     int64_t rows, int64_t d, int dtype, int norm, float eps, int8_t* q, int64_t ldq, float* scale, void* h, int64_t ldh, void* stream);
 /* Gradients:  dx = (weight * dy - h * r^2 * mean(h * weight * dy)) * r + dh,  dweight = sum_rows dy * h * r  (the residual's gradient is dx).
  * h: what hwer_rms_norm was taken of (its h, or x without a residual).  dh (nullable): gradient that reaches h directly.
  * dweight (nullable) needs the workspace; its sum has a fixed order (no atomics).  dx shares memory with no input. */
-size_t hwer_rms_norm_backward_workspace_bytes(int64_t rows, int d);
+size_t hwer_rms_norm_backward_workspace_bytes(int64_t rows, int64_t d);
 int hwer_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* weight /*nullable*/, int weight_dtype,
-                           const void* dh /*nullable*/, int64_t lddh, int64_t rows, int d, int dtype, float eps, void* dx, int64_t lddx,
+                           const void* dh /*nullable*/, int64_t lddh, int64_t rows, int64_t d, int dtype, float eps, void* dx, int64_t lddx,
                            void* dweight /*nullable*/, void* workspace, size_t workspace_bytes, void* stream);
 
 /* out[m][n] = (sum_k a[m][k] b[n][k]) * a_scale[m] * b_scale[n] (+ bias[n]): int8 rows with a float32 scale each on both sides (tokens / queries on the
  * left, channels / catalogue rows on the right), exact 32-bit sums (k <= 131071), out float32 / float16 / bfloat16. */
 int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* b, int64_t ldb, const float* b_scale, const float* bias /*nullable*/,
-                   int64_t m, int64_t n, int k, void* out, int64_t ldo, int out_dtype, void* stream);
+                   int64_t m, int64_t n, int64_t k, void* out, int64_t ldo, int out_dtype, void* stream);
 
 /* Softmax cross entropy of n query rows over all v rows of a catalogue, logits z = scale * <q_r, e_v> + bias_v never stored:
  *   loss_r = log sum_v exp z_rv - z_{r, target_r}.  target -1: the row does not count (loss 0, no gradient); any other target outside 0 .. v - 1:
@@ -569,17 +570,17 @@ int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int
  * Workspace: hwer_catalogue_ce_workspace_bytes(..., q_in_place, e_in_place = hwer_catalogue_ce_reads_in_place(rows, ld, d, dtype), ...); with a bias the table
  *   is never read in place (e_in_place = 0). */
 int hwer_catalogue_ce_max_dim(void);
-int hwer_catalogue_ce_reads_in_place(const void* rows, int64_t ld, int d, int dtype);
-size_t hwer_catalogue_ce_workspace_bytes(int64_t n, int64_t v, int d, int dtype, int q_in_place, int e_in_place, int want_gradients);
+int hwer_catalogue_ce_reads_in_place(const void* rows, int64_t ld, int64_t d, int dtype);
+size_t hwer_catalogue_ce_workspace_bytes(int64_t n, int64_t v, int64_t d, int dtype, int q_in_place, int e_in_place, int want_gradients);
 int hwer_catalogue_ce(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias /*nullable*/, const int64_t* target, int64_t n, int64_t v,
-                      int d, int dtype, float scale, int reduction, float* loss_rows, float* state, float* loss, float* counted, float* mean /*nullable*/, void* workspace,
+                      int64_t d, int dtype, float scale, int reduction, float* loss_rows, float* state, float* loss, float* counted, float* mean /*nullable*/, void* workspace,
                       size_t workspace_bytes, void* stream);
 int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias /*nullable*/, const int64_t* target, int64_t n,
-                               int64_t v, int d, int dtype, float scale, int reduction, const float* grad, const float* state, const float* counted,
+                               int64_t v, int64_t d, int dtype, float scale, int reduction, const float* grad, const float* state, const float* counted,
                                const float* mean, void* dq /*nullable*/, int64_t lddq, void* de /*nullable*/, int64_t ldde, float* dbias /*nullable*/,
                                void* workspace, size_t workspace_bytes, void* stream);
 int hwer_catalogue_ce_grads(const void* q, int64_t ldq, const void* e, int64_t lde, const float* bias /*nullable*/, const int64_t* target, int64_t n, int64_t v,
-                            int d, int dtype, float scale, int reduction, float* loss, void* dq, int64_t lddq, void* de, int64_t ldde,
+                            int64_t d, int dtype, float scale, int reduction, float* loss, void* dq, int64_t lddq, void* de, int64_t ldde,
                             float* dbias /*nullable*/, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -1,0 +1,52 @@
+"""The learned head's operators (hwer/head.py) at the edges of what a call may hold: sizes beyond 32 bits, arguments of other kinds, derivatives that
+are not offered, values at the ends of a type's range, many rows.  Tolerances as in test_head.py, whose plain implementations are used."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from test_head import TINY, TYPES, U, U32, ce_inputs, ce_reference, ce_tolerances, close, codes_reference, gpu, norm_reference, rnd
+
+
+@pytest.fixture(scope="module")
+def hw():
+    import hwer
+    from hwer import native
+    native.lib()
+    return hwer
+
+
+# ---------------------------------------------------------------------------------------------------------------- refusals (no GPU)
+WRAPS = [(1 << 32) + 8, (1 << 31) - (1 << 14) + 1, (1 << 31) - 1, 1 << 31, 1 << 40]
+
+
+@pytest.mark.parametrize("d", WRAPS)
+def test_widths_beyond_32_bits_are_refused(hw, d):
+    """a width that 32 bits cut off to 8, and those near 2^31 whose columns the wide kernels would count past it (no rows, or addresses that are never read)"""
+    from hwer import native
+    lib, p, E = native.lib(), ctypes.c_void_p(4096), native.HWER_EINVAL
+    for n in (0, 2):
+        assert lib.hwer_rms_norm(p, d, None, 0, None, 0, n, d, 0, 1e-6, p, d, None, 0, None) == E
+        assert lib.hwer_rms_norm_q8(p, d, None, 0, None, 0, n, d, 0, 1, 1e-6, p, d, p, None, 0, None) == E
+        assert lib.hwer_rms_norm_backward(p, d, p, d, None, 0, None, 0, n, d, 0, 1e-6, p, d, None, None, 0, None) == E
+    assert lib.hwer_rms_norm_backward_workspace_bytes(2, d) == 16
+    for m in (0, 2):
+        assert lib.hwer_matmul_q8(p, d, p, p, d, p, None, m, 2, d, p, 2, 0, None) == E
+        assert lib.hwer_catalogue_ce(p, d, p, d, None, p, m, 3, d, 0, 1.0, 1, p, p, p, p, None, p, 1 << 50, None) == E
+    assert lib.hwer_catalogue_ce_workspace_bytes(2, 3, d, 0, 0, 0, 1) == 0 and lib.hwer_catalogue_ce_reads_in_place(p, d, d, 1) == 0
+    # in Python, before anything of that size is allocated (one element that is broadcast)
+    x, q, s = torch.zeros(1, 1).expand(2, d), torch.zeros(1, 1, dtype=torch.int8).expand(2, d), torch.zeros(2)
+    for f in (lambda: hw.rms_norm(x), lambda: hw.rms_norm_grads(x, x), lambda: hw.rms_norm_q8(x), lambda: hw.quantize_rows_q8(x)):
+        with pytest.raises(ValueError, match="at most"):
+            f()
+    with pytest.raises(native.HwerNativeError):
+        hw.matmul_q8(q, s, q, s)      # (host tensors)
+
+
+@gpu
+def test_rows_of_too_many_codes_are_refused(hw):
+    for k in (131072, (1 << 32) + 16):
+        q, s = torch.zeros(1, 1, dtype=torch.int8, device="cuda").expand(2, k), torch.zeros(2, device="cuda")
+        with pytest.raises(ValueError, match="131071 codes"):
+            hw.matmul_q8(q, s, q, s)
