@@ -8,7 +8,8 @@
 Everything takes and returns device tensors on their own device, runs on its current stream, never synchronises and may be captured into a
 hipGraph.  `rms_norm` and `catalogue_cross_entropy` take part in autograd where an input requires a gradient; the `_grads` functions return
 the gradients directly and keep nothing (what a resident training step calls, and the simple form to capture: torch's own accumulators of leaf
-gradients belong to the stream that made them, so a captured `backward()` needs leaves of which no graph from outside the capture is alive).  The reference trains in DGL / PyTorch (hwer/gcn_ncf.py:126-327:
+gradients belong to the stream that made them, so a captured `backward()` needs leaves of which no graph from outside the capture is alive).
+Forward-mode derivatives are not offered: a dual tensor raises NotImplementedError.  The reference trains in DGL / PyTorch (hwer/gcn_ncf.py:126-327:
 out of scope here); what it hands to the search are rows (hwer/gcn_ncf.py:431,447-456).
 
 Errors: wrong shapes, types or devices raise before anything is launched (ValueError / TypeError; HwerNativeError from the library).  Values are
@@ -19,6 +20,7 @@ import contextlib
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import native
 
@@ -68,6 +70,10 @@ def _check_rows(name, t, dtypes=_DTYPES, dim=2):
 
 
 def _check_device(t, *others):
+    if _forward_ad._current_level >= 0:
+        for o in (t,) + others:
+            if isinstance(o, torch.Tensor) and _forward_ad.unpack_dual(o).tangent is not None:
+                raise NotImplementedError("the learned head's operators have no forward-mode derivative: got a dual tensor")
     index = t.get_device()
     if index < 0:
         raise native.HwerNativeError("hwer (MI355X build) needs device tensors: got one on %s; there is no CPU fallback for this path" % t.device)
@@ -107,13 +113,13 @@ def _weight(weight, x):
     return (weight if weight.is_contiguous() else weight.contiguous()), _DTYPES[weight.dtype]
 
 
-def _norm_checks(x, weight, residual, eps):
+def _norm_checks(x, weight, residual, eps, dy=None):
     _check_rows("x", x, dim=None)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x: rows of at least one element needed, got shape %s" % (tuple(x.shape),))
     if x.shape[-1] > _MAX_WIDTH:
         raise ValueError("x: rows of at most %d elements, got %d" % (_MAX_WIDTH, x.shape[-1]))
-    _check_device(x, weight, residual)
+    _check_device(x, weight, residual, dy)
     if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
         raise ValueError("residual: shape and type of x needed (%s %s), got %s %s" % (tuple(x.shape), x.dtype, tuple(residual.shape), residual.dtype))
     if not 0.0 <= float(eps) < float("inf"):
@@ -141,10 +147,9 @@ def rms_norm_grads(dy, h, weight=None, eps: float = 1e-6, dh=None):
 
 
 def _norm_backward(dy, h, weight, eps, dh, want_dw):
-    _norm_checks(h, weight, dh, eps)
+    _norm_checks(h, weight, dh, eps, dy)
     if dy.shape != h.shape or dy.dtype != h.dtype:
         raise ValueError("dy: shape and type of h needed")
-    _check_device(h, dy)
     w, wt = _weight(weight, h)
     (hr, ldh), (gr, ldg) = _flat(h), _flat(dy)
     ar, lda = _flat(dh) if dh is not None else (None, 0)

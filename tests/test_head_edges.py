@@ -50,3 +50,22 @@ def test_rows_of_too_many_codes_are_refused(hw):
         q, s = torch.zeros(1, 1, dtype=torch.int8, device="cuda").expand(2, k), torch.zeros(2, device="cuda")
         with pytest.raises(ValueError, match="131071 codes"):
             hw.matmul_q8(q, s, q, s)
+
+
+def test_dual_tensors_are_refused(hw):
+    """a forward-mode tangent would be lost without a word: requires_grad is False on a dual tensor"""
+    import torch.autograd.forward_ad as fw
+    x, w, t, q, s = torch.ones(3, 8), torch.ones(8), torch.zeros(3, dtype=torch.int64), torch.zeros(3, 8, dtype=torch.int8), torch.ones(3)
+    with fw.dual_level():
+        dual = lambda a: fw.make_dual(a, torch.ones_like(a))  # noqa: E731
+        for f in (lambda: hw.rms_norm(dual(x)), lambda: hw.rms_norm(x, dual(w)), lambda: hw.rms_norm(x, w, dual(x)), lambda: hw.rms_norm_grads(dual(x), x),
+                  lambda: hw.rms_norm_grads(x, x, dh=dual(x)), lambda: hw.rms_norm_q8(dual(x)), lambda: hw.quantize_rows_q8(dual(x)), lambda: hw.matmul_q8(q, dual(s), q, s),
+                  lambda: hw.matmul_q8(q, s, q, s, bias=dual(s)), lambda: hw.catalogue_cross_entropy(dual(x), x, t), lambda: hw.catalogue_cross_entropy(x, dual(x), t),
+                  lambda: hw.catalogue_cross_entropy(x, x, t, bias=dual(s)), lambda: hw.catalogue_cross_entropy_grads(dual(x), x, t)):
+            with pytest.raises(NotImplementedError):
+                f()
+        with pytest.raises(Exception):      # (beside a leaf torch's own refusal may come first)
+            hw.rms_norm(dual(x), torch.ones(8, requires_grad=True))
+        from hwer import native
+        with pytest.raises(native.HwerNativeError):      # no dual among the operands: as ever (these are on the host)
+            hw.rms_norm(x)
