@@ -60,6 +60,11 @@ def _wants_grad(*tensors):
     return False
 
 
+def _refuse_grad(what, *tensors):
+    if _wants_grad(*tensors):
+        raise NotImplementedError("%s has no gradient, and an operand requires one: call it under torch.no_grad(), or with detached operands" % what)
+
+
 def _check_rows(name, t, dtypes=_DTYPES, dim=2):
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s: a device tensor is needed, got %s" % (name, type(t).__name__))
@@ -215,14 +220,17 @@ def _codes(x, weight, residual, eps, norm):
 
 def rms_norm_q8(x, weight=None, residual=None, eps: float = 1e-6):
     """`rms_norm` whose y comes as int8 codes and one float32 scale for each row: -> (codes, scales) or (codes, scales, h).  y = codes * scale to half a
-    step, max|y| / 254.  No gradient (codes are for serving)."""
+    step, max|y| / 254.  No gradient, of h neither (codes are for serving): an operand that requires one raises where gradients are enabled."""
     _norm_checks(x, weight, residual, eps)
+    _refuse_grad("rms_norm_q8", x, weight, residual)
     return _codes(x, weight, residual, float(eps), 1)
 
 
 def quantize_rows_q8(x):
-    """Rows as int8 codes and one float32 scale each, x = codes * scale to half a step: -> (codes, scales).  What a catalogue is stored as for `matmul_q8`."""
+    """Rows as int8 codes and one float32 scale each, x = codes * scale to half a step: -> (codes, scales).  What a catalogue is stored as for `matmul_q8`.
+    No gradient: rows that require one (a trained table) raise where gradients are enabled."""
     _norm_checks(x, None, None, 0.0)
+    _refuse_grad("quantize_rows_q8", x)
     return _codes(x, None, None, 0.0, 0)
 
 
@@ -234,10 +242,12 @@ def _check_vector(name, t, n):
 
 def matmul_q8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
     """out = (a @ b.T) * a_scale[:, None] * b_scale (+ bias): a (m, k) and b (n, k) int8 codes, a_scale (m,), b_scale (n,), bias (n,) float32;
-    out (m, n) float32 / float16 / bfloat16.  The integer sums are exact (k <= 131 071)."""
+    out (m, n) float32 / float16 / bfloat16.  The integer sums are exact (k <= 131 071).  No gradient: scales or a bias that
+    require one raise where gradients are enabled."""
     _check_rows("a", a, (torch.int8,))
     _check_rows("b", b, (torch.int8,))
     _check_device(a, b, a_scale, b_scale, bias)
+    _refuse_grad("matmul_q8", a_scale, b_scale, bias)
     if a.shape[1] != b.shape[1]:
         raise ValueError("rows of %d against rows of %d codes" % (a.shape[1], b.shape[1]))
     if a.shape[1] > _MAX_CODES:

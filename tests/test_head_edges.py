@@ -69,3 +69,19 @@ def test_dual_tensors_are_refused(hw):
         from hwer import native
         with pytest.raises(native.HwerNativeError):      # no dual among the operands: as ever (these are on the host)
             hw.rms_norm(x)
+
+
+# ---------------------------------------------------------------------------------------------------------------- what a call may be given (GPU)
+@gpu
+def test_operators_without_a_gradient_say_so(hw):
+    x, w, q, s = torch.ones(3, 8, device="cuda"), torch.ones(8, device="cuda"), torch.zeros(3, 8, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda")
+    p = lambda a: a.clone().requires_grad_()  # noqa: E731
+    calls = (lambda: hw.rms_norm_q8(p(x)), lambda: hw.rms_norm_q8(x, p(w)), lambda: hw.rms_norm_q8(x, w, p(x)), lambda: hw.quantize_rows_q8(p(x)), lambda: hw.matmul_q8(q, p(s), q, s),
+             lambda: hw.matmul_q8(q, s, q, p(s)), lambda: hw.matmul_q8(q, s, q, s, bias=p(s)))
+    for f in calls:
+        with pytest.raises(NotImplementedError, match="no_grad"):
+            f()
+        with torch.no_grad():
+            f()
+    # the gradients' own functions take parameters as they are
+    assert hw.rms_norm_grads(x, x, p(w))[1].shape == (8,) and hw.catalogue_cross_entropy_grads(p(x), p(x), torch.zeros(3, dtype=torch.int64, device="cuda"))[1].shape == (3, 8)
