@@ -55,7 +55,7 @@ def _like(t, dtype=None):
 def _wants_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
-            if t is not None and t.requires_grad:
+            if getattr(t, "requires_grad", False):      # (anything else than a tensor is refused by the checks)
                 return True
     return False
 
@@ -75,9 +75,12 @@ def _check_rows(name, t, dtypes=_DTYPES, dim=2):
 
 
 def _check_device(t, *others):
+    for o in others:
+        if o is not None and not isinstance(o, torch.Tensor):
+            raise TypeError("a device tensor is needed, got %s" % type(o).__name__)
     if _forward_ad._current_level >= 0:
         for o in (t,) + others:
-            if isinstance(o, torch.Tensor) and _forward_ad.unpack_dual(o).tangent is not None:
+            if o is not None and _forward_ad.unpack_dual(o).tangent is not None:
                 raise NotImplementedError("the learned head's operators have no forward-mode derivative: got a dual tensor")
     index = t.get_device()
     if index < 0:
@@ -152,6 +155,7 @@ def rms_norm_grads(dy, h, weight=None, eps: float = 1e-6, dh=None):
 
 
 def _norm_backward(dy, h, weight, eps, dh, want_dw):
+    _check_rows("dy", dy, dim=None)
     _norm_checks(h, weight, dh, eps, dy)
     if dy.shape != h.shape or dy.dtype != h.dtype:
         raise ValueError("dy: shape and type of h needed")
@@ -236,6 +240,8 @@ def quantize_rows_q8(x):
 
 # ---------------------------------------------------------------------------------------------------------------- 8-bit product
 def _check_vector(name, t, n):
+    if t is None:
+        raise TypeError("%s: a device tensor is needed, got None" % name)
     if t.dtype is not torch.float32 or not _is_vector(t, n):
         raise ValueError("%s: float32 of shape (%d,) needed, got %s %s" % (name, n, t.dtype, tuple(t.shape)))
 
@@ -276,6 +282,8 @@ class _CeCall:
         _check_rows("table", table)
         if table.dtype != queries.dtype or table.shape[1] != queries.shape[1]:
             raise ValueError("table: rows of the queries' width and type needed (%d %s), got %s %s" % (queries.shape[1], queries.dtype, tuple(table.shape), table.dtype))
+        if targets is None:
+            raise TypeError("targets: a device tensor is needed, got None")
         _check_device(queries, table, targets, bias)
         if targets.dtype not in (torch.int64, torch.int32) or not _is_vector(targets, queries.shape[0]):
             raise ValueError("targets: int64 or int32 of shape (%d,) needed, got %s %s" % (queries.shape[0], targets.dtype, tuple(targets.shape)))

@@ -85,3 +85,19 @@ def test_operators_without_a_gradient_say_so(hw):
             f()
     # the gradients' own functions take parameters as they are
     assert hw.rms_norm_grads(x, x, p(w))[1].shape == (8,) and hw.catalogue_cross_entropy_grads(p(x), p(x), torch.zeros(3, dtype=torch.int64, device="cuda"))[1].shape == (3, 8)
+
+
+@gpu
+def test_operands_that_are_no_tensors_raise_type_errors(hw):
+    x, w, q, s, t = torch.ones(3, 8, device="cuda"), torch.ones(8, device="cuda"), torch.zeros(3, 8, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    for bad in ([1.0] * 8, 1.0, w.cpu().numpy()):
+        for f in (lambda: hw.rms_norm(bad), lambda: hw.rms_norm(x, bad), lambda: hw.rms_norm(x, w, bad), lambda: hw.rms_norm_grads(bad, x), lambda: hw.rms_norm_grads(x, bad),
+                  lambda: hw.rms_norm_grads(x, x, bad), lambda: hw.rms_norm_grads(x, x, dh=bad), lambda: hw.rms_norm_q8(x, bad), lambda: hw.rms_norm_q8(x, w, bad),
+                  lambda: hw.quantize_rows_q8(bad), lambda: hw.matmul_q8(bad, s, q, s), lambda: hw.matmul_q8(q, bad, q, s), lambda: hw.matmul_q8(q, s, q, bad),
+                  lambda: hw.matmul_q8(q, s, q, s, bias=bad), lambda: hw.catalogue_cross_entropy(bad, x, t), lambda: hw.catalogue_cross_entropy(x, bad, t),
+                  lambda: hw.catalogue_cross_entropy(x, x, bad), lambda: hw.catalogue_cross_entropy(x, x, t, bias=bad), lambda: hw.catalogue_cross_entropy_grads(x, x, bad)):
+            with pytest.raises(TypeError):
+                f()
+    for f in (lambda: hw.rms_norm_grads(None, x), lambda: hw.matmul_q8(q, None, q, s), lambda: hw.matmul_q8(q, s, q, None), lambda: hw.catalogue_cross_entropy(x, x, None)):
+        with pytest.raises(TypeError):
+            f()
