@@ -869,6 +869,7 @@ __global__ __launch_bounds__(256) void ce_de_kernel(const float* __restrict__ o,
 
 // ---------------------------------------------------------------------------------------------------------------- host
 constexpr int kCeMaxDim = 256;
+constexpr int64_t kCeMaxRows = (int64_t(1) << 26) - 256;
 static int ce_width(int64_t d) { return d >= 1 && d <= kCeMaxDim ? int(d) : 0; }      // 0: refused by CeCall::check
 static int ce_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
@@ -963,8 +964,9 @@ struct CeCall {
     int check(const char* what, void* workspace, size_t bytes, bool want_mean, void* stream) {
         if (!known_dtype(dtype)) return fail(HWER_EINVAL, "%s: unknown element type %d", what, dtype);
         if (d < 1) return fail(HWER_EINVAL, "%s: rows of 1..%d elements are supported", what, kCeMaxDim);
-        const int64_t most = (int64_t(1) << 31) - 256;
-        if (n < 0 || v < 1 || n > most || v > most) return fail(HWER_EINVAL, "%s: %lld rows, %lld classes", what, (long long)n, (long long)v);
+        // classes are 32-bit numbers; a wave for each query has to stay below a launch's 2^32 threads
+        if (n < 0 || v < 1 || n > kCeMaxRows || v > (int64_t(1) << 31) - 256)
+            return fail(HWER_EINVAL, "%s: %lld rows (at most %lld), %lld classes (at most 2^31 - 256)", what, (long long)n, (long long)kCeMaxRows, (long long)v);
         if (!(scale > 0.f) || !(scale < INFINITY)) return fail(HWER_EINVAL, "%s: scale must be positive and finite", what);
         if (n && (!q || !target)) return fail(HWER_EINVAL, "%s: null queries or targets", what);
         if (!e || ldq < d || lde < d) return fail(HWER_EINVAL, "%s: null table or a row stride below d", what);

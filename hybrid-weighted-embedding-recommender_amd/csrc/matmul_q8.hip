@@ -454,6 +454,13 @@ constexpr int kFewRows = 32;
 // 24 x 356 x 2 490: 20 and 9
 constexpr int kFewWholeK = 512;
 
+// A launch has fewer than 2^32 threads: 256 for 64 or 16 rows against a few, or for 128 x 128 of the output, 512 for 128 x 256
+static bool matmul_q8_fits(int64_t m, int64_t n, int64_t k) {
+    if (m > (int64_t(1) << 31) - 256 || n > (int64_t(1) << 31) - 256) return false;
+    if (std::min(m, n) <= kFewRows) return cdiv64(std::max(m, n), k <= kFewWholeK ? 64 : 16) < (int64_t(1) << 24);
+    return cdiv64(m, 128) * std::max(cdiv64(n, 128), 2 * cdiv64(n, 256)) < (int64_t(1) << 24) - 8;
+}
+
 template <typename O, bool ALIGNED>
 static void matmul_q8_launch(const QmmArgs& g, hipStream_t st) {
     if (std::min(g.m, g.n) <= kFewRows) {
@@ -499,7 +506,7 @@ extern "C" int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale
     if (!known_dtype(out_dtype)) return fail(HWER_EINVAL, "matmul_q8: unknown output type %d", out_dtype);
     if (m < 0 || n < 0 || k < 0 || k > 131071) return fail(HWER_EINVAL, "matmul_q8: m=%lld, n=%lld, k=%lld (k <= 131071: sums stay in 32 bits)", (long long)m, (long long)n, (long long)k);
     if (m == 0 || n == 0) return HWER_OK;
-    if (m > (int64_t(1) << 31) - 256 || n > (int64_t(1) << 31) - 256 || cdiv64(m, 64) * cdiv64(n, 64) > (int64_t(1) << 30))
+    if (!matmul_q8_fits(m, n, k))
         return fail(HWER_EINVAL, "matmul_q8: m=%lld, n=%lld: too many tiles for one call", (long long)m, (long long)n);
     if ((k && (!a || !b)) || !a_scale || !b_scale || !out) return fail(HWER_EINVAL, "matmul_q8: null operand");
     if (lda < k || ldb < k || ldo < n) return fail(HWER_EINVAL, "matmul_q8: a row stride is below the row's length");

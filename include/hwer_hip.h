@@ -551,7 +551,8 @@ int hwer_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t 
                            void* dweight /*nullable*/, void* workspace, size_t workspace_bytes, void* stream);
 
 /* out[m][n] = (sum_k a[m][k] b[n][k]) * a_scale[m] * b_scale[n] (+ bias[n]): int8 rows with a float32 scale each on both sides (tokens / queries on the
- * left, channels / catalogue rows on the right), exact 32-bit sums (k <= 131071), out float32 / float16 / bfloat16. */
+ * left, channels / catalogue rows on the right), exact 32-bit sums (k <= 131071), out float32 / float16 / bfloat16.
+ * A launch has fewer than 2^32 threads: up to 32 rows against fewer than 2^30 (k > 512: 2^28), otherwise fewer than 2^24 tiles of 128 x 128. */
 int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* b, int64_t ldb, const float* b_scale, const float* bias /*nullable*/,
                    int64_t m, int64_t n, int64_t k, void* out, int64_t ldo, int out_dtype, void* stream);
 
@@ -561,6 +562,7 @@ int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int
  *   Losses and gradients keep their digits where p_target is close to 1 (the target is left out of the sums).
  *   reduction 0 none, 1 mean over counted rows (0 without any), 2 sum.  1 <= d <= hwer_catalogue_ce_max_dim().
  *   loss_rows (n), state (n, 4; 16-byte aligned: what the backward call needs of every row), loss (1, reduction 1 / 2), counted (1, the number of counted rows); mean (n, d) float32, nullable: the mean of a row's classes but its target under their probabilities, which the backward call needs for dq.
+ *   n <= 2^26 - 256, v <= 2^31 - 256.
  * Backward: grad = upstream gradient of the reduced loss (one value, nullable = 1) or of each row (reduction 0).  dq, de, dbias nullable; dbias
  *   comes with de.  dq / de in the rows' type.  Every sum has a fixed order (no atomics).
  * hwer_catalogue_ce_grads: loss (reduction 1 / 2) and gradients in one call, without what the two calls hand over; float32 rows are laid out for the

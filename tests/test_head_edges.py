@@ -52,6 +52,18 @@ def test_rows_of_too_many_codes_are_refused(hw):
             hw.matmul_q8(q, s, q, s)
 
 
+def test_more_rows_than_a_launch_has_threads_for_are_refused(hw):
+    """before anything is launched (these calls used to fail at a later launch; the addresses are never read)"""
+    from hwer import native
+    lib, p, E = native.lib(), ctypes.c_void_p(4096), native.HWER_EINVAL
+    for n in ((1 << 26) - 255, 1 << 26, 1 << 30):
+        assert lib.hwer_catalogue_ce(p, 8, p, 8, None, p, n, 3, 8, 0, 1.0, 1, p, p, p, p, None, p, 1 << 50, None) == E
+        assert lib.hwer_catalogue_ce_grads(p, 8, p, 8, None, p, n, 3, 8, 0, 1.0, 1, p, p, 8, p, 8, None, p, 1 << 50, None) == E
+        assert lib.hwer_catalogue_ce_backward(p, 8, p, 8, None, p, n, 3, 8, 0, 1.0, 1, p, p, p, p, p, 8, p, 8, None, p, 1 << 50, None) == E
+    for m, n, k in ((1, 1 << 30, 16), (1 << 30, 32, 512), (1 << 28, 5, 513), (40, (1 << 31) - 256, 64), (1 << 30, 1 << 30, 8), (1 << 31, 2, 8)):
+        assert lib.hwer_matmul_q8(p, k, p, p, k, p, None, m, n, k, p, n, 0, None) == E, (m, n, k)
+
+
 def test_dual_tensors_are_refused(hw):
     """a forward-mode tangent would be lost without a word: requires_grad is False on a dual tensor"""
     import torch.autograd.forward_ad as fw
