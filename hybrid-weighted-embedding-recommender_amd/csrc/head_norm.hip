@@ -47,16 +47,26 @@ __device__ __forceinline__ void store_pack(E* row, int c, int d, const Pack<E, N
 
 // A code is round_half_even(127 v / top) of exact values.  The float32 quotient t = fl(v) (127 / fl(top)) is off by at most 4 * 2^-24 |t|, which leaves two
 // codes open next to the border between them - seldom for products of float32 weights, often for 16-bit rows, whose quotients can BE borders.  Then the
-// exact sign of 127 v - border * top decides, from products and their exact rounding errors (one fma each).
+// sign of 127 v - border * top decides: both products next to their rounding errors (one fma each), the products' difference, which has no error (they
+// are within a factor of two), and the errors' difference, which has few bits.  That is exact where v and top are float32 values.  Products of float32
+// weights have low parts, whose own roundings leave 2^-45.7 of the product: closer than 2^-44 to a border a code is done once more, in 64 bits.
 __device__ __forceinline__ bool q8_open(float t, float c) { return fabsf(fabsf(t - c) - 0.5f) <= 3e-7f * fabsf(t); }
-// v = vh + ve, top = th + te
-__device__ __forceinline__ float q8_settle(float t, float c, float vh, float ve, float th, float te) {
-    const float side = t > c ? 1.f : -1.f, border = c + 0.5f * side;
-    const float p = 127.f * vh, q = border * th;
-    const float d = ((p - q) + (fmaf(127.f, vh, -p) - fmaf(border, th, -q)) + (127.f * ve - border * te)) * side;
+// v = vh + ve, top = th + te; 127 and the border over 128, which keeps the products in range
+__device__ __forceinline__ float q8_settle(float t, float c, float vh, float ve, float th, float te, bool& unsure) {
+    const float side = t > c ? 1.f : -1.f, border = c + 0.5f * side, k = 127.f / 128.f, l = border * (1.f / 128.f);
+    const float p = k * vh, q = l * th;
+    const float d = ((p - q) + (fmaf(k, vh, -p) - fmaf(l, th, -q)) + (k * ve - l * te)) * side;
+    unsure = unsure || ((ve != 0.f || te != 0.f) && fabsf(d) <= 0x1p-44f * fabsf(p));
     return d > 0.f ? c + side : d < 0.f ? c : rintf(border);      // (on the border: the even one)
 }
-__device__ __forceinline__ int q8_exact(float h, float w, double top) { return int(rint(127.0 * (double(h) * double(w)) / top)); }
+// the same in 64 bits, which hold the 48 of a product: 127 v and border * top have 56, and their errors 3
+__device__ __forceinline__ int q8_exact(float h, float w, double top) {
+    const double v = double(h) * double(w), t = 127.0 * v / top, c = rint(t);
+    if (!(fabs(fabs(t - c) - 0.5) <= 1e-13 * fabs(t))) return int(c);
+    const double side = t > c ? 1.0 : -1.0, border = c + 0.5 * side, p = 127.0 * v, q = border * top;
+    const double d = ((p - q) + (fma(127.0, v, -p) - fma(border, top, -q))) * side;
+    return int(d > 0.0 ? c + side : d < 0.0 ? c : rint(border));
+}
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }      // ordered like |v|, infinities and NaN above all else
 constexpr uint32_t kInfBits = 0x7f800000u, kTinyBits = 0x0da24260u;      // 1e-30: below it 127 / top and the products' errors leave float32's range
 
@@ -86,8 +96,15 @@ __device__ __forceinline__ float row_sum(float v, float* slots, int flip) {
     return v;
 }
 
+// Waves of a SIMD that registers are shared out for: as they come, but codes of 16-bit rows with float32 weights held by 8 waves would take 130 registers, and a
+// CU one workgroup.
+template <typename E, typename W, int T, bool Q8>
+constexpr int norm_fwd_waves() {
+    return Q8 && T == 512 && sizeof(E) < sizeof(W) ? 4 : 1;
+}
+
 template <typename E, typename W, int T, int VPT, int VW, bool Q8>
-__global__ __launch_bounds__(norm_block(T)) void norm_fwd_kernel(NormFwdArgs a) {
+__global__ __launch_bounds__(norm_block(T), (norm_fwd_waves<E, W, T, Q8>())) void norm_fwd_kernel(NormFwdArgs a) {
     constexpr int B = norm_block(T), R = B / T;     // R rows at a time
     __shared__ float s_sum[2 * (T > 64 ? T / 64 : 1)];
     __shared__ uint32_t s_top[2 * (T > 64 ? T / 64 : 1)];
@@ -162,6 +179,7 @@ __global__ __launch_bounds__(norm_block(T)) void norm_fwd_kernel(NormFwdArgs a) 
             const float top = __uint_as_float(top_bits), inv = fine ? 127.f / top : 0.f;
             if (on && t == 0) a.scale[r] = top_bits < kInfBits ? top * rstd / 127.f : NAN;      // a row with a NaN or an infinity: codes 0, scale NaN
             const bool tiny = fine && top_bits < kTinyBits;
+            bool unsure = false;      // is a code of this lane too close to a border for float32?
             int8_t* q = static_cast<int8_t*>(a.y) + rc * a.ldy;
             constexpr bool PAIR = std::is_same<W, float>::value;      // weights of 24 bits: products have a low part (16-bit rows and weights: exact)
             float te = 0.f;      // low part of the largest product, needed where a code is open
@@ -215,38 +233,42 @@ __global__ __launch_bounds__(norm_block(T)) void norm_fwd_kernel(NormFwdArgs a) 
                 for (int j = 0; j < VW; ++j) {
                     const float hv = float(h[p].e[j]), wv = w[p * VW + j], v = hv * wv, quo = v * inv;
                     float c = rintf(quo);
-                    if (q8_open(quo, c)) c = q8_settle(quo, c, v, PAIR ? fmaf(hv, wv, -v) : 0.f, top, te);
+                    if (q8_open(quo, c)) c = q8_settle(quo, c, v, PAIR ? fmaf(hv, wv, -v) : 0.f, top, te, unsure);
                     out.e[j] = fine ? int8_t(int(c)) : int8_t(0);
                 }
                 store_pack<int8_t, VW>(q, (p * T + t) * VW, own, out);
             }
             }
-            // Rows of nothing but tiny products: once more from memory, in 64 bits
+            // Once more from memory, in 64 bits: rows of nothing but tiny products, and a lane's elements with a code that is still open
             bool again;
             if constexpr (T > 64) again = tiny;
             else again = __any(tiny);
-            if (again) {
+            const bool mine = tiny || (PAIR && unsure && fine);
+            if (again || mine) {
                 const E* hp = rp ? static_cast<const E*>(a.h) + rc * a.ldh : xp + rc * a.ldx;
-                const int mine = tiny ? own : 0;
-                double exact = 0.0;
+                double exact = double(top) + double(te);
+                if (again) {
+                    double v = 0.0;
+#pragma unroll 1
+                    for (int i = 0; i < VPT * VW; ++i) {
+                        const int c = (i / VW * T + t) * VW + i % VW;
+                        if (tiny && c < own) v = fmax(v, fabs(double(float(hp[c])) * double(wp ? float(wp[c]) : 1.f)));
+                    }
+                    v = lanes_max<(T < 64 ? T : 64)>(v);
+                    if constexpr (T > 64) {
+                        __syncthreads();
+                        if ((threadIdx.x & 63) == 0) s_exact[threadIdx.x >> 6] = v;
+                        __syncthreads();
+                        v = s_exact[0];
+#pragma unroll 1
+                        for (int i = 1; i < T / 64; ++i) v = fmax(v, s_exact[i]);
+                    }
+                    if (tiny) exact = v;
+                }
 #pragma unroll 1
                 for (int i = 0; i < VPT * VW; ++i) {
                     const int c = (i / VW * T + t) * VW + i % VW;
-                    if (c < mine) exact = fmax(exact, fabs(double(float(hp[c])) * double(wp ? float(wp[c]) : 1.f)));
-                }
-                exact = lanes_max<(T < 64 ? T : 64)>(exact);
-                if constexpr (T > 64) {
-                    __syncthreads();
-                    if ((threadIdx.x & 63) == 0) s_exact[threadIdx.x >> 6] = exact;
-                    __syncthreads();
-                    exact = s_exact[0];
-#pragma unroll 1
-                    for (int i = 1; i < T / 64; ++i) exact = fmax(exact, s_exact[i]);
-                }
-#pragma unroll 1
-                for (int i = 0; i < VPT * VW; ++i) {
-                    const int c = (i / VW * T + t) * VW + i % VW;
-                    if (c < mine) q[c] = int8_t(q8_exact(float(hp[c]), wp ? float(wp[c]) : 1.f, exact));
+                    if (mine && c < own) q[c] = int8_t(q8_exact(float(hp[c]), wp ? float(wp[c]) : 1.f, exact));
                 }
             }
         }

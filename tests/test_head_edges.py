@@ -113,3 +113,54 @@ def test_operands_that_are_no_tensors_raise_type_errors(hw):
     for f in (lambda: hw.rms_norm_grads(None, x), lambda: hw.matmul_q8(q, None, q, s), lambda: hw.matmul_q8(q, s, q, None), lambda: hw.catalogue_cross_entropy(x, x, None)):
         with pytest.raises(TypeError):
             f()
+
+
+# ---------------------------------------------------------------------------------------------------------------- codes
+def exact_codes(h, w):
+    """round_half_even(127 v / max|v|) of one row in integers (values as fractions)"""
+    from fractions import Fraction
+    v = [Fraction(float(a)) * Fraction(float(b)) for a, b in zip(h, w)]
+    top = max(abs(a) for a in v)
+    return torch.tensor([round(127 * a / top) for a in v], dtype=torch.int8)      # (Python rounds fractions to even)
+
+
+# 24-bit factors h, w and H, W of a row's largest product, whose quotient 127 h w / (H W) misses a border between two codes by about 2^-52 of itself
+NEAR_BORDERS = [(9421653, 11442761, 11141540, 15856770), (11326493, 15955928, 14549902, 14674142)]
+
+
+@gpu
+@pytest.mark.parametrize("d", [4, 24, 1000, 4096, 40961])
+def test_q8_codes_next_to_a_border_are_exact(hw, d):
+    for h, w, top_h, top_w in NEAR_BORDERS:
+        for near in (0, 1, -1):      # beside it: the same product one step of a factor further
+            x, y = torch.zeros(2, d), torch.ones(d)
+            x[0, :4] = torch.tensor([float(top_h), float(h), -float(h), float(h + near)])
+            y[:4] = torch.tensor([float(top_w), float(w), float(w), float(w)])
+            x[1] = 0.5 * x[0]
+            want = exact_codes(x[0], y)
+            q = hw.rms_norm_q8(x.cuda(), y.cuda())[0].cpu()
+            assert torch.equal(q[0], want) and torch.equal(q[1], want), (q[:, :4], want[:4])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("d", [9, 24, 250, 4096, 40961])
+def test_q8_codes_of_the_largest_values_are_exact(hw, d, dtype):
+    """rows that reach 127 * 2^121, whose 127-fold is beyond float32: values on the borders between two codes, and next to them"""
+    steps = torch.tensor([127.0, 0.5, 1.5, 2.5, -0.5, -1.5, 3.5, 100.5, -126.5])
+    x = torch.zeros(2, d, dtype=torch.float64)
+    x[0, :9], x[0, 9:] = steps, 50 * torch.tanh(rnd(d, d - 9))
+    x[1, :9] = -steps
+    x = (x * 2.0 ** 121).to(dtype)
+    if dtype == torch.float32 and d > 9:
+        x[:, 9] = torch.nextafter(x[:, 7], x[:, 0])      # 100.5 and -100.5, one step of float32 upwards / away
+        x[:, 10] = torch.nextafter(x[:, 8], x[:, 0])
+    codes, top = codes_reference(x, None)
+    q, s = hw.quantize_rows_q8(x.cuda())
+    assert torch.equal(q.cpu(), codes)
+    close(s, top / 127, top / 127 * 3 * U32, "scale")
+    # the same as products: rows of 2^41 (their squares are in range) and weights of 2^80
+    for w in (torch.full((d,), 2.0 ** 80), torch.full((d,), 2.0 ** 80).to(dtype)):
+        q, s = hw.rms_norm_q8((x.double() * 2.0 ** -80).to(dtype).cuda(), w.cuda())
+        assert torch.equal(q.cpu(), codes)
+
