@@ -177,7 +177,7 @@ __global__ __launch_bounds__(norm_block(T), (norm_fwd_waves<E, W, T, Q8>())) voi
             }
             const bool fine = top_bits > 0 && top_bits < kInfBits;
             const float top = __uint_as_float(top_bits), inv = fine ? 127.f / top : 0.f;
-            if (on && t == 0) a.scale[r] = top_bits < kInfBits ? top * rstd / 127.f : NAN;      // a row with a NaN or an infinity: codes 0, scale NaN
+            if (on && t == 0) a.scale[r] = fine ? top * rstd / 127.f : top_bits == 0 ? 0.f : NAN;      // (zeros: 0, without eps too; a NaN or an infinity: NaN)
             const bool tiny = fine && top_bits < kTinyBits;
             bool unsure = false;      // is a code of this lane too close to a border for float32?
             int8_t* q = static_cast<int8_t*>(a.y) + rc * a.ldy;
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_fwd_wide_kernel(NormFwdArgs
             for (int i = 1; i < kWideThreads / 64; ++i) top = fmax(top, s_top[i]);
             fine = top > 0.0 && top < double(INFINITY);
             inv = fine ? 127.f / float(top) : 0.f;
-            if (t == 0) a.scale[r] = top < double(INFINITY) ? float(top) * rstd / 127.f : NAN;
+            if (t == 0) a.scale[r] = fine ? float(top) * rstd / 127.f : top == 0.0 ? 0.f : NAN;
         }
         for (int c = t * VW; c < a.d; c += kWideThreads * VW) {
             const PE h = load(c);

@@ -534,12 +534,13 @@ int hwer_pack_exchange(const int64_t* idx, const double* score, const double* di
 
 /* Root-mean-square norm:  h = x + residual rounded to the rows' type (written when there is a residual; outputs share memory with no input),
  *   y = h * weight / sqrt(mean(h^2) + eps).  weight (nullable = ones): float32 or the rows' type.  One pass over memory.
- * 1 <= d <= 2^31 - 2^14.  The sum of squares is float32: |h| below 1.8e19 / sqrt(d).  A NaN or an infinity stays in its row. */
+ * 1 <= d <= 2^31 - 2^14.  The sum of squares is float32: |h| below 1.8e19 / sqrt(d), and with eps below 1e-32 a largest |h|
+ * above 1e-16.  A NaN or an infinity stays in its row. */
 int hwer_rms_norm(const void* x, int64_t ldx, const void* residual /*nullable*/, int64_t ldr, const void* weight /*nullable*/, int weight_dtype,
                   int64_t rows, int64_t d, int dtype, float eps, void* y, int64_t ldy, void* h, int64_t ldh, void* stream);
 /* The same rows as int8 codes with one scale a row: q = round_half_even(127 v / max|v|), v = h * weight, scale = max|v| / (127 sqrt(mean(h^2) + eps));
  * norm = 0: scale = max|v| / 127 (plain quantisation).  The codes are exact for their definition.  A row of zeros: codes 0, scale 0; a row
- * with a NaN or an infinity: codes 0, scale NaN. */
+ * with a NaN or an infinity (a product beyond float32 is one): codes 0, scale NaN. */
 int hwer_rms_norm_q8(const void* x, int64_t ldx, const void* residual /*nullable*/, int64_t ldr, const void* weight /*nullable*/, int weight_dtype,
                      int64_t rows, int64_t d, int dtype, int norm, float eps, int8_t* q, int64_t ldq, float* scale, void* h, int64_t ldh, void* stream);
 /* Gradients:  dx = (weight * dy - h * r^2 * mean(h * weight * dy)) * r + dh,  dweight = sum_rows dy * h * r  (the residual's gradient is dx).

@@ -164,3 +164,12 @@ def test_q8_codes_of_the_largest_values_are_exact(hw, d, dtype):
         q, s = hw.rms_norm_q8((x.double() * 2.0 ** -80).to(dtype).cuda(), w.cuda())
         assert torch.equal(q.cpu(), codes)
 
+@gpu
+@pytest.mark.parametrize("d", [24, 4096, 40961])
+def test_q8_scale_of_a_row_of_zeros_is_zero(hw, d):
+    """... whatever eps is: without one its norm is 0 / 0, but the codes' scale is not"""
+    x = torch.zeros(3, d)
+    x[1, 2] = 1.0
+    for w in (None, torch.ones(d).cuda(), torch.zeros(d).cuda()):
+        q, s = hw.rms_norm_q8(x.cuda(), w, eps=0.0)
+        assert float(s[0]) == 0 and float(s[2]) == 0 and not q[0].any() and not q[2].any() and torch.isfinite(s).all()
