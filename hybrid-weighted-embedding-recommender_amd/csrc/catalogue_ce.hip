@@ -720,7 +720,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
     }
     // in powers of two, 64 bits: the other classes' lse (all of them where no target counts) and the target's logit
     const int64_t t = a.target[r];
-    const bool on = t >= 0 && t < a.v;
+    const bool on = t >= 0 && t < a.v, there = on && !(BIAS && a.bias[t] == -INFINITY);      // (a target that is taken out has no row and no gradient)
     const double rest = sum == 0.f ? -double(INFINITY) : double(top) * double(unit) + log2(double(sum)) - double(a.off);
     double lse = rest, miss = 0.0, loss = 0.0;
     if (on) {
@@ -749,7 +749,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
     }
     if (t_in == 0) {
         a.loss_rows[r] = float(loss);
-        if constexpr (GRADS) ce_put_rowp<BIAS>(a, r, on, hi, low, float(miss), on ? 1.f : 0.f, t);
+        if constexpr (GRADS) ce_put_rowp<BIAS>(a, r, on, hi, low, float(miss), on ? 1.f : 0.f, there ? t : -1);
         else a.state[r] = {hi, low, float(miss), 0.f};
     }
     if (!GRADS && !a.mean) return;
@@ -778,13 +778,13 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
     }
     const float f = sum == 0.f ? 0.f : (F32 ? a.sc->unscale_e : 1.f) / sum;
     const float mean[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
-    const E* e = static_cast<const E*>(a.e) + (on ? t : 0) * a.lde;
+    const E* e = static_cast<const E*>(a.e) + (there ? t : 0) * a.lde;
     const float fq = a.scale * g * float(miss);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int c = 4 * c4 + j;
         if (c >= a.d) break;
-        if constexpr (GRADS) static_cast<E*>(a.dq)[r * a.lddq + c] = E(on ? fq * (mean[j] - float(e[c])) : 0.f);
+        if constexpr (GRADS) static_cast<E*>(a.dq)[r * a.lddq + c] = E(on ? fq * (mean[j] - (there ? float(e[c]) : 0.f)) : 0.f);
         else a.mean[r * a.d + c] = mean[j];
     }
 }
@@ -824,16 +824,16 @@ __global__ __launch_bounds__(256) void ce_dq_kernel(CeRows a) {
         return;
     }
     const int64_t t = a.target[r];
-    const bool on = t >= 0 && t < a.v;
+    const bool on = t >= 0 && t < a.v, there = on && !(BIAS && a.bias[t] == -INFINITY);
     const float4 st = a.state[r];
     const float gr = a.per_row ? a.grad[r] : g;
-    if (a.rowp && lane == 0) ce_put_rowp<BIAS>(a, r, on, st.x, st.y, st.z, !on ? 0.f : a.per_row ? (g > 0.f ? gr / g : gr) : 1.f, t);
+    if (a.rowp && lane == 0) ce_put_rowp<BIAS>(a, r, on, st.x, st.y, st.z, !on ? 0.f : a.per_row ? (g > 0.f ? gr / g : gr) : 1.f, there ? t : -1);
     if (!F32 && a.rowp) ce_copy_query(a, r, on, lane);
     if (a.dq) {
         E* dq = static_cast<E*>(a.dq) + r * a.lddq;
-        const E* e = static_cast<const E*>(a.e) + (on ? t : 0) * a.lde;
+        const E* e = static_cast<const E*>(a.e) + (there ? t : 0) * a.lde;
         const float f = a.scale * gr * st.z;
-        for (int c = lane; c < a.d; c += 64) dq[c] = E(on ? f * (a.mean[r * a.d + c] - float(e[c])) : 0.f);
+        for (int c = lane; c < a.d; c += 64) dq[c] = E(on ? f * (a.mean[r * a.d + c] - (there ? float(e[c]) : 0.f)) : 0.f);
     }
 }
 

@@ -534,8 +534,8 @@ int hwer_pack_exchange(const int64_t* idx, const double* score, const double* di
 
 /* Root-mean-square norm:  h = x + residual rounded to the rows' type (written when there is a residual; outputs share memory with no input),
  *   y = h * weight / sqrt(mean(h^2) + eps).  weight (nullable = ones): float32 or the rows' type.  One pass over memory.
- * 1 <= d <= 2^31 - 2^14.  The sum of squares is float32: |h| below 1.8e19 / sqrt(d), and with eps below 1e-32 a largest |h|
- * above 1e-16.  A NaN or an infinity stays in its row. */
+ * 1 <= d <= 2^31 - 2^14.  The sum of squares is float32: |h| below 1.8e19 / sqrt(d), and with eps below 1e-28 a largest |h|
+ * above 1e-14.  A NaN or an infinity stays in its row. */
 int hwer_rms_norm(const void* x, int64_t ldx, const void* residual /*nullable*/, int64_t ldr, const void* weight /*nullable*/, int weight_dtype,
                   int64_t rows, int64_t d, int dtype, float eps, void* y, int64_t ldy, void* h, int64_t ldh, void* stream);
 /* The same rows as int8 codes with one scale a row: q = round_half_even(127 v / max|v|), v = h * weight, scale = max|v| / (127 sqrt(mean(h^2) + eps));
@@ -560,6 +560,7 @@ int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int
 /* Softmax cross entropy of n query rows over all v rows of a catalogue, logits z = scale * <q_r, e_v> + bias_v never stored:
  *   loss_r = log sum_v exp z_rv - z_{r, target_r}.  target -1: the row does not count (loss 0, no gradient); any other target outside 0 .. v - 1:
  *   loss NaN, no gradient.  bias (nullable, float32, per class): -inf takes a class out; with every class out the loss is +inf and p = 0.
+ *   A target that is taken out makes its row's loss +inf; its class stays out all the same: a row of zeros in dq, without gradients of its own.
  *   Losses and gradients keep their digits where p_target is close to 1 (the target is left out of the sums).
  *   reduction 0 none, 1 mean over counted rows (0 without any), 2 sum.  1 <= d <= hwer_catalogue_ce_max_dim().
  *   loss_rows (n), state (n, 4; 16-byte aligned: what the backward call needs of every row), loss (1, reduction 1 / 2), counted (1, the number of counted rows); mean (n, d) float32, nullable: the mean of a row's classes but its target under their probabilities, which the backward call needs for dq.

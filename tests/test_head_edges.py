@@ -173,3 +173,45 @@ def test_q8_scale_of_a_row_of_zeros_is_zero(hw, d):
     for w in (None, torch.ones(d).cuda(), torch.zeros(d).cuda()):
         q, s = hw.rms_norm_q8(x.cuda(), w, eps=0.0)
         assert float(s[0]) == 0 and float(s[2]) == 0 and not q[0].any() and not q[2].any() and torch.isfinite(s).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------- cross entropy
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,d", [(40, 333, 64), (70, 150, 100), (300, 90, 256)])
+def test_cross_entropy_of_a_target_that_is_taken_out(hw, n, v, d, dtype):
+    """its row's loss is infinite; whatever the class holds reaches no gradient, and it has none itself"""
+    x, e, t, b = ce_inputs(n + d, n, v, d, dtype, bias=True)
+    b[3::7] = float("-inf")
+    t[::4] = 3
+    t[1::4] = 10
+    t[2] = -1
+    gone = torch.isinf(b)
+    bad, clean = e.clone(), e.clone()
+    clean[gone] = 0
+    bad[gone] = float("nan")
+    bad[10], bad[17] = float("inf"), torch.finfo(dtype).max
+    out_of = gone[t.clamp_min(0)] & (t >= 0)
+    # a class of its own, at -inf, that the target names: neither its row nor its gradients are of the table
+    ref_e, ref_b, ref_t = torch.cat([clean, torch.zeros(1, d, dtype=dtype)]), torch.cat([b, b[3:4]]), torch.where(out_of, torch.tensor(v), t)
+    up = torch.linspace(-1, 1, n).double()
+    up[out_of & (torch.arange(n) % 8 < 4)] = 0          # the caller drops some of the infinite losses
+    counted = int((t >= 0).sum())
+    one = torch.full((n,), 1.0 / counted, dtype=torch.float64)
+    for form, g in (("grads", one), ("mean", one), ("none", up)):
+        ref = ce_reference(x, ref_e, ref_t, 4.0, ref_b, g)
+        tol = ce_tolerances(ref, dtype, n, v, d)
+        if form == "grads":
+            loss, dx, de, db = hw.catalogue_cross_entropy_grads(x.cuda(), bad.cuda(), t.cuda(), scale=4.0, bias=b.cuda())
+        else:
+            leaves = [a.cuda().requires_grad_() for a in (x, bad, b)]
+            loss = hw.catalogue_cross_entropy(leaves[0], leaves[1], t.cuda(), scale=4.0, bias=leaves[2], reduction=form)
+            loss.backward(None if form == "mean" else up.float().cuda())
+            dx, de, db = (a.grad for a in leaves)
+        if form == "none":
+            assert torch.isinf(loss.detach().cpu()[out_of]).all() and torch.isfinite(loss.detach().cpu()[~out_of]).all()
+        else:
+            assert float(loss.detach()) == float("inf")
+        for got, key in ((dx, "dx"), (de, "de"), (db, "db")):
+            close(got, ref[key] if key == "dx" else ref[key][:v], 1.01 * (tol[key] if key == "dx" else tol[key][:v]) + (ref[key + "_size"] * 4 * U32)[:v if key != "dx" else n], form + " " + key)
+        assert not de[gone.cuda()].any() and not db[gone.cuda()].any()
