@@ -61,6 +61,16 @@ struct CeScalars {
     float unscale_s, unscale_q, unscale_e;      // float32 rows: 2^-(eq + ee), 2^-eq, 2^-ee, which undo the operands' powers of two
     float fac_e, fac_b;                          // factors of de and db
     float g_top;                                 // largest |upstream gradient| of a row
+    int counted;                                 // counted rows, of more than kCountedByRow
+};
+
+// A sum over the rows: one workgroup walks over up to kSumRows of them, more are summed in kSumParts parts first (1 M rows by one workgroup 0.5 ms).
+constexpr int64_t kSumRows = 16384;
+constexpr int kSumParts = 256;
+struct CeSums {
+    double loss[kSumParts];
+    float top[kSumParts];
+    int counted[kSumParts];
 };
 
 struct CePass {
@@ -74,6 +84,7 @@ struct CePass {
     const int64_t* target;       // per query its target
     int* counts;                 // pass 1: counted rows of each 32 queries
     const float* loss_rows;      // pass 2, nullable: the queries' losses, reduced by one more workgroup
+    const CeSums* sums;          // (nullable: those of more than kSumRows queries are summed in parts)
     float* loss;
     int reduction;
     float* zt;                   // pass 1: per query its target's logit, in the unit of m
@@ -112,14 +123,18 @@ constexpr int kFewTerms = 128;
 
 // Sum or mean of the rows' losses, and how many rows count; with no row counted the mean is 0.  One workgroup, 64-bit sums in a fixed order.
 template <int T>
-__device__ __forceinline__ void ce_reduce_loss(const float* loss_rows, const int64_t* target, int64_t n, int reduction, float* loss, float* counted) {
+__device__ __forceinline__ void ce_reduce_loss(const float* loss_rows, const int64_t* target, const CeSums* sums, int64_t n, int reduction, float* loss, float* counted) {
     __shared__ double s_sum[T / 64];
     __shared__ int s_cnt[T / 64];
     double sum = 0.0;
     int cnt = 0;      // n < 2^31
-    for (int64_t r = threadIdx.x; r < n; r += T) {
-        sum += double(loss_rows[r]);
-        cnt += target[r] != -1;
+    if (sums) {
+        for (int i = threadIdx.x; i < kSumParts; i += T) sum += sums->loss[i], cnt += sums->counted[i];
+    } else {
+        for (int64_t r = threadIdx.x; r < n; r += T) {
+            sum += double(loss_rows[r]);
+            cnt += target[r] != -1;
+        }
     }
     sum = wave_sum_f64(sum);
     cnt = wave_sum_i32(cnt);
@@ -132,6 +147,26 @@ __device__ __forceinline__ void ce_reduce_loss(const float* loss_rows, const int
         for (int i = 1; i < T / 64; ++i) sum += s_sum[i], cnt += s_cnt[i];
         if (loss) *loss = float(reduction == 1 ? sum / double(max(cnt, 1)) : sum);
         if (counted) *counted = float(cnt);
+    }
+}
+
+// ... one part of them
+__global__ __launch_bounds__(256) void ce_loss_parts_kernel(const float* loss_rows, const int64_t* target, int64_t n, CeSums* sums) {
+    __shared__ double s_sum[4];
+    __shared__ int s_cnt[4];
+    double sum = 0.0;
+    int cnt = 0;
+    for (int64_t r = int64_t(blockIdx.x) * 256 + threadIdx.x; r < n; r += kSumParts * 256) {
+        sum += double(loss_rows[r]);
+        cnt += target[r] != -1;
+    }
+    sum = wave_sum_f64(sum);
+    cnt = wave_sum_i32(cnt);
+    if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum, s_cnt[threadIdx.x >> 6] = cnt;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sums->loss[blockIdx.x] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+        sums->counted[blockIdx.x] = (s_cnt[0] + s_cnt[1]) + (s_cnt[2] + s_cnt[3]);
     }
 }
 
@@ -160,7 +195,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
     __shared__ __align__(16) float s_par[RING][MODE == kTable ? 4 : 1][TS];      // pass 1: bias; pass 2: CePass::rowp
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l31 = lane & 31;
     if constexpr (MODE == kTable) {
-        if (blockIdx.x + 1 == gridDim.x && a.loss) return ce_reduce_loss<256>(a.loss_rows, a.target, a.n_strm, a.reduction, a.loss, nullptr);
+        if (blockIdx.x + 1 == gridDim.x && a.loss) return ce_reduce_loss<256>(a.loss_rows, a.target, a.sums, a.n_strm, a.reduction, a.loss, nullptr);
     }
     // consecutive numbers stay on one XCD (workgroup id mod 8), and consecutive numbers share a split: the tiles they stream meet in that XCD's L2
     const int total = a.stat_blocks * a.n_splits, per = (total + 7) / 8;
@@ -665,6 +700,8 @@ struct CeRows {
     short* q_copy;
 };
 constexpr int kCUs = 256, kMaxSplits = 512;      // splits of a streaming side
+// Every row adds up to so many counts of 32 rows by itself (8 192 rows: 4 loads a lane); more are added once, by a launch of their own
+constexpr int kCountedByRow = 256;
 
 // What a row's state {lse, its low part, 1 - p_t} means to pass 2 (CePass::rowp); rel: its gradient relative to the largest.  Rows from n on: weights of zero.
 template <bool BIAS>
@@ -737,9 +774,13 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
     float g = 1.f;
     if constexpr (GRADS) {
         if (a.reduction == 1) {
-            int cnt = 0;
-            for (int i = lane; i < a.n_counts; i += 64) cnt += a.counts[i];
-            g = 1.f / float(max(wave_sum_i32(cnt), 1));
+            int cnt = a.sc->counted;
+            if (a.n_counts <= kCountedByRow) {
+                cnt = 0;
+                for (int i = lane; i < a.n_counts; i += 64) cnt += a.counts[i];
+                cnt = wave_sum_i32(cnt);
+            }
+            g = 1.f / float(max(cnt, 1));
         }
         if (blockIdx.x == 0 && threadIdx.x == 0) {
             const float unoff = __builtin_amdgcn_exp2f(-a.off2);
@@ -789,21 +830,39 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
     }
 }
 
-__global__ __launch_bounds__(1024) void ce_loss_kernel(const float* loss_rows, const int64_t* target, int64_t n, int reduction, float* loss, float* counted) {
-    ce_reduce_loss<1024>(loss_rows, target, n, reduction, loss, counted);
+__global__ __launch_bounds__(1024) void ce_count_kernel(const int* counts, int n_counts, CeScalars* sc) {
+    __shared__ int s[16];
+    int cnt = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n_counts; i += 1024) cnt += counts[i];
+    cnt = wave_sum_i32(cnt);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = cnt;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; ++i) cnt += s[i];
+        sc->counted = cnt;
+    }
 }
 
-// (of the rows that count: another row's gradient may be anything)
-__global__ __launch_bounds__(1024) void ce_grad_top_kernel(const float* grad, const int64_t* target, int64_t n, int64_t v, CeScalars* sc) {
+__global__ __launch_bounds__(1024) void ce_loss_kernel(const float* loss_rows, const int64_t* target, const CeSums* sums, int64_t n, int reduction, float* loss, float* counted) {
+    ce_reduce_loss<1024>(loss_rows, target, sums, n, reduction, loss, counted);
+}
+
+// Largest |upstream gradient| of the rows that count (another row's may be anything): of all by one workgroup, or a part of them by each of kSumParts ones;
+// with grad = nullptr of the parts.
+__global__ __launch_bounds__(1024) void ce_grad_top_kernel(const float* grad, const int64_t* target, int64_t n, int64_t v, CeScalars* sc, CeSums* sums) {
     __shared__ float s[16];
     float top = 0.f;
-    for (int64_t r = threadIdx.x; r < n; r += 1024) top = fmaxf(top, target[r] >= 0 && target[r] < v ? fabsf(grad[r]) : 0.f);
+    if (grad)
+        for (int64_t r = int64_t(blockIdx.x) * 1024 + threadIdx.x; r < n; r += int64_t(gridDim.x) * 1024) top = fmaxf(top, target[r] >= 0 && target[r] < v ? fabsf(grad[r]) : 0.f);
+    else if (threadIdx.x < kSumParts) top = sums->top[threadIdx.x];
     top = wave_max_f32(top);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-        sc->g_top = top;
+        if (gridDim.x > 1) sums->top[blockIdx.x] = top;
+        else sc->g_top = top;
     }
 }
 
@@ -907,7 +966,7 @@ static size_t up(size_t b) { return (b + 255) & ~size_t(255); }
 
 // Where a call's workspace keeps what.  The head (scalars, laid-out operands) serves both passes of a call.
 struct CeLayout {
-    size_t tops, q_hi, q_lo, e_hi, e_lo, loss_rows, counts, rowp, head, zt, m, l, o, fwd_end, l2, o2, bwd_end;
+    size_t sums, tops, q_hi, q_lo, e_hi, e_lo, loss_rows, counts, rowp, head, zt, m, l, o, fwd_end, l2, o2, bwd_end;
     CeSplit f, b;      // of pass 1 and 2
     size_t bytes(bool want_mean) const { return std::max<size_t>(256, want_mean ? std::max(fwd_end, bwd_end) : fwd_end); }
 };
@@ -916,6 +975,7 @@ static CeLayout ce_layout(int64_t n, int64_t v, int d, int dtype, bool q_direct,
     CeLayout y{};
     const CeSplit f = y.f = ce_split(n, v, d), b = y.b = ce_split(v, n, d);
     size_t at = 256;      // CeScalars
+    y.sums = at, at += n > kSumRows ? up(sizeof(CeSums)) : 0;
     y.tops = at, at += dtype == HWER_F32 ? 2 * kTopBlocks * 4 : 0;
     y.q_hi = at, at += q_direct && !want_mean ? 0 : up(size_t(n) * dp * 2);
     y.q_lo = at, at += dtype == HWER_F32 ? up(size_t(n) * dp * 2) : 0;
@@ -978,6 +1038,17 @@ struct CeCall {
         return HWER_OK;
     }
 
+    CeSums* sums() const { return n > kSumRows ? at<CeSums>(y.sums) : nullptr; }      // (nullptr: one workgroup does it)
+    // before a workgroup reduces the rows' losses
+    void sum_losses(const float* loss_rows) const {
+        if (sums()) ce_loss_parts_kernel<<<dim3(kSumParts), dim3(256), 0, st>>>(loss_rows, target, n, sums());
+    }
+    void grad_top(const float* grad) const {
+        CeScalars* sc = at<CeScalars>(0);
+        ce_grad_top_kernel<<<dim3(sums() ? kSumParts : 1), dim3(1024), 0, st>>>(grad, target, n, v, sc, sums());
+        if (sums()) ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, st>>>(nullptr, target, n, v, sc, sums());
+    }
+
     // lays out what the passes cannot read in place
     int prepare() const {
         CePack p{{q, e}, {nullptr, nullptr}, {nullptr, nullptr}, {n, v}, {ldq, lde}, d, dp, at<float>(y.tops), 0, at<CeScalars>(0), target, bias};
@@ -1028,7 +1099,8 @@ struct CeCall {
         p.l = at<float>(y.l2), p.o = at<float>(y.o2);
         p.rowp = at<float>(y.rowp), p.ld_rowp = ce_rowp_ld(n), p.out = de, p.out_b = dbias, p.ld_out = ldde, p.d = d;
         p.out_vec = d % 4 == 0 && aligned_to(de, ldde * dtype_bytes(dtype), 4 * dtype_bytes(dtype));
-        p.target = target, p.loss_rows = loss_rows, p.loss = loss, p.reduction = reduction;
+        p.target = target, p.loss_rows = loss_rows, p.sums = sums(), p.loss = loss, p.reduction = reduction;
+        if (loss) sum_losses(loss_rows);
         ce_pass_any<kTable>(p, dp, dtype, rowg, st);
         if (int rc = check_launch("catalogue_ce(table pass)")) return rc;
         if (s.splits > 1) {
@@ -1070,6 +1142,7 @@ struct CeCall {
 
     template <bool GRADS>
     int join(const CeRows& r) const {
+        if (GRADS && reduction == 1 && r.n_counts > kCountedByRow) ce_count_kernel<<<dim3(1), dim3(1024), 0, st>>>(r.counts, r.n_counts, r.sc);
         if (dtype == HWER_F32) join_typed<float, true, GRADS>(r);
         else if (dtype == HWER_F16) join_typed<f16_t, false, GRADS>(r);
         else join_typed<bf16_t, false, GRADS>(r);
@@ -1126,7 +1199,8 @@ int hwer_catalogue_ce(const void* q, int64_t ldq, const void* e, int64_t lde, co
         r.loss_rows = loss_rows, r.state = reinterpret_cast<float4*>(state), r.mean = mean;
         if (int rc = c.join<false>(r)) return rc;
     }
-    ce_loss_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(loss_rows, target, n, reduction, loss, counted);
+    c.sum_losses(loss_rows);
+    ce_loss_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(loss_rows, target, c.sums(), n, reduction, loss, counted);
     return check_launch("catalogue_ce");
 }
 
@@ -1144,7 +1218,7 @@ int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_
     CeRows r = c.rows();
     r.state = reinterpret_cast<float4*>(const_cast<float*>(state)), r.mean = const_cast<float*>(mean), r.counted = counted, r.grad = grad, r.per_row = reduction == 0;
     r.dq = dq, r.lddq = lddq, r.rowp = de ? c.at<float>(c.y.rowp) : nullptr;
-    if (reduction == 0) ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(grad, target, n, v, r.sc);
+    if (reduction == 0) c.grad_top(grad);
     if (int rc = c.backward_rows(r)) return rc;
     return de ? c.pass2(de, ldde, dbias, reduction == 0, nullptr, nullptr) : HWER_OK;
 }
@@ -1166,7 +1240,7 @@ int hwer_catalogue_ce_grads(const void* q, int64_t ldq, const void* e, int64_t l
         if (int rc = c.join<true>(r)) return rc;
     } else {
         r.per_row = 1, r.grad = loss_rows;      // no rows: the factors of a sum over nothing
-        ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, c.st>>>(loss_rows, target, 0, v, r.sc);
+        c.grad_top(loss_rows);
         if (int rc = c.backward_rows(r)) return rc;
     }
     return c.pass2(de, ldde, dbias, false, loss_rows, loss);

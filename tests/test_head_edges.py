@@ -215,3 +215,39 @@ def test_cross_entropy_of_a_target_that_is_taken_out(hw, n, v, d, dtype):
         for got, key in ((dx, "dx"), (de, "de"), (db, "db")):
             close(got, ref[key] if key == "dx" else ref[key][:v], 1.01 * (tol[key] if key == "dx" else tol[key][:v]) + (ref[key + "_size"] * 4 * U32)[:v if key != "dx" else n], form + " " + key)
         assert not de[gone.cuda()].any() and not db[gone.cuda()].any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,d", [(2049, 300, 64), (5000, 129, 128), (8192, 40, 32), (8193, 40, 32), (16384, 33, 20), (16385, 33, 20), (20000, 300, 64), (70001, 17, 130)])
+def test_cross_entropy_of_many_rows(hw, n, v, d, dtype):
+    """counts, losses and the largest upstream gradient of more rows than a wave's lanes, a row's share and a workgroup's, in each form; the same every time"""
+    x, e, t, _ = ce_inputs(n + v, n, v, d, dtype)
+    t[::5] = -1
+    t[n - 1] = 1
+    counted = int((t >= 0).sum())
+    dev = [a.cuda() for a in (x, e, t)]
+    up = rnd(7, n)
+    up[::4] = 0
+    up[n - 2] = 9.0                  # the largest one, among the last rows
+    t64 = [a.cuda() for a in (x, e, t)]
+    for form, g in (("mean", torch.full((n,), 1.0 / counted, dtype=torch.float64)), ("sum", torch.ones(n, dtype=torch.float64)), ("none", up)):
+        ref = {k: a.cpu() for k, a in ce_reference(t64[0], t64[1], t64[2], 4.0, None, g.cuda()).items()}
+        tol = ce_tolerances(ref, dtype, n, v, d)
+        low = 0.0 if dtype == torch.bfloat16 or form != "none" else 2.0 ** -40 * 4.0 * up.abs().max() * x.double().abs().sum(0)
+        want = ref["rows"].sum() / (counted if form == "mean" else 1)
+        if form != "none":
+            out = hw.catalogue_cross_entropy_grads(*dev, scale=4.0, reduction=form)
+            close(out[0], want, tol["loss"] * (1 if form == "mean" else n) + want.abs() * 2 * U32, form + " loss")
+            close(out[1], ref["dx"], tol["dx"], form + " dqueries")
+            close(out[2], ref["de"], tol["de"], form + " dtable")
+            assert all(torch.equal(p, q) for p, q in zip(out, hw.catalogue_cross_entropy_grads(*dev, scale=4.0, reduction=form)))
+        q, tab = dev[0].clone().requires_grad_(), dev[1].clone().requires_grad_()
+        loss = hw.catalogue_cross_entropy(q, tab, dev[2], scale=4.0, reduction=form)
+        if form == "none":
+            close(loss, ref["rows"], tol["loss"] + ref["rows"].abs() * U32, "rows")
+        else:
+            assert torch.equal(loss.detach(), out[0])
+        loss.backward(up.float().cuda() if form == "none" else None)
+        close(q.grad, ref["dx"], 1.01 * tol["dx"] + ref["dx_size"] * 4 * U32, form + " autograd dqueries")
+        close(tab.grad, ref["de"], 1.01 * tol["de"] + ref["de_size"] * 4 * U32 + low, form + " autograd dtable")
