@@ -217,7 +217,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
         for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
     const float scl = fmaxf(TERMS == 2 ? a.scale * a.sc->unscale_s : a.scale, 1.2e-38f), c = fmaxf(scl * kLog2e, 1.2e-38f);      // (never 0: 0 * -inf)
     const float thr = BIAS ? kStale * kLn2 : kStale / c;
-    float m = kLowest, renew = kLowest, l = 0.f;
+    float m = kLowest, renew = kLowest, l = 0.f, l_low = 0.f;      // l_low: what l is too large by
     const int64_t target = MODE != kTable && my < a.n_stat ? a.target[my] : -1;
     if (MODE != kTable && split == 0) {      // (-1 once per row: both halves of a wave hold the same rows)
         const int cnt = __builtin_popcountll(__ballot(half == 0 && target != -1));
@@ -373,6 +373,14 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
             }
         }
     };
+    // The sum of a lane's weights, over up to millions of rows: 16 at a time as a tree, added with the last addition's rounding error (one after the other, a million
+    // equal weights lost 8e-3 of their sum).
+    auto add_weights = [&](const float (&w)[16]) __attribute__((always_inline)) {
+        const float a0 = (w[0] + w[1]) + (w[2] + w[3]), a1 = (w[4] + w[5]) + (w[6] + w[7]), a2 = (w[8] + w[9]) + (w[10] + w[11]), a3 = (w[12] + w[13]) + (w[14] + w[15]);
+        const float add = ((a0 + a1) + (a2 + a3)) - l_low, sum = l + add;
+        l_low = (sum - l) - add;
+        l = sum;
+    };
     // S -> weights.  row: the first of the 32; reads: the first fragment reads of the product phase, issued before the exponentials
     float sub = BIAS ? 0.f : OFF;      // what exponents are taken against (without a maximum yet: 0)
     auto weights = [&](int slot, int sb, int64_t row, int my_target, bool hit, auto reads) __attribute__((always_inline)) {
@@ -398,10 +406,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
                     w[4 * q + 3] = __float_as_int(t.w) == int(my) ? v.w : w[4 * q + 3];
                 }
             }
-            if (BIAS) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) l += w[j];
-            }
+            if (BIAS) add_weights(w);
         } else {
             if (row + 32 > a.n_strm) {      // rows past the end
 #pragma unroll
@@ -434,7 +439,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
                 m = mn;
                 renew = m == kLowest ? kLowest : m + thr;
                 sub = m == kLowest ? (BIAS ? 0.f : OFF) : (BIAS ? m : OFF - m * c);
-                l *= f;
+                l *= f, l_low *= f;
                 if constexpr (MODE == kMean) {
 #pragma unroll
                     for (int i = 0; i < DB; ++i)
@@ -446,10 +451,8 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
             for (int j = 0; j < 16; ++j) w[j] = BIAS ? fmaf(s[j] - sub, kLog2e, OFF) : fmaf(s[j], c, sub);
             reads();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                w[j] = __builtin_amdgcn_exp2f(w[j]);
-                l += w[j];
-            }
+            for (int j = 0; j < 16; ++j) w[j] = __builtin_amdgcn_exp2f(w[j]);
+            add_weights(w);
         }
         if constexpr (MODE != kLse) {
 #pragma unroll
@@ -938,7 +941,10 @@ static bool ce_direct(const void* p, int64_t ld, int d, int dtype) {
 
 // Splits of the streaming side, in 32s of its rows.  A call takes as long as its fullest CU (which holds two workgroups, or one of the widest rows): rounds of
 // workgroups times (a split's 32s + about 4 for its start and end); and each split leaves sums behind that are written and read again, about 3 MB in the
-// time of 32 rows (with 2: 8 192 x 4 000 x 128 bfloat16 95 us, 83 so, 86 with 6; 2 000 x 3 000 x 100 float32 80, 76 and 73; 100 000 x 129 x 128 334, 337 and 339).
+// time of 32 rows (with 2: 8 192 x 4 000 x 128 bfloat16 101 us, 89 so, 89 with 6; 2 000 x 3 000 x 100 float32 77, 74 and 70; 100 000 x 129 x 128 the same).
+// A split is no longer than its products' sums can bear: the matrix instructions add to one float32 sum twice for 32 rows (float32 rows: six times), and with
+// terms of one direction (equal rows) N additions leave up to N 2^-25 of it.  float32 rows: 1 536 additions, 4.6e-5; 16-bit rows: 8 192, 2.4e-4, half a rounding
+// of float16.  As long as the splits' sums fit into kSplitBytes: 65 536 x 1.2 M float32 rows of 64 are 147 splits, 2.5 GB.
 // Tried for pass 2: one workgroup for each place on the CUs with an equal share of all blocks' work.  No last round that is not full (1 037 x 50 021 x 250
 // float16 256 -> 241 us), but no workgroup takes over from a slower one either, and the loop over blocks costs registers: 4 096 x 1.25 M x 128 bfloat16
 // 4.90 -> 5.00 ms, x 400 k x 64 0.97 -> 1.04, x 400 k x 256 4.0 -> 4.7.
@@ -946,12 +952,15 @@ struct CeSplit {
     int blocks, splits, subs;
 };
 constexpr int kRows = 128;      // stationary rows of a workgroup
-static CeSplit ce_split(int64_t n_stat, int64_t n_strm, int d) {
+constexpr int64_t kSplitBytes = int64_t(8) << 30;
+static CeSplit ce_split(int64_t n_stat, int64_t n_strm, int d, int dtype) {
     const int dp = ce_padded(d);
     const int64_t blocks = cdiv64(n_stat, kRows), subs = std::max<int64_t>(1, cdiv64(n_strm, 32)), slots = (dp == 256 ? 1 : 2) * kCUs;
+    const int64_t most = std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, kSplitBytes / (std::max<int64_t>(blocks, 1) * kRows * dp * 4)));
+    const int64_t least = std::min(most, cdiv64(subs, dtype == HWER_F32 ? 256 : 4096));
     double best = INFINITY;
-    int64_t per = subs;
-    for (int64_t s = 1; s <= std::min<int64_t>(subs, kMaxSplits) && (s == 1 || blocks * s <= 8 * slots); ++s) {
+    int64_t per = cdiv64(subs, least);
+    for (int64_t s = least; s <= std::min<int64_t>(subs, kMaxSplits) && (s == least || blocks * s <= 8 * slots); ++s) {
         const int64_t p = cdiv64(subs, s), n = cdiv64(subs, p);
         const double cost = double(cdiv64(blocks * n, slots) * (p + 4)) + (n > 1 ? double(blocks * kRows * dp * 8) * double(n) / 3e6 : 0.0);
         if (cost < best) best = cost, per = p;
@@ -973,7 +982,7 @@ struct CeLayout {
 static CeLayout ce_layout(int64_t n, int64_t v, int d, int dtype, bool q_direct, bool e_direct, bool want_mean) {
     const size_t dp = ce_padded(d);
     CeLayout y{};
-    const CeSplit f = y.f = ce_split(n, v, d), b = y.b = ce_split(v, n, d);
+    const CeSplit f = y.f = ce_split(n, v, d, dtype), b = y.b = ce_split(v, n, d, dtype);
     size_t at = 256;      // CeScalars
     y.sums = at, at += n > kSumRows ? up(sizeof(CeSums)) : 0;
     y.tops = at, at += dtype == HWER_F32 ? 2 * kTopBlocks * 4 : 0;

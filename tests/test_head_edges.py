@@ -251,3 +251,65 @@ def test_cross_entropy_of_many_rows(hw, n, v, d, dtype):
         loss.backward(up.float().cuda() if form == "none" else None)
         close(q.grad, ref["dx"], 1.01 * tol["dx"] + ref["dx_size"] * 4 * U32, form + " autograd dqueries")
         close(tab.grad, ref["de"], 1.01 * tol["de"] + ref["de_size"] * 4 * U32 + low, form + " autograd dtable")
+
+
+def equal_rows(n, v, d, dtype, bias):
+    """Four kinds of queries over a catalogue of one row again and again, one that is a little better and one that is far off (the target of most): every
+    weight of a long sum is the same value, so that its roundings have one direction.  Products of rows are exact in every type (a few bits each).
+    -> operands on the device, and the 64-bit results"""
+    a = torch.tensor([1.0, 0.5, 0.25, 0.75]).repeat(d // 4).to(dtype).cuda()
+    unit = torch.tensor([2.0, 4.0, 0.0, 0.0]).repeat(d // 4).to(dtype).cuda() / d          # <unit, a> = 1
+    table = a.repeat(v, 1)
+    table[0] = a * 1.25          # (the first one, so that the others' weights are below 1 from the start)
+    table[v - 1] = a * -0.25
+    kind = torch.arange(n, device="cuda") % 4
+    kinds = torch.stack([unit * c for c in (0.875, 1.25, 1.75, 2.875)])
+    queries = kinds[kind]
+    target = torch.where(torch.arange(n, device="cuda") % 5 == 0, v // 2, v - 1)
+    b = None
+    if bias:
+        b = torch.full((v,), 0.37, device="cuda")
+        b[v // 5] = -1.0
+    z = kinds.double() @ table.double().t() + (0 if b is None else b.double())
+    lse = torch.logsumexp(z, 1)
+    p = torch.exp(z - lse[:, None])
+    rows = lse[kind] - z[kind, target]
+    mean = p @ table.double()
+    dx = (mean[kind] - table[target].double()) / n
+    dx_size = (p @ table.double().abs())[kind] / n + table[target].double().abs() / n
+    w, wa = torch.zeros_like(p), torch.zeros_like(p)
+    for k in range(4):
+        hot = torch.zeros(v, dtype=torch.float64, device="cuda")
+        for c in (v // 2, v - 1):
+            hot[c] = int(((kind == k) & (target == c)).sum())
+        w[k], wa[k] = (p[k] * int((kind == k).sum()) - hot) / n, (p[k] * int((kind == k).sum()) + hot) / n
+    de, de_size = w.t() @ kinds.double(), wa.t() @ kinds.double().abs()
+    return (queries, table, target, b), dict(rows=rows, dx=dx, dx_size=dx_size, de=de, de_size=de_size, db=w.sum(0), db_size=wa.sum(0))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,bias", [(65536, 1200001, False), (4096, 1200001, True), (1200001, 65536, True), (512, 2500000, False)])
+def test_cross_entropy_sums_over_long_catalogues_and_batches(hw, n, v, bias, dtype):
+    """float32 sums of a million equal terms.  The sums of probabilities are compensated: off by a few roundings, whatever their length.  The products'
+    sums are added by the matrix instructions, at most 1 536 (float32 rows) or 8 192 of them one after the other: each rounding is up to 2^-24 of a sum that is
+    half of the last one on the average, so N of one direction leave up to N 2^-25; and joined from up to 512 parts, which may leave 512 2^-25 more."""
+    d = 64
+    (x, e, t, b), ref = equal_rows(n, v, d, dtype, bias)
+    f32 = dtype == torch.float32
+    # a logit of |z| < 4 in powers of two: the factor's and the product's rounding, and that of a sum below 16; a probability: two of them, and the
+    # exponential's and the sums' few roundings
+    dz = 4 * 2 * U32 + 2.0 ** -21
+    dp = 2 * dz + 16 * U32
+    rows = hw.catalogue_cross_entropy(x, e, t, bias=b, reduction="none")
+    close(rows, ref["rows"].cpu(), dz + 16 * U32 + ref["rows"].cpu().abs() * U32, "rows")
+    out = hw.catalogue_cross_entropy_grads(x, e, t, bias=b)
+    assert abs(float(out[0]) - float(ref["rows"].mean())) <= dz + 32 * U32
+    long = ((1536 if f32 else 8192) + 512) * 2.0 ** -25
+    w = 2.0 ** -22 if f32 else U[dtype]
+    low = 0.0 if dtype == torch.bfloat16 else 2.0 ** -36 * 4 * float(e.double().abs().amax()) / n
+    close(out[1], ref["dx"].cpu(), ref["dx"].cpu().abs() * U[dtype] + ref["dx_size"].cpu() * (dp + long + w) + low + 4 * TINY[dtype], "dqueries")
+    floor = 0.0 if dtype == torch.bfloat16 else 2.0 ** -40 * float(x.double().abs().amax())
+    close(out[2], ref["de"].cpu(), ref["de"].cpu().abs() * U[dtype] + ref["de_size"].cpu() * (dp + long + w) + floor + 4 * TINY[dtype], "dtable")
+    if bias:
+        close(out[3], ref["db"].cpu(), ref["db_size"].cpu() * (dp + 512 * 2.0 ** -25) + 1e-30, "dbias")
