@@ -58,8 +58,9 @@ template <> struct CeType<bf16_t> {
 
 // device-side scalars of a call (in its workspace)
 struct CeScalars {
-    float unscale_s, unscale_q, unscale_e;      // float32 rows: 2^-(eq + ee), 2^-eq, 2^-ee, which undo the operands' powers of two
-    float fac_e, fac_b;                          // factors of de and db
+    int shift_s;                                 // float32 rows: -(eq + ee), -eq as a factor and -ee: they undo the operands' powers of two 2^eq and 2^ee
+    float unscale_q, unscale_e;
+    float fac_e, fac_b;                          // factors of de (float32 rows: and unscale_q, alone, as both together may leave float32's range) and db
     float g_top;                                 // largest |upstream gradient| of a row
     int counted;                                 // counted rows, of more than kCountedByRow
 };
@@ -215,7 +216,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
     for (int i = 0; i < (MODE == kLse ? 1 : DB); ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-    const float scl = fmaxf(TERMS == 2 ? a.scale * a.sc->unscale_s : a.scale, 1.2e-38f), c = fmaxf(scl * kLog2e, 1.2e-38f);      // (never 0: 0 * -inf)
+    const float scl = fmaxf(TERMS == 2 ? ldexpf(a.scale, a.sc->shift_s) : a.scale, 1.2e-38f), c = fmaxf(scl * kLog2e, 1.2e-38f);      // (never 0: 0 * -inf)
     const float thr = BIAS ? kStale * kLn2 : kStale / c;
     float m = kLowest, renew = kLowest, l = 0.f, l_low = 0.f;      // l_low: what l is too large by
     const int64_t target = MODE != kTable && my < a.n_stat ? a.target[my] : -1;
@@ -543,7 +544,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
     }
     if constexpr (MODE == kTable) {
         typedef typename std::conditional<TERMS == 2, float, E>::type OUT;
-        const float f = a.sc->fac_e;
+        const float f = a.sc->fac_e, un = TERMS == 2 ? a.sc->unscale_q : 1.f;
         OUT* out = static_cast<OUT*>(a.out) + my * a.ld_out;
         if (BIAS && half == 0 && a.out_b) a.out_b[my] = l * a.sc->fac_b;
 #pragma unroll
@@ -552,7 +553,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
             for (int q = 0; q < 4; ++q) {
                 const int col = 32 * i + 8 * q + 4 * half;
                 typedef OUT out4 __attribute__((ext_vector_type(4)));
-                const out4 v = {OUT(o[i][4 * q] * f), OUT(o[i][4 * q + 1] * f), OUT(o[i][4 * q + 2] * f), OUT(o[i][4 * q + 3] * f)};
+                const out4 v = {OUT(o[i][4 * q] * f * un), OUT(o[i][4 * q + 1] * f * un), OUT(o[i][4 * q + 2] * f * un), OUT(o[i][4 * q + 3] * f * un)};
                 if (a.out_vec) {
                     if (col < a.d) *reinterpret_cast<out4*>(out + col) = v;
                 } else {
@@ -633,10 +634,10 @@ __global__ __launch_bounds__(256) void ce_top_kernel(CePack a) {
     if (threadIdx.x == 0) a.tops[w * kTopBlocks + blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
 }
 
-// exponent that puts `top` into [2^14, 2^15)
+// exponent that puts `top` into [2^14, 2^15), as far as 2^126 does
 __device__ __forceinline__ int ce_exponent(float top) {
     if (!(top > 0.f) || !(top < INFINITY)) return 0;
-    return max(-100, min(100, 14 - ilogbf(top)));
+    return min(126, 14 - ilogbf(top));
 }
 
 __global__ __launch_bounds__(256) void ce_split_kernel(CePack a) {
@@ -651,7 +652,7 @@ __global__ __launch_bounds__(256) void ce_split_kernel(CePack a) {
     __syncthreads();
     const int eq = ce_exponent(s[0]), ee = ce_exponent(s[1]);
     if (blockIdx.x == 0 && w == 0 && threadIdx.x == 0) {
-        a.sc->unscale_s = ldexpf(1.f, -eq - ee);
+        a.sc->shift_s = -eq - ee;
         a.sc->unscale_q = ldexpf(1.f, -eq);
         a.sc->unscale_e = ldexpf(1.f, -ee);
     }
@@ -733,7 +734,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
         if (GRADS && r < a.ld_rowp && t_in == 0) ce_put_rowp<BIAS>(a, r, false, 0.f, 0.f, 0.f, 0.f, -1);
         return;
     }
-    const float unit = BIAS ? kLog2e : fmaxf((F32 ? a.scale * a.sc->unscale_s : a.scale) * kLog2e, 1.2e-38f);      // from the maxima's unit to powers of two (as in the pass)
+    const float unit = BIAS ? kLog2e : fmaxf((F32 ? ldexpf(a.scale, a.sc->shift_s) : a.scale) * kLog2e, 1.2e-38f);      // from the maxima's unit to powers of two (as in the pass)
     float top = kLowest;
     for (int s = t_in; s < a.n_splits; s += TR) top = fmaxf(top, a.m[int64_t(s) * a.n + r]);
     top = wave_max_f32(top);
@@ -787,7 +788,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
         }
         if (blockIdx.x == 0 && threadIdx.x == 0) {
             const float unoff = __builtin_amdgcn_exp2f(-a.off2);
-            a.sc->fac_e = a.scale * g * unoff * (F32 ? a.sc->unscale_q : 1.f);
+            a.sc->fac_e = a.scale * g * unoff;
             a.sc->fac_b = g * unoff;
         }
     }
@@ -820,8 +821,8 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
         }
         if (grp) return;
     }
-    const float f = sum == 0.f ? 0.f : (F32 ? a.sc->unscale_e : 1.f) / sum;
-    const float mean[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+    const float f = sum == 0.f ? 0.f : 1.f / sum, un = F32 ? a.sc->unscale_e : 1.f;      // (one after the other: both may leave float32's range)
+    const float mean[4] = {v.x * f * un, v.y * f * un, v.z * f * un, v.w * f * un};
     const E* e = static_cast<const E*>(a.e) + (there ? t : 0) * a.lde;
     const float fq = a.scale * g * float(miss);
 #pragma unroll
@@ -878,7 +879,7 @@ __global__ __launch_bounds__(256) void ce_dq_kernel(CeRows a) {
     const float g = a.per_row ? a.sc->g_top : (a.grad ? a.grad[0] : 1.f) / (a.reduction == 1 ? fmaxf(a.counted[0], 1.f) : 1.f);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         const float unoff = __builtin_amdgcn_exp2f(-a.off2);
-        a.sc->fac_e = a.scale * g * unoff * (F32 ? a.sc->unscale_q : 1.f);
+        a.sc->fac_e = a.scale * g * unoff;
         a.sc->fac_b = g * unoff;
     }
     if (r >= a.n) {
@@ -904,7 +905,7 @@ template <typename E>
 __global__ __launch_bounds__(256) void ce_de_kernel(const float* __restrict__ o, const float* __restrict__ l, int n_splits, int64_t v, int d, int dp,
                                                    const CeScalars* sc, E* __restrict__ de, int64_t ldde, float* __restrict__ db) {
     const int per = dp / 4, shift = 31 - __clz(per);
-    const float fe = sc->fac_e, fb = sc->fac_b;
+    const float fe = sc->fac_e, fb = sc->fac_b, un = std::is_same<E, float>::value ? sc->unscale_q : 1.f;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < v * per; i += int64_t(gridDim.x) * 256) {
         const int64_t r = i >> shift;
         const int c = int(i & (per - 1)) * 4;
@@ -916,10 +917,10 @@ __global__ __launch_bounds__(256) void ce_de_kernel(const float* __restrict__ o,
                 s.x += t.x, s.y += t.y, s.z += t.z, s.w += t.w;
             }
             E* out = de + r * ldde + c;
-            out[0] = E(s.x * fe);
-            if (c + 1 < d) out[1] = E(s.y * fe);
-            if (c + 2 < d) out[2] = E(s.z * fe);
-            if (c + 3 < d) out[3] = E(s.w * fe);
+            out[0] = E(s.x * fe * un);
+            if (c + 1 < d) out[1] = E(s.y * fe * un);
+            if (c + 2 < d) out[2] = E(s.z * fe * un);
+            if (c + 3 < d) out[3] = E(s.w * fe * un);
         }
         if (db && c == 0) {
             float s = l[r];

@@ -313,3 +313,26 @@ def test_cross_entropy_sums_over_long_catalogues_and_batches(hw, n, v, bias, dty
     close(out[2], ref["de"].cpu(), ref["de"].cpu().abs() * U[dtype] + ref["de_size"].cpu() * (dp + long + w) + floor + 4 * TINY[dtype], "dtable")
     if bias:
         close(out[3], ref["db"].cpu(), ref["db_size"].cpu() * (dp + 512 * 2.0 ** -25) + 1e-30, "dbias")
+
+
+@gpu
+@pytest.mark.parametrize("n,v,d", [(5, 9, 64), (70, 333, 100), (300, 2000, 128), (40, 150, 256)])
+@pytest.mark.parametrize("exponent", [-118, -100, 60, 90, 118])
+def test_cross_entropy_of_float32_rows_far_from_one(hw, n, v, d, exponent):
+    """queries of size 2^k against rows of size 2^-k: the logits are ordinary, and so are the relative errors of everything"""
+    x, e, t, b = ce_inputs(n + d, n, v, d, torch.float32, bias=True)
+    x, e = (x.double() * 2.0 ** exponent).float(), (e.double() * 2.0 ** -exponent).float()
+    t[::5] = -1
+    counted = int((t >= 0).sum())
+    for bias in (None, b):
+        ref = ce_reference(x, e, t, 5.0, bias, torch.full((n,), 1.0 / counted, dtype=torch.float64))
+        tol = ce_tolerances(ref, torch.float32, n, v, d)
+        grads = hw.catalogue_cross_entropy_grads(x.cuda(), e.cuda(), t.cuda(), scale=5.0, bias=None if bias is None else bias.cuda())
+        leaves = [None if a is None else a.cuda().requires_grad_() for a in (x, e, bias)]
+        loss = hw.catalogue_cross_entropy(leaves[0], leaves[1], t.cuda(), scale=5.0, bias=leaves[2])
+        loss.backward()
+        for out in (grads, [loss] + [a.grad for a in leaves if a is not None]):
+            close(out[0], ref["rows"].sum() / counted, tol["loss"] + ref["rows"].sum().abs() / counted * 2 * U32, "loss")
+            for got, key in zip(out[1:], ("dx", "de", "db")):
+                # (results below the smallest normal value keep its step)
+                close(got, ref[key], 1.01 * (tol[key] - (4 * TINY[torch.float32] if key != "db" else 0)) + ref[key + "_size"] * 4 * U32 + 2.0 ** -148, key)
