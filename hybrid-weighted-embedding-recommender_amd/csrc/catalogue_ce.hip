@@ -118,8 +118,11 @@ __device__ __forceinline__ int ce_swz(int r) {
     else return ((r & 3) << 2) | ((r >> 2) & 3);
 }
 
-// WT: 16-bit terms of a weight.  Two for float32 rows; and where a sum has few terms (kFewTerms), whose roundings do not average out: with four queries
-// one rounding of each target's weight is the error of its class's whole gradient (1.6 times the plain form's, measured).
+// WT: 16-bit terms of a weight.  Two for float32 rows; and where a sum has few terms (kFewTerms), whose roundings do not average out.  In longer sums of 16-bit
+// rows one, but two for targets' weights in pass 2, each of which may be the better part of its class's gradient: 2-norm errors of de are those of one rounding
+// to the type then (1 037 x 50 021 x 250 float16 2.40e-4, with one term for all 2.94e-4; 4 096 x 1.25 M x 128 bfloat16 1.67e-3 and 2.00e-3).  That costs
+// 1 - 3 % where targets are spread over the catalogue, up to 10 % where the first hundreds of classes are most queries' targets (4 096 x 26 744 x 128 bfloat16 160
+// and 175 us); in the phases of the product itself, under a branch for each matrix instruction, 184.
 constexpr int kFewTerms = 128;
 
 // Sum or mean of the rows' losses, and how many rows count; with no row counted the mean is 0.  One workgroup, 64-bit sums in a fixed order.
@@ -311,17 +314,20 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
     s16x8 ring[DEPTH][TERMS];
     typedef const __attribute__((address_space(3))) s16x8* lds8_t;
     typedef __attribute__((address_space(3))) s16x4* lds4_t;
+    auto read_transposed = [&](int t, int row, auto i_) __attribute__((always_inline)) {      // 16 streaming rows x 32 columns
+        constexpr int i = decltype(i_)::value;
+        const uint32_t p = HELD ? tr_at[i % (SWZ / 4) * HELD] : tr_at[0] ^ (64 * (i % (SWZ / 4)));
+        const int off = t * PLANE + row * ROWB + 16 * SWZ * (i / (SWZ / 4));
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds4_t>(p + off));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds4_t>((p ^ 32) + (off + 8 * ROWB)));      // (8 rows on, the swizzle differs by 2)
+        return s16x8(__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
     auto read = [&](auto u_, auto sb2_, auto sb1_) __attribute__((always_inline)) {
         constexpr int u = decltype(u_)::value, sb2 = decltype(sb2_)::value, sb1 = decltype(sb1_)::value;
 #pragma unroll
         for (int t = 0; t < TERMS; ++t) {
-            if constexpr (u < N2) {      // 16 streaming rows x 32 columns, transposed
-                constexpr int k = u / DB, i = u % DB;
-                const uint32_t p = HELD ? tr_at[i % (SWZ / 4) * HELD] : tr_at[0] ^ (64 * (i % (SWZ / 4)));
-                const int off = t * PLANE + (sb2 * 32 + 16 * k) * ROWB + 16 * SWZ * (i / (SWZ / 4));
-                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds4_t>(p + off));
-                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds4_t>((p ^ 32) + (off + 8 * ROWB)));      // (8 rows on, the swizzle differs by 2)
-                ring[u % DEPTH][t] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+            if constexpr (u < N2) {
+                ring[u % DEPTH][t] = read_transposed(t, sb2 * 32 + 16 * (u / DB), std::integral_constant<int, u % DB>());
             } else {
                 constexpr int k = u - N2;
                 ring[u % DEPTH][t] = *reinterpret_cast<lds8_t>((HELD ? fr_at[k % (SWZ / 2) * HELD] : fr_at[0] ^ (32 * (k % (SWZ / 2)))) + (t * PLANE + sb1 * 32 * ROWB + 16 * SWZ * (k / (SWZ / 2))));
@@ -384,9 +390,10 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
     };
     // S -> weights.  row: the first of the 32; reads: the first fragment reads of the product phase, issued before the exponentials
     float sub = BIAS ? 0.f : OFF;      // what exponents are taken against (without a maximum yet: 0)
-    auto weights = [&](int slot, int sb, int64_t row, int my_target, bool hit, auto reads) __attribute__((always_inline)) {
+    auto weights = [&](int slot, int sb, int64_t row, int my_target, uint32_t hits, auto reads) __attribute__((always_inline)) {
         if constexpr (HAS_X && !EARLY) read_params(slot, sb);
         float w[16];
+        typename X::x8 low[MODE == kTable && WT == 1 ? 2 : 1];      // what rounding leaves of targets' weights
         if constexpr (MODE == kTable) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[j] = BIAS ? fmaf(fmaf(s[j], scl, my_bias) - px[j], kLog2e, OFF) : fmaf(s[j], c, -px[j]);
@@ -396,15 +403,22 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
                 w[j] = __builtin_amdgcn_exp2f(w[j]);
                 if constexpr (MUL) w[j] *= pm[j];
             }
-            if (hit) {      // (popular classes are hit in every tile: four rows' targets and weights at a time, not one after the other)
+            if (hits) {      // (popular classes are hit in every tile: four rows' targets and weights at a time, not one after the other)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
+                    if constexpr (WT == 1)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) low[q / 2][4 * (q % 2) + j] = E(0.f);
+                    if (!(hits >> (8 * q) & 255)) continue;
                     const int r = sb * 32 + 8 * q + 4 * half;
                     const float4 t = *reinterpret_cast<const float4*>(&s_par[slot][3][r]), v = *reinterpret_cast<const float4*>(&s_par[slot][2][r]);
-                    w[4 * q] = __float_as_int(t.x) == int(my) ? v.x : w[4 * q];
-                    w[4 * q + 1] = __float_as_int(t.y) == int(my) ? v.y : w[4 * q + 1];
-                    w[4 * q + 2] = __float_as_int(t.z) == int(my) ? v.z : w[4 * q + 2];
-                    w[4 * q + 3] = __float_as_int(t.w) == int(my) ? v.w : w[4 * q + 3];
+                    const float ts[4] = {t.x, t.y, t.z, t.w}, vs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool mine = __float_as_int(ts[j]) == int(my);
+                        w[4 * q + j] = mine ? vs[j] : w[4 * q + j];
+                        if constexpr (WT == 1) low[q / 2][4 * (q % 2) + j] = E(mine ? vs[j] - float(E(vs[j])) : 0.f);
+                    }
                 }
             }
             if (BIAS) add_weights(w);
@@ -418,7 +432,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
 #pragma unroll
                 for (int j = 0; j < 16; ++j) s[j] = fmaf(s[j], scl, px[j]);
             }
-            if (hit) {      // a target in this tile, and perhaps among these 32 rows: its logit is noted, and it is left out
+            if (hits) {      // a target in this tile, and perhaps among these 32 rows: its logit is noted, and it is left out
                 const int at = my_target - sb * 32;
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
@@ -467,6 +481,20 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
                 ph[k] = __builtin_bit_cast(s16x8, hi);
                 if (WT == 2) pl[k] = __builtin_bit_cast(s16x8, lo);
             }
+            // Targets' weights have a second term in one-term products too: ONE rounding would be the error of the gradient of a class that is seldom a target.  Its
+            // product is made by itself, for 16 rows with a target among them.
+            if constexpr (MODE == kTable && WT == 1) {
+                if (hits) {
+                    ce_static_for<0, 2>([&](auto k_) __attribute__((always_inline)) {
+                        constexpr int k = decltype(k_)::value;
+                        if (!(hits >> (16 * k) & 65535)) return;
+                        ce_static_for<0, DB>([&](auto i_) __attribute__((always_inline)) {
+                            constexpr int i = decltype(i_)::value;
+                            o[i] = X::mfma(read_transposed(0, sb * 32 + 16 * k, i_), __builtin_bit_cast(s16x8, low[k]), o[i]);
+                        });
+                    });
+                }
+            }
         }
     };
 
@@ -482,11 +510,11 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
         const int next = (slot + 1) % RING;
         const int64_t row = strm0 + int64_t(tile) * TS, from_tile = target - row;
         const int my_target = MODE != kTable && from_tile >= 0 && from_tile < TS ? int(from_tile) : -1;
-        bool hit = __any(my_target >= 0);
-        if (MODE == kTable) {      // does any of the tile's queries have its target among this wave's rows?
+        uint64_t hits = __any(my_target >= 0) ? ~uint64_t(0) : 0;
+        if (MODE == kTable) {      // which of the tile's queries have their target among this wave's rows?
             const int t = (TS >= 64 || lane < TS) ? __float_as_int(s_par[slot][MODE == kTable ? 3 : 0][lane & (TS - 1)]) : -1;
             static_assert(TS <= 64, "a lane a row");
-            hit = __any(t >= row0 && t < row0 + 32);
+            hits = __ballot(t >= row0 && t < row0 + 32);
         }
         ce_static_for<0, SB>([&](auto sb_) __attribute__((always_inline)) {
             constexpr int sb = decltype(sb_)::value, sb1 = sb == SB - 1 ? 0 : sb + 1;
@@ -495,7 +523,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
                 fetch_params(tile + 1, next);
                 if (tile + 2 < tiles) fetch(tile + 2, (slot + 2) % RING);
             }
-            weights(slot, sb, row + sb * 32, my_target, hit, [&]() __attribute__((always_inline)) {
+            weights(slot, sb, row + sb * 32, my_target, uint32_t(hits >> (32 * sb)), [&]() __attribute__((always_inline)) {
                 __builtin_amdgcn_sched_barrier(0);
                 ce_static_for<0, PRE>([&](auto u) __attribute__((always_inline)) { read(u, sb_, std::integral_constant<int, sb1>()); });
                 __builtin_amdgcn_sched_barrier(0);

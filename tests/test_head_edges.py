@@ -336,3 +336,29 @@ def test_cross_entropy_of_float32_rows_far_from_one(hw, n, v, d, exponent):
             for got, key in zip(out[1:], ("dx", "de", "db")):
                 # (results below the smallest normal value keep its step)
                 close(got, ref[key], 1.01 * (tol[key] - (4 * TINY[torch.float32] if key != "db" else 0)) + ref[key + "_size"] * 4 * U32 + 2.0 ** -148, key)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("n,v,d", [(200, 4000, 64), (1000, 1300, 100), (700, 5000, 128), (300, 900, 256)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_cross_entropy_gradient_of_a_class_that_is_a_target_once(hw, n, v, d, dtype, bias):
+    """its one large weight, the target's, is not rounded to 16 bits: what is left is the rounding of the gradient itself and of the small weights"""
+    x, e, _, b = ce_inputs(n + d, n, v, d, dtype, bias=bias, spread=0.0)
+    t = torch.randperm(v, generator=torch.Generator().manual_seed(n))[:n]
+    t[::9] = -1
+    for form in ("mean", "none"):
+        up = (0.5 + torch.rand(n, generator=torch.Generator().manual_seed(d))).double() / n if form == "none" else torch.full((n,), 1.0 / int((t >= 0).sum()), dtype=torch.float64)
+        ref = ce_reference(x, e, t, 3.0, b, up)
+        tol = ce_tolerances(ref, dtype, n, v, d)
+        z = 3.0 * (x.double() @ e.double().t()) + (0 if b is None else b.double())
+        p = torch.softmax(z, 1) * torch.where(t >= 0, up, torch.zeros_like(up))[:, None]
+        hot = torch.zeros_like(p).scatter_(1, t.clamp_min(0)[:, None], 1.0) * torch.where(t >= 0, up, torch.zeros_like(up))[:, None]
+        small, large = 3.0 * (p.t() @ x.double().abs()), 3.0 * (hot.t() @ x.double().abs())
+        u = U[dtype]
+        want = tol["de"] - ref["de_p"] * u + small * u + large * 2 * u * u + ref["de_size"] * 4 * U32
+        tab = e.cuda().requires_grad_()
+        hw.catalogue_cross_entropy(x.cuda(), tab, t.cuda(), scale=3.0, bias=None if b is None else b.cuda(), reduction=form).backward(up.float().cuda() if form == "none" else None)
+        close(tab.grad, ref["de"], want, form + " dtable")
+        if form == "mean":
+            close(hw.catalogue_cross_entropy_grads(x.cuda(), e.cuda(), t.cuda(), scale=3.0, bias=None if b is None else b.cuda())[2], ref["de"], want, "dtable in one call")
