@@ -326,11 +326,11 @@ def read_profile(lib):
 
 
 def library_digest():
-    """sha256 over the library's sources + flags (csrc/build.py::_digest): what `lib/libhwer_hip.so.sha256` holds for the library that ran"""
+    """sha256 over the sources of the search's kernels + flags (csrc/build.py::search_digest)"""
     try:
         sys.path.insert(0, os.path.join(ROOT, "hybrid-weighted-embedding-recommender_amd", "csrc"))
         import build as hip_build
-        return hip_build._digest()
+        return hip_build.search_digest()
     except Exception:
         return None
     finally:
@@ -341,10 +341,10 @@ def load_traffic(config):
     """HBM-side bytes of the screen stage per launch from the committed rocprofv3 PMC passes of THIS command
     ((2 * FETCH_SIZE + WRITE_SIZE) * 1024; gfx950 counts wide reads at half their bytes - MI355X_MICROARCH.md §HBM).  The
     counters cannot be read from inside the run: the value is labelled with the file it comes from, and it is only reported when
-    that file carries the digest of the library that is running (`library_digest`; tools/pmc_summary.py writes it) - counters of
+    that file carries the digest of the search's sources that are running (`library_digest`; tools/collect_profiles.py writes it) - counters of
     another build of the kernels are not this run's traffic: then `traffic` is null and `traffic_source` says why."""
     dig = library_digest()
-    for fn in ("r6_pmc_traffic.json", "r5_pmc_traffic.json", "r4_pmc_traffic.json"):
+    for fn in ("search_pmc_traffic.json", "r6_pmc_traffic.json"):
         try:
             with open(os.path.join(ROOT, "profiles", fn)) as fh:
                 doc = json.load(fh)

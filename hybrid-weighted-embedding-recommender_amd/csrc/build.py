@@ -16,9 +16,10 @@ LIBDIR = os.path.join(os.path.dirname(HERE), "lib")
 # HWER_LIB_NAME=libhwer_hip_diag.so HIPCC_EXTRA=-DHWER_DIAG_STAMPS python build.py: a diagnostic library beside the production one (own objects)
 LIB = os.path.join(LIBDIR, os.environ.get("HWER_LIB_NAME", "libhwer_hip.so"))
 OBJ_TAG = "" if os.path.basename(LIB) == "libhwer_hip.so" else "." + os.path.basename(LIB).replace(".so", "")
-SOURCES = ["rowops.hip", "knn_screen.hip", "knn_small.hip", "knn_select.hip", "knn_select_f64.hip", "fit_pca.hip", "rows_f64.hip", "knn_wide.hip", "head_norm.hip", "matmul_q8.hip",
-           "catalogue_ce.hip"]
-HEADERS = ["hwer_common.h", "head_common.h", "knn_internal.h", "knn_select_kernels.h", os.path.join(ROOT, "include", "hwer_hip.h")]
+SEARCH_SOURCES = ["rowops.hip", "knn_screen.hip", "knn_small.hip", "knn_select.hip", "knn_select_f64.hip", "fit_pca.hip", "rows_f64.hip", "knn_wide.hip"]
+SEARCH_HEADERS = ["hwer_common.h", "knn_internal.h", "knn_select_kernels.h"]
+SOURCES = SEARCH_SOURCES + ["head_norm.hip", "matmul_q8.hip", "catalogue_ce.hip"]
+HEADERS = SEARCH_HEADERS + ["head_common.h", os.path.join(ROOT, "include", "hwer_hip.h")]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math",
          # no packed float32 instructions (v_pk_add / mul / fma_f32): -O3 forms them from ordinary float code, and some of their forms have given
          # wrong results on this chip now and then (hipcc's host pass does not know the feature and warns: harmless)
@@ -28,9 +29,15 @@ FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-ffp-contract=o
 # scheduling barriers; the production build has none)
 
 
-def _digest():
+def search_digest():
+    """Digest of what the search's kernels are made of (their sources, the flags; not the interface's declarations, nor the other operators' sources): what
+    profiles of the search are bound to."""
+    return _digest(SEARCH_SOURCES + SEARCH_HEADERS)
+
+
+def _digest(files=None):
     h = hashlib.sha256()
-    for f in SOURCES + HEADERS + [os.path.abspath(__file__)]:
+    for f in files or SOURCES + HEADERS + [os.path.abspath(__file__)]:
         with open(os.path.join(HERE, f) if not os.path.isabs(f) else f, "rb") as fh:
             h.update(fh.read())
     # (flags with the checkout's own location taken out: the digest of one source tree is the same wherever it is checked out - a GPU box runs

@@ -83,6 +83,27 @@ def test_dual_tensors_are_refused(hw):
             hw.rms_norm(x)
 
 
+def test_profiles_of_the_search_are_bound_to_the_search():
+    """the digest that the search's traffic counters carry covers every file that its kernels include, and none of the learned head's"""
+    import os
+    import re
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    csrc = os.path.join(root, "hybrid-weighted-embedding-recommender_amd", "csrc")
+    sys.path.insert(0, csrc)
+    try:
+        import build as hip_build
+    finally:
+        sys.path.pop(0)
+    mine = set(hip_build.SEARCH_SOURCES + hip_build.SEARCH_HEADERS)
+    assert not {f for f in mine if "head_" in f or "catalogue" in f or "q8" in f} and set(hip_build.SEARCH_SOURCES) < set(hip_build.SOURCES)
+    for f in mine:
+        with open(os.path.join(csrc, f)) as fh:
+            for inc in re.findall(r'#include "([^"]+)"', fh.read()):
+                assert inc in mine or inc == "hwer_hip.h", (f, inc)
+    assert hip_build.search_digest() not in (hip_build._digest(), hip_build._digest(hip_build.SEARCH_SOURCES))
+
+
 # ---------------------------------------------------------------------------------------------------------------- what a call may be given (GPU)
 @gpu
 def test_operators_without_a_gradient_say_so(hw):

@@ -1,9 +1,9 @@
 #!/usr/bin/env python3
-"""Copy the summaries of a tools/profile_round.sh run (gpurun_out/<dir>) into profiles/ under this round's names (r<ROUND>_*) and
-rebuild profiles/r<ROUND>_pmc_traffic.json (the HBM-side bytes of the screen stage per launch that bench.py labels `traffic`),
-stamped with the digest of the library sources the counters were collected on (bench.py reports `traffic` only for that build).
+"""Copy the summaries of a tools/profile_round.sh run (<dir>) into profiles/ under the names <PREFIX>_* and rebuild
+profiles/<PREFIX>_pmc_traffic.json (the HBM-side bytes of the screen stage per launch that bench.py labels `traffic`),
+stamped with the digest of the search's sources the counters were collected on (bench.py reports `traffic` only for those).
 
-    python tools/collect_profiles.py gpurun_out/prof "c1 c2 c3 c4" [ROUND=4]
+    python tools/collect_profiles.py <dir> "c1 c2 c3 c4" [PREFIX=search]
 """
 import json
 import os
@@ -12,7 +12,7 @@ import sys
 
 src = sys.argv[1]
 cfgs = (sys.argv[2] if len(sys.argv) > 2 else "c1 c2 c3 c4").split()
-RND = "r%s" % (sys.argv[3] if len(sys.argv) > 3 else "4")
+RND = sys.argv[3] if len(sys.argv) > 3 else "search"
 CMD = "python3 bench.py --config %s --no-cpu-baseline --sweep-only --no-graph"
 
 
@@ -38,7 +38,7 @@ traffic = {"_comment": "HBM-side traffic per launch from rocprofv3 PMC passes of
            "pre-pass (dense-mode screen over the sample) and its threshold kernel."}
 for c in cfgs:
     j = json.load(open(f"{src}/stats_{c}_bench.json"))
-    hdr = [f"# rocprofv3 --kernel-trace --stats -- {CMD % c} --steps N --warmup 5   (MI355X, " + RND + "; tools/profile_round.sh)",
+    hdr = [f"# rocprofv3 --kernel-trace --stats -- {CMD % c} --steps N --warmup 5   (MI355X; tools/profile_round.sh)",
            "# bench line under the profiler: ms_per_step=%.4f kernels=%s" % (j["ms_per_step"], json.dumps({k["kernel"][:28]: round(k["ms_per_step"], 4) for k in j["kernels"]}))]
     open(f"profiles/{RND}_rocprof_stats_{c}.txt", "w").write(
         "\n".join(hdr) + "\n" + open(f"{src}/stats_{c}.txt").read() +
@@ -83,7 +83,7 @@ for c in cfgs:
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hybrid-weighted-embedding-recommender_amd", "csrc"))
 import build as hip_build  # noqa: E402
 dig_file = os.path.join(src, "library_digest.txt")      # written on the GPU box by tools/profile_round.sh next to the counters
-traffic["library_digest"] = open(dig_file).read().strip() if os.path.exists(dig_file) else hip_build._digest()
+traffic["library_digest"] = open(dig_file).read().strip() if os.path.exists(dig_file) else hip_build.search_digest()
 json.dump(traffic, open("profiles/%s_pmc_traffic.json" % RND, "w"), indent=1)
 for c in cfgs:
     print(c, traffic[c]["knn_screen_bytes_per_launch"] / 1e6, "MB per screen launch")
