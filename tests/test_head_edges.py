@@ -196,6 +196,44 @@ def test_q8_scale_of_a_row_of_zeros_is_zero(hw, d):
         assert float(s[0]) == 0 and float(s[2]) == 0 and not q[0].any() and not q[2].any() and torch.isfinite(s).all()
 
 
+# ---------------------------------------------------------------------------------------------------------------- strides
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,d", [(1, 7), (9, 100), (130, 250), (33, 1024), (5, 4100), (3, 20001)])
+def test_norm_of_strided_operands(hw, n, d, dtype):
+    """every operand as rows of a wider tensor (at any alignment), transposed, broadcast and with a leading dimension: the same bits as of copies"""
+    x, res, dy, dh = (rnd(n + i, n, d).to(dtype).cuda() for i in range(4))
+    w = (1 + 0.2 * rnd(9, d)).to(dtype).cuda()
+
+    def wide(t, left):
+        out = torch.full((n, d + 13), float("nan"), dtype=dtype, device="cuda")
+        out[:, left:left + d] = t
+        return out[:, left:left + d]
+    views = {"wide": lambda t, i: wide(t, 1 + 2 * i), "transposed": lambda t, i: t.t().contiguous().t(), "leading": lambda t, i: wide(t, i).unsqueeze(1),
+             "every second": lambda t, i: torch.stack([t, t], -1).reshape(n, 2 * d)[:, ::2]}
+    weights = torch.stack([w, w], 1).reshape(-1)[::2]
+    y, h = hw.rms_norm(x, w, res)
+    dx, dw = hw.rms_norm_grads(dy, h, w, dh=dh)
+    q, s, hq = hw.rms_norm_q8(x, w, res)
+    plain, scale = hw.quantize_rows_q8(x)
+    for name, view in views.items():
+        vx, vr, vy, vd, vh = (view(t, i) for i, t in enumerate((x, res, dy, dh, h)))
+        got = (hw.rms_norm(vx, weights, vr), hw.rms_norm_grads(vy, vh, weights, dh=vd), hw.rms_norm_q8(vx, weights, vr), hw.quantize_rows_q8(vx))
+        for out, want in zip(got, ((y, h), (dx, dw), (q, s, hq), (plain, scale))):
+            assert all(torch.equal(a.reshape(b.shape), b) for a, b in zip(out, want)), name
+        leaves = [t.detach().requires_grad_() for t in (vx, weights, vr)]
+        out, hidden = hw.rms_norm(leaves[0], leaves[1], leaves[2])
+        torch.autograd.backward([out, hidden], [vy, vd])
+        assert torch.equal(leaves[0].grad.reshape(n, d), dx) and torch.equal(leaves[2].grad.reshape(n, d), dx) and torch.equal(leaves[1].grad, dw), name
+    # one row for all, and one gradient for all
+    row = x[:1].expand(n, d)
+    assert torch.equal(hw.rms_norm(row, w, res)[0], hw.rms_norm(row.contiguous(), w, res)[0]) and torch.equal(hw.rms_norm_q8(row, w)[0], hw.rms_norm_q8(row.contiguous(), w)[0])
+    assert torch.equal(hw.rms_norm_grads(dy[:1].expand(n, d), h, w)[0], hw.rms_norm_grads(dy[:1].expand(n, d).contiguous(), h, w)[0])
+    z = x.clone().requires_grad_()
+    hw.rms_norm(z, w).sum().backward()
+    assert torch.equal(z.grad, hw.rms_norm_grads(torch.ones_like(x), x, w)[0])
+
+
 # ---------------------------------------------------------------------------------------------------------------- cross entropy
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
