@@ -375,9 +375,12 @@ def catalogue_cross_entropy(queries, table, targets, scale: float = 1.0, bias: O
     reduction "none" one for each row).  Logits are never in memory; gradients for queries, table and bias through autograd.
 
     queries (n, d), table (v, d): float32 / float16 / bfloat16 of one type, 1 <= d <= 256.  targets (n,): -1 = the row does not count (an unknown
-    node, as everywhere in this package; padding); any other value outside the table makes its loss NaN.  scale > 0: 1 / temperature.  bias (v,) float32,
+    node, as everywhere in this package; padding); any other value outside the table makes its loss NaN.  scale > 0, a number: 1 / temperature (a learned
+    one belongs on the queries).  bias (v,) float32,
     e.g. a correction for popularity; -inf takes a row out of the catalogue.  Rows that do not count or are taken out may hold anything, NaN and
     infinities included; their gradients are zero.  A target that is taken out: a loss of +inf, and the gradients as if its row were zeros.  float32 products keep 2^-22 of an element and 2^-40 of its operand's largest one.  "mean" divides by the counted rows and is 0 without any."""
+    if _wants_grad(scale):
+        raise NotImplementedError("scale has no gradient here: multiply the queries by a learned temperature, or pass a number")
     if _wants_grad(queries, table, bias):
         return _CatalogueCrossEntropy.apply(queries, table, bias, targets, scale, reduction)
     call = _CeCall(queries, table, targets, scale, bias, reduction)

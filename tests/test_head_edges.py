@@ -104,6 +104,20 @@ def test_profiles_of_the_search_are_bound_to_the_search():
     assert hip_build.search_digest() not in (hip_build._digest(), hip_build._digest(hip_build.SEARCH_SOURCES))
 
 
+def test_a_learned_scale_is_refused(hw):
+    """its gradient would be lost without a word"""
+    x, t = torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64)
+    scale = torch.tensor(20.0, requires_grad=True)
+    with pytest.raises(NotImplementedError, match="queries"):
+        hw.catalogue_cross_entropy(x, x, t, scale=scale)
+    from hwer import native
+    for other in (scale.detach(), 20):
+        with pytest.raises(native.HwerNativeError):      # (host tensors)
+            hw.catalogue_cross_entropy(x, x, t, scale=other)
+    with torch.no_grad(), pytest.raises(native.HwerNativeError):
+        hw.catalogue_cross_entropy(x, x, t, scale=scale)
+
+
 # ---------------------------------------------------------------------------------------------------------------- what a call may be given (GPU)
 @gpu
 def test_operators_without_a_gradient_say_so(hw):
