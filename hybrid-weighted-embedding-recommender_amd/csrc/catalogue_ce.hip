@@ -880,12 +880,12 @@ __global__ __launch_bounds__(1024) void ce_loss_kernel(const float* loss_rows, c
     ce_reduce_loss<1024>(loss_rows, target, sums, n, reduction, loss, counted);
 }
 
-// Largest |upstream gradient| of the rows that count (another row's may be anything): of all by one workgroup, or a part of them by each of kSumParts ones;
-// with grad = nullptr of the parts.
-__global__ __launch_bounds__(1024) void ce_grad_top_kernel(const float* grad, const int64_t* target, int64_t n, int64_t v, CeScalars* sc, CeSums* sums) {
+// Largest |upstream gradient| of the rows that count (another row's may be anything): of all by one workgroup, or a part of them by each of kSumParts ones, and
+// then of the parts.  (0 without rows.)
+__global__ __launch_bounds__(1024) void ce_grad_top_kernel(const float* grad, const int64_t* target, int64_t n, int64_t v, CeScalars* sc, CeSums* sums, bool of_parts) {
     __shared__ float s[16];
     float top = 0.f;
-    if (grad)
+    if (!of_parts)
         for (int64_t r = int64_t(blockIdx.x) * 1024 + threadIdx.x; r < n; r += int64_t(gridDim.x) * 1024) top = fmaxf(top, target[r] >= 0 && target[r] < v ? fabsf(grad[r]) : 0.f);
     else if (threadIdx.x < kSumParts) top = sums->top[threadIdx.x];
     top = wave_max_f32(top);
@@ -1083,8 +1083,8 @@ struct CeCall {
     }
     void grad_top(const float* grad) const {
         CeScalars* sc = at<CeScalars>(0);
-        ce_grad_top_kernel<<<dim3(sums() ? kSumParts : 1), dim3(1024), 0, st>>>(grad, target, n, v, sc, sums());
-        if (sums()) ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, st>>>(nullptr, target, n, v, sc, sums());
+        ce_grad_top_kernel<<<dim3(sums() ? kSumParts : 1), dim3(1024), 0, st>>>(grad, target, n, v, sc, sums(), false);
+        if (sums()) ce_grad_top_kernel<<<dim3(1), dim3(1024), 0, st>>>(grad, target, n, v, sc, sums(), true);
     }
 
     // lays out what the passes cannot read in place
@@ -1247,7 +1247,7 @@ int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_
                                int64_t lddq, void* de, int64_t ldde, float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
     CeCall c{q, e, ldq, lde, bias, target, n, v, ce_width(d), dtype, scale, reduction};
     if (int rc = c.check("catalogue_ce_backward", workspace, workspace_bytes, true, stream)) return rc;
-    if (reduction < 0 || reduction > 2 || (reduction == 0 && !grad)) return fail(HWER_EINVAL, "catalogue_ce_backward: unknown reduction %d, or rows' losses without their gradients", reduction);
+    if (reduction < 0 || reduction > 2 || (reduction == 0 && n && !grad)) return fail(HWER_EINVAL, "catalogue_ce_backward: unknown reduction %d, or rows' losses without their gradients", reduction);
     if (!counted || (n && (!state || (dq && !mean)))) return fail(HWER_EINVAL, "catalogue_ce_backward: what the forward call left is missing");
     if ((dq && lddq < d) || (de && ldde < d)) return fail(HWER_EINVAL, "catalogue_ce_backward: a row stride is below d");
     if (dbias && (!bias || !de)) return fail(HWER_EINVAL, "catalogue_ce_backward: dbias needs the bias, and comes with the table's gradient");
@@ -1277,8 +1277,8 @@ int hwer_catalogue_ce_grads(const void* q, int64_t ldq, const void* e, int64_t l
         r.loss_rows = loss_rows, r.dq = dq, r.lddq = lddq, r.rowp = c.at<float>(c.y.rowp);
         if (int rc = c.join<true>(r)) return rc;
     } else {
-        r.per_row = 1, r.grad = loss_rows;      // no rows: the factors of a sum over nothing
-        c.grad_top(loss_rows);
+        r.per_row = 1;      // no rows: the factors of a sum over nothing
+        c.grad_top(nullptr);
         if (int rc = c.backward_rows(r)) return rc;
     }
     return c.pass2(de, ldde, dbias, false, loss_rows, loss);

@@ -435,3 +435,47 @@ def test_cross_entropy_gradient_of_a_class_that_is_a_target_once(hw, n, v, d, dt
         close(tab.grad, ref["de"], want, form + " dtable")
         if form == "mean":
             close(hw.catalogue_cross_entropy_grads(x.cuda(), e.cuda(), t.cuda(), scale=3.0, bias=None if b is None else b.cuda())[2], ref["de"], want, "dtable in one call")
+
+
+@gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_cross_entropy_of_no_rows_through_autograd(hw, reduction):
+    """an empty batch: losses and gradients of a sum over nothing"""
+    for dtype in TYPES:
+        q, e, b = torch.zeros(0, 40, dtype=dtype, device="cuda").requires_grad_(), rnd(1, 70, 40).to(dtype).cuda().requires_grad_(), rnd(2, 70).float().cuda().requires_grad_()
+        loss = hw.catalogue_cross_entropy(q, e, torch.zeros(0, dtype=torch.int64, device="cuda"), bias=b, reduction=reduction)
+        assert loss.shape == ((0,) if reduction == "none" else ()) and not loss.detach().any()
+        loss.backward(torch.zeros(0, device="cuda") if reduction == "none" else None)
+        assert q.grad.shape == (0, 40) and not e.grad.any() and not b.grad.any()
+
+
+@gpu
+def test_cross_entropy_of_many_rows_captured(hw):
+    """the sums in parts inside two graphs, replayed in turn on new contents, with eager calls between"""
+    n, v, d = 20000, 300, 64
+    make = lambda seed: tuple(a.cuda() for a in ce_inputs(seed, n, v, d, torch.bfloat16)[:3])  # noqa: E731
+    bufs, graphs, outs = [make(1), make(2)], [], []
+
+    def call(x, e, t):
+        rows = hw.catalogue_cross_entropy(x, e, t, scale=4.0, reduction="none")
+        return (rows,) + tuple(hw.catalogue_cross_entropy_grads(x, e, t, scale=4.0)) + (hw.catalogue_cross_entropy(x, e, t, scale=4.0),)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for b in bufs:
+            call(*b)
+    torch.cuda.current_stream().wait_stream(side)
+    for b in bufs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(*b))
+        graphs.append(g)
+    for turn in range(3):
+        for k in (0, 1):
+            new = make(10 + 2 * turn + k)
+            for dst, src in zip(bufs[k], new):
+                dst.copy_(src)
+            graphs[k].replay()
+            want = call(*new)
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(outs[k], want)), (turn, k)
