@@ -32,6 +32,7 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 # only where it is another one, the raw stream handle).
 _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _STAY = contextlib.nullcontext()
+_Tensor = torch.Tensor
 
 
 def P(t):
@@ -55,7 +56,7 @@ def _like(t, dtype=None):
 def _wants_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
-            if getattr(t, "requires_grad", False):      # (anything else than a tensor is refused by the checks)
+            if t is not None and getattr(t, "requires_grad", False):      # (anything else than a tensor is refused by the checks)
                 return True
     return False
 
@@ -75,19 +76,19 @@ def _check_rows(name, t, dtypes=_DTYPES, dim=2):
 
 
 def _check_device(t, *others):
-    for o in others:
-        if o is not None and not isinstance(o, torch.Tensor):
-            raise TypeError("a device tensor is needed, got %s" % type(o).__name__)
     if _forward_ad._current_level >= 0:
         for o in (t,) + others:
-            if o is not None and _forward_ad.unpack_dual(o).tangent is not None:
+            if isinstance(o, _Tensor) and _forward_ad.unpack_dual(o).tangent is not None:
                 raise NotImplementedError("the learned head's operators have no forward-mode derivative: got a dual tensor")
     index = t.get_device()
     if index < 0:
         raise native.HwerNativeError("hwer (MI355X build) needs device tensors: got one on %s; there is no CPU fallback for this path" % t.device)
     for o in others:
-        if o is not None and o.get_device() != index:
-            raise ValueError("operands on two devices: %s and %s" % (t.device, o.device))
+        if o is not None:
+            if not isinstance(o, _Tensor):
+                raise TypeError("a device tensor is needed, got %s" % type(o).__name__)
+            if o.get_device() != index:
+                raise ValueError("operands on two devices: %s and %s" % (t.device, o.device))
 
 
 def _rows(t):
