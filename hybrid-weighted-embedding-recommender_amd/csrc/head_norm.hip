@@ -7,7 +7,7 @@
 // The codes do not depend on r: they are quotients of two exact values, rounded once, and equal in every implementation that rounds right.
 //
 // All three are bound by memory: a row is read once, held in registers (raw, 16 bytes per load), reduced over the lanes that hold it and
-// written once.  T lanes hold a row (16, a wave, 4 waves, 16 waves) with VPT vectors each; a workgroup keeps its share of the weights in
+// written once.  T lanes hold a row (16, or 1 to 16 waves: NormPlan) with VPT vectors each; a workgroup keeps its share of the weights in
 // registers and walks over rows.
 #include <algorithm>
 
