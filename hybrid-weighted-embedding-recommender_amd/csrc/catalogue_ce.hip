@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
     // and the one after that: a tile is fetched while two are worked on.
     constexpr int RING = 4;
     // The factor carries a query's own upstream gradient, and the part of its lse that float32 cannot hold beside |lse| ~ 40 (2^-19 of a weight):
-    // of no account in 16-bit gradients, so plain 16-bit passes save the multiplication.
+    // of no account in 16-bit gradients, so plain 16-bit passes save the multiplication, but for tiles with a row beyond FAR.
     constexpr bool MUL = MODE == kTable && (ROWG || BIAS || TERMS == 2);
     constexpr float OFF = X::offset[MODE == kTable];
     __shared__ __align__(16) char s_tile[RING][TERMS][PLANE];
@@ -350,8 +350,9 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
             }
             s = X::mfma(hi, xf[0][k], s);
             if constexpr (TERMS == 2) {
-                s = X::mfma(lo, xf[0][k], s);
-                s = X::mfma(hi, xf[1][k], s);
+                // (in the same order of the operands in both passes: a logit has the same bits in either)
+                s = MODE == kTable ? X::mfma(hi, xf[1][k], s) : X::mfma(lo, xf[0][k], s);
+                s = MODE == kTable ? X::mfma(lo, xf[0][k], s) : X::mfma(hi, xf[1][k], s);
             }
         }
     };
@@ -390,6 +391,11 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
     };
     // S -> weights.  row: the first of the 32; reads: the first fragment reads of the product phase, issued before the exponentials
     float sub = BIAS ? 0.f : OFF;      // what exponents are taken against (without a maximum yet: 0)
+    // Without a bias that is OFF - m c rounded, next to which an exponent's 2^-24 count where it is large: `far` rows' weights are put right by `fix`
+    // (pass 1, per lane), or the row's factor (pass 2).
+    constexpr float FAR = 256.f;
+    float fix = 1.f;
+    bool far = false;
     auto weights = [&](int slot, int sb, int64_t row, int my_target, uint32_t hits, auto reads) __attribute__((always_inline)) {
         if constexpr (HAS_X && !EARLY) read_params(slot, sb);
         float w[16];
@@ -402,6 +408,13 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
             for (int j = 0; j < 16; ++j) {
                 w[j] = __builtin_amdgcn_exp2f(w[j]);
                 if constexpr (MUL) w[j] *= pm[j];
+            }
+            if (!MUL && far) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float4 u = *reinterpret_cast<const float4*>(&s_par[slot][1][sb * 32 + 4 * half + 8 * q]);
+                    w[4 * q] *= u.x, w[4 * q + 1] *= u.y, w[4 * q + 2] *= u.z, w[4 * q + 3] *= u.w;
+                }
             }
             if (hits) {      // (popular classes are hit in every tile: four rows' targets and weights at a time, not one after the other)
 #pragma unroll
@@ -453,7 +466,13 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
                 const float f = m == kLowest ? 1.f : __builtin_amdgcn_exp2f((m - mn) * (BIAS ? kLog2e : c));
                 m = mn;
                 renew = m == kLowest ? kLowest : m + thr;
-                sub = m == kLowest ? (BIAS ? 0.f : OFF) : (BIAS ? m : OFF - m * c);
+                if (renew - m > 1.01f * thr) renew = m;      // (float32's steps at m are larger: the weights' range would not hold)
+                sub = m == kLowest ? (BIAS ? 0.f : OFF) : (BIAS ? m : fmaf(-m, c, OFF));
+                if (!BIAS) {
+                    const bool mine = fabsf(sub) > FAR && m != kLowest;
+                    fix = mine ? __builtin_amdgcn_exp2f(OFF - fmaf(m, c, sub)) : 1.f;
+                    far = __any(mine);
+                }
                 l *= f, l_low *= f;
                 if constexpr (MODE == kMean) {
 #pragma unroll
@@ -467,6 +486,10 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
             reads();
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[j] = __builtin_amdgcn_exp2f(w[j]);
+            if (!BIAS && far) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j] *= fix;
+            }
             add_weights(w);
         }
         if constexpr (MODE != kLse) {
@@ -515,6 +538,10 @@ __global__ __launch_bounds__(256, (ce_waves<TERMS, DP>())) void ce_pass_kernel(C
             const int t = (TS >= 64 || lane < TS) ? __float_as_int(s_par[slot][MODE == kTable ? 3 : 0][lane & (TS - 1)]) : -1;
             static_assert(TS <= 64, "a lane a row");
             hits = __ballot(t >= row0 && t < row0 + 32);
+            if (!MUL) {
+                const float off = (TS >= 64 || lane < TS) ? fabsf(s_par[slot][0][lane & (TS - 1)]) : 0.f;
+                far = __any(off > FAR && off < INFINITY);
+            }
         }
         ce_static_for<0, SB>([&](auto sb_) __attribute__((always_inline)) {
             constexpr int sb = decltype(sb_)::value, sb1 = sb == SB - 1 ? 0 : sb + 1;
@@ -739,7 +766,12 @@ constexpr int kCountedByRow = 256;
 template <bool BIAS>
 __device__ __forceinline__ void ce_put_rowp(const CeRows& a, int64_t r, bool on, float lse, float low, float miss, float rel, int64_t t) {
     const bool some = on && lse != kLowest;
-    a.rowp[r] = some ? (BIAS ? lse : lse - a.off2) : INFINITY;
+    const float px = BIAS ? lse : lse - a.off2;
+    if (!BIAS && some) {      // (what that subtraction leaves)
+        const float back = px - lse;
+        low += (lse - (px - back)) - (a.off2 + back);
+    }
+    a.rowp[r] = some ? px : INFINITY;
     a.rowp[a.ld_rowp + r] = on ? rel * __builtin_amdgcn_exp2f(BIAS ? -low * kLog2e : -low) : 0.f;
     a.rowp[2 * a.ld_rowp + r] = -rel * miss * __builtin_amdgcn_exp2f(a.off2);
     a.rowp[3 * a.ld_rowp + r] = __int_as_float(on ? int(t) : -1);
@@ -801,7 +833,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
     } else if (t != -1) {
         loss = NAN;      // no such class: nothing to learn from, and seen in the loss
     }
-    if (BIAS) lse *= kLn2d;
+    if (BIAS) lse /= double(unit);      // (the inverse of the factor that the passes' exponents have)
     const float hi = float(lse), low = hi == kLowest ? 0.f : float(lse - double(hi));
     float g = 1.f;
     if constexpr (GRADS) {

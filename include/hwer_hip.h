@@ -564,7 +564,7 @@ int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int
  *   Losses and gradients keep their digits where p_target is close to 1 (the target is left out of the sums).
  *   reduction 0 none, 1 mean over counted rows (0 without any), 2 sum.  1 <= d <= hwer_catalogue_ce_max_dim().
  *   loss_rows (n), state (n, 4; 16-byte aligned: what the backward call needs of every row), loss (1, reduction 1 / 2), counted (1, the number of counted rows); mean (n, d) float32, nullable: the mean of a row's classes but its target under their probabilities, which the backward call needs for dq.
- *   n <= 2^26 - 256, v <= 2^31 - 256.
+ *   n <= 2^26 - 256, v <= 2^31 - 256.  |z| below 1e8 (a class at a finite offset of any size is as good as gone beside others).
  * Backward: grad = upstream gradient of the reduced loss (one value, nullable = 1) or of each row (reduction 0).  dq, de, dbias nullable; dbias
  *   comes with de.  dq / de in the rows' type.  Every sum has a fixed order (no atomics).
  * hwer_catalogue_ce_grads: loss (reduction 1 / 2) and gradients in one call, without what the two calls hand over; float32 rows are laid out for the

@@ -479,3 +479,62 @@ def test_cross_entropy_of_many_rows_captured(hw):
             want = call(*new)
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(outs[k], want)), (turn, k)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("mask", [-1e4, -1.7e7, -4e7, -5e7, -6.5e7, -1e8, -1e9, -1e30])
+def test_cross_entropy_of_finite_masks(hw, dtype, mask):
+    """classes put far away by a finite offset, whole tiles of them first, with logits that rise: as good as gone, whatever float32's steps are out there"""
+    n, v, d, gone = 300, 60000, 64, 40000          # (several tiles to a split)
+    x, e, t, b = ce_inputs(77, n, v, d, dtype, bias=True, spread=0.0)
+    e[:gone] = (e[:gone].float() * torch.linspace(1, 6, 128).repeat(gone // 128 + 1)[:gone, None]).to(dtype)
+    b[:gone] = mask
+    t = gone + t % (v - gone)
+    kept = torch.arange(v) >= gone
+    one = torch.full((n,), 1.0 / n, dtype=torch.float64)
+    ref = {k: a.cpu() for k, a in ce_reference(x.cuda(), e.cuda(), t.cuda(), 30.0, torch.where(kept, b, torch.tensor(float("-inf"))).cuda(), one.cuda()).items()}
+    tol = ce_tolerances(ref, dtype, n, v, d)
+    loss, dx, de, db = hw.catalogue_cross_entropy_grads(x.cuda(), e.cuda(), t.cuda(), scale=30.0, bias=b.cuda())
+    close(loss, ref["rows"].mean(), tol["loss"] + ref["rows"].mean().abs() * 2 * U32, "loss")
+    close(dx, ref["dx"], tol["dx"], "dqueries")
+    close(de, ref["de"], tol["de"], "dtable")
+    close(db, ref["db"], tol["db"], "dbias")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("scale", [1e4, 3e6, 1e7, 3e7, 1e8])
+@pytest.mark.parametrize("bias", [False, True])
+def test_cross_entropy_of_huge_logits(hw, dtype, scale, bias):
+    """logits whose float32 steps are beyond one: each row's probability is at one class, and everything stays finite"""
+    n, v, d = 200, 700, 64
+    x, e, t, _ = ce_inputs(5, n, v, d, dtype, spread=0.0)
+    x, e = (x.float() * 2).to(dtype), (e.float() * 2).to(dtype)
+    z = x.double() @ e.double().t()
+    best = z.topk(2, 1)
+    clear = (best.values[:, 0] - best.values[:, 1]) * scale > 200 + 64 * scale * 2.0 ** -22      # (the second class is out of reach)
+    t[::3] = best.indices[::3, 0]
+    t[~clear] = -1
+    assert int((t >= 0).sum()) > n // 2
+    up = torch.full((n,), 0.01 / scale, dtype=torch.float64)
+    leaves = [a.cuda().requires_grad_() for a in (x, e)]
+    b = torch.zeros(v, device="cuda") if bias else None
+    rows = hw.catalogue_cross_entropy(leaves[0], leaves[1], t.cuda(), scale=scale, bias=b, reduction="none")
+    rows.backward(up.float().cuda())
+    on = (t >= 0)
+    at = t.clamp_min(0)
+    want = torch.where(on, scale * (best.values[:, 0] - z.gather(1, at[:, None])[:, 0]), 0.0)
+    size = scale * (x.double().abs() @ e.double().abs().t()).amax(1)
+    close(rows, want, size * (9 * 2.0 ** -22 + 40 * U32) + 1e-30, "rows")
+    g = (scale * up * on)[:, None]
+    top, mine = e.double()[best.indices[:, 0]], e.double()[at]
+    u = U[dtype]
+    close(leaves[0].grad, g * (top - mine), g * (top.abs() + mine.abs()) * (2 * u + 1e-5) + 4 * TINY[dtype], "dqueries")
+    de, de_size = torch.zeros(v, d, dtype=torch.float64), torch.zeros(v, d, dtype=torch.float64)
+    for sign, idx in ((1, best.indices[:, 0]), (-1, at)):
+        de.index_add_(0, idx, sign * g * x.double())
+        de_size.index_add_(0, idx, g * x.double().abs())
+    # a probability next to 1 comes from a difference of logits: float32's step there, up to the probability itself
+    step = min(1.0, float(size.max()) * 8 * U32)
+    close(leaves[1].grad, de, de_size * (2 * u + 1e-5 + 2 * step) + 4 * TINY[dtype], "dtable")
