@@ -992,7 +992,9 @@ __global__ __launch_bounds__(256) void ce_de_kernel(const float* __restrict__ o,
 
 // ---------------------------------------------------------------------------------------------------------------- host
 constexpr int kCeMaxDim = 256;
+// Classes are 32-bit numbers; a wave for each query has to stay below a launch's 2^32 threads
 constexpr int64_t kCeMaxRows = (int64_t(1) << 26) - 256;
+static bool ce_rows_fit(int64_t n, int64_t v) { return n >= 0 && n <= kCeMaxRows && v >= 1 && v <= (int64_t(1) << 31) - 256; }
 static int ce_width(int64_t d) { return d >= 1 && d <= kCeMaxDim ? int(d) : 0; }      // 0: refused by CeCall::check
 static int ce_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
@@ -1094,8 +1096,7 @@ struct CeCall {
     int check(const char* what, void* workspace, size_t bytes, bool want_mean, void* stream) {
         if (!known_dtype(dtype)) return fail(HWER_EINVAL, "%s: unknown element type %d", what, dtype);
         if (d < 1) return fail(HWER_EINVAL, "%s: rows of 1..%d elements are supported", what, kCeMaxDim);
-        // classes are 32-bit numbers; a wave for each query has to stay below a launch's 2^32 threads
-        if (n < 0 || v < 1 || n > kCeMaxRows || v > (int64_t(1) << 31) - 256)
+        if (!ce_rows_fit(n, v))
             return fail(HWER_EINVAL, "%s: %lld rows (at most %lld), %lld classes (at most 2^31 - 256)", what, (long long)n, (long long)kCeMaxRows, (long long)v);
         if (!(scale > 0.f) || !(scale < INFINITY)) return fail(HWER_EINVAL, "%s: scale must be positive and finite", what);
         if (n && (!q || !target)) return fail(HWER_EINVAL, "%s: null queries or targets", what);
@@ -1251,7 +1252,7 @@ int hwer_catalogue_ce_max_dim(void) { return kCeMaxDim; }
 int hwer_catalogue_ce_reads_in_place(const void* rows, int64_t ld, int64_t d, int dtype) { return ce_width(d) && ce_direct(rows, ld, int(d), dtype) ? 1 : 0; }
 
 size_t hwer_catalogue_ce_workspace_bytes(int64_t n, int64_t v, int64_t d, int dtype, int q_in_place, int e_in_place, int want_gradients) {
-    if (!known_dtype(dtype) || !ce_width(d) || n < 0 || v < 1) return 0;
+    if (!known_dtype(dtype) || !ce_width(d) || !ce_rows_fit(n, v)) return 0;      // (what the calls refuse)
     return ce_layout(n, v, int(d), dtype, q_in_place != 0, e_in_place != 0, want_gradients != 0).bytes(want_gradients != 0);
 }
 

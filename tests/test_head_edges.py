@@ -59,6 +59,7 @@ def test_more_rows_than_a_launch_has_threads_for_are_refused(hw):
     for n in ((1 << 26) - 255, 1 << 26, 1 << 30):
         assert lib.hwer_catalogue_ce(p, 8, p, 8, None, p, n, 3, 8, 0, 1.0, 1, p, p, p, p, None, p, 1 << 50, None) == E
         assert lib.hwer_catalogue_ce_grads(p, 8, p, 8, None, p, n, 3, 8, 0, 1.0, 1, p, p, 8, p, 8, None, p, 1 << 50, None) == E
+        assert lib.hwer_catalogue_ce_workspace_bytes(n, 3, 8, 0, 0, 0, 1) == 0 and lib.hwer_catalogue_ce_workspace_bytes(3, 64 * n, 8, 0, 0, 0, 1) == 0
         assert lib.hwer_catalogue_ce_backward(p, 8, p, 8, None, p, n, 3, 8, 0, 1.0, 1, p, p, p, p, p, 8, p, 8, None, p, 1 << 50, None) == E
     for m, n, k in ((1, 1 << 30, 16), (1 << 30, 32, 512), (1 << 28, 5, 513), (40, (1 << 31) - 256, 64), (1 << 30, 1 << 30, 8), (1 << 31, 2, 8)):
         assert lib.hwer_matmul_q8(p, k, p, p, k, p, None, m, n, k, p, n, 0, None) == E, (m, n, k)
