@@ -829,7 +829,8 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeRows a) {
         const bool none = sum == 0.f && z == -double(INFINITY);      // every class masked
         loss = none ? double(INFINITY) : x > 64.0 ? x * kLn2d : log1p(exp2(x));
         miss = none ? 1.0 : 1.0 / (1.0 + exp2(-x));
-        if (!none && z != -double(INFINITY)) lse = z + loss / kLn2d;
+        // (from the larger one: beside a target at float32's lowest value the sum of the others would be lost)
+        if (!none && z != -double(INFINITY)) lse = x > 0.0 ? rest + log1p(exp2(-x)) / kLn2d : z + loss / kLn2d;
     } else if (t != -1) {
         loss = NAN;      // no such class: nothing to learn from, and seen in the loss
     }

@@ -505,6 +505,34 @@ def test_cross_entropy_of_finite_masks(hw, dtype, mask):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("mask", [-1e4, -4e7, -1e9, -1e30, -3e38, float(torch.finfo(torch.float32).min)])
+@pytest.mark.parametrize("n,v,d", [(60, 90, 64), (300, 2000, 100)])
+def test_cross_entropy_of_a_target_at_a_finite_mask(hw, n, v, d, dtype, mask):
+    """its loss is as large as the mask, its probability nothing, and everything else as if it were far away"""
+    x, e, t, b = ce_inputs(n + d, n, v, d, dtype, bias=True, spread=0.0)
+    b[: v // 3] = mask
+    t = v // 3 + t % (v - v // 3)
+    t[::5] = 7
+    t[1::10] = -1
+    far = t == 7
+    counted = int((t >= 0).sum())
+    up = torch.where(t >= 0, 1.0 / counted, 0.0).double()
+    ref = ce_reference(x, e, t, 4.0, b, up)
+    tol = ce_tolerances(ref, dtype, n, v, d)
+    leaves = [a.cuda().requires_grad_() for a in (x, e, b)]
+    rows = hw.catalogue_cross_entropy(leaves[0], leaves[1], t.cuda(), scale=4.0, bias=leaves[2], reduction="none")
+    # (the target's logit is rounded at the mask's size)
+    close(rows, ref["rows"].clamp_max(float(torch.finfo(torch.float32).max)), tol["loss"] + ref["rows"].abs() * U32 + torch.where(far, abs(mask) * 2 * U32, 0.0), "rows")
+    rows.backward(up.float().cuda())
+    grads = hw.catalogue_cross_entropy_grads(x.cuda(), e.cuda(), t.cuda(), scale=4.0, bias=b.cuda())
+    for dx, de, db in (tuple(a.grad for a in leaves), grads[1:]):
+        close(dx, ref["dx"], 1.01 * tol["dx"] + ref["dx_size"] * 4 * U32, "dqueries")
+        close(de, ref["de"], 1.01 * tol["de"] + ref["de_size"] * 4 * U32, "dtable")
+        close(db, ref["db"], 1.01 * tol["db"] + ref["db_size"] * 4 * U32, "dbias")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("scale", [1e4, 3e6, 1e7, 3e7, 1e8])
 @pytest.mark.parametrize("bias", [False, True])
 def test_cross_entropy_of_huge_logits(hw, dtype, scale, bias):
