@@ -197,7 +197,8 @@ class _RmsNorm(torch.autograd.Function):
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-6):
     """y = h * weight / sqrt(mean(h^2, last dimension) + eps) with h = x, or h = x + residual rounded to their type: -> y, or (y, h) with a residual.
-    x: float32 / float16 / bfloat16, any number of leading dimensions; weight: (d,) float32 or x's type, None = ones."""
+    x: float32 / float16 / bfloat16, any number of leading dimensions; weight: (d,) float32 or x's type, None = ones.  Squares are summed in float32:
+    |h| below 1.8e19 / sqrt(d), and with eps below 1e-28 a row's largest above 1e-14."""
     _norm_checks(x, weight, residual, eps)
     eps = float(eps)
     if _wants_grad(x, weight, residual):
@@ -379,7 +380,8 @@ def catalogue_cross_entropy(queries, table, targets, scale: float = 1.0, bias: O
     node, as everywhere in this package; padding); any other value outside the table makes its loss NaN.  scale > 0, a number: 1 / temperature (a learned
     one belongs on the queries).  bias (v,) float32,
     e.g. a correction for popularity; -inf takes a row out of the catalogue.  Rows that do not count or are taken out may hold anything, NaN and
-    infinities included; their gradients are zero.  A target that is taken out: a loss of +inf, and the gradients as if its row were zeros.  float32 products keep 2^-22 of an element and 2^-40 of its operand's largest one.  "mean" divides by the counted rows and is 0 without any."""
+    infinities included; their gradients are zero.  A target that is taken out: a loss of +inf, and the gradients as if its row were zeros.  float32 products keep 2^-22 of an element and 2^-40 of its operand's largest one;
+    float16 and float32 rows' gradients keep a probability's 2^-40 of the largest (of the largest upstream gradient, with one for each row).  "mean" divides by the counted rows and is 0 without any."""
     if _wants_grad(scale):
         raise NotImplementedError("scale has no gradient here: multiply the queries by a learned temperature, or pass a number")
     if _wants_grad(queries, table, bias):

@@ -570,6 +570,8 @@ int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int
  * hwer_catalogue_ce_grads: loss (reduction 1 / 2) and gradients in one call, without what the two calls hand over; float32 rows are laid out for the
  *   matrix instructions once.
  *   float32 rows are multiplied as two float16 terms relative to the operand's largest finite element: elements keep 2^-22 of themselves and 2^-40 of it.
+ *   Probabilities enter the gradients' products in 16 bits (float32 rows: two terms): float16 terms end at 2^-36 of a row's largest in dq and 2^-40 of the
+ *   largest row's gradient in de (contributions below that are lost), bfloat16 at float32's smallest.
  *   Rows of q that do not count, and rows of e whose bias is -inf, may hold anything (NaN, infinities): they reach no other row.
  * Workspace: hwer_catalogue_ce_workspace_bytes(..., q_in_place, e_in_place = hwer_catalogue_ce_reads_in_place(rows, ld, d, dtype), ...); with a bias the table
  *   is never read in place (e_in_place = 0). */
