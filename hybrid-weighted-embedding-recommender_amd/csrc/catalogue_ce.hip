@@ -1106,6 +1106,7 @@ struct CeCall {
         y = ce_layout(n, v, d, dtype, q_direct, e_direct, want_mean);
         const size_t need = y.bytes(want_mean);
         if (!workspace || bytes < need) return fail(HWER_EWORKSPACE, "%s: workspace of %zu bytes needed", what, need);
+        if (!aligned_to(workspace, 0, 256)) return fail(HWER_EINVAL, "%s: the workspace must be 256-byte aligned", what);
         ws = static_cast<unsigned char*>(workspace), st = as_stream(stream);
         return HWER_OK;
     }
@@ -1264,6 +1265,7 @@ int hwer_catalogue_ce(const void* q, int64_t ldq, const void* e, int64_t lde, co
     if (int rc = c.check("catalogue_ce", workspace, workspace_bytes, mean != nullptr, stream)) return rc;
     if (reduction < 0 || reduction > 2) return fail(HWER_EINVAL, "catalogue_ce: unknown reduction %d", reduction);
     if (!counted || (reduction && !loss) || (n && (!loss_rows || !state))) return fail(HWER_EINVAL, "catalogue_ce: null output");
+    if (!aligned_to(state, 0, 16)) return fail(HWER_EINVAL, "catalogue_ce: state must be 16-byte aligned");
     if (n) {
         CeRows r;
         if (int rc = c.prepare()) return rc;
@@ -1283,6 +1285,7 @@ int hwer_catalogue_ce_backward(const void* q, int64_t ldq, const void* e, int64_
     if (int rc = c.check("catalogue_ce_backward", workspace, workspace_bytes, true, stream)) return rc;
     if (reduction < 0 || reduction > 2 || (reduction == 0 && n && !grad)) return fail(HWER_EINVAL, "catalogue_ce_backward: unknown reduction %d, or rows' losses without their gradients", reduction);
     if (!counted || (n && (!state || (dq && !mean)))) return fail(HWER_EINVAL, "catalogue_ce_backward: what the forward call left is missing");
+    if (!aligned_to(state, 0, 16)) return fail(HWER_EINVAL, "catalogue_ce_backward: state must be 16-byte aligned");
     if ((dq && lddq < d) || (de && ldde < d)) return fail(HWER_EINVAL, "catalogue_ce_backward: a row stride is below d");
     if (dbias && (!bias || !de)) return fail(HWER_EINVAL, "catalogue_ce_backward: dbias needs the bias, and comes with the table's gradient");
     if (de || dtype == HWER_F32)

@@ -693,6 +693,7 @@ int hwer_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t 
     if (rows && (!dy || !dx || lddy < d || lddx < d || (dh && lddh < d))) return fail(HWER_EINVAL, "rms_norm_backward: null rows or a row stride below d");
     if (dweight && (!workspace || workspace_bytes < hwer_rms_norm_backward_workspace_bytes(rows, d)))
         return fail(HWER_EWORKSPACE, "rms_norm_backward: workspace of %zu bytes needed", hwer_rms_norm_backward_workspace_bytes(rows, d));
+    if (dweight && !aligned_to(workspace, 0, 16)) return fail(HWER_EINVAL, "rms_norm_backward: the workspace must be 16-byte aligned");
     hipStream_t st = as_stream(stream);
     NormBwdArgs a{dy, h, weight, dh, dx, dweight ? static_cast<float*>(workspace) : nullptr, rows, lddy, ldh, lddh, lddx, int(d), eps};
     int parts = 0;

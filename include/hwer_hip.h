@@ -545,7 +545,7 @@ int hwer_rms_norm_q8(const void* x, int64_t ldx, const void* residual /*nullable
                      int64_t rows, int64_t d, int dtype, int norm, float eps, int8_t* q, int64_t ldq, float* scale, void* h, int64_t ldh, void* stream);
 /* Gradients:  dx = (weight * dy - h * r^2 * mean(h * weight * dy)) * r + dh,  dweight = sum_rows dy * h * r  (the residual's gradient is dx).
  * h: what hwer_rms_norm was taken of (its h, or x without a residual).  dh (nullable): gradient that reaches h directly.
- * dweight (nullable) needs the workspace; its sum has a fixed order (no atomics).  dx shares memory with no input. */
+ * dweight (nullable) needs the workspace (16-byte aligned); its sum has a fixed order (no atomics).  dx shares memory with no input. */
 size_t hwer_rms_norm_backward_workspace_bytes(int64_t rows, int64_t d);
 int hwer_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* weight /*nullable*/, int weight_dtype,
                            const void* dh /*nullable*/, int64_t lddh, int64_t rows, int64_t d, int dtype, float eps, void* dx, int64_t lddx,
@@ -573,7 +573,7 @@ int hwer_matmul_q8(const int8_t* a, int64_t lda, const float* a_scale, const int
  *   Probabilities enter the gradients' products in 16 bits (float32 rows: two terms): float16 terms end at 2^-36 of a row's largest in dq and 2^-40 of the
  *   largest row's gradient in de (contributions below that are lost), bfloat16 at float32's smallest.
  *   Rows of q that do not count, and rows of e whose bias is -inf, may hold anything (NaN, infinities): they reach no other row.
- * Workspace: hwer_catalogue_ce_workspace_bytes(..., q_in_place, e_in_place = hwer_catalogue_ce_reads_in_place(rows, ld, d, dtype), ...); with a bias the table
+ * Workspace (256-byte aligned): hwer_catalogue_ce_workspace_bytes(..., q_in_place, e_in_place = hwer_catalogue_ce_reads_in_place(rows, ld, d, dtype), ...); with a bias the table
  *   is never read in place (e_in_place = 0). */
 int hwer_catalogue_ce_max_dim(void);
 int hwer_catalogue_ce_reads_in_place(const void* rows, int64_t ld, int64_t d, int dtype);

@@ -65,6 +65,20 @@ def test_more_rows_than_a_launch_has_threads_for_are_refused(hw):
         assert lib.hwer_matmul_q8(p, k, p, p, k, p, None, m, n, k, p, n, 0, None) == E, (m, n, k)
 
 
+def test_workspaces_off_their_alignment_are_refused(hw):
+    from hwer import native
+    lib, p, E = native.lib(), ctypes.c_void_p(4096), native.HWER_EINVAL
+    at = lambda off: ctypes.c_void_p(4096 + off)  # noqa: E731
+    for off in (1, 4, 16, 128):
+        assert lib.hwer_catalogue_ce(p, 8, p, 8, None, p, 2, 3, 8, 0, 1.0, 1, p, p, p, p, None, at(off), 1 << 40, None) == E
+        assert lib.hwer_catalogue_ce_grads(p, 8, p, 8, None, p, 2, 3, 8, 0, 1.0, 1, p, p, 8, p, 8, None, at(off), 1 << 40, None) == E
+        assert lib.hwer_catalogue_ce_backward(p, 8, p, 8, None, p, 2, 3, 8, 0, 1.0, 1, p, p, p, p, p, 8, p, 8, None, at(off), 1 << 40, None) == E
+    for off in (1, 4, 8):
+        assert lib.hwer_catalogue_ce(p, 8, p, 8, None, p, 2, 3, 8, 0, 1.0, 1, p, at(off), p, p, None, p, 1 << 40, None) == E
+        assert lib.hwer_catalogue_ce_backward(p, 8, p, 8, None, p, 2, 3, 8, 0, 1.0, 1, p, at(off), p, p, p, 8, p, 8, None, p, 1 << 40, None) == E
+        assert lib.hwer_rms_norm_backward(p, 8, p, 8, p, 0, None, 0, 2, 8, 0, 1e-6, p, 8, p, at(off), 1 << 40, None) == E
+
+
 def test_dual_tensors_are_refused(hw):
     """a forward-mode tangent would be lost without a word: requires_grad is False on a dual tensor"""
     import torch.autograd.forward_ad as fw
